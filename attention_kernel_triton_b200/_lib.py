@@ -26,7 +26,7 @@ AKT_BFLOAT16 = 1
 
 DEVICE_STATUS_NAMES = {0: "ok", 1: "wait timeout", 2: "page id outside the pool",
                        3: "token index outside the sequence", 4: "malformed indptr",
-                       5: "kept-index list longer than its buffer"}
+                       5: "list longer than its buffer", 6: "no dead page left to copy to"}
 
 
 class AktError(RuntimeError):
@@ -147,6 +147,58 @@ class AppendPagedArgs(Structure):
     ]
 
 
+class RotaryArgs(Structure):
+    _fields_ = [
+        ("q", c_void_p), ("q_stride_token", c_int64), ("q_stride_head", c_int64), ("q_stride_dim", c_int64),
+        ("k", c_void_p), ("k_stride_token", c_int64), ("k_stride_head", c_int64), ("k_stride_dim", c_int64),
+        ("q_out", c_void_p), ("q_out_stride_token", c_int64), ("q_out_stride_head", c_int64),
+        ("q_out_stride_dim", c_int64),
+        ("k_out", c_void_p), ("k_out_stride_token", c_int64), ("k_out_stride_head", c_int64),
+        ("k_out_stride_dim", c_int64),
+        ("cos_sin", c_void_p), ("cos_sin_stride", c_int64), ("max_positions", c_int64), ("positions", c_void_p),
+        ("num_tokens", c_int64),
+        ("num_qo_heads", c_int32), ("num_kv_heads", c_int32), ("head_dim", c_int32), ("rotary_dim", c_int32),
+        ("interleaved", c_int32), ("inverse", c_int32), ("dtype", c_int32),
+    ]
+
+
+class AppendRotaryArgs(Structure):
+    _fields_ = [
+        ("append", AppendPagedArgs),
+        ("q", c_void_p), ("q_stride_token", c_int64), ("q_stride_head", c_int64), ("q_stride_dim", c_int64),
+        ("q_out", c_void_p), ("q_out_stride_token", c_int64), ("q_out_stride_head", c_int64),
+        ("q_out_stride_dim", c_int64),
+        ("cos_sin", c_void_p), ("cos_sin_stride", c_int64), ("max_positions", c_int64),
+        ("num_qo_heads", c_int32), ("rotary_dim", c_int32), ("interleaved", c_int32),
+    ]
+
+
+class PagePool(Structure):
+    _fields_ = [
+        ("kv_cache", c_void_p), ("stride_layer", c_int64), ("stride_page", c_int64), ("stride_kv", c_int64),
+        ("stride_head", c_int64), ("stride_token", c_int64), ("stride_dim", c_int64), ("num_pages", c_int64),
+        ("num_layers", c_int32), ("num_kv_heads", c_int32), ("page_size", c_int32), ("head_dim", c_int32),
+    ]
+
+
+class ForkPagedArgs(Structure):
+    _fields_ = [
+        ("pool", PagePool),
+        ("kv_page_indptr", c_void_p), ("kv_page_indices", c_void_p), ("kv_last_page_len", c_void_p),
+        ("num_page_entries", c_int64), ("parents", c_void_p), ("reserved", c_void_p),
+        ("out_indptr", c_void_p), ("out_indices", c_void_p), ("out_last_page_len", c_void_p),
+        ("max_entries", c_int64), ("batch", c_int32), ("num_children", c_int32),
+    ]
+
+
+class CompactPagedArgs(Structure):
+    _fields_ = [
+        ("pool", PagePool),
+        ("kv_page_indices", c_void_p), ("num_page_entries", c_int64), ("reserved", c_void_p),
+        ("out_indices", c_void_p), ("pages_used", c_void_p),
+    ]
+
+
 AKT_MAX_PEERS = 8
 
 
@@ -200,6 +252,16 @@ SIGNATURES = {
                                             c_void_p]),
     "akt_mask_to_sparse_index": (c_int, [POINTER(MaskToIndexArgs), c_void_p]),
     "akt_sparse_index_to_mask": (c_int, [POINTER(IndexToMaskArgs), c_void_p]),
+    "akt_rotary": (c_int, [POINTER(RotaryArgs), c_void_p]),
+    "akt_append_rotary_paged_kv": (c_int, [POINTER(AppendRotaryArgs), c_void_p]),
+    "akt_copy_kv_pages": (c_int, [POINTER(PagePool), c_void_p, c_void_p, c_int64, c_void_p]),
+    "akt_fork_paged_workspace_size": (c_size_t, [POINTER(ForkPagedArgs)]),
+    "akt_fork_paged": (c_int, [POINTER(ForkPagedArgs), c_void_p, c_size_t, c_void_p]),
+    "akt_compact_paged_workspace_size": (c_size_t, [POINTER(CompactPagedArgs)]),
+    "akt_compact_paged": (c_int, [POINTER(CompactPagedArgs), c_void_p, c_size_t, c_void_p]),
+    "akt_free_kv_pages_workspace_size": (c_size_t, [c_int64]),
+    "akt_free_kv_pages": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_size_t,
+                                  c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,250 @@
+"""Rotary positions: the table of angles, the rotation of plain tensors (with
+its gradient) and the rotation fused with the append to a paged KV cache.
+
+The reference starts from queries and keys that are already rotated; these are
+the steps before it.  A model keeps one table, ``rotary_cos_sin(...)``
+(``[max_positions, rotary_dim]`` fp32: the cosines of ``rotary_dim / 2`` angles,
+then their sines), and hands it to every call.  Pair ``i`` of a head's first
+``rotary_dim`` values, ``(x[i], x[i + rotary_dim / 2])`` or, ``interleaved``,
+``(x[2i], x[2i + 1])``, becomes ``(a c - b s, b c + a s)``; the values past
+``rotary_dim`` are copied.  Sums are in fp32, rounded once to the tensors' type.
+Runs ``akt_rotary`` / ``akt_append_rotary_paged_kv`` (sm_100a) on torch's
+current stream.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+
+
+def rotary_frequencies(rotary_dim, base=10000.0, scaling=None):
+    """``(angles per position, fp64 [rotary_dim / 2]; factor on cos and sin)``.
+
+    ``scaling`` (a dict) stretches the angles for contexts past the trained length:
+
+    * ``{"type": "linear", "factor": f}``: every angle divided by ``f``;
+    * ``{"type": "ntk", "factor": f}``: the base raised to
+      ``base * f ** (rotary_dim / (rotary_dim - 2))``, which divides the slowest
+      angle by ``f`` and leaves the fastest;
+    * ``{"type": "yarn", "factor": f, "original_max_positions": n}`` (optional
+      ``beta_fast`` 32, ``beta_slow`` 1, ``attention_factor`` ``0.1 ln f + 1``):
+      angles that turn more than ``beta_fast`` times in ``n`` positions are kept,
+      those that turn less than ``beta_slow`` times divided by ``f``, and the ones
+      between mixed linearly over their index (Peng et al., "YaRN", 2023);
+    * ``{"type": "banded", "factor": f, "original_max_positions": n,
+      "low_freq_factor": a, "high_freq_factor": b}``: by wave length ``w = 2 pi /
+      angle``: kept below ``n / b``, divided by ``f`` above ``n / a``, between them
+      mixed linearly in ``n / w``.
+    """
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be positive and even")
+    if not base > 0:
+        raise ValueError("base must be positive")
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    freq = float(base) ** (-2 * i / rotary_dim)
+    if scaling is None:
+        return freq, 1.0
+    kind = scaling.get("type")
+    f = float(scaling["factor"])
+    if not f > 0:
+        raise ValueError("scaling factor must be positive")
+    if kind == "linear":
+        return freq / f, 1.0
+    if kind == "ntk":
+        if rotary_dim == 2:
+            raise ValueError("ntk scaling needs rotary_dim > 2")
+        return (float(base) * f ** (rotary_dim / (rotary_dim - 2))) ** (-2 * i / rotary_dim), 1.0
+    if kind == "yarn":
+        n = float(scaling["original_max_positions"])
+
+        def index_of(turns):  # index of the angle that makes so many turns in n positions
+            return rotary_dim * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+        lo = max(math.floor(index_of(float(scaling.get("beta_fast", 32.0)))), 0)
+        hi = min(math.ceil(index_of(float(scaling.get("beta_slow", 1.0)))), rotary_dim - 1)
+        ramp = ((i - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        default = 0.1 * math.log(f) + 1.0 if f > 1 else 1.0
+        return freq / f * ramp + freq * (1 - ramp), float(scaling.get("attention_factor", default))
+    if kind == "banded":
+        n = float(scaling["original_max_positions"])
+        a, b = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        if not b > a:
+            raise ValueError("high_freq_factor must exceed low_freq_factor")
+        keep = ((n * freq / (2 * math.pi) - a) / (b - a)).clamp(0, 1)
+        return freq * keep + freq / f * (1 - keep), 1.0
+    raise ValueError(f"unknown rotary scaling {kind!r}")
+
+
+def rotary_cos_sin(max_positions, rotary_dim, base=10000.0, scaling=None, device="cuda"):
+    """The table ``[max_positions, rotary_dim]`` (fp32) for the calls below, built once:
+    angles in fp64 (an fp32 product is off by 0.008 at position 131072), rounded at the end."""
+    freq, factor = rotary_frequencies(rotary_dim, base, scaling)
+    angle = torch.arange(max_positions, dtype=torch.float64)[:, None] * freq
+    return torch.cat((angle.cos() * factor, angle.sin() * factor), 1).float().to(device)
+
+
+def _check_table(cos_sin, D, dev):
+    if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32 or cos_sin.device != dev:
+        raise ValueError("cos_sin must be fp32 [max_positions, rotary_dim] on the tensors' device")
+    R = cos_sin.shape[1]
+    if R % 2 or R > D:
+        raise ValueError("rotary_dim (the table's width) must be even and at most the head dim")
+    return cos_sin if cos_sin.stride(1) == 1 and cos_sin.stride(0) >= R else cos_sin.contiguous()
+
+
+def _unit(x):
+    return x if x.stride(-1) == 1 else x.contiguous()
+
+
+def rotary_into(q_out, k_out, q, k, cos_sin, positions, interleaved=False, inverse=False):
+    """Rotate ``q [T, Hq, D]`` into ``q_out`` and, unless ``k`` is None, ``k [T, Hkv, D]``
+    into ``k_out`` (either may be its input: in place)."""
+    ts = (q, q_out) if k is None else (q, q_out, k, k_out)
+    dev = _lib.require_cuda(*ts, cos_sin)
+    for t in ts:
+        if t.dim() != 3 or t.shape[0] != q.shape[0] or t.shape[2] != q.shape[2]:
+            raise ValueError("tensors must be [tokens, heads, head_dim] with the same tokens and head_dim")
+        if t.dtype != q.dtype:
+            raise TypeError("q, k and the outputs must share one dtype")
+    if q_out.shape != q.shape or (k is not None and k_out.shape != k.shape):
+        raise ValueError("an output must have its input's shape")
+    T, Hq, D = q.shape
+    table = _check_table(cos_sin, D, dev)
+    pos = _lib.as_int32(positions, dev)
+    if pos.dim() != 1 or pos.numel() != T:
+        raise ValueError("positions must hold one position per token")
+    pos = pos.contiguous()
+    a = _lib.RotaryArgs()
+    q = _unit(q)
+    a.q, (a.q_stride_token, a.q_stride_head, a.q_stride_dim) = q.data_ptr(), q.stride()
+    a.q_out, (a.q_out_stride_token, a.q_out_stride_head, a.q_out_stride_dim) = q_out.data_ptr(), q_out.stride()
+    if k is not None:
+        k = _unit(k)
+        a.k, (a.k_stride_token, a.k_stride_head, a.k_stride_dim) = k.data_ptr(), k.stride()
+        a.k_out, (a.k_out_stride_token, a.k_out_stride_head, a.k_out_stride_dim) = k_out.data_ptr(), k_out.stride()
+        a.num_kv_heads = k.shape[1]
+    a.cos_sin, a.cos_sin_stride, a.max_positions = table.data_ptr(), table.stride(0), table.shape[0]
+    a.positions, a.num_tokens = pos.data_ptr(), T
+    a.num_qo_heads, a.head_dim, a.rotary_dim = Hq, D, table.shape[1]
+    a.interleaved, a.inverse, a.dtype = int(bool(interleaved)), int(bool(inverse)), _lib.dtype_code(q)
+    with _lib.on_device(dev):
+        _lib.check(_lib.lib().akt_rotary(ctypes.byref(a), _lib.stream_ptr(dev)))
+    return q_out, k_out
+
+
+def _forward(q, k, cos_sin, positions, interleaved, inverse):
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    return rotary_into(q_out, k_out, q, k, cos_sin, positions, interleaved, inverse)
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, cos_sin, positions, interleaved, inverse):
+        ctx.save_for_backward(cos_sin, positions)
+        ctx.how = interleaved, inverse
+        return _forward(q, k, cos_sin, positions, interleaved, inverse)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        cos_sin, positions = ctx.saved_tensors
+        interleaved, inverse = ctx.how
+        q_in, k_in = _forward(dq, dk, cos_sin, positions, interleaved, not inverse)
+        return q_in, k_in, None, None, None, None
+
+
+def apply_rotary_qk(q, k, cos_sin, positions, interleaved=False, inverse=False):
+    """
+    q: [T, Hq, D], k: [T, Hkv, D] (fp16 or bf16; any strides with unit dim stride)
+    cos_sin: [max_positions, rotary_dim] (fp32), positions: [T] (int32)
+    returns (q', k') of the same shapes; a position outside the table gives zeros (status 3)
+
+    ``inverse`` turns the other way, which is the gradient too: a training step either
+    calls it on the outputs' gradients or lets autograd do so.
+    """
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+        return _Rotary.apply(q, k, cos_sin, positions, interleaved, inverse)
+    return _forward(q, k, cos_sin, positions, interleaved, inverse)
+
+
+def apply_rotary(x, cos_sin, positions, interleaved=False, inverse=False):
+    """``apply_rotary_qk`` for one tensor ``x [T, H, D]``."""
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _RotaryOne.apply(x, cos_sin, positions, interleaved, inverse)
+    return _forward(x, None, cos_sin, positions, interleaved, inverse)[0]
+
+
+class _RotaryOne(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, cos_sin, positions, interleaved, inverse):
+        ctx.save_for_backward(cos_sin, positions)
+        ctx.how = interleaved, inverse
+        return _forward(x, None, cos_sin, positions, interleaved, inverse)[0]
+
+    @staticmethod
+    def backward(ctx, dx):
+        cos_sin, positions = ctx.saved_tensors
+        interleaved, inverse = ctx.how
+        return _forward(dx, None, cos_sin, positions, interleaved, not inverse)[0], None, None, None, None
+
+
+def append_rotary_paged_kv_cache(paged_kv_cache, q, append_k, append_v, append_indptr, kv_page_indptr,
+                                 kv_page_indices, kv_last_page_len, cos_sin, interleaved=False):
+    """``paged_kv_append.append_paged_kv_cache`` with the keys rotated to their positions in
+    their sequences on the way, and the rotated queries ``[num_append, Hq, D]`` returned.
+
+    ``q`` (or None: nothing is returned), ``append_k`` and ``append_v`` are
+    ``[num_append, heads, D]``, ragged by ``append_indptr [B + 1]``; the page table already
+    describes the sequences after the append.  One pass: the rotated keys are never stored
+    outside the pool.
+    """
+    dev = _lib.require_cuda(paged_kv_cache, append_k, append_v, cos_sin)
+    if not (paged_kv_cache.dtype == append_k.dtype == append_v.dtype):
+        raise TypeError("the pool and the appended rows must share one dtype")
+    if paged_kv_cache.dim() != 5 or paged_kv_cache.shape[1] != 2:
+        raise ValueError("paged_kv_cache must be [num_pages, 2, Hkv, page_size, D]")
+    _, _, Hkv, P, D = paged_kv_cache.shape
+    if append_k.dim() != 3 or append_k.shape[1:] != (Hkv, D) or append_v.shape != append_k.shape:
+        raise ValueError("append_k and append_v must be [num_append, Hkv, D]")
+    table = _check_table(cos_sin, D, dev)
+    indptr = _lib.as_int32(kv_page_indptr, dev).contiguous()
+    indices = _lib.as_int32(kv_page_indices, dev).contiguous()
+    last = _lib.as_int32(kv_last_page_len, dev).contiguous()
+    app = _lib.as_int32(append_indptr, dev).contiguous()
+    B = indptr.numel() - 1
+    if app.numel() != B + 1 or last.numel() != B:
+        raise ValueError("append_indptr and kv_page_indptr must have B+1 entries and kv_last_page_len B entries")
+    k, v = _unit(append_k), _unit(append_v)
+    x = _lib.AppendRotaryArgs()
+    a = x.append
+    a.kv_cache = paged_kv_cache.data_ptr()
+    (a.kv_stride_page, a.kv_stride_kv, a.kv_stride_head, a.kv_stride_token, a.kv_stride_dim) = paged_kv_cache.stride()
+    a.num_pages = paged_kv_cache.shape[0]
+    a.kv_page_indptr, a.kv_page_indices, a.kv_last_page_len = indptr.data_ptr(), indices.data_ptr(), last.data_ptr()
+    a.num_page_entries = indices.numel()
+    a.append_k, (a.k_stride_token, a.k_stride_head, a.k_stride_dim) = k.data_ptr(), k.stride()
+    a.append_v, (a.v_stride_token, a.v_stride_head, a.v_stride_dim) = v.data_ptr(), v.stride()
+    a.append_indptr, a.num_append = app.data_ptr(), k.shape[0]
+    a.batch, a.num_kv_heads, a.page_size, a.head_dim = B, Hkv, P, D
+    a.dtype = _lib.dtype_code(k)
+    q_out = None
+    if q is not None:
+        _lib.require_cuda(paged_kv_cache, q)
+        if q.dtype != append_k.dtype:
+            raise TypeError("the pool and the appended rows must share one dtype")
+        if q.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != D:
+            raise ValueError("q must be [num_append, Hq, D]")
+        q = _unit(q)
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        x.q, (x.q_stride_token, x.q_stride_head, x.q_stride_dim) = q.data_ptr(), q.stride()
+        x.q_out, (x.q_out_stride_token, x.q_out_stride_head, x.q_out_stride_dim) = q_out.data_ptr(), q_out.stride()
+        x.num_qo_heads = q.shape[1]
+    x.cos_sin, x.cos_sin_stride, x.max_positions = table.data_ptr(), table.stride(0), table.shape[0]
+    x.rotary_dim, x.interleaved = table.shape[1], int(bool(interleaved))
+    with _lib.on_device(dev):
+        _lib.check(_lib.lib().akt_append_rotary_paged_kv(ctypes.byref(x), _lib.stream_ptr(dev)))
+    return q_out

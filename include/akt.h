@@ -46,7 +46,8 @@ int akt_abi_version(void);
 const char* akt_last_error(void);
 /* First error code any kernel recorded on `device` since the last clear
  * (0 = none; 1 wait timeout, 2 page id out of pool, 3 token index out of
- * sequence, 4 malformed indptr, 5 kept-index list longer than its buffer).
+ * sequence, 4 malformed indptr, 5 list longer than its buffer, 6 no dead page
+ * left to copy to).
  * Synchronises that device. */
 int akt_device_status(int device, unsigned int* status_out);
 int akt_clear_device_status(int device);
@@ -411,6 +412,135 @@ typedef struct akt_index_to_mask_args {
 } akt_index_to_mask_args;
 
 int akt_sparse_index_to_mask(const akt_index_to_mask_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* rotary positions (no reference counterpart: its inputs come rotated)     */
+/* Row cos_sin[p] of the fp32 table holds the cosines of rotary_dim / 2     */
+/* angles of position p, then their sines.  The first rotary_dim values of  */
+/* a head form pairs, (x[i], x[i + rotary_dim / 2]) or, interleaved,        */
+/* (x[2i], x[2i + 1]); pair i becomes (a c - b s, b c + a s); values past   */
+/* rotary_dim are copied.  inverse turns the other way (-s), which is also  */
+/* the gradient.  Token t's position is positions[t]; one outside           */
+/* [0, max_positions) gives a row of zeros and is recorded (status 3).      */
+/* k may be absent (num_kv_heads 0).  Outputs may be the inputs themselves, */
+/* with the same strides (in place); no other overlap.  No workspace.       */
+/* ------------------------------------------------------------------------ */
+typedef struct akt_rotary_args {
+  const void* q; /* [num_tokens, num_qo_heads, head_dim] */
+  int64_t q_stride_token, q_stride_head, q_stride_dim;
+  const void* k; /* [num_tokens, num_kv_heads, head_dim] */
+  int64_t k_stride_token, k_stride_head, k_stride_dim;
+  void* q_out;
+  int64_t q_out_stride_token, q_out_stride_head, q_out_stride_dim;
+  void* k_out;
+  int64_t k_out_stride_token, k_out_stride_head, k_out_stride_dim;
+  const float* cos_sin; /* [max_positions, rotary_dim], unit stride in a row */
+  int64_t cos_sin_stride, max_positions;
+  const int32_t* positions; /* [num_tokens] */
+  int64_t num_tokens;
+  int32_t num_qo_heads, num_kv_heads, head_dim, rotary_dim;
+  int32_t interleaved, inverse, dtype;
+} akt_rotary_args;
+
+int akt_rotary(const akt_rotary_args* args, void* stream);
+
+/* Rotary positions and the append in one pass: akt_append_paged_kv with the */
+/* appended keys turned to their positions in the sequence (those the page   */
+/* table gives them) on their way into the pool, and the new tokens' queries */
+/* turned into q_out.  A token whose row the page table does not place is    */
+/* skipped and recorded as there; its query row is zeros.  num_qo_heads 0:   */
+/* no queries.                                                               */
+typedef struct akt_append_rotary_args {
+  akt_append_paged_args append;
+  const void* q; /* [num_append, num_qo_heads, head_dim] */
+  int64_t q_stride_token, q_stride_head, q_stride_dim;
+  void* q_out;
+  int64_t q_out_stride_token, q_out_stride_head, q_out_stride_dim;
+  const float* cos_sin; /* [max_positions, rotary_dim] */
+  int64_t cos_sin_stride, max_positions;
+  int32_t num_qo_heads, rotary_dim, interleaved;
+} akt_append_rotary_args;
+
+int akt_append_rotary_paged_kv(const akt_append_rotary_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* pages of a paged KV cache: copy, fork, compact, free (no reference       */
+/* counterpart: its drivers build one fixed table)                          */
+/* A page is live when the table names it (or `reserved`, a byte per page,  */
+/* or NULL, marks it); every other page is dead and may be written.  The    */
+/* pool is [num_layers, num_pages, 2, num_kv_heads, page_size, head_dim]    */
+/* of a 2-byte type, any strides with unit dim stride; one layer is the     */
+/* pool of the paged decodes.                                               */
+/* ------------------------------------------------------------------------ */
+typedef struct akt_page_pool {
+  void* kv_cache;
+  int64_t stride_layer, stride_page, stride_kv, stride_head, stride_token, stride_dim;
+  int64_t num_pages;
+  int32_t num_layers, num_kv_heads, page_size, head_dim;
+} akt_page_pool;
+
+/* Page src_pages[i] copied to page dst_pages[i] for i < num_copies, in every */
+/* layer.  No destination may be another copy's source or destination.  A   */
+/* copy with a page outside the pool is skipped and recorded (status 2).    */
+int akt_copy_kv_pages(const akt_page_pool* pool, const int32_t* src_pages, const int32_t* dst_pages,
+                      int64_t num_copies, void* stream);
+
+/* A new batch of sequences from parents: child c continues sequence        */
+/* parents[c] of the table.  The first child of a parent takes its pages    */
+/* over; each further one shares the full pages and gets a copy of a partly */
+/* filled last page in the lowest-numbered dead page that no earlier child  */
+/* took.  Dead is what neither a named parent's pages nor `reserved` holds, */
+/* so sequences that no child names are dropped.  Writes the children's     */
+/* table: out_indptr [num_children + 1], out_indices [max_entries] (-1 past */
+/* its end), out_last_page_len [num_children]; it must not overlap the      */
+/* input table.  Children past max_entries entries are cut (status 5);      */
+/* where no dead page is left the child's last entry is -1 (status 6); a    */
+/* parent outside the batch or with bad bounds gives an empty child (status */
+/* 4), one with a bad page id keeps that id and is recorded (status 2).     */
+typedef struct akt_fork_paged_args {
+  akt_page_pool pool;
+  const int32_t* kv_page_indptr;   /* [batch + 1] */
+  const int32_t* kv_page_indices;  /* [num_page_entries] */
+  const int32_t* kv_last_page_len; /* [batch] */
+  int64_t num_page_entries;
+  const int32_t* parents;  /* [num_children] */
+  const uint8_t* reserved; /* [num_pages] or NULL */
+  int32_t* out_indptr;
+  int32_t* out_indices;
+  int32_t* out_last_page_len;
+  int64_t max_entries;
+  int32_t batch, num_children;
+} akt_fork_paged_args;
+
+size_t akt_fork_paged_workspace_size(const akt_fork_paged_args* args);
+int akt_fork_paged(const akt_fork_paged_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Live pages moved to the lowest page numbers that `reserved` leaves open  */
+/* (reserved pages stay): with n pages named by the table, the targets are  */
+/* the n lowest such numbers; pages there already stay, the others move to  */
+/* the empty targets, both in ascending order.  out_indices                 */
+/* [num_page_entries] is the table's index array after the moves (negative  */
+/* entries stay; ids outside the pool stay and are recorded, status 2),     */
+/* pages_used one past the highest page then in use or reserved.  The old   */
+/* places keep their contents.                                              */
+typedef struct akt_compact_paged_args {
+  akt_page_pool pool;
+  const int32_t* kv_page_indices; /* [num_page_entries] */
+  int64_t num_page_entries;
+  const uint8_t* reserved; /* [num_pages] or NULL */
+  int32_t* out_indices;    /* [num_page_entries] */
+  int32_t* pages_used;     /* [1] */
+} akt_compact_paged_args;
+
+size_t akt_compact_paged_workspace_size(const akt_compact_paged_args* args);
+int akt_compact_paged(const akt_compact_paged_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The dead pages in ascending order: free_pages [num_pages] (-1 past their */
+/* count), num_free [1].                                                    */
+size_t akt_free_kv_pages_workspace_size(int64_t num_pages);
+int akt_free_kv_pages(const int32_t* kv_page_indices, int64_t num_page_entries, const uint8_t* reserved,
+                      int64_t num_pages, int32_t* free_pages, int32_t* num_free, void* workspace,
+                      size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
