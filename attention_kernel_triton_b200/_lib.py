@@ -147,6 +147,21 @@ class AppendPagedArgs(Structure):
     ]
 
 
+class ChunkPagedArgs(Structure):
+    _fields_ = [
+        ("q", c_void_p), ("q_stride_token", c_int64), ("q_stride_head", c_int64), ("q_stride_dim", c_int64),
+        ("q_indptr", c_void_p), ("num_tokens", c_int64),
+        ("kv_cache", c_void_p), ("kv_stride_page", c_int64), ("kv_stride_kv", c_int64), ("kv_stride_head", c_int64),
+        ("kv_stride_token", c_int64), ("kv_stride_dim", c_int64), ("num_pages", c_int64),
+        ("kv_page_indptr", c_void_p), ("kv_page_indices", c_void_p), ("kv_last_page_len", c_void_p),
+        ("num_page_entries", c_int64),
+        ("out", c_void_p), ("out_stride_token", c_int64), ("out_stride_head", c_int64), ("out_stride_dim", c_int64),
+        ("lse", c_void_p), ("lse_stride_token", c_int64), ("lse_stride_head", c_int64),
+        ("batch", c_int32), ("num_qo_heads", c_int32), ("num_kv_heads", c_int32), ("page_size", c_int32),
+        ("head_dim", c_int32), ("causal", c_int32), ("dtype", c_int32), ("softmax_scale", c_float),
+    ]
+
+
 class RotaryArgs(Structure):
     _fields_ = [
         ("q", c_void_p), ("q_stride_token", c_int64), ("q_stride_head", c_int64), ("q_stride_dim", c_int64),
@@ -252,6 +267,8 @@ SIGNATURES = {
                                             c_void_p]),
     "akt_mask_to_sparse_index": (c_int, [POINTER(MaskToIndexArgs), c_void_p]),
     "akt_sparse_index_to_mask": (c_int, [POINTER(IndexToMaskArgs), c_void_p]),
+    "akt_chunk_paged_workspace_size": (c_size_t, [POINTER(ChunkPagedArgs)]),
+    "akt_chunk_paged": (c_int, [POINTER(ChunkPagedArgs), c_void_p, c_size_t, c_void_p]),
     "akt_rotary": (c_int, [POINTER(RotaryArgs), c_void_p]),
     "akt_append_rotary_paged_kv": (c_int, [POINTER(AppendRotaryArgs), c_void_p]),
     "akt_copy_kv_pages": (c_int, [POINTER(PagePool), c_void_p, c_void_p, c_int64, c_void_p]),

@@ -414,6 +414,49 @@ typedef struct akt_index_to_mask_args {
 int akt_sparse_index_to_mask(const akt_index_to_mask_args* args, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* attention of a chunk of new tokens over a paged cache (prompt chunks,    */
+/* drafted tokens to verify, single tokens, mixed in one batch; the         */
+/* reference has the one-token form only, decode_flash_attention_redundant_ */
+/* var_len_paged.py:228-274)                                                */
+/* The page table already covers the new tokens (as after the append):      */
+/* sequence b holds len_b = (pages_b - 1) * page_size + kv_last_page_len[b] */
+/* tokens (the last clamped to [0, page_size]), its queries are rows        */
+/* q_indptr[b] .. q_indptr[b+1] of q, the n_b newest: row i stands at       */
+/* position len_b - n_b + i and sees the keys up to it (causal) or all      */
+/* len_b keys.  A row that sees no key gives zeros and lse -inf, and so do  */
+/* rows before q_indptr[0] and from q_indptr[batch] on (padding).  Bad page */
+/* bounds make a sequence empty, bad query bounds leave its rows out (both  */
+/* status 4); K and V rows of pages outside the pool read as zeros (status  */
+/* 2).  A value row that is not finite reaches the rows that see it only.   */
+/* lse [num_tokens, num_qo_heads] (fp32, or NULL): natural-log sum-exp of   */
+/* the scaled scores.  head_dim 64 or 128.                                  */
+/* ------------------------------------------------------------------------ */
+typedef struct akt_chunk_paged_args {
+  const void* q; /* [num_tokens, num_qo_heads, head_dim] */
+  int64_t q_stride_token, q_stride_head, q_stride_dim;
+  const int32_t* q_indptr; /* [batch + 1] */
+  int64_t num_tokens;
+  const void* kv_cache; /* [num_pages, 2, num_kv_heads, page_size, head_dim] */
+  int64_t kv_stride_page, kv_stride_kv, kv_stride_head, kv_stride_token, kv_stride_dim;
+  int64_t num_pages;
+  const int32_t* kv_page_indptr;   /* [batch + 1] */
+  const int32_t* kv_page_indices;  /* [num_page_entries] */
+  const int32_t* kv_last_page_len; /* [batch] */
+  int64_t num_page_entries;
+  void* out; /* [num_tokens, num_qo_heads, head_dim] */
+  int64_t out_stride_token, out_stride_head, out_stride_dim;
+  float* lse; /* [num_tokens, num_qo_heads] or NULL */
+  int64_t lse_stride_token, lse_stride_head;
+  int32_t batch, num_qo_heads, num_kv_heads, page_size, head_dim;
+  int32_t causal;
+  int32_t dtype;
+  float softmax_scale;
+} akt_chunk_paged_args;
+
+size_t akt_chunk_paged_workspace_size(const akt_chunk_paged_args* args);
+int akt_chunk_paged(const akt_chunk_paged_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* rotary positions (no reference counterpart: its inputs come rotated)     */
 /* Row cos_sin[p] of the fp32 table holds the cosines of rotary_dim / 2     */
 /* angles of position p, then their sines.  The first rotary_dim values of  */

@@ -7,6 +7,7 @@ from attention_kernel_triton_b200 import _lib
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 STRUCTS = {
+    "akt_chunk_paged_args": _lib.ChunkPagedArgs,
     "akt_rotary_args": _lib.RotaryArgs,
     "akt_append_rotary_args": _lib.AppendRotaryArgs,
     "akt_page_pool": _lib.PagePool,
