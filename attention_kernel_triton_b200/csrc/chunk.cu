@@ -1,23 +1,78 @@
-// Attention of a chunk of new tokens over a paged cache: prompt chunks,
-// drafted tokens to verify and single tokens, ragged in one batch.
+// Attention of a chunk of new tokens over a paged cache, on the 5th-generation
+// tensor cores (tcgen05 + TMEM): prompt chunks, drafted tokens to verify and
+// single tokens, ragged in one batch.  The reference has the one-token form only
+// (decode_flash_attention_redundant_var_len_paged.py:228-274).
 //
 // O_i = sum_j softmax_j(q_i . k_j s) v_j over the keys j that row i sees; row i
-// of sequence b stands at position len_b - n_b + i.  First form: one warp per
-// (token, query head) walks the keys with the running maximum and sum of the
-// softmax in fp32.
+// of sequence b stands at position len_b - n_b + i.  One pass over the keys with
+// the softmax's running maximum and sum in fp32; P is rounded to the input type
+// before P.V, as in the reference's decode (DP:39-57).
+//
+// Rows and units.  The G query heads of a kv head share K and V, so a 128-row
+// tile holds TQ = floor(128 / G) tokens x G heads (row = token * G + head) and
+// each K/V row is read once for all of them.  A unit is (sequence, kv head, 2 TQ
+// consecutive tokens): two tiles ("slots") that share every K/V tile of 128
+// keys.  A unit whose rows fit one tile (decoding, verification) puts the same
+// rows in both slots and gives slot t every other key tile: the two slots'
+// (O, max, sum) are joined from TMEM at its end.
+//
+// Work split.  The units' key tiles stand on a line, (sequence, kv head, unit).
+// Whole units are dealt to the CTAs (one per SM) round by round while no CTA
+// gets more than its share of all tiles; the rest of the line is cut so that
+// every CTA ends with the same count, also inside a unit.  A unit in parts
+// leaves its normalised fp32 partial outputs and log-sum-exps in the workspace
+// (at most two parts per CTA), which chunk_merge_kernel joins.  So one long
+// sequence of one token fills the GPU and a batch of prompts has no tail.
+//
+// Warps of a CTA (12):
+//   0-3 / 4-7  softmax of slot 0 / 1: thread i owns row i = TMEM lane i
+//   8          loader of the K and V ring: tensor-map boxes inside the pages, or
+//              16-byte cp.async rows where no box fits a page (TMA template)
+//   9 / 11     Q loads and MMAs of slot 0 / 1 (one thread)
+//   10         scheduler: the CTA's segments, a few ahead, through shared memory;
+//              and the V tiles at the mask's edge (below)
+// TMEM (512 columns): S[2] (128 each), O[2] (D each).  P_t overwrites S_t: a
+// slot's MMAs are issued by one thread in the order S_j, P.V_j, S_j+1, and while
+// one slot's softmax runs the tensor pipe works for the other.
+//
+// What lies behind the mask.  Scores are masked by selection, so K may hold
+// anything there.  A masked weight is 0, but 0 x NaN is NaN in P.V, so in V tiles
+// that a mask crosses the rows past the sequence are cleared, and values that are
+// not finite are cleared and their tokens noted; a row that does see such a token
+// gets the value added to its output at the end.
+//
+// Built without -rdc (setmaxnreg needs whole-program device code).
+#define AKT_WHOLE_PROGRAM 1
 #include "common.cuh"
 #include "profile.cuh"
+#include "tensor_map.h"
 
+#include <algorithm>
 #include <string>
+#include <type_traits>
 
 namespace akt {
 int set_error(int code, const std::string& msg);
 
 namespace {
 
+constexpr int BM = 128;            // rows of a slot
+constexpr int BN = 128;            // keys of a tile
+constexpr int kThreads = 384;
+constexpr int kLoadWarp = 8;
+constexpr int kMmaWarp0 = 9;
+constexpr int kSchedWarp = 10;
+// 2 * 128 * 216 + 128 * 64 <= 384 * 168 registers
+constexpr int kLaunchRegs = 168, kSoftmaxRegs = 216, kControlRegs = 64;
+static_assert(256 * kSoftmaxRegs + 128 * kControlRegs <= kThreads * kLaunchRegs, "register split");
+constexpr float kRescaleThreshold = 8.0f;  // log2 units
+constexpr int kSegs = 4;           // segments in flight between the scheduler and the others
+constexpr int kSegReaders = 12;    // loader, 2 issuers, 8 softmax warps, scheduler (its V duty)
+constexpr int kTableSeqs = 96;     // sequences whose table fits the CTA's shared memory
+constexpr int kMaxCtas = 384;      // of the main kernel (one per SM)
+
 struct ChunkParams {
   const char* q;
-  int64_t q_tok, q_head;  // bytes
   const int32_t* q_indptr;
   int64_t num_tokens;
   const char* kv;
@@ -30,72 +85,1270 @@ struct ChunkParams {
   int64_t o_tok, o_head;  // bytes
   float* lse;
   int64_t l_tok, l_head;  // elements
-  int B, Hq, Hkv, group, P, causal;
+  int B, Hq, Hkv, group, P, causal, D;
   float scale_log2;
+  int TQ;             // tokens of a slot
+  FastDiv div_group;  // row -> (token, head)
+  FastDiv div_page;   // key -> (page, row)
+  int box_rows;       // rows of one tensor-map box (divides the page size), TMA loads
+  int grid;           // CTAs of the main kernel
+  // workspace
+  struct Part* parts;  // [grid][2]
+  float* part_o;       // [grid][2][part_rows][D]
+  float* part_lse;     // [grid][2][part_rows] natural log, -inf: no key
+  int part_rows;
+  // tables in the workspace, for more than kTableSeqs sequences
+  int64_t* plan_cost;  // [B + 1]
+  int* plan_units;     // [B + 1]
+  struct Plan* plan;
+  int64_t* plan_share; // [grid + 1]
 };
 
-constexpr int kWarps = 8;
+// A unit's part that one CTA left in the workspace (written for both of a
+// CTA's places; keys == 0: none).
+struct Part {
+  int used, first, last;  // whether it is one; the unit's first / last keys
+  int q0, ntok, kvh, single, pad;
+};
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kWarps * 32) chunk_rows_kernel(const ChunkParams p) {
-  constexpr int N = D / 32;  // values of a row per lane
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (row >= p.num_tokens * p.Hq) return;
-  const int64_t tok = row / p.Hq;
-  const int h = (int)(row - tok * p.Hq), kvh = h / p.group;
-  int lo = 0, hi = p.B - 1;  // the last b with q_indptr[b] <= tok
+// How the line of units is dealt: rounds of whole units, then the cuts.
+struct Plan {
+  int64_t base;  // tiles of the dealt units: where the cut part of the line starts
+  int rounds;
+};
+
+// A run of key tiles of one unit for one CTA.
+struct Seg {
+  int q0;      // the unit's first row of q (token); -1: no more segments
+  int ntok;    // its tokens
+  int vis0;    // keys that the first token sees
+  int kvh;
+  int page0;   // the sequence's first entry of the index array
+  int len;     // its keys
+  int t0, t1;  // key tiles
+  int nt;      // key tiles of the whole unit
+  int single;  // one tile of rows: the slots take turns at the key tiles
+  int part;    // -1: the whole unit; else the place of the partial result
+  int noted;   // tokens in `bad`
+  uint32_t bad[3][BN / 32];  // tokens from tile vis0 / BN on whose V row is not finite
+};
+
+template <int D>
+struct Cfg {
+  static constexpr int DB = D / 64;  // 64-column (128-byte) swizzle blocks of a row
+  static constexpr int COL_S = 0, COL_O = 2 * BN, TMEM_COLS = 512;
+  static_assert(COL_O + 2 * D <= TMEM_COLS, "TMEM budget");
+  static constexpr uint32_t Q_BYTES = BM * D * 2, KV_BYTES = BN * D * 2;
+  static constexpr int NS = D == 64 ? 12 : 5;  // ring stages, K and V in turn
+  static constexpr uint32_t OFF_Q = 0, OFF_KV = 2 * Q_BYTES, OFF_BAR = OFF_KV + NS * KV_BYTES;
+  // full, empty, ready [NS]; q_full, s_full, p_full, o_full [slot]; seg_full,
+  // seg_empty [kSegs]; join (slot 1 done), joined; mma_idle
+  static constexpr int N_BARS = 3 * NS + 8 + 2 * kSegs + 3;
+  static constexpr uint32_t OFF_MISC = OFF_BAR + (N_BARS * 8 + 15) / 16 * 16;  // TMEM address, abort flag
+  static constexpr uint32_t OFF_SEG = OFF_MISC + 16;
+  static constexpr uint32_t OFF_TABLE = OFF_SEG + kSegs * sizeof(Seg);
+  static constexpr uint32_t SMEM = OFF_TABLE + (kTableSeqs + 1) * 12 + 16;
+  static_assert(SMEM <= 227 * 1024, "shared memory budget");
+  // slot 1's maxima and sums for the join, in the ring's place of nothing else
+  static constexpr uint32_t OFF_STAT = (SMEM + 15) / 16 * 16;
+  static constexpr uint32_t SMEM_ALL = OFF_STAT + 2 * BM * 4;
+  static_assert(SMEM_ALL <= 227 * 1024, "shared memory budget");
+};
+
+// -------------------------------------------------------------------------
+// the sequences and their units
+// -------------------------------------------------------------------------
+struct Seq {
+  int a0, n, page0, len;  // first row of q, queries, first index entry, keys
+};
+
+// Sequence b's bounds; a malformed one is empty (recorded by the planner).
+__device__ __forceinline__ Seq load_seq(const ChunkParams& p, int b, bool record) {
+  Seq s;
+  const int a1 = __ldg(p.q_indptr + b + 1), e = __ldg(p.indptr + b + 1), last = __ldg(p.last + b);
+  s.a0 = __ldg(p.q_indptr + b);
+  s.page0 = __ldg(p.indptr + b);
+  s.n = a1 - s.a0;
+  s.len = 0;
+  if (s.a0 < 0 || a1 < s.a0 || a1 > p.num_tokens) {
+    if (record) record_status(kStatusBadIndptr);
+    s.n = 0;
+  }
+  if (s.page0 < 0 || e < s.page0 || e > p.num_page_entries) {
+    if (record) record_status(kStatusBadIndptr);
+  } else if (e > s.page0) {
+    s.len = (e - s.page0 - 1) * p.P + min(max(last, 0), p.P);
+  }
+  return s;
+}
+
+__device__ __forceinline__ int num_units(const ChunkParams& p, const Seq& s) {
+  return s.n ? (s.n - 1) / (2 * p.TQ) + 1 : 0;
+}
+
+// Key tiles of unit u, and what it costs (a unit without keys writes zeros)
+__device__ __forceinline__ int unit_tiles(const ChunkParams& p, const Seq& s, int u) {
+  const int vis = p.causal ? s.len - s.n + min((u + 1) * 2 * p.TQ, s.n) : s.len;
+  return vis > 0 ? (vis - 1) / BN + 1 : 0;
+}
+__device__ __forceinline__ int unit_cost(const ChunkParams& p, const Seq& s, int u) {
+  return max(unit_tiles(p, s, u), 1);
+}
+
+// Tables: cost[b] and units[b] count the tiles and units before sequence b.
+struct Tables {
+  const int64_t* cost;
+  const int* units;
+};
+
+// Largest b in [0, B) with t[b] <= x (the entry that holds x; empty ones are passed over).
+template <typename V>
+__device__ __forceinline__ int find_seq(const V* t, int B, V x) {
+  int lo = 0, hi = B - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (__ldg(p.q_indptr + mid) <= tok) lo = mid; else hi = mid - 1;
+    if (t[mid] <= x) lo = mid; else hi = mid - 1;
   }
-  const int64_t a0 = __ldg(p.q_indptr + lo), a1 = __ldg(p.q_indptr + lo + 1);
-  const int s = __ldg(p.indptr + lo), e = __ldg(p.indptr + lo + 1);
-  int64_t keys = 0;
-  if (tok < __ldg(p.q_indptr) || tok >= __ldg(p.q_indptr + p.B)) {
-    // padding: no sequence
-  } else if (a0 < 0 || tok < a0 || tok >= a1 || a1 > p.num_tokens || s < 0 || e < s || e > p.num_page_entries) {
-    if (lane == 0) record_status(kStatusBadIndptr);
-  } else if (e > s) {
-    const int64_t len = (int64_t)(e - s - 1) * p.P + min(max(__ldg(p.last + lo), 0), p.P);
-    keys = p.causal ? max((int64_t)0, len - (a1 - a0) + (tok - a0) + 1) : len;
-  }
-  float q[N], o[N];
-  const T* qr = reinterpret_cast<const T*>(p.q + tok * p.q_tok + h * p.q_head);
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    q[i] = Elem<T>::to_float(qr[lane + 32 * i]) * p.scale_log2;
-    o[i] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  for (int64_t j0 = 0; j0 < keys; j0 += p.P) {
-    const int page = __ldg(p.indices + s + j0 / p.P);
-    const bool bad = page < 0 || page >= p.num_pages;  // reads as zeros
-    if (bad && lane == 0) record_status(kStatusBadPage);
-    const char* k = p.kv + (bad ? 0 : (int64_t)page * p.s_page + kvh * p.s_head);
-    const int n = (int)min((int64_t)p.P, keys - j0);
-    for (int t = 0; t < n; ++t, k += bad ? 0 : p.s_tok) {
-      const T* kr = reinterpret_cast<const T*>(k);
-      const T* vr = reinterpret_cast<const T*>(k + p.s_kv);
-      float x = 0.f;
-      if (!bad) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) x = fmaf(q[i], Elem<T>::to_float(kr[lane + 32 * i]), x);
-      }
-#pragma unroll
-      for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-      const float m2 = fmaxf(m, x), a = fast_exp2(m - m2), w = fast_exp2(x - m2);
-      m = m2;
-      l = l * a + w;
-#pragma unroll
-      for (int i = 0; i < N; ++i) o[i] = bad ? o[i] * a : fmaf(w, Elem<T>::to_float(vr[lane + 32 * i]), o[i] * a);
+  return lo;
+}
+
+// Unit i of the line: its sequence, kv head and number (a sequence's units run
+// from the last, longest one down).
+__device__ __forceinline__ void unit_at(const ChunkParams& p, const Tables& t, int i, int& b, Seq& s, int& kvh, int& u) {
+  b = find_seq(t.units, p.B, i);
+  s = load_seq(p, b, false);
+  const int U = num_units(p, s), r = i - t.units[b];
+  kvh = r / U;
+  u = U - 1 - (r - kvh * U);
+}
+
+// Fills the tables (threads of one CTA, `nthreads` of them; cost and units in
+// shared or global memory) -- the caller syncs before and after.
+__device__ void build_tables(const ChunkParams& p, int64_t* cost, int* units, int nthreads) {
+  // a team of threads per sequence sums its units' costs
+  int team = 32;
+  while (team > 1 && (nthreads / team) < p.B) team >>= 1;
+  const int lane = threadIdx.x % team;
+  for (int b0 = 0; b0 < p.B; b0 += nthreads / team) {
+    const int b = b0 + threadIdx.x / team;
+    int U = 0;
+    int64_t c = 0;
+    if (b < p.B) {
+      const Seq s = load_seq(p, b, lane == 0);
+      U = num_units(p, s);
+      for (int u = lane; u < U; u += team) c += unit_cost(p, s, u);
+    }
+    for (int o = team >> 1; o; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+    if (b < p.B && lane == 0) {
+      cost[b + 1] = c * p.Hkv;
+      units[b + 1] = U * p.Hkv;
     }
   }
-  T* orow = reinterpret_cast<T*>(p.out + tok * p.o_tok + h * p.o_head);
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  __syncthreads();
+  if (threadIdx.x < 32) {  // running sums
+    int64_t c0 = 0;
+    int u0 = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      const int b = b0 + threadIdx.x;
+      int64_t c = b < p.B ? cost[b + 1] : 0;
+      int u = b < p.B ? units[b + 1] : 0;
 #pragma unroll
-  for (int i = 0; i < N; ++i) orow[lane + 32 * i] = Elem<T>::from_float(o[i] * inv);
-  if (p.lse && lane == 0) p.lse[tok * p.l_tok + h * p.l_head] = l > 0.f ? (m + __log2f(l)) * kLn2 : -INFINITY;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t cy = __shfl_up_sync(0xffffffffu, c, o);
+        const int uy = __shfl_up_sync(0xffffffffu, u, o);
+        if (threadIdx.x >= o) {
+          c += cy;
+          u += uy;
+        }
+      }
+      if (b < p.B) {
+        cost[b + 1] = c0 + c;
+        units[b + 1] = u0 + u;
+      }
+      c0 += __shfl_sync(0xffffffffu, c, 31);
+      u0 += __shfl_sync(0xffffffffu, u, 31);
+    }
+    if (threadIdx.x == 0) {
+      cost[0] = 0;
+      units[0] = 0;
+    }
+  }
+  __syncthreads();
+}
+
+// The unit that CTA c gets in round r of whole units: rounds run left to right
+// and right to left in turn, which evens out costs that fall along the line.
+__device__ __forceinline__ int dealt_unit(const ChunkParams& p, int r, int c) {
+  return r * p.grid + ((r & 1) ? p.grid - 1 - c : c);
+}
+
+// Deals whole units and cuts the rest (at least p.grid threads of one CTA, all
+// call it).  share[c] .. share[c + 1] is CTA c's range of the cut part, in tiles
+// from plan.base.  scratch: 2 int64.
+__device__ Plan make_plan(const ChunkParams& p, const Tables& t, int64_t* share, int64_t* scratch) {
+  const int64_t W = t.cost[p.B];
+  const int N = t.units[p.B];
+  const int64_t target = (W + p.grid - 1) / p.grid;
+  Plan pl{0, 0};
+  int64_t mine = 0;
+  // Dealing pays by the CTAs of a round sharing K/V tiles in L2 and by fewer
+  // parts; with one unit per (sequence, kv head) there is nothing to share.
+  const int most = N > (int64_t)p.B * p.Hkv ? N / p.grid : 0;
+  for (int r = 0; r < most; ++r) {
+    int64_t c = 0;
+    if (threadIdx.x < p.grid) {
+      int b, kvh, u;
+      Seq s;
+      unit_at(p, t, dealt_unit(p, r, threadIdx.x), b, s, kvh, u);
+      c = unit_cost(p, s, u);
+    }
+    if (__syncthreads_or(mine + c > target)) break;
+    mine += c;
+    ++pl.rounds;
+  }
+  // what each CTA still lacks, scaled to what is left
+  if (threadIdx.x < p.grid) share[threadIdx.x] = mine;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    int64_t dealt = 0, lacks = 0;
+    for (int c0 = 0; c0 < p.grid; c0 += 32) {
+      const int c = c0 + threadIdx.x;
+      const int64_t m = c < p.grid ? share[c] : target;
+      int64_t l = target - m, d = c < p.grid ? m : 0, x = l;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (threadIdx.x >= o) x += y;
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+      __syncwarp();
+      if (c < p.grid) share[c] = lacks + x - l;  // before CTA c
+      lacks += __shfl_sync(0xffffffffu, x, 31);
+      dealt += d;
+    }
+    if (threadIdx.x == 0) {
+      scratch[0] = dealt;
+      scratch[1] = lacks;
+    }
+  }
+  __syncthreads();
+  pl.base = scratch[0];
+  const int64_t rest = W - scratch[0], lacks = scratch[1];
+  __syncthreads();
+  // lacks >= rest, and equal but for the rounding of the target
+  if (threadIdx.x < p.grid) {
+    const double f = lacks > 0 ? (double)share[threadIdx.x] / (double)lacks : 0.0;
+    share[threadIdx.x] = min((int64_t)(f * (double)rest), rest);
+  }
+  if (threadIdx.x == 0) share[p.grid] = rest;
+  __syncthreads();
+  return pl;
+}
+
+// -------------------------------------------------------------------------
+// PTX helpers
+// -------------------------------------------------------------------------
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+  d |= (uint64_t)((lbo >> 4) & 0x3FFFu) << 16;
+  d |= (uint64_t)((sbo >> 4) & 0x3FFFu) << 32;
+  d |= (uint64_t)1 << 46;  // descriptor version for sm_100
+  d |= (uint64_t)2 << 61;  // 128-byte swizzle
+  return d;
+}
+
+__host__ __device__ constexpr uint32_t idesc_f16(int fmt, int M, int N, int b_mn_major) {
+  return (1u << 4) | ((uint32_t)fmt << 7) | ((uint32_t)fmt << 10) | ((uint32_t)b_mn_major << 16) |
+         ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// A shared-memory descriptor as two words; an offset of the tile is an add on the low one.
+struct Desc {
+  uint32_t lo, hi;
+};
+__device__ __forceinline__ Desc desc_words(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  const uint64_t d = desc_sw128(saddr, lbo, sbo);
+  return Desc{(uint32_t)d, (uint32_t)(d >> 32)};
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+                                       uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 da, {%1, %2};\n\t"
+      "mov.b64 db, {%3, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(tmem_d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                       uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+// 16 bytes global -> shared, or zeros when src_bytes is 0
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t src_bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// generic-proxy writes to shared memory before later async-proxy reads (the MMAs)
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Slow path of a bounded mbarrier wait: every 256 polls it gives up if another
+// role of the CTA has, or, after kWaitLimitNs, records kStatusWaitTimeout and
+// raises the abort flag itself.
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  const uint64_t t0 = globaltimer_ns();
+  for (uint32_t it = 1;; ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 255u) == 0u) {
+      if (*abort_flag) return false;
+      if (globaltimer_ns() - t0 > kWaitLimitNs) {
+        record_status(kStatusWaitTimeout);
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  }
+}
+
+// 16-bit values of w that are not finite, as a mask of their bits
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u;
+  return __vcmpeq2(w & e, e);
+}
+
+// The rare end of a row that sees tokens whose V row is not finite (their
+// values were cleared for the MMAs): each such value added to the output.
+template <typename T, int D, typename O>
+__device__ __forceinline__ void add_not_finite(const ChunkParams& p, const Seg& sg, int vis, O* row) {
+  const int first = max(sg.vis0, 0) / BN * BN;
+#pragma unroll 1
+  for (int i = 0; i < 3 * BN; ++i) {
+    if (!(sg.bad[i / BN][(i / 32) % (BN / 32)] >> (i & 31) & 1u)) continue;
+    const int key = first + i;
+    if (key >= vis) continue;
+    const int pg = (int)fdiv((uint32_t)key, p.div_page);
+    const int page = __ldg(p.indices + sg.page0 + pg);
+    if (page < 0 || page >= p.num_pages) continue;
+    const T* v = reinterpret_cast<const T*>(p.kv + (int64_t)page * p.s_page + p.s_kv + (int64_t)sg.kvh * p.s_head +
+                                            (int64_t)(key - pg * p.P) * p.s_tok);
+#pragma unroll 1
+    for (int d = 0; d < D; ++d) {
+      const float x = Elem<T>::to_float(v[d]);
+      if (!isfinite(x)) {
+        if constexpr (std::is_same<O, float>::value) row[d] += x;
+        else row[d] = Elem<T>::from_float(Elem<T>::to_float(row[d]) + x);
+      }
+    }
+  }
+}
+
+// 32 columns of a finished row: fp32 partial, or the output type
+template <typename T>
+__device__ __forceinline__ void store32(const float (&o)[32], T* out) {
+#pragma unroll
+  for (int e = 0; e < 32; e += 8)
+    reinterpret_cast<uint4*>(out)[e / 8] =
+        make_uint4(Elem<T>::pack2(o[e], o[e + 1]), Elem<T>::pack2(o[e + 2], o[e + 3]), Elem<T>::pack2(o[e + 4], o[e + 5]),
+                   Elem<T>::pack2(o[e + 6], o[e + 7]));
+}
+__device__ __forceinline__ void store32(const float (&o)[32], float* out) {
+#pragma unroll
+  for (int e = 0; e < 32; e += 4) reinterpret_cast<float4*>(out)[e / 4] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+}
+
+// -------------------------------------------------------------------------
+// the planner of batches past the CTA's own table
+// -------------------------------------------------------------------------
+__global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
+  __shared__ int64_t scratch[2];
+  build_tables(p, p.plan_cost, p.plan_units, 1024);
+  const Plan pl = make_plan(p, Tables{p.plan_cost, p.plan_units}, p.plan_share, scratch);
+  if (threadIdx.x == 0) *p.plan = pl;
+}
+
+// -------------------------------------------------------------------------
+// main kernel
+// -------------------------------------------------------------------------
+template <typename T, int D, bool TMA>
+__global__ void __launch_bounds__(kThreads, 1)
+    chunk_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                     const __grid_constant__ CUtensorMap tmV, const ChunkParams p) {
+  using C = Cfg<D>;
+  constexpr int NS = C::NS;
+  constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
+  constexpr uint32_t IDESC_S = idesc_f16(fmt, BM, BN, 0);
+  constexpr uint32_t IDESC_PV = idesc_f16(fmt, BM, D, 1);
+
+  extern __shared__ __align__(1024) unsigned char smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* full = bars;             // [NS] loaded
+  uint64_t* empty = full + NS;       // [NS] both issuers done with it
+  uint64_t* ready = empty + NS;      // [NS] seen (and, for V at a mask's edge, cleaned) by the scheduler warp
+  uint64_t* q_full = ready + NS;     // [slot]
+  uint64_t* s_full = q_full + 2;     // [slot]
+  uint64_t* p_full = s_full + 2;     // [slot]
+  uint64_t* o_full = p_full + 2;     // [slot] the segment's last P.V is done
+  uint64_t* seg_full = o_full + 2;   // [kSegs]
+  uint64_t* seg_empty = seg_full + kSegs;
+  uint64_t* join = seg_empty + kSegs;  // slot 1's statistics are in shared memory
+  uint64_t* joined = join + 1;         // slot 0 has read slot 1's output
+  uint64_t* mma_idle = joined + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  Seg* segs = reinterpret_cast<Seg*>(smem + C::OFF_SEG);
+  float* stat = reinterpret_cast<float*>(smem + C::OFF_STAT);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 2);
+      mbar_init(&ready[s], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&q_full[t], 1);
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&o_full[t], 1);
+    }
+    for (int i = 0; i < kSegs; ++i) {
+      mbar_init(&seg_full[i], 1);
+      mbar_init(&seg_empty[i], kSegReaders);
+    }
+    mbar_init(join, 4);
+    mbar_init(joined, 4);
+    mbar_init(mma_idle, 2);
+    *abort_flag = (smem_u32(smem) & 1023u) ? 1 : 0;  // swizzled tiles need a 1024-byte aligned base
+    if (*abort_flag) record_status(kStatusWaitTimeout);
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "n"(C::TMEM_COLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  // the tables and the plan: built by every CTA for itself, or read from the planner's
+  int64_t begin, end;
+  Plan plan;
+  Tables tab;
+  if (p.B <= kTableSeqs) {
+    int64_t* cost = reinterpret_cast<int64_t*>(smem + C::OFF_TABLE);
+    int* units = reinterpret_cast<int*>(cost + p.B + 1);
+    // the shares live where slot 0's Q tile goes later
+    int64_t* share = reinterpret_cast<int64_t*>(smem + C::OFF_Q);
+    build_tables(p, cost, units, kThreads);
+    tab = Tables{cost, units};
+    plan = make_plan(p, tab, share, share + p.grid + 1);
+    begin = share[blockIdx.x];
+    end = share[blockIdx.x + 1];
+    // generic reads before the async-proxy writes of the Q tile
+    fence_async_smem();
+  } else {
+    grid_dep_wait();
+    tab = Tables{p.plan_cost, p.plan_units};
+    plan = *p.plan;
+    begin = p.plan_share[blockIdx.x];
+    end = p.plan_share[blockIdx.x + 1];
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+    if (mbar_try_wait(bar, parity)) return true;
+    return wait_or_abort(bar, parity, abort_flag);
+  };
+  // first key tile of the CTA's slot t in a segment, the step and the end
+  struct Tiles {
+    int j0, step, j1;
+  };
+  auto slot_tiles = [&](int t, int t0, int t1, int single, int ntok, int vis0, int len) -> Tiles {
+    if (single) return Tiles{t0 + t, 2, t1};
+    const int tok = min(p.TQ * (t + 1), ntok) - 1;  // the slot's last token
+    if (tok < p.TQ * t) return Tiles{t0, 1, t0};
+    const int vis = p.causal ? vis0 + tok : len;
+    return Tiles{t0, 1, min(t1, vis > 0 ? (vis - 1) / BN + 1 : 0)};
+  };
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
+    if (warp == kSchedWarp) {
+      // ===================== scheduler, and V at the mask's edge =====================
+      int round = 0;               // rounds of whole units done
+      int64_t x = plan.base + begin;
+      const int64_t x_end = plan.base + end;
+      int b = -1, kvh = 0, u = 0, U = 0, stream = 0;  // the line's current unit
+      int64_t unit_x = 0;          // where it starts
+      Seq s{};
+      int n_pub = 0;
+      bool ok = true, more = true;
+      // the next segment into ring place n_pub; false when there was none left
+      auto publish = [&]() -> void {
+        Seg sg{};
+        sg.q0 = -1;
+        if (round < plan.rounds) {
+          int bb, k, uu;
+          Seq q;
+          unit_at(p, tab, dealt_unit(p, round, blockIdx.x), bb, q, k, uu);
+          ++round;
+          const int X = 2 * p.TQ;
+          sg.q0 = q.a0 + uu * X;
+          sg.ntok = min(X, q.n - uu * X);
+          sg.vis0 = p.causal ? q.len - q.n + uu * X + 1 : q.len;
+          sg.kvh = k;
+          sg.page0 = q.page0;
+          sg.len = q.len;
+          sg.nt = unit_tiles(p, q, uu);
+          sg.t0 = 0;
+          sg.t1 = sg.nt;
+          sg.part = -1;
+        } else if (x < x_end) {
+          if (b < 0) {  // the unit that holds x
+            b = find_seq(tab.cost, p.B, x);
+            s = load_seq(p, b, false);
+            U = num_units(p, s);
+            const int64_t per_head = (tab.cost[b + 1] - tab.cost[b]) / p.Hkv;
+            const int64_t rel = x - tab.cost[b];
+            kvh = (int)(rel / per_head);
+            unit_x = tab.cost[b] + kvh * per_head;
+            for (int i0 = 0;; i0 += 32) {  // 32 units at a time
+              const int i = i0 + lane;
+              int64_t c = i < U ? unit_cost(p, s, U - 1 - i) : 0, run = c;
+#pragma unroll
+              for (int o = 1; o < 32; o <<= 1) {
+                const int64_t y = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= o) run += y;
+              }
+              const unsigned m = __ballot_sync(0xffffffffu, i < U && unit_x + run > x);
+              if (m || i0 + 32 >= U) {
+                const int at = m ? __ffs(m) - 1 : 31;
+                u = U - 1 - min(i0 + at, U - 1);
+                unit_x += __shfl_sync(0xffffffffu, run - c, at);
+                break;
+              }
+              unit_x += __shfl_sync(0xffffffffu, run, 31);
+            }
+          }
+          const int X = 2 * p.TQ, cost = unit_cost(p, s, u);
+          sg.q0 = s.a0 + u * X;
+          sg.ntok = min(X, s.n - u * X);
+          sg.vis0 = p.causal ? s.len - s.n + u * X + 1 : s.len;
+          sg.kvh = kvh;
+          sg.page0 = s.page0;
+          sg.len = s.len;
+          sg.nt = unit_tiles(p, s, u);
+          const int64_t to = min(x_end - unit_x, (int64_t)cost);
+          sg.t0 = (int)(x - unit_x);
+          sg.t1 = min((int)to, sg.nt);
+          const bool whole = sg.t0 == 0 && to == cost;
+          sg.part = whole ? -1 : (stream ? 1 : 0);
+          if (sg.t0 > sg.t1) sg.t0 = sg.t1;
+          if (!whole && lane == 0) {
+            Part& pt = p.parts[2 * blockIdx.x + sg.part];
+            pt.used = 1;
+            pt.first = x == unit_x;
+            pt.last = to == cost;
+            pt.q0 = sg.q0;
+            pt.ntok = sg.ntok;
+            pt.kvh = kvh;
+            pt.single = sg.ntok <= p.TQ;
+          }
+          ++stream;
+          x = unit_x + to;
+          if (to == cost) {  // on to the next unit of the line
+            unit_x = x;
+            if (u > 0) {
+              --u;
+            } else if (kvh + 1 < p.Hkv) {
+              ++kvh;
+              u = U - 1;
+            } else {
+              b = -1;
+            }
+          }
+        }
+        sg.single = sg.ntok <= p.TQ;
+        more = sg.q0 >= 0;
+        const int e = n_pub % kSegs;
+        if (n_pub >= kSegs && !wait(&seg_empty[e], ((n_pub / kSegs) - 1) & 1)) {
+          ok = false;
+          return;
+        }
+        if (lane == 0) {
+          segs[e] = sg;
+          mbar_arrive(&seg_full[e]);
+        }
+        __syncwarp();
+        ++n_pub;
+      };
+      if (lane < 2) p.parts[2 * blockIdx.x + lane].used = 0;
+      __syncwarp();
+      uint32_t st = 0, ph = 0;
+      publish();
+      for (int k = 0; ok && k < n_pub; ++k) {
+        if (more) publish();  // one ahead of the segment whose V tiles are looked at
+        if (!ok) break;
+        Seg* sg = &segs[k % kSegs];
+        const int t0 = sg->t0, t1 = sg->t1, vis0 = sg->vis0, len = sg->len, j_edge = max(vis0, 0) / BN;
+        if (sg->q0 < 0) break;
+        for (int j = t0; ok && j < t1; ++j) {
+#pragma unroll 1
+          for (int op = 0; op < 2; ++op) {
+            if (!wait(&full[st], ph)) {
+              ok = false;
+              break;
+            }
+            if (op && ((p.causal && (j + 1) * BN > vis0) || (j + 1) * BN > len)) {
+              unsigned char* v = smem + C::OFF_KV + st * C::KV_BYTES;
+              const int rows = len - j * BN;  // the others are past the sequence
+              for (int c = lane; c < BN * D / 8; c += 32) {  // 16-byte pieces
+                const int r = (c >> 3) & (BN - 1);           // piece c: half c / (8 BN), row, chunk
+                uint4* w = reinterpret_cast<uint4*>(v + c * 16);
+                if (r >= rows) {
+                  *w = make_uint4(0, 0, 0, 0);
+                } else if (p.causal) {
+                  uint4 y = *w;
+                  const uint32_t m0 = not_finite2<T>(y.x), m1 = not_finite2<T>(y.y), m2 = not_finite2<T>(y.z),
+                                 m3 = not_finite2<T>(y.w);
+                  if (m0 | m1 | m2 | m3) {
+                    *w = make_uint4(y.x & ~m0, y.y & ~m1, y.z & ~m2, y.w & ~m3);
+                    atomicOr(&sg->bad[j - j_edge][r >> 5], 1u << (r & 31));
+                    sg->noted = 1;
+                  }
+                }
+              }
+              fence_async_smem();
+              __syncwarp();
+            }
+            if (lane == 0) mbar_arrive(&ready[st]);
+            if (++st == NS) {
+              st = 0;
+              ph ^= 1u;
+            }
+          }
+        }
+        if (lane == 0) mbar_arrive(&seg_empty[k % kSegs]);
+      }
+    } else if (warp == kLoadWarp) {
+      // ============================ K and V loader ============================
+      uint32_t st = 0, ph = 0, n_load = 0;
+      bool ok = true;
+      const int boxes = TMA ? (BN / p.box_rows) * C::DB : 0;  // of one tile of K or V, at most 32
+      int held = -1;  // cp.async: the stage whose copies are not known to have landed
+      auto hand_over = [&]() {
+        if (held < 0) return;
+        cp_async_wait<0>();
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[held]);
+        held = -1;
+      };
+      for (int k = 0; ok; ++k) {
+        if (!wait(&seg_full[k % kSegs], (k / kSegs) & 1)) break;
+        const Seg* sg = &segs[k % kSegs];
+        const int q0 = sg->q0, t0 = sg->t0, t1 = sg->t1, kvh = sg->kvh, page0 = sg->page0, len = sg->len;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&seg_empty[k % kSegs]);
+        if (q0 < 0) break;
+        if constexpr (TMA) {
+          // lane l loads box l of each tile: rows [rb, rb + box_rows) of the tile, 64 columns
+          const int db = lane % C::DB, rb = lane / C::DB * p.box_rows;
+          auto page_of = [&](int j, int& row) -> int {  // past the sequence and bad ids: past the pool (zeros)
+            const int key = j * BN + rb;
+            row = 0;
+            if (lane >= boxes || key >= len) return (int)p.num_pages;
+            const int pg = (int)fdiv((uint32_t)key, p.div_page);
+            row = key - pg * p.P;
+            const int id = __ldg(p.indices + page0 + pg);
+            if (id >= 0 && id < p.num_pages) return id;
+            record_status(kStatusBadPage);
+            return (int)p.num_pages;
+          };
+          int row, page = 0;
+          if (t0 < t1) page = page_of(t0, row);
+          for (int j = t0; ok && j < t1; ++j) {
+            int row_next = 0, page_next = 0;
+            if (j + 1 < t1) page_next = page_of(j + 1, row_next);  // on its way while this tile is issued
+#pragma unroll
+            for (int op = 0; op < 2; ++op) {
+              if (n_load >= NS && !wait(&empty[st], ph ^ 1u)) {
+                ok = false;
+                break;
+              }
+              if (lane == 0) mbar_arrive_expect_tx(&full[st], C::KV_BYTES);
+              __syncwarp();
+              if (lane < boxes)
+                tma_load_4d(smem + C::OFF_KV + st * C::KV_BYTES + db * (BN * 128) + rb * 128, op ? &tmV : &tmK, db * 64,
+                            row, kvh, page, &full[st]);
+              ++n_load;
+              if (++st == NS) {
+                st = 0;
+                ph ^= 1u;
+              }
+            }
+            row = row_next;
+            page = page_next;
+          }
+        } else {
+          // every half warp (D = 128) or quarter (D = 64) copies whole rows in 16-byte pieces
+          constexpr int CH = D / 8, RW = 32 / CH;  // pieces of a row; rows a step
+          const int ch = lane % CH, rl = lane / CH;
+          for (int j = t0; ok && j < t1; ++j) {
+            // the addresses of rows lane, lane + 32, ... of the tile's keys (null: zeros)
+            const char* src[BN / 32];
+#pragma unroll
+            for (int i = 0; i < BN / 32; ++i) {
+              const int key = j * BN + i * 32 + lane;
+              src[i] = nullptr;
+              if (key < len) {
+                const int pg = (int)fdiv((uint32_t)key, p.div_page);
+                const int id = __ldg(p.indices + page0 + pg);
+                if (id >= 0 && id < p.num_pages)
+                  src[i] = p.kv + (int64_t)id * p.s_page + (int64_t)kvh * p.s_head + (int64_t)(key - pg * p.P) * p.s_tok;
+                else record_status(kStatusBadPage);
+              }
+            }
+#pragma unroll 1
+            for (int op = 0; op < 2; ++op) {
+              if (n_load >= NS && !__all_sync(0xffffffffu, mbar_try_wait(&empty[st], ph ^ 1u))) {
+                hand_over();  // nothing else to do: what was copied last need not wait for the next copy
+                if (!wait(&empty[st], ph ^ 1u)) {
+                  ok = false;
+                  break;
+                }
+              }
+              const uint32_t tile = smem_u32(smem + C::OFF_KV + st * C::KV_BYTES);
+#pragma unroll
+              for (int i = 0; i < BN / 32; ++i) {
+#pragma unroll 4
+                for (int r0 = 0; r0 < 32; r0 += RW) {
+                  const int r = r0 + rl;
+                  const char* row = reinterpret_cast<const char*>(
+                      __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src[i]), r));
+                  const uint32_t dst = tile + (ch >> 3) * (BN * 128) + (i * 32 + r) * 128 + (((ch & 7) ^ (r & 7)) << 4);
+                  cp_async16(dst, row ? row + (op ? p.s_kv : 0) + ch * 16 : p.q, row ? 16u : 0u);
+                }
+              }
+              cp_async_commit();
+              if (held >= 0) {  // the stage before this one has landed
+                cp_async_wait<1>();
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[held]);
+              }
+              held = (int)st;
+              ++n_load;
+              if (++st == NS) {
+                st = 0;
+                ph ^= 1u;
+              }
+            }
+          }
+          hand_over();  // the segment's last stage
+        }
+      }
+      if (TMA && *abort_flag && lane == 0) {  // loads still in flight into this CTA's shared memory
+        for (uint32_t g = n_load > NS ? n_load - NS : 0; g < n_load; ++g) mbar_wait(&full[g % NS], (g / NS) & 1);
+      }
+      if (!TMA) cp_async_wait<0>();
+    } else if (lane == 0) {
+      // ============================ MMA issuers ============================
+      const int t = warp == kMmaWarp0 ? 0 : 1;
+      const Desc dq = desc_words(smem_u32(smem + C::OFF_Q + t * C::Q_BYTES), 16, 1024);
+      const Desc dk = desc_words(smem_u32(smem + C::OFF_KV), 16, 1024);
+      const Desc dv = desc_words(smem_u32(smem + C::OFF_KV), BN * 128, 1024);
+      uint32_t st = 0, ph = 0, qn = 0, pc = 0;
+      bool ok = true, q_loading = false;
+      // Q of segment k, once the slot's earlier S MMAs are known to be done; true if there is one
+      auto load_q = [&](int k) -> bool {
+        if (!wait(&seg_full[k % kSegs], (k / kSegs) & 1)) {
+          ok = false;
+          return false;
+        }
+        const Seg* sg = &segs[k % kSegs];
+        if (sg->q0 < 0) return false;
+        const Tiles tl = slot_tiles(t, sg->t0, sg->t1, sg->single, sg->ntok, sg->vis0, sg->len);
+        if (tl.j0 >= tl.j1) return false;
+        const int tok = sg->q0 + (sg->single ? 0 : t * p.TQ);
+        mbar_arrive_expect_tx(&q_full[t], (uint32_t)(p.TQ * p.group * 128 * C::DB));
+#pragma unroll
+        for (int db = 0; db < C::DB; ++db)
+          tma_load_4d(smem + C::OFF_Q + t * C::Q_BYTES + db * (BM * 128), &tmQ, db * 64, 0, sg->kvh, tok, &q_full[t]);
+        ++qn;
+        return true;
+      };
+      for (int k = 0; ok; ++k) {
+        if (!wait(&seg_full[k % kSegs], (k / kSegs) & 1)) break;
+        const Seg* sg = &segs[k % kSegs];
+        const int t0 = sg->t0, t1 = sg->t1;
+        if (sg->q0 < 0) {
+          mbar_arrive(&seg_empty[k % kSegs]);
+          break;
+        }
+        const Tiles tl = slot_tiles(t, t0, t1, sg->single, sg->ntok, sg->vis0, sg->len);
+        const bool active = tl.j0 < tl.j1;
+        const int j_last = active ? tl.j0 + (tl.j1 - 1 - tl.j0) / tl.step * tl.step : -1;
+        if (active && !q_loading) load_q(k);
+        q_loading = false;
+        int next = tl.j0;
+        for (int j = t0; ok && j < t1; ++j) {
+          const bool mine = active && j == next && j < tl.j1;
+          // ---- S = Q K^T
+          if (!wait(&full[st], ph)) { ok = false; break; }
+          if (mine) {
+            if (j == tl.j0 && !wait(&q_full[t], (qn - 1) & 1)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t k_lo = dk.lo + st * (C::KV_BYTES >> 4);
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              const uint32_t off = (i >> 2) * (BN * 128) + (i & 3) * 32;  // Q and K tiles have 128 rows each
+              mma_ss(tmem + C::COL_S + t * BN, dq.lo + (off >> 4), dq.hi, k_lo + (off >> 4), dk.hi, IDESC_S, i > 0);
+            }
+            mma_commit(&s_full[t]);
+            mma_commit(&empty[st]);
+          } else {
+            mbar_arrive(&empty[st]);
+          }
+          if (++st == NS) { st = 0; ph ^= 1u; }
+          // ---- O += P V
+          if (!wait(&ready[st], ph)) { ok = false; break; }
+          if (mine) {
+            if (!wait(&p_full[t], pc & 1)) { ok = false; break; }
+            ++pc;
+            if (j == j_last) q_loading = load_q(k + 1);  // S of this segment is done: P came from it
+            tc_fence_after();
+            const uint32_t v_lo = dv.lo + st * (C::KV_BYTES >> 4);
+#pragma unroll
+            for (int i = 0; i < BN / 16; ++i)
+              mma_ts(tmem + C::COL_O + t * D, tmem + C::COL_S + t * BN + i * 8, v_lo + i * (2048 >> 4), dv.hi, IDESC_PV,
+                     (j > tl.j0 || i > 0) ? 1u : 0u);
+            mma_commit(&empty[st]);
+            if (j == j_last) mma_commit(&o_full[t]);
+            next += tl.step;
+          } else {
+            mbar_arrive(&empty[st]);
+          }
+          if (++st == NS) { st = 0; ph ^= 1u; }
+        }
+        mbar_arrive(&seg_empty[k % kSegs]);
+      }
+      if (*abort_flag && qn) mbar_wait(&q_full[t], (qn - 1) & 1);  // a Q load still in flight
+      // every MMA issued by this thread has finished before the CTA can exit
+      mma_commit(mma_idle);
+      mbar_wait(mma_idle, 0);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    // ============================ softmax ============================
+    const int t = warp >> 2;
+    const int r = threadIdx.x & (BM - 1);  // row = TMEM lane
+    const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + lane_addr + C::COL_S + t * BN;
+    const uint32_t tO = tmem + lane_addr + C::COL_O;
+    const int rtok = (int)fdiv((uint32_t)r, p.div_group), rhead = r - rtok * p.group;
+    uint32_t sc = 0, oc0 = 0, oc1 = 0, nj = 0;  // S tiles, finished outputs of slots 0 and 1, joins
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      if (!wait(&seg_full[k % kSegs], (k / kSegs) & 1)) break;
+      const Seg* sg = &segs[k % kSegs];
+      const int q0 = sg->q0, ntok = sg->ntok, vis0 = sg->vis0, len = sg->len, single = sg->single, part = sg->part;
+      if (q0 < 0) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&seg_empty[k % kSegs]);
+        break;
+      }
+      const Tiles tl = slot_tiles(t, sg->t0, sg->t1, single, ntok, vis0, len);
+      const int tok = (single ? 0 : t * p.TQ) + rtok;  // of the unit
+      const bool valid = rtok < p.TQ && tok < ntok;
+      const int vis = p.causal ? vis0 + tok : len;     // keys that this row sees
+      const int vis_min = p.causal ? vis0 + (single ? 0 : t * p.TQ) : len;  // and that every row of the slot sees
+      const bool warp_valid = __any_sync(0xffffffffu, valid);
+      float m_use = -INFINITY, l = 0.f;
+      for (int j = tl.j0; j < tl.j1; j += tl.step) {
+        if (!wait(&s_full[t], sc & 1)) { ok = false; break; }
+        ++sc;
+        if (warp_valid) {
+          tc_fence_after();
+          float x[BN];
+          {
+            uint32_t rr[BN / 32][32];
+#pragma unroll
+            for (int c = 0; c < BN / 32; ++c) tmem_ld32(tS + c * 32, rr[c]);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < BN / 32; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[c * 32 + e] = __uint_as_float(rr[c][e]);
+          }
+          if ((j + 1) * BN > vis_min) {
+            const int lim = vis - j * BN;  // columns from lim on are hidden
+#pragma unroll
+            for (int c = 0; c < BN; ++c) x[c] = c >= lim ? -INFINITY : x[c];
+          }
+          // row maximum of the raw scores (the scale is positive): 4 chains of 3-input maxima
+          float mx;
+          {
+            float a0 = fmaxf(x[0], x[4]), a1 = fmaxf(x[1], x[5]), a2 = fmaxf(x[2], x[6]), a3 = fmaxf(x[3], x[7]);
+#pragma unroll
+            for (int c = 8; c < BN; c += 8) {
+              a0 = max3f(a0, x[c + 0], x[c + 1]);
+              a1 = max3f(a1, x[c + 2], x[c + 3]);
+              a2 = max3f(a2, x[c + 4], x[c + 5]);
+              a3 = max3f(a3, x[c + 6], x[c + 7]);
+            }
+            mx = max3f(a0, a1, fmaxf(a2, a3)) * p.scale_log2;
+          }
+          // the maximum in use only moves when it grows by more than 8 (log2), so O is rescaled
+          // rarely; P <= 2^8 stays as exact and the quotient O / l is the same
+          const float m_new = fmaxf(m_use, mx);
+          const bool need = m_new > m_use + kRescaleThreshold || (m_use == -INFINITY && m_new != -INFINITY);
+          float alpha = 1.f;
+          if (need) {
+            alpha = fast_exp2(m_use - m_new);
+            m_use = m_new;
+          }
+          const float m_sub = m_use == -INFINITY ? 0.f : m_use;
+          const float2 sl2 = make_float2(p.scale_log2, p.scale_log2), nm2 = make_float2(-m_sub, -m_sub);
+          float2 rs2[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) rs2[e] = make_float2(0.f, 0.f);
+          uint32_t pk[BN / 64][32];
+#pragma unroll
+          for (int e = 0; e < BN / 2; ++e) {
+            const float2 v = ffma2(make_float2(x[2 * e], x[2 * e + 1]), sl2, nm2);
+            const float2 ev = make_float2(fast_exp2(v.x), fast_exp2(v.y));
+            rs2[e & 3] = __fadd2_rn(rs2[e & 3], ev);
+            pk[e >> 5][e & 31] = Elem<T>::pack2(ev.x, ev.y);
+          }
+          const float2 rs01 = __fadd2_rn(rs2[0], rs2[1]), rs23 = __fadd2_rn(rs2[2], rs2[3]);
+          const float2 rsum = __fadd2_rn(rs01, rs23);
+          l = l * alpha + (rsum.x + rsum.y);
+          // S_j's commit covered P.V_j-1, so O may be rescaled here
+          if (j > tl.j0 && __any_sync(0xffffffffu, need)) {
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t rr[32];
+              tmem_ld32(tO + t * D + c * 32, rr);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) rr[e] = __float_as_uint(__uint_as_float(rr[e]) * alpha);
+              tmem_st32(tO + t * D + c * 32, rr);
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < BN / 64; ++c) tmem_st32(tS + c * 32, pk[c]);
+          tmem_wait_st();
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+      }
+      if (!ok) break;
+      // ---- the segment's output: the whole row, or its partial result
+      const bool mine = tl.j0 < tl.j1;
+      float w0 = 0.f, w1 = 0.f, total = l, m_row = m_use;
+      bool other = false;
+      if (mine) {
+        if (!wait(&o_full[t], (t ? oc1 : oc0) & 1)) break;
+        if (t) ++oc1; else ++oc0;
+        tc_fence_after();
+      }
+      if (single) {
+        if (t == 1) {  // hand the statistics over; slot 0 reads O from TMEM
+          stat[r] = m_use;
+          stat[BM + r] = mine ? l : 0.f;
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(join);
+          if (!wait(joined, nj & 1)) break;
+          ++nj;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&seg_empty[k % kSegs]);
+          continue;
+        }
+        if (!wait(join, nj & 1)) break;
+        ++nj;
+        tc_fence_after();
+        const float m1 = stat[r], l1 = stat[BM + r];
+        other = l1 > 0.f || l1 != l1;
+        m_row = fmaxf(m_use, other ? m1 : -INFINITY);
+        const float m_sub = m_row == -INFINITY ? 0.f : m_row;
+        w0 = fast_exp2(m_use - m_sub);
+        w1 = other ? fast_exp2(m1 - m_sub) : 0.f;
+        total = l * w0 + (other ? l1 * w1 : 0.f);
+      } else {
+        w0 = 1.f;
+      }
+      const bool any = total > 0.f || total != total;  // a row that sees no key: zeros
+      const float inv = any ? 1.f / total : 0.f;
+      w0 *= inv;
+      w1 *= inv;
+      const bool take1 = single && __any_sync(0xffffffffu, other);
+      const int head = sg->kvh * p.group + rhead;
+      const int64_t grow = (int64_t)q0 + tok;
+      T* orow = reinterpret_cast<T*>(p.out + grow * p.o_tok + (int64_t)head * p.o_head);
+      const int prow = (single ? 0 : t * BM) + r;
+      const int64_t pidx = ((int64_t)(2 * blockIdx.x) + max(part, 0)) * p.part_rows + prow;
+      if (warp_valid) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t a[32], b[32];
+          float o[32];
+          if (mine) tmem_ld32(tO + t * D + c * 32, a);
+          if (take1) tmem_ld32(tO + D + c * 32, b);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            float y = mine && any ? __uint_as_float(a[e]) * w0 : 0.f;
+            if (other) y = fmaf(__uint_as_float(b[e]), w1, y);
+            o[e] = y;
+          }
+          if (valid) {
+            if (part < 0) store32(o, orow + c * 32);
+            else store32(o, p.part_o + pidx * D + c * 32);
+          }
+        }
+        const float row_lse = any ? (m_row + __log2f(total)) * kLn2 : -INFINITY;
+        if (valid) {
+          if (part >= 0) p.part_lse[pidx] = row_lse;
+          else if (p.lse) p.lse[grow * p.l_tok + (int64_t)head * p.l_head] = row_lse;
+          if (sg->noted) {
+            if (part < 0) add_not_finite<T, D, T>(p, *sg, vis, orow);
+            else add_not_finite<T, D, float>(p, *sg, vis, p.part_o + pidx * D);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (single && lane == 0) mbar_arrive(joined);
+      if (lane == 0) mbar_arrive(&seg_empty[k % kSegs]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp0) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::TMEM_COLS));
+  }
+}
+
+// -------------------------------------------------------------------------
+// merge of units in parts, and zeros for rows of no sequence
+// -------------------------------------------------------------------------
+// O = sum_i e^{lse_i - M} O_i / sum_i e^{lse_i - M}.  The unit's parts are the one
+// with its first keys and then place 0 of the CTAs after it, up to the one with
+// its last keys.  CTA (x, y): place x, rows [32 y, 32 y + 32); a warp per row.
+constexpr int kMergeThreads = 256, kMergeRows = 32;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const ChunkParams p) {
+  grid_dep_wait();
+  constexpr int N = D / 32;  // columns per lane
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // padding rows of q (none in a batch that fills it)
+  if (blockIdx.y == 0) {
+    const int64_t lo = min(max((int64_t)__ldg(p.q_indptr), (int64_t)0), p.num_tokens);
+    const int64_t hi = min(max((int64_t)__ldg(p.q_indptr + p.B), lo), p.num_tokens);
+    const int64_t none = (lo + p.num_tokens - hi) * p.Hq;
+    for (int64_t i = (int64_t)blockIdx.x * (kMergeThreads / 32) + warp; i < none;
+         i += (int64_t)gridDim.x * (kMergeThreads / 32)) {
+      int64_t tok = i / p.Hq;
+      const int h = (int)(i - tok * p.Hq);
+      if (tok >= lo) tok += hi - lo;
+      T* row = reinterpret_cast<T*>(p.out + tok * p.o_tok + (int64_t)h * p.o_head);
+#pragma unroll
+      for (int e = 0; e < N; ++e) row[lane + 32 * e] = Elem<T>::from_float(0.f);
+      if (p.lse && lane == 0) p.lse[tok * p.l_tok + (int64_t)h * p.l_head] = -INFINITY;
+    }
+  }
+  const int c0 = blockIdx.x >> 1;
+  const Part me = p.parts[blockIdx.x];
+  if (!me.used || !me.first) return;
+  const int rows = me.single ? me.ntok * p.group : BM + (me.ntok - p.TQ) * p.group;
+  if ((int)blockIdx.y * kMergeRows >= rows) return;
+  // how many CTAs follow with parts of this unit (those without one are passed over)
+  int last = c0;
+  for (int base = c0 + 1; base < p.grid; base += 32) {
+    const int c = base + lane;
+    const bool ends = c < p.grid && p.parts[2 * c].used && p.parts[2 * c].last;
+    const unsigned m = __ballot_sync(0xffffffffu, ends);
+    if (m) {
+      last = base + __ffs(m) - 1;
+      break;
+    }
+  }
+  const int count = last - c0 + 1;
+  for (int r = blockIdx.y * kMergeRows + warp; r < min(rows, (int)(blockIdx.y + 1) * kMergeRows); r += kMergeThreads / 32) {
+    const int slot = me.single ? 0 : r >> 7, rr = r & (BM - 1);
+    const int rtok = (int)fdiv((uint32_t)rr, p.div_group), tok = slot * p.TQ + rtok;
+    if (rtok >= p.TQ || tok >= me.ntok) continue;
+    const int head = me.kvh * p.group + rr - rtok * p.group;
+    auto place = [&](int i) -> int64_t {
+      return ((int64_t)(i ? 2 * (c0 + i) : (int)blockIdx.x)) * p.part_rows + r;
+    };
+    auto lse_of = [&](int i) -> float {
+      return i < count && (i == 0 || p.parts[2 * (c0 + i)].used) ? p.part_lse[place(i)] : -INFINITY;
+    };
+    float M = -INFINITY;
+    for (int i = lane; i < count; i += 32) M = fmaxf(M, lse_of(i));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float Ms = M == -INFINITY ? 0.f : M;
+    float acc[N] = {}, den = 0.f;
+    for (int i0 = 0; i0 < count; i0 += 32) {
+      const float mine = fast_exp2((lse_of(i0 + lane) - Ms) * kLog2e);  // NaN stays NaN
+      const int n = min(32, count - i0);
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const float w = __shfl_sync(0xffffffffu, mine, i);
+        if (w == 0.f) continue;
+        den += w;
+        const float* o = p.part_o + place(i0 + i) * D + lane * N;
+        if constexpr (N == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(o);
+          acc[0] = fmaf(w, v.x, acc[0]); acc[1] = fmaf(w, v.y, acc[1]);
+          acc[2] = fmaf(w, v.z, acc[2]); acc[3] = fmaf(w, v.w, acc[3]);
+        } else {
+          const float2 v = *reinterpret_cast<const float2*>(o);
+          acc[0] = fmaf(w, v.x, acc[0]); acc[1] = fmaf(w, v.y, acc[1]);
+        }
+      }
+    }
+    const bool any = den > 0.f || den != den;
+    const float inv = any ? 1.f / den : 0.f;
+    const int64_t grow = (int64_t)me.q0 + tok;
+    T* row = reinterpret_cast<T*>(p.out + grow * p.o_tok + (int64_t)head * p.o_head) + lane * N;
+    if constexpr (N == 4)
+      *reinterpret_cast<uint2*>(row) = make_uint2(Elem<T>::pack2(acc[0] * inv, acc[1] * inv), Elem<T>::pack2(acc[2] * inv, acc[3] * inv));
+    else
+      *reinterpret_cast<uint32_t*>(row) = Elem<T>::pack2(acc[0] * inv, acc[1] * inv);
+    if (p.lse && lane == 0)
+      p.lse[grow * p.l_tok + (int64_t)head * p.l_head] = any ? Ms + __log2f(den) * kLn2 : -INFINITY;
+  }
+}
+
+// -------------------------------------------------------------------------
+// host
+// -------------------------------------------------------------------------
+bool al16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
+
+int sm_count() {
+  static std::atomic<int> counts[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  int n = counts[dev].load(std::memory_order_relaxed);
+  if (!n) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+    counts[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+
+struct Layout {
+  int grid, part_rows, TQ;
+  size_t parts, lse, o, cost, units, plan, share, bytes;
+};
+
+// The grid is one CTA per SM, or less where the tables' bounds show that there
+// are fewer tiles: a sequence has at most one unit more per head than its rows
+// fill, and a unit at most as many tiles as all pages hold.
+Layout make_layout(const akt_chunk_paged_args* a) {
+  Layout y{};
+  const int G = a->num_qo_heads / a->num_kv_heads;
+  y.TQ = BM / G;
+  const int64_t units = ((int64_t)a->num_tokens / (2 * y.TQ) + std::min<int64_t>(a->batch, a->num_tokens)) * a->num_kv_heads;
+  const int64_t tiles = a->num_page_entries * a->page_size / BN + 1;
+  y.grid = std::min({sm_count(), kMaxCtas, 1024});
+  if (units < y.grid && units * tiles < y.grid) y.grid = (int)std::max<int64_t>(1, units * tiles);
+  y.part_rows = (int)std::min<int64_t>(2 * BM, a->num_tokens * G <= BM ? a->num_tokens * G : 2 * BM);
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t p = at;
+    at += round256(n);
+    return p;
+  };
+  y.parts = take((size_t)y.grid * 2 * sizeof(Part));
+  y.lse = take((size_t)y.grid * 2 * y.part_rows * 4);
+  y.o = take((size_t)y.grid * 2 * y.part_rows * a->head_dim * 4);
+  if (a->batch > kTableSeqs) {
+    y.cost = take(((size_t)a->batch + 1) * 8);
+    y.units = take(((size_t)a->batch + 1) * 4);
+    y.plan = take(sizeof(Plan));
+    y.share = take(((size_t)y.grid + 1) * 8);
+  }
+  y.bytes = at;
+  return y;
 }
 
 int check_args(const akt_chunk_paged_args* a) {
@@ -107,47 +1360,113 @@ int check_args(const akt_chunk_paged_args* a) {
   if (a->dtype != AKT_FLOAT16 && a->dtype != AKT_BFLOAT16) return set_error(AKT_ERR_INVALID, "dtype");
   if (a->head_dim != 64 && a->head_dim != 128)
     return set_error(AKT_ERR_UNSUPPORTED, "chunk_paged: head_dim must be 64 or 128");
+  if (a->num_qo_heads / a->num_kv_heads > BM)
+    return set_error(AKT_ERR_UNSUPPORTED, "chunk_paged: at most 128 query heads per kv head");
   if (!(a->softmax_scale > 0.f) || a->softmax_scale == INFINITY)
     return set_error(AKT_ERR_INVALID, "chunk_paged: softmax_scale must be positive and finite");
-  if (a->num_tokens > 0x7fffffff / a->num_qo_heads || a->num_page_entries > 0x7fffffff / a->page_size)
+  // positions, rows and pages are 32-bit in the kernels (addresses are 64-bit)
+  if (a->num_tokens > 0x3fffffff / a->num_qo_heads || a->num_page_entries > 0x3fffffff / a->page_size ||
+      a->num_pages > 0x7ffffff0)
     return set_error(AKT_ERR_INVALID, "chunk_paged: too many tokens");
   if (a->num_tokens == 0) return AKT_OK;
   if (!a->q || !a->out || !a->q_indptr || !a->kv_page_indptr || !a->kv_last_page_len ||
-      (a->num_page_entries > 0 && (!a->kv_page_indices || !a->kv_cache)))
+      (a->num_page_entries > 0 && (!a->kv_page_indices || (!a->kv_cache && a->num_pages > 0))))
     return set_error(AKT_ERR_INVALID, "chunk_paged: missing tensor");
   if (a->batch == 0) return set_error(AKT_ERR_INVALID, "chunk_paged: tokens without sequences");
   if (a->q_stride_dim != 1 || a->kv_stride_dim != 1 || a->out_stride_dim != 1)
     return set_error(AKT_ERR_UNSUPPORTED, "chunk_paged: unit dim stride required");
+  const int64_t strides[] = {a->q_stride_token,  a->q_stride_head,  a->kv_stride_page,   a->kv_stride_kv,
+                             a->kv_stride_head,  a->kv_stride_token, a->out_stride_token, a->out_stride_head};
+  for (int64_t s : strides)
+    if (s % 8) return set_error(AKT_ERR_UNSUPPORTED, "chunk_paged: strides must be multiples of 16 bytes");
+  if (!al16(a->q) || !al16(a->kv_cache) || !al16(a->out))
+    return set_error(AKT_ERR_UNSUPPORTED, "chunk_paged: 16-byte alignment required");
   return AKT_OK;
 }
 
-template <typename T>
-int launch(const ChunkParams& p, int D, cudaStream_t st) {
-  const unsigned grid = (unsigned)((p.num_tokens * p.Hq + kWarps - 1) / kWarps);
+int make_map(CUtensorMap* m, const void* base, int dtype, const cuuint64_t (&dims)[4], const int64_t (&strides)[3],
+             cuuint32_t box1, cuuint32_t box3) {
+  auto fn = tensor_map_encoder();
+  if (!fn) return set_error(AKT_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  // an extent of one has no stride of its own (torch gives any)
+  cuuint64_t st[3];
+  for (int i = 0; i < 3; ++i) st[i] = (cuuint64_t)(dims[i + 1] > 1 ? strides[i] : 16);
+  cuuint32_t box[4] = {64, box1, 1, box3};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r =
+      fn(m, dtype == AKT_FLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+         const_cast<void*>(base), dims, st, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(AKT_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+  return AKT_OK;
+}
+
+template <typename T, int D, bool TMA>
+int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const ChunkParams& p,
+                 cudaStream_t st) {
+  auto kern = chunk_fwd_kernel<T, D, TMA>;
+  constexpr int smem = (int)Cfg<D>::SMEM_ALL;
+  // the register split in the kernel is only valid at the compiled count
+  static const int regs = [&] {
+    cudaFuncAttributes fa;
+    return cudaFuncGetAttributes(&fa, kern) == cudaSuccess ? fa.numRegs : 0;
+  }();
+  if (regs != kLaunchRegs)
+    return set_error(AKT_ERR_CUDA, "chunk kernel compiled with " + std::to_string(regs) + " registers, expected " +
+                                       std::to_string(kLaunchRegs));
+  cudaError_t e = ensure_smem_limit<chunk_fwd_kernel<T, D, TMA>>((size_t)smem);
+  if (e != cudaSuccess) return set_error(AKT_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
+  const bool planned = p.B > kTableSeqs;
+  if (planned) chunk_plan_kernel<<<1, 1024, 0, st>>>(p);
   {
     ProfileScope prof(st);
-    if (D == 64) chunk_rows_kernel<T, 64><<<grid, kWarps * 32, 0, st>>>(p);
-    else chunk_rows_kernel<T, 128><<<grid, kWarps * 32, 0, st>>>(p);
+    if (planned) e = launch_dependent(kern, dim3(p.grid), dim3(kThreads), smem, st, mq, mk, mv, p);
+    else kern<<<p.grid, kThreads, smem, st>>>(mq, mk, mv, p);
   }
-  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess)
+    e = launch_dependent(chunk_merge_kernel<T, D>, dim3(2 * p.grid, (p.part_rows + kMergeRows - 1) / kMergeRows),
+                         dim3(kMergeThreads), 0, st, p);
+  if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? AKT_OK : set_error(AKT_ERR_CUDA, std::string("chunk_paged: ") + cudaGetErrorString(e));
 }
 
+template <typename T, int D>
+int dispatch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const ChunkParams& p,
+                   cudaStream_t st) {
+  return p.box_rows ? launch_chunk<T, D, true>(mq, mk, mv, p, st) : launch_chunk<T, D, false>(mq, mk, mv, p, st);
+}
+
 }  // namespace
+
+cudaError_t chunk_status_read(unsigned int* v) { return cudaMemcpyFromSymbol(v, g_device_status_local, sizeof(*v)); }
+
+cudaError_t chunk_status_clear() {
+  const unsigned int z = 0;
+  return cudaMemcpyToSymbol(g_device_status_local, &z, sizeof(z));
+}
+
 }  // namespace akt
 
 using namespace akt;
 
-extern "C" size_t akt_chunk_paged_workspace_size(const akt_chunk_paged_args* a) { return 0; }
+extern "C" size_t akt_chunk_paged_workspace_size(const akt_chunk_paged_args* a) {
+  if (!a || a->num_qo_heads <= 0 || a->num_kv_heads <= 0 || a->num_qo_heads % a->num_kv_heads || a->num_tokens <= 0 ||
+      a->batch <= 0 || a->num_qo_heads / a->num_kv_heads > BM || a->page_size <= 0 || a->head_dim <= 0 ||
+      a->num_page_entries < 0)
+    return 0;
+  return make_layout(a).bytes;
+}
 
 extern "C" int akt_chunk_paged(const akt_chunk_paged_args* a, void* workspace, size_t workspace_bytes, void* stream) {
   if (!a) return set_error(AKT_ERR_INVALID, "null args");
-  const int rc = check_args(a);
+  int rc = check_args(a);
   if (rc || a->num_tokens == 0) return rc;
+  const Layout y = make_layout(a);
+  if (!workspace || workspace_bytes < y.bytes)
+    return set_error(AKT_ERR_WORKSPACE, "chunk_paged: workspace of " + std::to_string(y.bytes) + " bytes required");
   ChunkParams p{};
   p.q = static_cast<const char*>(a->q);
-  p.q_tok = a->q_stride_token * 2;
-  p.q_head = a->q_stride_head * 2;
   p.q_indptr = a->q_indptr;
   p.num_tokens = a->num_tokens;
   p.kv = static_cast<const char*>(a->kv_cache);
@@ -172,7 +1491,46 @@ extern "C" int akt_chunk_paged(const akt_chunk_paged_args* a, void* workspace, s
   p.group = p.Hq / p.Hkv;
   p.P = a->page_size;
   p.causal = a->causal ? 1 : 0;
+  p.D = a->head_dim;
   p.scale_log2 = a->softmax_scale * kLog2e;
+  p.TQ = y.TQ;
+  p.div_group = make_fastdiv((uint32_t)p.group);
+  p.div_page = make_fastdiv((uint32_t)p.P);
+  p.grid = y.grid;
+  char* ws = static_cast<char*>(workspace);
+  p.parts = reinterpret_cast<Part*>(ws + y.parts);
+  p.part_lse = reinterpret_cast<float*>(ws + y.lse);
+  p.part_o = reinterpret_cast<float*>(ws + y.o);
+  p.part_rows = y.part_rows;
+  if (p.B > kTableSeqs) {
+    p.plan_cost = reinterpret_cast<int64_t*>(ws + y.cost);
+    p.plan_units = reinterpret_cast<int*>(ws + y.units);
+    p.plan = reinterpret_cast<Plan*>(ws + y.plan);
+    p.plan_share = reinterpret_cast<int64_t*>(ws + y.share);
+  }
+  // a box holds rows of one page: the largest power of two from 8 (the swizzle's
+  // row period) to 128 that divides the page size
+  p.box_rows = 0;
+  for (int r = 128; r >= 8 && !p.box_rows; r >>= 1)
+    if (p.P % r == 0) p.box_rows = r;
+  CUtensorMap mq, mk, mv;
+  const int64_t qs[3] = {a->q_stride_head * 2, a->q_stride_head * 2 * p.group, a->q_stride_token * 2};
+  const cuuint64_t qd[4] = {(cuuint64_t)p.D, (cuuint64_t)p.group, (cuuint64_t)p.Hkv, (cuuint64_t)p.num_tokens};
+  rc = make_map(&mq, a->q, a->dtype, qd, qs, (cuuint32_t)p.group, (cuuint32_t)p.TQ);
+  if (rc) return rc;
+  if (p.box_rows && p.num_pages > 0) {
+    const int64_t ks[3] = {p.s_tok, p.s_head, p.s_page};
+    const cuuint64_t kd[4] = {(cuuint64_t)p.D, (cuuint64_t)p.P, (cuuint64_t)p.Hkv, (cuuint64_t)p.num_pages};
+    rc = make_map(&mk, p.kv, a->dtype, kd, ks, (cuuint32_t)p.box_rows, 1);
+    if (!rc) rc = make_map(&mv, p.kv + p.s_kv, a->dtype, kd, ks, (cuuint32_t)p.box_rows, 1);
+    if (rc) return rc;
+  } else {
+    mk = mv = mq;
+    p.box_rows = 0;
+  }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return a->dtype == AKT_FLOAT16 ? launch<__half>(p, a->head_dim, st) : launch<__nv_bfloat16>(p, a->head_dim, st);
+  if (a->dtype == AKT_FLOAT16)
+    return p.D == 64 ? dispatch_chunk<__half, 64>(mq, mk, mv, p, st) : dispatch_chunk<__half, 128>(mq, mk, mv, p, st);
+  return p.D == 64 ? dispatch_chunk<__nv_bfloat16, 64>(mq, mk, mv, p, st)
+                   : dispatch_chunk<__nv_bfloat16, 128>(mq, mk, mv, p, st);
 }
