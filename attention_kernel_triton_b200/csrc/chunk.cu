@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ __align__(1024) unsigned char smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* full = bars;             // [NS] loaded
-  uint64_t* empty = full + NS;       // [NS] both issuers done with it
+  uint64_t* empty = full + NS;       // [NS] both issuers and the scheduler warp done with it
   uint64_t* ready = empty + NS;      // [NS] seen (and, for V at a mask's edge, cleaned) by the scheduler warp
   uint64_t* q_full = ready + NS;     // [slot]
   uint64_t* s_full = q_full + 2;     // [slot]
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 2);
+      mbar_init(&empty[s], 3);
       mbar_init(&ready[s], 1);
     }
     for (int t = 0; t < 2; ++t) {
@@ -788,7 +788,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               fence_async_smem();
               __syncwarp();
             }
-            if (lane == 0) mbar_arrive(&ready[st]);
+            if (lane == 0) {
+              mbar_arrive(&ready[st]);
+              // K too is refilled only once this warp has seen it: its view of the
+              // barriers' phases must not fall a whole turn of the ring behind
+              mbar_arrive(&empty[st]);
+            }
             if (++st == NS) {
               st = 0;
               ph ^= 1u;

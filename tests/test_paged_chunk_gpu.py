@@ -80,6 +80,7 @@ class Case:
     def check(self, causal, scale=None, **kw):
         got, lse = flash_attention_chunk_paged_with_lse(*self.args(), causal=causal, softmax_scale=scale, **kw)
         self.close(got, lse, causal, scale)
+        assert _lib.device_status(0) == 0
         return got, lse
 
     def close(self, got, lse, causal, scale=None):
@@ -158,6 +159,15 @@ def test_chunk_many_units_per_cta():
     c = Case([1500, 700, 2100], [1500, 300, 2000], Hkv=8, G=4, D=64, dtype=FP16, seed=3)
     c.check(True)
     c.check(False)
+
+
+@pytest.mark.parametrize("new", [1, 5, 40])
+def test_chunk_many_segments_and_tiles_per_cta(new):
+    # each CTA walks several units of many key tiles, of one tile of rows and of two
+    lens = [300 + 97 * i for i in range(64)]
+    c = Case(lens, [new] * 64, Hkv=8, G=4, D=128, seed=new)
+    c.check(True)
+    assert _lib.device_status(0) == 0
 
 
 def test_chunk_one_token_is_the_decode():
