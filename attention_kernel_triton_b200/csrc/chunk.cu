@@ -427,6 +427,14 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -1024,17 +1032,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int k = 0; ok; ++k) {
       if (!wait(&seg_full[k % kSegs], (k / kSegs) & 1)) break;
       const Seg* sg = &segs[k % kSegs];
-      const int q0 = sg->q0, ntok = sg->ntok, vis0 = sg->vis0, len = sg->len, single = sg->single, part = sg->part;
-      if (q0 < 0) {
+      if (sg->q0 < 0) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&seg_empty[k % kSegs]);
         break;
       }
-      const Tiles tl = slot_tiles(t, sg->t0, sg->t1, single, ntok, vis0, len);
-      const int tok = (single ? 0 : t * p.TQ) + rtok;  // of the unit
-      const bool valid = rtok < p.TQ && tok < ntok;
-      const int vis = p.causal ? vis0 + tok : len;     // keys that this row sees
-      const int vis_min = p.causal ? vis0 + (single ? 0 : t * p.TQ) : len;  // and that every row of the slot sees
+      const bool single = sg->single;
+      const Tiles tl = slot_tiles(t, sg->t0, sg->t1, single, sg->ntok, sg->vis0, sg->len);
+      const bool mine = tl.j0 < tl.j1;
+      const int tok0 = single ? 0 : t * p.TQ;                        // the slot's first token of the unit
+      const int vis_min = p.causal ? sg->vis0 + tok0 : sg->len;      // keys that every row of the slot sees
+      const int vis = vis_min + (p.causal ? rtok : 0);               // and that this row sees
+      const bool valid = rtok < p.TQ && tok0 + rtok < sg->ntok;
       const bool warp_valid = __any_sync(0xffffffffu, valid);
       float m_use = -INFINITY, l = 0.f;
       for (int j = tl.j0; j < tl.j1; j += tl.step) {
@@ -1085,13 +1094,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           float2 rs2[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) rs2[e] = make_float2(0.f, 0.f);
-          uint32_t pk[BN / 64][32];
+          // 32 columns at a time: P goes out as it is made (columns of S already read)
 #pragma unroll
-          for (int e = 0; e < BN / 2; ++e) {
-            const float2 v = ffma2(make_float2(x[2 * e], x[2 * e + 1]), sl2, nm2);
-            const float2 ev = make_float2(fast_exp2(v.x), fast_exp2(v.y));
-            rs2[e & 3] = __fadd2_rn(rs2[e & 3], ev);
-            pk[e >> 5][e & 31] = Elem<T>::pack2(ev.x, ev.y);
+          for (int c = 0; c < BN / 32; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int i = c * 16 + e;
+              const float2 v = ffma2(make_float2(x[2 * i], x[2 * i + 1]), sl2, nm2);
+              const float2 ev = make_float2(fast_exp2(v.x), fast_exp2(v.y));
+              rs2[e & 3] = __fadd2_rn(rs2[e & 3], ev);
+              pk[e] = Elem<T>::pack2(ev.x, ev.y);
+            }
+            tmem_st16(tS + c * 16, pk);
           }
           const float2 rs01 = __fadd2_rn(rs2[0], rs2[1]), rs23 = __fadd2_rn(rs2[2], rs2[3]);
           const float2 rsum = __fadd2_rn(rs01, rs23);
@@ -1108,8 +1123,6 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_st32(tO + t * D + c * 32, rr);
             }
           }
-#pragma unroll
-          for (int c = 0; c < BN / 64; ++c) tmem_st32(tS + c * 32, pk[c]);
           tmem_wait_st();
           tc_fence_before();
         }
@@ -1118,7 +1131,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       // ---- the segment's output: the whole row, or its partial result
-      const bool mine = tl.j0 < tl.j1;
       float w0 = 0.f, w1 = 0.f, total = l, m_row = m_use;
       bool other = false;
       if (mine) {
@@ -1157,11 +1169,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       w0 *= inv;
       w1 *= inv;
       const bool take1 = single && __any_sync(0xffffffffu, other);
-      const int head = sg->kvh * p.group + rhead;
-      const int64_t grow = (int64_t)q0 + tok;
+      // (read again here rather than kept through the loop, which has no registers to spare)
+      const volatile Seg* sv = sg;
+      const int part = sv->part, head = sv->kvh * p.group + rhead;
+      const int64_t grow = (int64_t)sv->q0 + tok0 + rtok;
       T* orow = reinterpret_cast<T*>(p.out + grow * p.o_tok + (int64_t)head * p.o_head);
-      const int prow = (single ? 0 : t * BM) + r;
-      const int64_t pidx = ((int64_t)(2 * blockIdx.x) + max(part, 0)) * p.part_rows + prow;
+      const int64_t pidx = ((int64_t)(2 * blockIdx.x) + max(part, 0)) * p.part_rows + (single ? 0 : t * BM) + r;
       if (warp_valid) {
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
