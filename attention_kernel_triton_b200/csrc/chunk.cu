@@ -26,14 +26,14 @@
 //
 // Warps of a CTA (12):
 //   0-3 / 4-7  softmax of slot 0 / 1: thread i owns row i = TMEM lane i
-//   8          loader of the K and V ring: tensor-map boxes inside the pages, or
-//              16-byte cp.async rows where no box fits a page (TMA template)
-//   9 / 11     Q loads and MMAs of slot 0 / 1 (one thread)
+//   8 / 11     loaders of K / of V and Q into a ring of tiles: tensor-map boxes inside
+//              the pages, or 16-byte cp.async rows where no box fits a page (TMA template)
+//   9          issuer of both slots' MMAs (one thread)
 //   10         scheduler: the CTA's segments, a few ahead, through shared memory;
 //              and the V tiles at the mask's edge (below)
 // TMEM (512 columns): S[2] (128 each), O[2] (D each).  P_t overwrites S_t: a
-// slot's MMAs are issued by one thread in the order S_j, P.V_j, S_j+1, and while
-// one slot's softmax runs the tensor pipe works for the other.
+// slot's MMAs are issued in the order S_j, P.V_j, S_j+1, and while one slot's
+// softmax runs the tensor pipe works for the other.
 //
 // What lies behind the mask.  Scores are masked by selection, so K may hold
 // anything there.  A masked weight is 0, but 0 x NaN is NaN in P.V, so in V tiles
@@ -59,15 +59,16 @@ namespace {
 constexpr int BM = 128;            // rows of a slot
 constexpr int BN = 128;            // keys of a tile
 constexpr int kThreads = 384;
-constexpr int kLoadWarp = 8;
-constexpr int kMmaWarp0 = 9;
+constexpr int kLoadWarp = 8;       // K
+constexpr int kMmaWarp = 9;
 constexpr int kSchedWarp = 10;
+constexpr int kLoadVWarp = 11;     // V and Q
 // 2 * 128 * 216 + 128 * 64 <= 384 * 168 registers
 constexpr int kLaunchRegs = 168, kSoftmaxRegs = 216, kControlRegs = 64;
 static_assert(256 * kSoftmaxRegs + 128 * kControlRegs <= kThreads * kLaunchRegs, "register split");
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
 constexpr int kSegs = 4;           // segments in flight between the scheduler and the others
-constexpr int kSegReaders = 12;    // loader, 2 issuers, 8 softmax warps, scheduler (its V duty)
+constexpr int kSegReaders = 12;    // 2 loaders, issuer, 8 softmax warps, scheduler (its V duty)
 constexpr int kTableSeqs = 96;     // sequences whose table fits the CTA's shared memory
 constexpr int kMaxCtas = 384;      // of the main kernel (one per SM)
 
@@ -126,10 +127,11 @@ struct Seg {
   int page0;   // the sequence's first entry of the index array
   int len;     // its keys
   int t0, t1;  // key tiles
-  int nt;      // key tiles of the whole unit
+  int n0, n1;  // how many of them slot 0 and slot 1 take
   int single;  // one tile of rows: the slots take turns at the key tiles
   int part;    // -1: the whole unit; else the place of the partial result
   int noted;   // tokens in `bad`
+  int pad[3];
   uint32_t bad[3][BN / 32];  // tokens from tile vis0 / BN on whose V row is not finite
 };
 
@@ -139,11 +141,11 @@ struct Cfg {
   static constexpr int COL_S = 0, COL_O = 2 * BN, TMEM_COLS = 512;
   static_assert(COL_O + 2 * D <= TMEM_COLS, "TMEM budget");
   static constexpr uint32_t Q_BYTES = BM * D * 2, KV_BYTES = BN * D * 2;
-  static constexpr int NS = D == 64 ? 12 : 5;  // ring stages, K and V in turn
+  static constexpr int NS = D == 64 ? 11 : 5;  // ring stages, K and V in turn
   static constexpr uint32_t OFF_Q = 0, OFF_KV = 2 * Q_BYTES, OFF_BAR = OFF_KV + NS * KV_BYTES;
-  // full, empty, ready [NS]; q_full, s_full, p_full, o_full [slot]; seg_full,
+  // full, empty, ready [NS]; q_full, q_empty, s_full, p_full, o_full [slot]; seg_full,
   // seg_empty [kSegs]; join (slot 1 done), joined; mma_idle
-  static constexpr int N_BARS = 3 * NS + 8 + 2 * kSegs + 3;
+  static constexpr int N_BARS = 3 * NS + 10 + 2 * kSegs + 3;
   static constexpr uint32_t OFF_MISC = OFF_BAR + (N_BARS * 8 + 15) / 16 * 16;  // TMEM address, abort flag
   static constexpr uint32_t OFF_SEG = OFF_MISC + 16;
   static constexpr uint32_t OFF_TABLE = OFF_SEG + kSegs * sizeof(Seg);
@@ -364,41 +366,38 @@ __host__ __device__ constexpr uint32_t idesc_f16(int fmt, int M, int N, int b_mn
          ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-// A shared-memory descriptor as two words; an offset of the tile is an add on the low one.
-struct Desc {
-  uint32_t lo, hi;
-};
-__device__ __forceinline__ Desc desc_words(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-  const uint64_t d = desc_sw128(saddr, lbo, sbo);
-  return Desc{(uint32_t)d, (uint32_t)(d >> 32)};
-}
-
-__device__ __forceinline__ void mma_ss(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
-                                       uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "mov.b64 da, {%1, %2};\n\t"
-      "mov.b64 db, {%3, %4};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(tmem_d),
-      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
 
-__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
-                                       uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "mov.b64 db, {%2, %3};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(tmem_d),
-      "r"(tmem_a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
 
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
+}
+
+// one lane of a converged warp
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
 }
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -458,6 +457,19 @@ __device__ __forceinline__ void cp_async_wait() {
 }
 // generic-proxy writes to shared memory before later async-proxy reads (the MMAs)
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// whether the phase with this parity has completed, without waiting
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 
 __device__ __forceinline__ float max3f(float a, float b, float c) {
   float r;
@@ -530,6 +542,51 @@ __device__ __forceinline__ void store32(const float (&o)[32], float* out) {
   for (int e = 0; e < 32; e += 4) reinterpret_cast<float4*>(out)[e / 4] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
 }
 
+// The end of a softmax warp's rows of a segment: O = w0 O_t (+ w1 O_1 where the
+// slots are joined), normalised, to the output or to the segment's partial
+// result.  flags: 1 the slot has an output of its own, 2 slot 1's is added.  A
+// function of its own: what it needs is read again from the segment, so the key
+// loop has its registers.
+template <typename T, int D>
+__device__ __noinline__ void finish_rows(const ChunkParams& p, const Seg* sg, uint32_t tO, int t, float w0, float w1,
+                                         float row_lse, int flags) {
+  const int r = threadIdx.x & (BM - 1), rtok = (int)fdiv((uint32_t)r, p.div_group);
+  const bool single = sg->single;
+  const int tok = (single ? 0 : t * p.TQ) + rtok, part = sg->part, head = sg->kvh * p.group + r - rtok * p.group;
+  const bool valid = rtok < p.TQ && tok < sg->ntok;
+  const int64_t grow = (int64_t)sg->q0 + tok;
+  T* orow = reinterpret_cast<T*>(p.out + grow * p.o_tok + (int64_t)head * p.o_head);
+  const int64_t pidx = ((int64_t)(2 * blockIdx.x) + max(part, 0)) * p.part_rows + (single ? 0 : t * BM) + r;
+  const bool take0 = __any_sync(0xffffffffu, flags & 1), take1 = __any_sync(0xffffffffu, flags & 2);
+#pragma unroll 1
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t a[32], b[32];
+    float o[32];
+    if (take0) tmem_ld32(tO + t * D + c * 32, a);
+    if (take1) tmem_ld32(tO + D + c * 32, b);
+    tmem_wait_ld();
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      float y = flags & 1 ? __uint_as_float(a[e]) * w0 : 0.f;
+      if (flags & 2) y = fmaf(__uint_as_float(b[e]), w1, y);
+      o[e] = y;
+    }
+    if (valid) {
+      if (part < 0) store32(o, orow + c * 32);
+      else store32(o, p.part_o + pidx * D + c * 32);
+    }
+  }
+  if (valid) {
+    if (part >= 0) p.part_lse[pidx] = row_lse;
+    else if (p.lse) p.lse[grow * p.l_tok + (int64_t)head * p.l_head] = row_lse;
+    if (sg->noted) {
+      const int vis = sg->vis0 + tok;
+      if (part < 0) add_not_finite<T, D, T>(p, *sg, vis, orow);
+      else add_not_finite<T, D, float>(p, *sg, vis, p.part_o + pidx * D);
+    }
+  }
+}
+
 // -------------------------------------------------------------------------
 // the planner of batches past the CTA's own table
 // -------------------------------------------------------------------------
@@ -546,7 +603,7 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
 template <typename T, int D, bool TMA>
 __global__ void __launch_bounds__(kThreads, 1)
     chunk_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                     const __grid_constant__ CUtensorMap tmV, const ChunkParams p) {
+                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ ChunkParams p) {
   using C = Cfg<D>;
   constexpr int NS = C::NS;
   constexpr int fmt = std::is_same<T, __half>::value ? 0 : 1;
@@ -556,10 +613,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ __align__(1024) unsigned char smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* full = bars;             // [NS] loaded
-  uint64_t* empty = full + NS;       // [NS] both issuers and the scheduler warp done with it
+  uint64_t* empty = full + NS;       // [NS] the issuer and the scheduler warp done with it
   uint64_t* ready = empty + NS;      // [NS] seen (and, for V at a mask's edge, cleaned) by the scheduler warp
   uint64_t* q_full = ready + NS;     // [slot]
-  uint64_t* s_full = q_full + 2;     // [slot]
+  uint64_t* q_empty = q_full + 2;    // [slot]
+  uint64_t* s_full = q_empty + 2;    // [slot]
   uint64_t* p_full = s_full + 2;     // [slot]
   uint64_t* o_full = p_full + 2;     // [slot] the segment's last P.V is done
   uint64_t* seg_full = o_full + 2;   // [kSegs]
@@ -577,11 +635,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 3);
+      mbar_init(&empty[s], 2);
       mbar_init(&ready[s], 1);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
+      mbar_init(&q_empty[t], 1);
       mbar_init(&s_full[t], 1);
       mbar_init(&p_full[t], 4);
       mbar_init(&o_full[t], 1);
@@ -592,12 +651,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(join, 4);
     mbar_init(joined, 4);
-    mbar_init(mma_idle, 2);
+    mbar_init(mma_idle, 1);
     *abort_flag = (smem_u32(smem) & 1023u) ? 1 : 0;  // swizzled tiles need a 1024-byte aligned base
     if (*abort_flag) record_status(kStatusWaitTimeout);
     fence_mbar_init();
   }
-  if (warp == kMmaWarp0) {
+  if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "n"(C::TMEM_COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -634,18 +693,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (mbar_try_wait(bar, parity)) return true;
     return wait_or_abort(bar, parity, abort_flag);
   };
-  // first key tile of the CTA's slot t in a segment, the step and the end
-  struct Tiles {
-    int j0, step, j1;
-  };
-  auto slot_tiles = [&](int t, int t0, int t1, int single, int ntok, int vis0, int len) -> Tiles {
-    if (single) return Tiles{t0 + t, 2, t1};
-    const int tok = min(p.TQ * (t + 1), ntok) - 1;  // the slot's last token
-    if (tok < p.TQ * t) return Tiles{t0, 1, t0};
-    const int vis = p.causal ? vis0 + tok : len;
-    return Tiles{t0, 1, min(t1, vis > 0 ? (vis - 1) / BN + 1 : 0)};
-  };
-
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
     if (warp == kSchedWarp) {
@@ -674,9 +721,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           sg.kvh = k;
           sg.page0 = q.page0;
           sg.len = q.len;
-          sg.nt = unit_tiles(p, q, uu);
           sg.t0 = 0;
-          sg.t1 = sg.nt;
+          sg.t1 = unit_tiles(p, q, uu);
           sg.part = -1;
         } else if (x < x_end) {
           if (b < 0) {  // the unit that holds x
@@ -712,10 +758,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           sg.kvh = kvh;
           sg.page0 = s.page0;
           sg.len = s.len;
-          sg.nt = unit_tiles(p, s, u);
           const int64_t to = min(x_end - unit_x, (int64_t)cost);
           sg.t0 = (int)(x - unit_x);
-          sg.t1 = min((int)to, sg.nt);
+          sg.t1 = min((int)to, unit_tiles(p, s, u));
           const bool whole = sg.t0 == 0 && to == cost;
           sg.part = whole ? -1 : (stream ? 1 : 0);
           if (sg.t0 > sg.t1) sg.t0 = sg.t1;
@@ -744,6 +789,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         sg.single = sg.ntok <= p.TQ;
+        const int n = sg.t1 - sg.t0;
+        if (sg.single) {
+          sg.n0 = (n + 1) >> 1;
+          sg.n1 = n >> 1;
+        } else {  // slot 1 holds the unit's last token, slot 0's may see fewer keys
+          const int vis = p.causal ? sg.vis0 + p.TQ - 1 : sg.len;
+          sg.n0 = max(0, min(sg.t1, vis > 0 ? (vis - 1) / BN + 1 : 0) - sg.t0);
+          sg.n1 = n;
+        }
         more = sg.q0 >= 0;
         const int e = n_pub % kSegs;
         if (n_pub >= kSegs && !wait(&seg_empty[e], ((n_pub / kSegs) - 1) & 1)) {
@@ -810,11 +864,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (lane == 0) mbar_arrive(&seg_empty[k % kSegs]);
       }
-    } else if (warp == kLoadWarp) {
-      // ============================ K and V loader ============================
-      uint32_t st = 0, ph = 0, n_load = 0;
+    } else if (warp == kLoadWarp || warp == kLoadVWarp) {
+      // ============================ K loader, V (and Q) loader ============================
+      // A warp each: one warp's boxes (72 cycles apiece) took as long as a tile's whole turn.
+      // The K of tile i is ring load 2 i, its V load 2 i + 1.
+      const int op = warp == kLoadVWarp;
+      uint32_t g = op, qn0 = 0, qn1 = 0;
       bool ok = true;
-      const int boxes = TMA ? (BN / p.box_rows) * C::DB : 0;  // of one tile of K or V, at most 32
+      const int boxes = TMA ? (BN / p.box_rows) * C::DB : 0;  // of one tile, at most 32
       int held = -1;  // cp.async: the stage whose copies are not known to have landed
       auto hand_over = [&]() {
         if (held < 0) return;
@@ -828,53 +885,64 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!wait(&seg_full[k % kSegs], (k / kSegs) & 1)) break;
         const Seg* sg = &segs[k % kSegs];
         const int q0 = sg->q0, t0 = sg->t0, t1 = sg->t1, kvh = sg->kvh, page0 = sg->page0, len = sg->len;
+        const int single = sg->single, n0 = sg->n0, n1 = sg->n1;
         __syncwarp();
         if (lane == 0) mbar_arrive(&seg_empty[k % kSegs]);
         if (q0 < 0) break;
+        if (op) {  // Q of both slots: the buffer is free once the slot's last S before is done
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            uint32_t& qn = t ? qn1 : qn0;
+            if (!(t ? n1 : n0)) continue;
+            if (qn && !wait(&q_empty[t], (qn - 1) & 1)) {
+              ok = false;
+              break;
+            }
+            ++qn;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&q_full[t], (uint32_t)(p.TQ * p.group * 128 * C::DB));
+#pragma unroll
+              for (int db = 0; db < C::DB; ++db)
+                tma_load_4d(smem + C::OFF_Q + t * C::Q_BYTES + db * (BM * 128), &tmQ, db * 64, 0, kvh,
+                            q0 + (single ? 0 : t * p.TQ), &q_full[t]);
+            }
+          }
+        }
         if constexpr (TMA) {
           // lane l loads box l of each tile: rows [rb, rb + box_rows) of the tile, 64 columns
           const int db = lane % C::DB, rb = lane / C::DB * p.box_rows;
-          auto page_of = [&](int j, int& row) -> int {  // past the sequence and bad ids: past the pool (zeros)
+          const bool mine = lane < boxes;
+          // the index entry of the box's page, a tile ahead of its use (the id is looked at then)
+          auto entry = [&](int j) -> int {
             const int key = j * BN + rb;
-            row = 0;
-            if (lane >= boxes || key >= len) return (int)p.num_pages;
-            const int pg = (int)fdiv((uint32_t)key, p.div_page);
-            row = key - pg * p.P;
-            const int id = __ldg(p.indices + page0 + pg);
-            if (id >= 0 && id < p.num_pages) return id;
-            record_status(kStatusBadPage);
-            return (int)p.num_pages;
+            return mine && key < len ? __ldg(p.indices + page0 + (int)fdiv((uint32_t)key, p.div_page)) : -1;
           };
-          int row, page = 0;
-          if (t0 < t1) page = page_of(t0, row);
-          for (int j = t0; ok && j < t1; ++j) {
-            int row_next = 0, page_next = 0;
-            if (j + 1 < t1) page_next = page_of(j + 1, row_next);  // on its way while this tile is issued
-#pragma unroll
-            for (int op = 0; op < 2; ++op) {
-              if (n_load >= NS && !wait(&empty[st], ph ^ 1u)) {
-                ok = false;
-                break;
-              }
-              if (lane == 0) mbar_arrive_expect_tx(&full[st], C::KV_BYTES);
-              __syncwarp();
-              if (lane < boxes)
-                tma_load_4d(smem + C::OFF_KV + st * C::KV_BYTES + db * (BN * 128) + rb * 128, op ? &tmV : &tmK, db * 64,
-                            row, kvh, page, &full[st]);
-              ++n_load;
-              if (++st == NS) {
-                st = 0;
-                ph ^= 1u;
-              }
+          int id_next = t0 < t1 ? entry(t0) : -1;
+          for (int j = t0; ok && j < t1; ++j, g += 2) {
+            const int id = id_next, key = j * BN + rb;
+            if (j + 1 < t1) id_next = entry(j + 1);
+            const uint32_t st = g % NS;
+            if (g >= NS && !wait(&empty[st], ((g / NS) - 1) & 1)) {
+              ok = false;
+              break;
             }
-            row = row_next;
-            page = page_next;
+            if (lane == 0) mbar_arrive_expect_tx(&full[st], C::KV_BYTES);
+            __syncwarp();
+            if (mine) {
+              // boxes past the sequence, and of bad ids, are asked for past the pool: zeros
+              const bool there = id >= 0 && id < p.num_pages;
+              const int row = key - (int)fdiv((uint32_t)key, p.div_page) * p.P;
+              tma_load_4d(smem + C::OFF_KV + st * C::KV_BYTES + db * (BN * 128) + rb * 128, op ? &tmV : &tmK, db * 64,
+                          there ? row : 0, kvh, there ? id : (int)p.num_pages, &full[st]);
+              if (!there && key < len) record_status(kStatusBadPage);
+            }
+            __syncwarp();
           }
         } else {
           // every half warp (D = 128) or quarter (D = 64) copies whole rows in 16-byte pieces
           constexpr int CH = D / 8, RW = 32 / CH;  // pieces of a row; rows a step
           const int ch = lane % CH, rl = lane / CH;
-          for (int j = t0; ok && j < t1; ++j) {
+          for (int j = t0; ok && j < t1; ++j, g += 2) {
             // the addresses of rows lane, lane + 32, ... of the tile's keys (null: zeros)
             const char* src[BN / 32];
 #pragma unroll
@@ -885,137 +953,173 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int pg = (int)fdiv((uint32_t)key, p.div_page);
                 const int id = __ldg(p.indices + page0 + pg);
                 if (id >= 0 && id < p.num_pages)
-                  src[i] = p.kv + (int64_t)id * p.s_page + (int64_t)kvh * p.s_head + (int64_t)(key - pg * p.P) * p.s_tok;
+                  src[i] = p.kv + (op ? p.s_kv : 0) + (int64_t)id * p.s_page + (int64_t)kvh * p.s_head +
+                           (int64_t)(key - pg * p.P) * p.s_tok;
                 else record_status(kStatusBadPage);
               }
             }
-#pragma unroll 1
-            for (int op = 0; op < 2; ++op) {
-              if (n_load >= NS && !__all_sync(0xffffffffu, mbar_try_wait(&empty[st], ph ^ 1u))) {
-                hand_over();  // nothing else to do: what was copied last need not wait for the next copy
-                if (!wait(&empty[st], ph ^ 1u)) {
-                  ok = false;
-                  break;
-                }
-              }
-              const uint32_t tile = smem_u32(smem + C::OFF_KV + st * C::KV_BYTES);
-#pragma unroll
-              for (int i = 0; i < BN / 32; ++i) {
-#pragma unroll 4
-                for (int r0 = 0; r0 < 32; r0 += RW) {
-                  const int r = r0 + rl;
-                  const char* row = reinterpret_cast<const char*>(
-                      __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src[i]), r));
-                  const uint32_t dst = tile + (ch >> 3) * (BN * 128) + (i * 32 + r) * 128 + (((ch & 7) ^ (r & 7)) << 4);
-                  cp_async16(dst, row ? row + (op ? p.s_kv : 0) + ch * 16 : p.q, row ? 16u : 0u);
-                }
-              }
-              cp_async_commit();
-              if (held >= 0) {  // the stage before this one has landed
-                cp_async_wait<1>();
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&full[held]);
-              }
-              held = (int)st;
-              ++n_load;
-              if (++st == NS) {
-                st = 0;
-                ph ^= 1u;
+            __syncwarp();
+            const uint32_t st = g % NS;
+            if (g >= NS && !__all_sync(0xffffffffu, mbar_try_wait(&empty[st], ((g / NS) - 1) & 1))) {
+              hand_over();  // nothing else to do: what was copied last need not wait for the next copy
+              if (!wait(&empty[st], ((g / NS) - 1) & 1)) {
+                ok = false;
+                break;
               }
             }
+            const uint32_t tile = smem_u32(smem + C::OFF_KV + st * C::KV_BYTES);
+#pragma unroll
+            for (int i = 0; i < BN / 32; ++i) {
+#pragma unroll 4
+              for (int r0 = 0; r0 < 32; r0 += RW) {
+                const int r = r0 + rl;
+                const char* row =
+                    reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src[i]), r));
+                const uint32_t dst = tile + (ch >> 3) * (BN * 128) + (i * 32 + r) * 128 + (((ch & 7) ^ (r & 7)) << 4);
+                cp_async16(dst, row ? row + ch * 16 : p.q, row ? 16u : 0u);
+              }
+            }
+            cp_async_commit();
+            if (held >= 0) {  // the stage before this one has landed
+              cp_async_wait<1>();
+              fence_async_smem();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&full[held]);
+            }
+            held = (int)st;
           }
           hand_over();  // the segment's last stage
         }
       }
-      if (TMA && *abort_flag && lane == 0) {  // loads still in flight into this CTA's shared memory
-        for (uint32_t g = n_load > NS ? n_load - NS : 0; g < n_load; ++g) mbar_wait(&full[g % NS], (g / NS) & 1);
+      if (*abort_flag && lane == 0) {  // loads still in flight into this CTA's shared memory
+        if (TMA)
+          for (uint32_t f = g > 2 * NS ? g - 2 * NS : (uint32_t)op; f < g; f += 2) mbar_wait(&full[f % NS], (f / NS) & 1);
+        if (qn0) mbar_wait(&q_full[0], (qn0 - 1) & 1);
+        if (qn1) mbar_wait(&q_full[1], (qn1 - 1) & 1);
       }
       if (!TMA) cp_async_wait<0>();
-    } else if (lane == 0) {
-      // ============================ MMA issuers ============================
-      const int t = warp == kMmaWarp0 ? 0 : 1;
-      const Desc dq = desc_words(smem_u32(smem + C::OFF_Q + t * C::Q_BYTES), 16, 1024);
-      const Desc dk = desc_words(smem_u32(smem + C::OFF_KV), 16, 1024);
-      const Desc dv = desc_words(smem_u32(smem + C::OFF_KV), BN * 128, 1024);
-      uint32_t st = 0, ph = 0, qn = 0, pc = 0;
-      bool ok = true, q_loading = false;
-      // Q of segment k, once the slot's earlier S MMAs are known to be done; true if there is one
-      auto load_q = [&](int k) -> bool {
-        if (!wait(&seg_full[k % kSegs], (k / kSegs) & 1)) {
-          ok = false;
-          return false;
-        }
-        const Seg* sg = &segs[k % kSegs];
-        if (sg->q0 < 0) return false;
-        const Tiles tl = slot_tiles(t, sg->t0, sg->t1, sg->single, sg->ntok, sg->vis0, sg->len);
-        if (tl.j0 >= tl.j1) return false;
-        const int tok = sg->q0 + (sg->single ? 0 : t * p.TQ);
-        mbar_arrive_expect_tx(&q_full[t], (uint32_t)(p.TQ * p.group * 128 * C::DB));
+    } else {
+      // ============================ MMA issuer ============================
+      // One warp issues both slots' MMAs, the slots in turn: P.V of slot t's tile,
+      // then S of its next tile (which overwrites that P).  So the slots' softmaxes
+      // run half a period apart: with an issuer per slot their MMAs mixed in the pipe,
+      // both waited for S at the same time and then fought for the exponentials
+      // (5.1K cycles a tile pair).  The whole warp runs the control flow on values that
+      // are the same in every lane (a reduction's result is a uniform register, which is
+      // what the MMA takes its descriptors from) and an elected lane issues: 50 cycles
+      // an MMA, against 117 from a branch of one lane.  A wait that is over already
+      // costs 150 cycles, so the ring is asked once per load: `ready` comes in the order
+      // of the loads, and what a later load has answered is known of the earlier ones.
+      auto uni = [&](int v) { return (int)__reduce_or_sync(0xffffffffu, (unsigned)v); };
+      auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool {
+        return __all_sync(0xffffffffu, wait(bar, parity));
+      };
+      const uint64_t dk = desc_sw128(smem_u32(smem + C::OFF_KV), 16, 1024);
+      const uint64_t dq = desc_sw128(smem_u32(smem + C::OFF_Q), 16, 1024);
+      const uint64_t dv = desc_sw128(smem_u32(smem + C::OFF_KV), BN * 128, 1024);
+      const uint32_t tmem_u = uni(tmem);
+      uint32_t par = 0;    // parities of the next p_full (bits 0, 1) and q_full (bits 2, 3) by slot
+      uint32_t begun = 0;  // bit t: slot t's first S of the segment is out already
+      uint32_t base = 0;   // ring loads before the current segment
+      uint32_t seen = 0;   // ring loads known to be ready
+      bool ok = true;
+      auto ring_wait = [&](uint32_t g) -> bool {
+        if (g < seen) return true;
+        seen = g + 1;
+        return wait_all(&ready[g % NS], (g / NS) & 1);
+      };
+      // S of slot t from the K tile that is ring load g
+      auto issue_s = [&](int t, uint32_t g, bool last, bool release) {
+        const uint32_t st = g % NS;
+        const uint64_t k = dk + st * (C::KV_BYTES >> 4), q = dq + t * (C::Q_BYTES >> 4);
+        const uint32_t d = tmem_u + C::COL_S + t * BN;
+        tc_fence_after();
+        if (elect_one()) {
 #pragma unroll
-        for (int db = 0; db < C::DB; ++db)
-          tma_load_4d(smem + C::OFF_Q + t * C::Q_BYTES + db * (BM * 128), &tmQ, db * 64, 0, sg->kvh, tok, &q_full[t]);
-        ++qn;
-        return true;
+          for (int i = 0; i < D / 16; ++i) {
+            const uint32_t off = ((i >> 2) * (BN * 128) + (i & 3) * 32) >> 4;  // Q and K tiles have 128 rows each
+            mma_ss(d, q + off, k + off, IDESC_S, i > 0);
+          }
+          mma_commit(&s_full[t]);
+          if (release) mma_commit(&empty[st]);
+          if (last) mma_commit(&q_empty[t]);
+        }
+        __syncwarp();
       };
       for (int k = 0; ok; ++k) {
-        if (!wait(&seg_full[k % kSegs], (k / kSegs) & 1)) break;
+        if (!wait_all(&seg_full[k % kSegs], (k / kSegs) & 1)) break;
         const Seg* sg = &segs[k % kSegs];
-        const int t0 = sg->t0, t1 = sg->t1;
-        if (sg->q0 < 0) {
-          mbar_arrive(&seg_empty[k % kSegs]);
-          break;
-        }
-        const Tiles tl = slot_tiles(t, t0, t1, sg->single, sg->ntok, sg->vis0, sg->len);
-        const bool active = tl.j0 < tl.j1;
-        const int j_last = active ? tl.j0 + (tl.j1 - 1 - tl.j0) / tl.step * tl.step : -1;
-        if (active && !q_loading) load_q(k);
-        q_loading = false;
-        int next = tl.j0;
-        for (int j = t0; ok && j < t1; ++j) {
-          const bool mine = active && j == next && j < tl.j1;
-          // ---- S = Q K^T
-          if (!wait(&full[st], ph)) { ok = false; break; }
-          if (mine) {
-            if (j == tl.j0 && !wait(&q_full[t], (qn - 1) & 1)) { ok = false; break; }
-            tc_fence_after();
-            const uint32_t k_lo = dk.lo + st * (C::KV_BYTES >> 4);
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-              const uint32_t off = (i >> 2) * (BN * 128) + (i & 3) * 32;  // Q and K tiles have 128 rows each
-              mma_ss(tmem + C::COL_S + t * BN, dq.lo + (off >> 4), dq.hi, k_lo + (off >> 4), dk.hi, IDESC_S, i > 0);
-            }
-            mma_commit(&s_full[t]);
-            mma_commit(&empty[st]);
-          } else {
-            mbar_arrive(&empty[st]);
+        const int q0 = uni(sg->q0), single = uni(sg->single), tiles = uni(sg->t1 - sg->t0);
+        const int n0 = uni(sg->n0), n1 = uni(sg->n1);
+        if (lane == 0) mbar_arrive(&seg_empty[k % kSegs]);
+        if (q0 < 0) break;
+        // both slots' first S, unless it went out at the end of the last segment
+#pragma unroll 1
+        for (int t = 0; t < 2; ++t) {
+          const int nt = t ? n1 : n0;
+          if (!nt || (begun >> t & 1u)) continue;
+          const uint32_t g = base + (single ? 2 * t : 0);
+          if (!wait_all(&q_full[t], par >> (2 + t) & 1u) || !ring_wait(g)) {
+            ok = false;
+            break;
           }
-          if (++st == NS) { st = 0; ph ^= 1u; }
+          par ^= 4u << t;
+          issue_s(t, g, nt == 1, single || t);
+        }
+        begun = 0;
+        // one slot's turn: P.V of its tile r, then S of its next one
+        auto turn_of = [&](int t, int r) -> bool {
+          const int nt = t ? n1 : n0;
+          if (r >= nt) return true;
+          const bool last = r + 1 == nt;
+          const int j = single ? 2 * r + t : r;  // the tile's number in the segment
+          const uint32_t g = base + 2 * j + 1, st = g % NS;
+          const uint64_t v = dv + st * (C::KV_BYTES >> 4);
+          // with two slots on a tile, one wait per tile: for the next K, which comes after this V
+          if (!ring_wait(single || last ? g : g + 1) || !wait_all(&p_full[t], par >> t & 1u)) return false;
+          par ^= 1u << t;
           // ---- O += P V
-          if (!wait(&ready[st], ph)) { ok = false; break; }
-          if (mine) {
-            if (!wait(&p_full[t], pc & 1)) { ok = false; break; }
-            ++pc;
-            if (j == j_last) q_loading = load_q(k + 1);  // S of this segment is done: P came from it
-            tc_fence_after();
-            const uint32_t v_lo = dv.lo + st * (C::KV_BYTES >> 4);
+          tc_fence_after();
+          if (elect_one()) {
 #pragma unroll
-            for (int i = 0; i < BN / 16; ++i)
-              mma_ts(tmem + C::COL_O + t * D, tmem + C::COL_S + t * BN + i * 8, v_lo + i * (2048 >> 4), dv.hi, IDESC_PV,
-                     (j > tl.j0 || i > 0) ? 1u : 0u);
-            mma_commit(&empty[st]);
-            if (j == j_last) mma_commit(&o_full[t]);
-            next += tl.step;
-          } else {
-            mbar_arrive(&empty[st]);
+            for (int e = 0; e < BN / 16; ++e)
+              mma_ts(tmem_u + C::COL_O + t * D, tmem_u + C::COL_S + t * BN + e * 8, v + e * (2048 >> 4), IDESC_PV,
+                     e > 0 ? 1u : (uint32_t)(r > 0));
+            if (single || t) mma_commit(&empty[st]);
+            if (last) mma_commit(&o_full[t]);
           }
-          if (++st == NS) { st = 0; ph ^= 1u; }
-        }
-        mbar_arrive(&seg_empty[k % kSegs]);
+          __syncwarp();
+          if (!last) {
+            const uint32_t gs = base + 2 * (single ? j + 2 : j + 1);
+            if (!ring_wait(gs)) return false;
+            issue_s(t, gs, r + 2 == nt, single || t);
+            return true;
+          }
+          // or S of its first tile of the next segment, if its Q and K are there.  Two slots
+          // share a K tile and slot 1's S releases it, so slot 1 never goes first.
+          if (!uni(mbar_test(&seg_full[(k + 1) % kSegs], ((k + 1) / kSegs) & 1))) return true;
+          const Seg* s2 = &segs[(k + 1) % kSegs];
+          const int single2 = uni(s2->single);
+          const bool turn = s2->q0 >= 0 && (single2 || t == 0 || (begun & 1u) || s2->n0 == 0);
+          const int nt2 = uni(turn ? (t ? s2->n1 : s2->n0) : 0);
+          const uint32_t gs = base + 2 * tiles + (single2 ? 2 * t : 0);
+          if (nt2 && uni(mbar_test(&q_full[t], par >> (2 + t) & 1u) &&
+                         (gs < seen || mbar_test(&ready[gs % NS], (gs / NS) & 1)))) {
+            seen = max(seen, gs + 1);
+            par ^= 4u << t;
+            issue_s(t, gs, nt2 == 1, single2 || t);
+            begun |= 1u << t;
+          }
+          return true;
+        };
+        const int turns = 2 * max(n0, n1);
+#pragma unroll 1
+        for (int i = 0; ok && i < turns; ++i) ok = turn_of(i & 1, i >> 1);  // (unrolled by slot it spills)
+        base += 2 * tiles;
       }
-      if (*abort_flag && qn) mbar_wait(&q_full[t], (qn - 1) & 1);  // a Q load still in flight
       // every MMA issued by this thread has finished before the CTA can exit
-      mma_commit(mma_idle);
+      if (elect_one()) mma_commit(mma_idle);
+      __syncwarp();
       mbar_wait(mma_idle, 0);
     }
   } else {
@@ -1026,7 +1130,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + lane_addr + C::COL_S + t * BN;
     const uint32_t tO = tmem + lane_addr + C::COL_O;
-    const int rtok = (int)fdiv((uint32_t)r, p.div_group), rhead = r - rtok * p.group;
+    const int rtok = (int)fdiv((uint32_t)r, p.div_group);
     uint32_t sc = 0, oc0 = 0, oc1 = 0, nj = 0;  // S tiles, finished outputs of slots 0 and 1, joins
     bool ok = true;
     for (int k = 0; ok; ++k) {
@@ -1038,15 +1142,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       const bool single = sg->single;
-      const Tiles tl = slot_tiles(t, sg->t0, sg->t1, single, sg->ntok, sg->vis0, sg->len);
-      const bool mine = tl.j0 < tl.j1;
+      const int n = t ? sg->n1 : sg->n0;                             // the slot's key tiles
+      const bool mine = n > 0;
       const int tok0 = single ? 0 : t * p.TQ;                        // the slot's first token of the unit
-      const int vis_min = p.causal ? sg->vis0 + tok0 : sg->len;      // keys that every row of the slot sees
-      const int vis = vis_min + (p.causal ? rtok : 0);               // and that this row sees
+      // keys past the slot's first tile that every row of the slot sees, and that this row sees more
+      const int key0 = (sg->t0 + (single ? t : 0)) * BN, key_step = single ? 2 * BN : BN;
+      int vis_min = (p.causal ? sg->vis0 + tok0 : sg->len) - key0;
+      const int more = p.causal ? rtok : 0;
       const bool valid = rtok < p.TQ && tok0 + rtok < sg->ntok;
       const bool warp_valid = __any_sync(0xffffffffu, valid);
       float m_use = -INFINITY, l = 0.f;
-      for (int j = tl.j0; j < tl.j1; j += tl.step) {
+      for (int i = 0; i < n; ++i, vis_min -= key_step) {
         if (!wait(&s_full[t], sc & 1)) { ok = false; break; }
         ++sc;
         if (warp_valid) {
@@ -1062,8 +1168,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int e = 0; e < 32; ++e) x[c * 32 + e] = __uint_as_float(rr[c][e]);
           }
-          if ((j + 1) * BN > vis_min) {
-            const int lim = vis - j * BN;  // columns from lim on are hidden
+          if (vis_min < BN) {
+            const int lim = vis_min + more;  // columns from lim on are hidden
 #pragma unroll
             for (int c = 0; c < BN; ++c) x[c] = c >= lim ? -INFINITY : x[c];
           }
@@ -1100,8 +1206,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const int i = c * 16 + e;
-              const float2 v = ffma2(make_float2(x[2 * i], x[2 * i + 1]), sl2, nm2);
+              const float2 v = ffma2(make_float2(x[c * 32 + 2 * e], x[c * 32 + 2 * e + 1]), sl2, nm2);
               const float2 ev = make_float2(fast_exp2(v.x), fast_exp2(v.y));
               rs2[e & 3] = __fadd2_rn(rs2[e & 3], ev);
               pk[e] = Elem<T>::pack2(ev.x, ev.y);
@@ -1112,7 +1217,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float2 rsum = __fadd2_rn(rs01, rs23);
           l = l * alpha + (rsum.x + rsum.y);
           // S_j's commit covered P.V_j-1, so O may be rescaled here
-          if (j > tl.j0 && __any_sync(0xffffffffu, need)) {
+          if (i > 0 && __any_sync(0xffffffffu, need)) {
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
               uint32_t rr[32];
@@ -1168,42 +1273,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float inv = any ? 1.f / total : 0.f;
       w0 *= inv;
       w1 *= inv;
-      const bool take1 = single && __any_sync(0xffffffffu, other);
-      // (read again here rather than kept through the loop, which has no registers to spare)
-      const volatile Seg* sv = sg;
-      const int part = sv->part, head = sv->kvh * p.group + rhead;
-      const int64_t grow = (int64_t)sv->q0 + tok0 + rtok;
-      T* orow = reinterpret_cast<T*>(p.out + grow * p.o_tok + (int64_t)head * p.o_head);
-      const int64_t pidx = ((int64_t)(2 * blockIdx.x) + max(part, 0)) * p.part_rows + (single ? 0 : t * BM) + r;
-      if (warp_valid) {
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t a[32], b[32];
-          float o[32];
-          if (mine) tmem_ld32(tO + t * D + c * 32, a);
-          if (take1) tmem_ld32(tO + D + c * 32, b);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            float y = mine && any ? __uint_as_float(a[e]) * w0 : 0.f;
-            if (other) y = fmaf(__uint_as_float(b[e]), w1, y);
-            o[e] = y;
-          }
-          if (valid) {
-            if (part < 0) store32(o, orow + c * 32);
-            else store32(o, p.part_o + pidx * D + c * 32);
-          }
-        }
-        const float row_lse = any ? (m_row + __log2f(total)) * kLn2 : -INFINITY;
-        if (valid) {
-          if (part >= 0) p.part_lse[pidx] = row_lse;
-          else if (p.lse) p.lse[grow * p.l_tok + (int64_t)head * p.l_head] = row_lse;
-          if (sg->noted) {
-            if (part < 0) add_not_finite<T, D, T>(p, *sg, vis, orow);
-            else add_not_finite<T, D, float>(p, *sg, vis, p.part_o + pidx * D);
-          }
-        }
-      }
+      if (warp_valid)
+        finish_rows<T, D>(p, sg, tO, t, w0, w1, any ? (m_row + __log2f(total)) * kLn2 : -INFINITY,
+                          (mine && any ? 1 : 0) | (other ? 2 : 0));
       tc_fence_before();
       __syncwarp();
       if (single && lane == 0) mbar_arrive(joined);
@@ -1212,7 +1284,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp0) {
+  if (warp == kMmaWarp) {
     __syncwarp();
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::TMEM_COLS));
