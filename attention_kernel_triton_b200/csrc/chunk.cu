@@ -70,7 +70,7 @@ constexpr float kRescaleThreshold = 8.0f;  // log2 units
 constexpr int kSegs = 4;           // segments in flight between the scheduler and the others
 constexpr int kSegReaders = 12;    // 2 loaders, issuer, 8 softmax warps, scheduler (its V duty)
 constexpr int kTableSeqs = 96;     // sequences whose table fits the CTA's shared memory
-constexpr int kMaxCtas = 384;      // of the main kernel (one per SM)
+constexpr int kMaxCtas = kThreads; // of the main kernel (one per SM)
 
 struct ChunkParams {
   const char* q;
@@ -284,66 +284,64 @@ __device__ __forceinline__ int dealt_unit(const ChunkParams& p, int r, int c) {
   return r * p.grid + ((r & 1) ? p.grid - 1 - c : c);
 }
 
+// a / b, by the short division where both fit 32 bits
+__device__ __forceinline__ int64_t div_small(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 // Deals whole units and cuts the rest (at least p.grid threads of one CTA, all
 // call it).  share[c] .. share[c + 1] is CTA c's range of the cut part, in tiles
-// from plan.base.  scratch: 2 int64.
-__device__ Plan make_plan(const ChunkParams& p, const Tables& t, int64_t* share, int64_t* scratch) {
+// from plan.base.  scratch: an int64 per 32 CTAs.
+__device__ Plan make_plan(const ChunkParams& p, const Tables& t, int64_t* share, int* scratch) {
   const int64_t W = t.cost[p.B];
-  const int N = t.units[p.B];
-  const int64_t target = (W + p.grid - 1) / p.grid;
+  const int N = t.units[p.B], c = threadIdx.x;
+  const int64_t per = div_small(W, p.grid), left = W - per * p.grid;
+  const int64_t target = per + (left ? 1 : 0);
   Plan pl{0, 0};
   int64_t mine = 0;
   // Dealing pays by the CTAs of a round sharing K/V tiles in L2 and by fewer
   // parts; with one unit per (sequence, kv head) there is nothing to share.
   const int most = N > (int64_t)p.B * p.Hkv ? N / p.grid : 0;
   for (int r = 0; r < most; ++r) {
-    int64_t c = 0;
-    if (threadIdx.x < p.grid) {
+    int64_t cost = 0;
+    if (c < p.grid) {
       int b, kvh, u;
       Seq s;
-      unit_at(p, t, dealt_unit(p, r, threadIdx.x), b, s, kvh, u);
-      c = unit_cost(p, s, u);
+      unit_at(p, t, dealt_unit(p, r, c), b, s, kvh, u);
+      cost = unit_cost(p, s, u);
     }
-    if (__syncthreads_or(mine + c > target)) break;
-    mine += c;
+    if (__syncthreads_or(mine + cost > target)) break;
+    mine += cost;
     ++pl.rounds;
   }
-  // what each CTA still lacks, scaled to what is left
-  if (threadIdx.x < p.grid) share[threadIdx.x] = mine;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    int64_t dealt = 0, lacks = 0;
-    for (int c0 = 0; c0 < p.grid; c0 += 32) {
-      const int c = c0 + threadIdx.x;
-      const int64_t m = c < p.grid ? share[c] : target;
-      int64_t l = target - m, d = c < p.grid ? m : 0, x = l;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if (threadIdx.x >= o) x += y;
-      }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-      __syncwarp();
-      if (c < p.grid) share[c] = lacks + x - l;  // before CTA c
-      lacks += __shfl_sync(0xffffffffu, x, 31);
-      dealt += d;
-    }
-    if (threadIdx.x == 0) {
-      scratch[0] = dealt;
-      scratch[1] = lacks;
-    }
+  if (!pl.rounds) {  // everything is cut: c W / grid, to the tile
+    if (c <= p.grid) share[c] = c * per + (int64_t)((uint32_t)(c * left) / (uint32_t)p.grid);
+    __syncthreads();
+    return pl;
   }
-  __syncthreads();
-  pl.base = scratch[0];
-  const int64_t rest = W - scratch[0], lacks = scratch[1];
-  __syncthreads();
-  // lacks >= rest, and equal but for the rounding of the target
-  if (threadIdx.x < p.grid) {
-    const double f = lacks > 0 ? (double)share[threadIdx.x] / (double)lacks : 0.0;
-    share[threadIdx.x] = min((int64_t)(f * (double)rest), rest);
+  // each CTA's range is what it lacks of the target (the sums of the lacks are
+  // below W; the rounding of the target, less than a tile a CTA, is the last ones' gain)
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t x = c < p.grid ? target - mine : 0;
+  const int64_t lack = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
   }
-  if (threadIdx.x == 0) share[p.grid] = rest;
+  int64_t* sums = reinterpret_cast<int64_t*>(scratch);  // of the first warps
+  const int warps = (p.grid + 31) / 32;
+  if (lane == 31 && warp < warps) sums[warp] = x;
+  __syncthreads();
+  int64_t before = 0, all = 0;
+  for (int w = 0; w < warps; ++w) {
+    before += w < warp ? sums[w] : 0;
+    all += sums[w];
+  }
+  pl.base = p.grid * target - all;
+  const int64_t rest = W - pl.base;
+  if (c < p.grid) share[c] = min(before + x - lack, rest);
+  if (c == p.grid) share[c] = rest;
   __syncthreads();
   return pl;
 }
@@ -495,6 +493,10 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, vo
   }
 }
 
+__device__ __noinline__ bool wait_or_abort_call(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return wait_or_abort(bar, parity, abort_flag);
+}
+
 // 16-bit values of w that are not finite, as a mask of their bits
 template <typename T>
 __device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
@@ -591,7 +593,7 @@ __device__ __noinline__ void finish_rows(const ChunkParams& p, const Seg* sg, ui
 // the planner of batches past the CTA's own table
 // -------------------------------------------------------------------------
 __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
-  __shared__ int64_t scratch[2];
+  __shared__ __align__(8) int scratch[64];
   build_tables(p, p.plan_cost, p.plan_units, 1024);
   const Plan pl = make_plan(p, Tables{p.plan_cost, p.plan_units}, p.plan_share, scratch);
   if (threadIdx.x == 0) *p.plan = pl;
@@ -672,7 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int64_t* share = reinterpret_cast<int64_t*>(smem + C::OFF_Q);
     build_tables(p, cost, units, kThreads);
     tab = Tables{cost, units};
-    plan = make_plan(p, tab, share, share + p.grid + 1);
+    plan = make_plan(p, tab, share, reinterpret_cast<int*>(share + p.grid + 1));
     begin = share[blockIdx.x];
     end = share[blockIdx.x + 1];
     // generic reads before the async-proxy writes of the Q tile
@@ -695,6 +697,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
+    auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+      if (mbar_try_wait(bar, parity)) return true;
+      return wait_or_abort_call(bar, parity, abort_flag);
+    };
     if (warp == kSchedWarp) {
       // ===================== scheduler, and V at the mask's edge =====================
       int round = 0;               // rounds of whole units done
@@ -729,9 +735,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             b = find_seq(tab.cost, p.B, x);
             s = load_seq(p, b, false);
             U = num_units(p, s);
-            const int64_t per_head = (tab.cost[b + 1] - tab.cost[b]) / p.Hkv;
+            const int64_t per_head = div_small(tab.cost[b + 1] - tab.cost[b], p.Hkv);
             const int64_t rel = x - tab.cost[b];
-            kvh = (int)(rel / per_head);
+            kvh = (int)div_small(rel, per_head);
             unit_x = tab.cost[b] + kvh * per_head;
             for (int i0 = 0;; i0 += 32) {  // 32 units at a time
               const int i = i0 + lane;
@@ -1419,7 +1425,7 @@ Layout make_layout(const akt_chunk_paged_args* a) {
   y.TQ = BM / G;
   const int64_t units = ((int64_t)a->num_tokens / (2 * y.TQ) + std::min<int64_t>(a->batch, a->num_tokens)) * a->num_kv_heads;
   const int64_t tiles = a->num_page_entries * a->page_size / BN + 1;
-  y.grid = std::min({sm_count(), kMaxCtas, 1024});
+  y.grid = std::min(sm_count(), kMaxCtas - 1);  // (the planning threads are one more)
   if (units < y.grid && units * tiles < y.grid) y.grid = (int)std::max<int64_t>(1, units * tiles);
   y.part_rows = (int)std::min<int64_t>(2 * BM, a->num_tokens * G <= BM ? a->num_tokens * G : 2 * BM);
   size_t at = 0;
