@@ -91,7 +91,8 @@ struct ChunkParams {
   int TQ;             // tokens of a slot
   FastDiv div_group;  // row -> (token, head)
   FastDiv div_page;   // key -> (page, row)
-  int box_rows;       // rows of one tensor-map box (divides the page size), TMA loads
+  int box_rows;       // keys of one tensor-map box (divides the page size), TMA loads
+  int linear;         // pages, K and V, and heads follow one another with one stride
   int grid;           // CTAs of the main kernel
   // workspace
   struct Part* parts;  // [grid][2]
@@ -141,7 +142,9 @@ struct Cfg {
   static constexpr int COL_S = 0, COL_O = 2 * BN, TMEM_COLS = 512;
   static_assert(COL_O + 2 * D <= TMEM_COLS, "TMEM budget");
   static constexpr uint32_t Q_BYTES = BM * D * 2, KV_BYTES = BN * D * 2;
-  static constexpr int NS = D == 64 ? 11 : 5;  // ring stages, K and V in turn
+  // a K or V tile: per 8 keys, per 64 columns, 8 rows of 128 bytes (swizzled)
+  static constexpr uint32_t HALF = 1024, GROUP = DB * 1024;
+  static constexpr int NS = D == 64 ? 11 : 5;  // ring stages
   static constexpr uint32_t OFF_Q = 0, OFF_KV = 2 * Q_BYTES, OFF_BAR = OFF_KV + NS * KV_BYTES;
   // full, empty, ready [NS]; q_full, q_empty, s_full, p_full, o_full [slot]; seg_full,
   // seg_empty [kSegs]; join (slot 1 done), joined; mma_idle
@@ -346,6 +349,12 @@ __device__ Plan make_plan(const ChunkParams& p, const Tables& t, int64_t* share,
   return pl;
 }
 
+// Order of a segment's n tiles in the ring: K0, K1, V0, K2, V1, ... V(n-1).  V
+// comes a tile after its K (it is needed a softmax later), so stages hold what
+// is wanted soon.  Load of tile i's K and V:
+__device__ __forceinline__ uint32_t ring_k(int i) { return i ? 2 * i - 1 : 0; }
+__device__ __forceinline__ uint32_t ring_v(int i, int n) { return i + 1 < n ? 2 * i + 2 : 2 * i + 1; }
+
 // -------------------------------------------------------------------------
 // PTX helpers
 // -------------------------------------------------------------------------
@@ -441,6 +450,14 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
       "[%2];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, int y, int z, int w, int v, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(y), "r"(z), "r"(w), "r"(v)
       : "memory");
 }
 
@@ -827,45 +844,47 @@ __global__ void __launch_bounds__(kThreads, 1)
         Seg* sg = &segs[k % kSegs];
         const int t0 = sg->t0, t1 = sg->t1, vis0 = sg->vis0, len = sg->len, j_edge = max(vis0, 0) / BN;
         if (sg->q0 < 0) break;
-        for (int j = t0; ok && j < t1; ++j) {
+        const int loads = 2 * (t1 - t0);
 #pragma unroll 1
-          for (int op = 0; op < 2; ++op) {
-            if (!wait(&full[st], ph)) {
-              ok = false;
-              break;
-            }
-            if (op && ((p.causal && (j + 1) * BN > vis0) || (j + 1) * BN > len)) {
-              unsigned char* v = smem + C::OFF_KV + st * C::KV_BYTES;
-              const int rows = len - j * BN;  // the others are past the sequence
-              for (int c = lane; c < BN * D / 8; c += 32) {  // 16-byte pieces
-                const int r = (c >> 3) & (BN - 1);           // piece c: half c / (8 BN), row, chunk
-                uint4* w = reinterpret_cast<uint4*>(v + c * 16);
-                if (r >= rows) {
-                  *w = make_uint4(0, 0, 0, 0);
-                } else if (p.causal) {
-                  uint4 y = *w;
-                  const uint32_t m0 = not_finite2<T>(y.x), m1 = not_finite2<T>(y.y), m2 = not_finite2<T>(y.z),
-                                 m3 = not_finite2<T>(y.w);
-                  if (m0 | m1 | m2 | m3) {
-                    *w = make_uint4(y.x & ~m0, y.y & ~m1, y.z & ~m2, y.w & ~m3);
-                    atomicOr(&sg->bad[j - j_edge][r >> 5], 1u << (r & 31));
-                    sg->noted = 1;
-                  }
+        for (int i = 0; i < loads; ++i) {
+          if (!wait(&full[st], ph)) {
+            ok = false;
+            break;
+          }
+          // V tiles are the even loads from the third on, and the last one
+          const int j = t0 + (i + 1 == loads ? (i >> 1) : (i >> 1) - 1);
+          const bool is_v = i + 1 == loads || (i >= 2 && !(i & 1));
+          if (is_v && ((p.causal && (j + 1) * BN > vis0) || (j + 1) * BN > len)) {
+            unsigned char* v = smem + C::OFF_KV + st * C::KV_BYTES;
+            const int rows = len - j * BN;  // the others are past the sequence
+            for (int c = lane; c < BN * D / 8; c += 32) {  // 16-byte pieces
+              const int r = c / (64 * C::DB) * 8 + ((c >> 3) & 7);
+              uint4* w = reinterpret_cast<uint4*>(v + c * 16);
+              if (r >= rows) {
+                *w = make_uint4(0, 0, 0, 0);
+              } else if (p.causal) {
+                uint4 y = *w;
+                const uint32_t m0 = not_finite2<T>(y.x), m1 = not_finite2<T>(y.y), m2 = not_finite2<T>(y.z),
+                               m3 = not_finite2<T>(y.w);
+                if (m0 | m1 | m2 | m3) {
+                  *w = make_uint4(y.x & ~m0, y.y & ~m1, y.z & ~m2, y.w & ~m3);
+                  atomicOr(&sg->bad[j - j_edge][r >> 5], 1u << (r & 31));
+                  sg->noted = 1;
                 }
               }
-              fence_async_smem();
-              __syncwarp();
             }
-            if (lane == 0) {
-              mbar_arrive(&ready[st]);
-              // K too is refilled only once this warp has seen it: its view of the
-              // barriers' phases must not fall a whole turn of the ring behind
-              mbar_arrive(&empty[st]);
-            }
-            if (++st == NS) {
-              st = 0;
-              ph ^= 1u;
-            }
+            fence_async_smem();
+            __syncwarp();
+          }
+          if (lane == 0) {
+            mbar_arrive(&ready[st]);
+            // K too is refilled only once this warp has seen it: its view of the
+            // barriers' phases must not fall a whole turn of the ring behind
+            mbar_arrive(&empty[st]);
+          }
+          if (++st == NS) {
+            st = 0;
+            ph ^= 1u;
           }
         }
         if (lane == 0) mbar_arrive(&seg_empty[k % kSegs]);
@@ -873,11 +892,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == kLoadWarp || warp == kLoadVWarp) {
       // ============================ K loader, V (and Q) loader ============================
       // A warp each: one warp's boxes (72 cycles apiece) took as long as a tile's whole turn.
-      // The K of tile i is ring load 2 i, its V load 2 i + 1.
       const int op = warp == kLoadVWarp;
-      uint32_t g = op, qn0 = 0, qn1 = 0;
+      uint32_t base = 0, qn0 = 0, qn1 = 0;  // ring loads before the segment; Q loads
       bool ok = true;
-      const int boxes = TMA ? (BN / p.box_rows) * C::DB : 0;  // of one tile, at most 32
+      const int boxes = TMA ? BN / p.box_rows : 0;  // of one tile, at most 16
+      uint32_t loaded = 0;  // stages this warp has loaded (bits 0 ..) and the parity of the last load (16 ..)
       int held = -1;  // cp.async: the stage whose copies are not known to have landed
       auto hand_over = [&]() {
         if (held < 0) return;
@@ -915,8 +934,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if constexpr (TMA) {
-          // lane l loads box l of each tile: rows [rb, rb + box_rows) of the tile, 64 columns
-          const int db = lane % C::DB, rb = lane / C::DB * p.box_rows;
+          // lane l loads box l of each tile: keys [rb, rb + box_rows) of the tile
+          const int rb = lane * p.box_rows;
           const bool mine = lane < boxes;
           // the index entry of the box's page, a tile ahead of its use (the id is looked at then)
           auto entry = [&](int j) -> int {
@@ -924,22 +943,27 @@ __global__ void __launch_bounds__(kThreads, 1)
             return mine && key < len ? __ldg(p.indices + page0 + (int)fdiv((uint32_t)key, p.div_page)) : -1;
           };
           int id_next = t0 < t1 ? entry(t0) : -1;
-          for (int j = t0; ok && j < t1; ++j, g += 2) {
+          for (int j = t0; ok && j < t1; ++j) {
             const int id = id_next, key = j * BN + rb;
             if (j + 1 < t1) id_next = entry(j + 1);
-            const uint32_t st = g % NS;
+            const uint32_t g = base + (op ? ring_v(j - t0, t1 - t0) : ring_k(j - t0)), st = g % NS;
             if (g >= NS && !wait(&empty[st], ((g / NS) - 1) & 1)) {
               ok = false;
               break;
             }
             if (lane == 0) mbar_arrive_expect_tx(&full[st], C::KV_BYTES);
+            loaded = (loaded & ~(0x10001u << st)) | 1u << st | ((g / NS) & 1u) << (16 + st);
             __syncwarp();
             if (mine) {
               // boxes past the sequence, and of bad ids, are asked for past the pool: zeros
               const bool there = id >= 0 && id < p.num_pages;
-              const int row = key - (int)fdiv((uint32_t)key, p.div_page) * p.P;
-              tma_load_4d(smem + C::OFF_KV + st * C::KV_BYTES + db * (BN * 128) + rb * 128, op ? &tmV : &tmK, db * 64,
-                          there ? row : 0, kvh, there ? id : (int)p.num_pages, &full[st]);
+              const int row = there ? key - (int)fdiv((uint32_t)key, p.div_page) * p.P : 0;
+              const int page = there ? id : (int)p.num_pages;
+              unsigned char* dst = smem + C::OFF_KV + st * C::KV_BYTES + (rb >> 3) * C::GROUP;
+              if (p.linear)  // [block of a page, kv and head][8-row group][64 columns][row]
+                tma_load_5d(dst, &tmK, 0, 0, row >> 3, (page * 2 + op) * p.Hkv + kvh, &full[st]);
+              else  // [page][head][64 columns][row]
+                tma_load_5d(dst, op ? &tmV : &tmK, row, 0, kvh, page, &full[st]);
               if (!there && key < len) record_status(kStatusBadPage);
             }
             __syncwarp();
@@ -948,7 +972,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // every half warp (D = 128) or quarter (D = 64) copies whole rows in 16-byte pieces
           constexpr int CH = D / 8, RW = 32 / CH;  // pieces of a row; rows a step
           const int ch = lane % CH, rl = lane / CH;
-          for (int j = t0; ok && j < t1; ++j, g += 2) {
+          for (int j = t0; ok && j < t1; ++j) {
             // the addresses of rows lane, lane + 32, ... of the tile's keys (null: zeros)
             const char* src[BN / 32];
 #pragma unroll
@@ -965,7 +989,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
             __syncwarp();
-            const uint32_t st = g % NS;
+            const uint32_t g = base + (op ? ring_v(j - t0, t1 - t0) : ring_k(j - t0)), st = g % NS;
             if (g >= NS && !__all_sync(0xffffffffu, mbar_try_wait(&empty[st], ((g / NS) - 1) & 1))) {
               hand_over();  // nothing else to do: what was copied last need not wait for the next copy
               if (!wait(&empty[st], ((g / NS) - 1) & 1)) {
@@ -981,7 +1005,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int r = r0 + rl;
                 const char* row =
                     reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src[i]), r));
-                const uint32_t dst = tile + (ch >> 3) * (BN * 128) + (i * 32 + r) * 128 + (((ch & 7) ^ (r & 7)) << 4);
+                const uint32_t dst = tile + (uint32_t)(i * 4 + (r >> 3)) * C::GROUP + (ch >> 3) * C::HALF + (r & 7) * 128 +
+                                     (((ch & 7) ^ (r & 7)) << 4);
                 cp_async16(dst, row ? row + ch * 16 : p.q, row ? 16u : 0u);
               }
             }
@@ -996,10 +1021,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           hand_over();  // the segment's last stage
         }
+        base += 2 * (t1 - t0);
       }
       if (*abort_flag && lane == 0) {  // loads still in flight into this CTA's shared memory
         if (TMA)
-          for (uint32_t f = g > 2 * NS ? g - 2 * NS : (uint32_t)op; f < g; f += 2) mbar_wait(&full[f % NS], (f / NS) & 1);
+          for (int st = 0; st < NS; ++st)  // whichever phase a stage is in, its load (if any) ends it
+            if (loaded >> st & 1u) mbar_wait(&full[st], loaded >> (16 + st) & 1u);
         if (qn0) mbar_wait(&q_full[0], (qn0 - 1) & 1);
         if (qn1) mbar_wait(&q_full[1], (qn1 - 1) & 1);
       }
@@ -1020,9 +1047,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool {
         return __all_sync(0xffffffffu, wait(bar, parity));
       };
-      const uint64_t dk = desc_sw128(smem_u32(smem + C::OFF_KV), 16, 1024);
+      const uint64_t dk = desc_sw128(smem_u32(smem + C::OFF_KV), 16, C::GROUP);
       const uint64_t dq = desc_sw128(smem_u32(smem + C::OFF_Q), 16, 1024);
-      const uint64_t dv = desc_sw128(smem_u32(smem + C::OFF_KV), BN * 128, 1024);
+      const uint64_t dv = desc_sw128(smem_u32(smem + C::OFF_KV), C::HALF, C::GROUP);
       const uint32_t tmem_u = uni(tmem);
       uint32_t par = 0;    // parities of the next p_full (bits 0, 1) and q_full (bits 2, 3) by slot
       uint32_t begun = 0;  // bit t: slot t's first S of the segment is out already
@@ -1043,8 +1070,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (elect_one()) {
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) {
-            const uint32_t off = ((i >> 2) * (BN * 128) + (i & 3) * 32) >> 4;  // Q and K tiles have 128 rows each
-            mma_ss(d, q + off, k + off, IDESC_S, i > 0);
+            const uint32_t in = (i & 3) * 32;  // inside a row's 128 bytes
+            mma_ss(d, q + (((i >> 2) * (BM * 128) + in) >> 4), k + (((i >> 2) * C::HALF + in) >> 4), IDESC_S, i > 0);
           }
           mma_commit(&s_full[t]);
           if (release) mma_commit(&empty[st]);
@@ -1064,7 +1091,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int t = 0; t < 2; ++t) {
           const int nt = t ? n1 : n0;
           if (!nt || (begun >> t & 1u)) continue;
-          const uint32_t g = base + (single ? 2 * t : 0);
+          const uint32_t g = base + ring_k(single ? t : 0);
           if (!wait_all(&q_full[t], par >> (2 + t) & 1u) || !ring_wait(g)) {
             ok = false;
             break;
@@ -1079,24 +1106,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (r >= nt) return true;
           const bool last = r + 1 == nt;
           const int j = single ? 2 * r + t : r;  // the tile's number in the segment
-          const uint32_t g = base + 2 * j + 1, st = g % NS;
+          const uint32_t g = base + ring_v(j, tiles), st = g % NS;
           const uint64_t v = dv + st * (C::KV_BYTES >> 4);
-          // with two slots on a tile, one wait per tile: for the next K, which comes after this V
-          if (!ring_wait(single || last ? g : g + 1) || !wait_all(&p_full[t], par >> t & 1u)) return false;
+          // (with two slots on a tile, this is the only wait for the ring: the next K comes before this V)
+          if (!ring_wait(g) || !wait_all(&p_full[t], par >> t & 1u)) return false;
           par ^= 1u << t;
           // ---- O += P V
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
             for (int e = 0; e < BN / 16; ++e)
-              mma_ts(tmem_u + C::COL_O + t * D, tmem_u + C::COL_S + t * BN + e * 8, v + e * (2048 >> 4), IDESC_PV,
+              mma_ts(tmem_u + C::COL_O + t * D, tmem_u + C::COL_S + t * BN + e * 8, v + e * (2 * C::GROUP >> 4), IDESC_PV,
                      e > 0 ? 1u : (uint32_t)(r > 0));
             if (single || t) mma_commit(&empty[st]);
             if (last) mma_commit(&o_full[t]);
           }
           __syncwarp();
           if (!last) {
-            const uint32_t gs = base + 2 * (single ? j + 2 : j + 1);
+            const uint32_t gs = base + ring_k(single ? j + 2 : j + 1);
             if (!ring_wait(gs)) return false;
             issue_s(t, gs, r + 2 == nt, single || t);
             return true;
@@ -1108,7 +1135,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int single2 = uni(s2->single);
           const bool turn = s2->q0 >= 0 && (single2 || t == 0 || (begun & 1u) || s2->n0 == 0);
           const int nt2 = uni(turn ? (t ? s2->n1 : s2->n0) : 0);
-          const uint32_t gs = base + 2 * tiles + (single2 ? 2 * t : 0);
+          const uint32_t gs = base + 2 * tiles + ring_k(single2 ? t : 0);
           if (nt2 && uni(mbar_test(&q_full[t], par >> (2 + t) & 1u) &&
                          (gs < seen || mbar_test(&ready[gs % NS], (gs / NS) & 1)))) {
             seen = max(seen, gs + 1);
@@ -1480,17 +1507,16 @@ int check_args(const akt_chunk_paged_args* a) {
   return AKT_OK;
 }
 
-int make_map(CUtensorMap* m, const void* base, int dtype, const cuuint64_t (&dims)[4], const int64_t (&strides)[3],
-             cuuint32_t box1, cuuint32_t box3) {
+int make_map(CUtensorMap* m, const void* base, int dtype, int rank, const cuuint64_t* dims, const int64_t* strides,
+             const cuuint32_t* box) {
   auto fn = tensor_map_encoder();
   if (!fn) return set_error(AKT_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   // an extent of one has no stride of its own (torch gives any)
-  cuuint64_t st[3];
-  for (int i = 0; i < 3; ++i) st[i] = (cuuint64_t)(dims[i + 1] > 1 ? strides[i] : 16);
-  cuuint32_t box[4] = {64, box1, 1, box3};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
+  cuuint64_t st[4];
+  for (int i = 0; i + 1 < rank; ++i) st[i] = (cuuint64_t)(dims[i + 1] > 1 ? strides[i] : 16);
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   const CUresult r =
-      fn(m, dtype == AKT_FLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+      fn(m, dtype == AKT_FLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank,
          const_cast<void*>(base), dims, st, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
@@ -1604,26 +1630,39 @@ extern "C" int akt_chunk_paged(const akt_chunk_paged_args* a, void* workspace, s
     p.plan = reinterpret_cast<Plan*>(ws + y.plan);
     p.plan_share = reinterpret_cast<int64_t*>(ws + y.share);
   }
-  // a box holds rows of one page: the largest power of two from 8 (the swizzle's
+  // a box holds keys of one page: the largest power of two from 8 (the swizzle's
   // row period) to 128 that divides the page size
   p.box_rows = 0;
   for (int r = 128; r >= 8 && !p.box_rows; r >>= 1)
     if (p.P % r == 0) p.box_rows = r;
+  if (p.num_pages == 0) p.box_rows = 0;
   CUtensorMap mq, mk, mv;
-  const int64_t qs[3] = {a->q_stride_head * 2, a->q_stride_head * 2 * p.group, a->q_stride_token * 2};
   const cuuint64_t qd[4] = {(cuuint64_t)p.D, (cuuint64_t)p.group, (cuuint64_t)p.Hkv, (cuuint64_t)p.num_tokens};
-  rc = make_map(&mq, a->q, a->dtype, qd, qs, (cuuint32_t)p.group, (cuuint32_t)p.TQ);
-  if (rc) return rc;
-  if (p.box_rows && p.num_pages > 0) {
-    const int64_t ks[3] = {p.s_tok, p.s_head, p.s_page};
-    const cuuint64_t kd[4] = {(cuuint64_t)p.D, (cuuint64_t)p.P, (cuuint64_t)p.Hkv, (cuuint64_t)p.num_pages};
-    rc = make_map(&mk, p.kv, a->dtype, kd, ks, (cuuint32_t)p.box_rows, 1);
-    if (!rc) rc = make_map(&mv, p.kv + p.s_kv, a->dtype, kd, ks, (cuuint32_t)p.box_rows, 1);
-    if (rc) return rc;
-  } else {
-    mk = mv = mq;
-    p.box_rows = 0;
+  const int64_t qs[3] = {a->q_stride_head * 2, a->q_stride_head * 2 * p.group, a->q_stride_token * 2};
+  const cuuint32_t qb[4] = {64, (cuuint32_t)p.group, 1, (cuuint32_t)p.TQ};
+  rc = make_map(&mq, a->q, a->dtype, 4, qd, qs, qb);
+  mk = mv = mq;
+  if (!rc && p.box_rows) {
+    const cuuint64_t halves = (cuuint64_t)(p.D / 64);
+    // Heads, K and V, and pages in one run (a contiguous pool): one dimension counts
+    // them, and a box takes all 8-row groups of its keys, 4 KB at 16 keys of 128
+    // values.  Other strides take two dimensions and a box 8 rows.
+    p.linear = p.s_kv == p.s_head * p.Hkv && p.s_page == 2 * p.s_kv && p.num_pages * 2 * p.Hkv < 0x7fff0000;
+    if (p.linear) {
+      const cuuint64_t kd[5] = {64, 8, halves, (cuuint64_t)(p.P / 8), (cuuint64_t)(p.num_pages * 2 * p.Hkv)};
+      const int64_t ks[4] = {p.s_tok, 128, 8 * p.s_tok, p.s_head};
+      const cuuint32_t kb[5] = {64, 8, (cuuint32_t)halves, (cuuint32_t)(p.box_rows / 8), 1};
+      rc = make_map(&mk, p.kv, a->dtype, 5, kd, ks, kb);
+    } else {
+      p.box_rows = 8;
+      const cuuint64_t kd[5] = {64, (cuuint64_t)p.P, halves, (cuuint64_t)p.Hkv, (cuuint64_t)p.num_pages};
+      const int64_t ks[4] = {p.s_tok, 128, p.s_head, p.s_page};
+      const cuuint32_t kb[5] = {64, 8, (cuuint32_t)halves, 1, 1};
+      rc = make_map(&mk, p.kv, a->dtype, 5, kd, ks, kb);
+      if (!rc) rc = make_map(&mv, p.kv + p.s_kv, a->dtype, 5, kd, ks, kb);
+    }
   }
+  if (rc) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (a->dtype == AKT_FLOAT16)
     return p.D == 64 ? dispatch_chunk<__half, 64>(mq, mk, mv, p, st) : dispatch_chunk<__half, 128>(mq, mk, mv, p, st);
