@@ -69,6 +69,10 @@ static_assert(256 * kSoftmaxRegs + 128 * kControlRegs <= kThreads * kLaunchRegs,
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
 constexpr int kSegs = 4;           // segments in flight between the scheduler and the others
 constexpr int kSegReaders = 12;    // 2 loaders, issuer, 8 softmax warps, scheduler (its V duty)
+// A unit's start and end (Q, the first tile's chain, the output), in key tiles.
+// A batch of 512 to 32768 tokens: without it the CTAs with the short sequences
+// were last, 830 us against KUNIT_US.
+constexpr int kUnitCost = 2;
 constexpr int kTableSeqs = 96;     // sequences whose table fits the CTA's shared memory
 constexpr int kMaxCtas = kThreads; // of the main kernel (one per SM)
 
@@ -191,13 +195,13 @@ __device__ __forceinline__ int num_units(const ChunkParams& p, const Seq& s) {
   return s.n ? (s.n - 1) / (2 * p.TQ) + 1 : 0;
 }
 
-// Key tiles of unit u, and what it costs (a unit without keys writes zeros)
+// Key tiles of unit u, and what it costs on the line
 __device__ __forceinline__ int unit_tiles(const ChunkParams& p, const Seq& s, int u) {
   const int vis = p.causal ? s.len - s.n + min((u + 1) * 2 * p.TQ, s.n) : s.len;
   return vis > 0 ? (vis - 1) / BN + 1 : 0;
 }
 __device__ __forceinline__ int unit_cost(const ChunkParams& p, const Seq& s, int u) {
-  return max(unit_tiles(p, s, u), 1);
+  return kUnitCost + unit_tiles(p, s, u);
 }
 
 // Tables: cost[b] and units[b] count the tiles and units before sequence b.
@@ -747,68 +751,75 @@ __global__ void __launch_bounds__(kThreads, 1)
           sg.t0 = 0;
           sg.t1 = unit_tiles(p, q, uu);
           sg.part = -1;
-        } else if (x < x_end) {
-          if (b < 0) {  // the unit that holds x
-            b = find_seq(tab.cost, p.B, x);
-            s = load_seq(p, b, false);
-            U = num_units(p, s);
-            const int64_t per_head = div_small(tab.cost[b + 1] - tab.cost[b], p.Hkv);
-            const int64_t rel = x - tab.cost[b];
-            kvh = (int)div_small(rel, per_head);
-            unit_x = tab.cost[b] + kvh * per_head;
-            for (int i0 = 0;; i0 += 32) {  // 32 units at a time
-              const int i = i0 + lane;
-              int64_t c = i < U ? unit_cost(p, s, U - 1 - i) : 0, run = c;
+        } else {
+          while (x < x_end) {
+            if (b < 0) {  // the unit that holds x
+              b = find_seq(tab.cost, p.B, x);
+              s = load_seq(p, b, false);
+              U = num_units(p, s);
+              const int64_t per_head = div_small(tab.cost[b + 1] - tab.cost[b], p.Hkv);
+              const int64_t rel = x - tab.cost[b];
+              kvh = (int)div_small(rel, per_head);
+              unit_x = tab.cost[b] + kvh * per_head;
+              for (int i0 = 0;; i0 += 32) {  // 32 units at a time
+                const int i = i0 + lane;
+                int64_t c = i < U ? unit_cost(p, s, U - 1 - i) : 0, run = c;
 #pragma unroll
-              for (int o = 1; o < 32; o <<= 1) {
-                const int64_t y = __shfl_up_sync(0xffffffffu, run, o);
-                if (lane >= o) run += y;
+                for (int o = 1; o < 32; o <<= 1) {
+                  const int64_t y = __shfl_up_sync(0xffffffffu, run, o);
+                  if (lane >= o) run += y;
+                }
+                const unsigned m = __ballot_sync(0xffffffffu, i < U && unit_x + run > x);
+                if (m || i0 + 32 >= U) {
+                  const int at = m ? __ffs(m) - 1 : 31;
+                  u = U - 1 - min(i0 + at, U - 1);
+                  unit_x += __shfl_sync(0xffffffffu, run - c, at);
+                  break;
+                }
+                unit_x += __shfl_sync(0xffffffffu, run, 31);
               }
-              const unsigned m = __ballot_sync(0xffffffffu, i < U && unit_x + run > x);
-              if (m || i0 + 32 >= U) {
-                const int at = m ? __ffs(m) - 1 : 31;
-                u = U - 1 - min(i0 + at, U - 1);
-                unit_x += __shfl_sync(0xffffffffu, run - c, at);
-                break;
+            }
+            const int X = 2 * p.TQ, nt = unit_tiles(p, s, u), cost = kUnitCost + nt;
+            const int to = (int)min(x_end - unit_x, (int64_t)cost);
+            sg.t0 = max(0, (int)(x - unit_x) - kUnitCost);
+            sg.t1 = max(0, to - kUnitCost);
+            // a range with none of the unit's tiles leaves it to the others (a unit without
+            // any is the last one's, which writes zeros)
+            const bool some = nt ? sg.t0 < sg.t1 : to == cost;
+            if (some) {
+              sg.q0 = s.a0 + u * X;
+              sg.ntok = min(X, s.n - u * X);
+              sg.vis0 = p.causal ? s.len - s.n + u * X + 1 : s.len;
+              sg.kvh = kvh;
+              sg.page0 = s.page0;
+              sg.len = s.len;
+              const bool whole = sg.t1 - sg.t0 == nt;
+              sg.part = whole ? -1 : (stream ? 1 : 0);
+              if (!whole && lane == 0) {
+                Part& pt = p.parts[2 * blockIdx.x + sg.part];
+                pt.used = 1;
+                pt.first = sg.t0 == 0;
+                pt.last = sg.t1 == nt;
+                pt.q0 = sg.q0;
+                pt.ntok = sg.ntok;
+                pt.kvh = kvh;
+                pt.single = sg.ntok <= p.TQ;
               }
-              unit_x += __shfl_sync(0xffffffffu, run, 31);
+              ++stream;
             }
-          }
-          const int X = 2 * p.TQ, cost = unit_cost(p, s, u);
-          sg.q0 = s.a0 + u * X;
-          sg.ntok = min(X, s.n - u * X);
-          sg.vis0 = p.causal ? s.len - s.n + u * X + 1 : s.len;
-          sg.kvh = kvh;
-          sg.page0 = s.page0;
-          sg.len = s.len;
-          const int64_t to = min(x_end - unit_x, (int64_t)cost);
-          sg.t0 = (int)(x - unit_x);
-          sg.t1 = min((int)to, unit_tiles(p, s, u));
-          const bool whole = sg.t0 == 0 && to == cost;
-          sg.part = whole ? -1 : (stream ? 1 : 0);
-          if (sg.t0 > sg.t1) sg.t0 = sg.t1;
-          if (!whole && lane == 0) {
-            Part& pt = p.parts[2 * blockIdx.x + sg.part];
-            pt.used = 1;
-            pt.first = x == unit_x;
-            pt.last = to == cost;
-            pt.q0 = sg.q0;
-            pt.ntok = sg.ntok;
-            pt.kvh = kvh;
-            pt.single = sg.ntok <= p.TQ;
-          }
-          ++stream;
-          x = unit_x + to;
-          if (to == cost) {  // on to the next unit of the line
-            unit_x = x;
-            if (u > 0) {
-              --u;
-            } else if (kvh + 1 < p.Hkv) {
-              ++kvh;
-              u = U - 1;
-            } else {
-              b = -1;
+            x = unit_x + to;
+            if (to == cost) {  // on to the next unit of the line
+              unit_x = x;
+              if (u > 0) {
+                --u;
+              } else if (kvh + 1 < p.Hkv) {
+                ++kvh;
+                u = U - 1;
+              } else {
+                b = -1;
+              }
             }
+            if (some) break;
           }
         }
         sg.single = sg.ntok <= p.TQ;
@@ -855,15 +866,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int j = t0 + (i + 1 == loads ? (i >> 1) : (i >> 1) - 1);
           const bool is_v = i + 1 == loads || (i >= 2 && !(i & 1));
           if (is_v && ((p.causal && (j + 1) * BN > vis0) || (j + 1) * BN > len)) {
+            // rows that every row of the unit sees stay as they are
             unsigned char* v = smem + C::OFF_KV + st * C::KV_BYTES;
             const int rows = len - j * BN;  // the others are past the sequence
-            for (int c = lane; c < BN * D / 8; c += 32) {  // 16-byte pieces
-              const int r = c / (64 * C::DB) * 8 + ((c >> 3) & 7);
-              uint4* w = reinterpret_cast<uint4*>(v + c * 16);
+            const int r0 = min(max(p.causal ? vis0 - j * BN : rows, 0), BN);
+#pragma unroll 2
+            for (int c = lane; c < (BN - r0) * (D / 8); c += 32) {  // 16-byte pieces
+              const int r = r0 + c / (D / 8), ch = c % (D / 8);     // (the swizzle stays inside a row)
+              uint4* w = reinterpret_cast<uint4*>(v + (r >> 3) * C::GROUP + (ch >> 3) * C::HALF + (r & 7) * 128 + (ch & 7) * 16);
               if (r >= rows) {
                 *w = make_uint4(0, 0, 0, 0);
-              } else if (p.causal) {
-                uint4 y = *w;
+              } else {
+                const uint4 y = *w;
                 const uint32_t m0 = not_finite2<T>(y.x), m1 = not_finite2<T>(y.y), m2 = not_finite2<T>(y.z),
                                m3 = not_finite2<T>(y.w);
                 if (m0 | m1 | m2 | m3) {
