@@ -63,16 +63,18 @@ constexpr int kLoadWarp = 8;       // K
 constexpr int kMmaWarp = 9;
 constexpr int kSchedWarp = 10;
 constexpr int kLoadVWarp = 11;     // V and Q
-// 2 * 128 * 216 + 128 * 64 <= 384 * 168 registers
-constexpr int kLaunchRegs = 168, kSoftmaxRegs = 216, kControlRegs = 64;
+// 2 * 128 * 208 + 128 * 80 <= 384 * 168 registers (no spills; 216 and 64 spill a little)
+constexpr int kLaunchRegs = 168, kSoftmaxRegs = 208, kControlRegs = 80;
 static_assert(256 * kSoftmaxRegs + 128 * kControlRegs <= kThreads * kLaunchRegs, "register split");
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
 constexpr int kSegs = 4;           // segments in flight between the scheduler and the others
 constexpr int kSegReaders = 12;    // 2 loaders, issuer, 8 softmax warps, scheduler (its V duty)
-// A unit's start and end (Q, the first tile's chain, the output), in key tiles.
-// A batch of 512 to 32768 tokens: without it the CTAs with the short sequences
-// were last, 830 us against KUNIT_US.
-constexpr int kUnitCost = 2;
+// A unit's start and end (Q, the first tile's chain, the output), in key tiles:
+// of one tile of rows, of two.  A verification of 5 tokens in 64 sequences of 512
+// to 32768: without it the CTAs with the short sequences were last, 1025 us; with
+// 2 and 2 787, 6 and 1 682, 6 and 3 680, 8 and 3 686.  Eight prompts of 2048 tokens:
+// 451, then 400, 414, 398, 390.
+constexpr int kUnitCost1 = 6, kUnitCost2 = 3;
 constexpr int kTableSeqs = 96;     // sequences whose table fits the CTA's shared memory
 constexpr int kMaxCtas = kThreads; // of the main kernel (one per SM)
 
@@ -200,8 +202,11 @@ __device__ __forceinline__ int unit_tiles(const ChunkParams& p, const Seq& s, in
   const int vis = p.causal ? s.len - s.n + min((u + 1) * 2 * p.TQ, s.n) : s.len;
   return vis > 0 ? (vis - 1) / BN + 1 : 0;
 }
+__device__ __forceinline__ int unit_extra(const ChunkParams& p, const Seq& s, int u) {
+  return s.n - u * 2 * p.TQ <= p.TQ ? kUnitCost1 : kUnitCost2;
+}
 __device__ __forceinline__ int unit_cost(const ChunkParams& p, const Seq& s, int u) {
-  return kUnitCost + unit_tiles(p, s, u);
+  return unit_extra(p, s, u) + unit_tiles(p, s, u);
 }
 
 // Tables: cost[b] and units[b] count the tiles and units before sequence b.
@@ -518,11 +523,19 @@ __device__ __noinline__ bool wait_or_abort_call(uint64_t* bar, uint32_t parity, 
   return wait_or_abort(bar, parity, abort_flag);
 }
 
-// 16-bit values of w that are not finite, as a mask of their bits
+// Values of w that are not finite: bit 15 of each half, whose exponent is all ones
+// exactly when adding one to it carries out
 template <typename T>
 __device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
   constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u;
-  return __vcmpeq2(w & e, e);
+  constexpr uint32_t one = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
+  return ((w & e) + one) & 0x80008000u;
+}
+// w without them
+template <typename T>
+__device__ __forceinline__ uint32_t without_not_finite2(uint32_t w) {
+  const uint32_t m = not_finite2<T>(w) >> 15;
+  return w & ~(m * 0xffffu);
 }
 
 // The rare end of a row that sees tokens whose V row is not finite (their
@@ -551,62 +564,101 @@ __device__ __forceinline__ void add_not_finite(const ChunkParams& p, const Seg& 
   }
 }
 
-// 32 columns of a finished row: fp32 partial, or the output type
-template <typename T>
-__device__ __forceinline__ void store32(const float (&o)[32], T* out) {
-#pragma unroll
-  for (int e = 0; e < 32; e += 8)
-    reinterpret_cast<uint4*>(out)[e / 8] =
-        make_uint4(Elem<T>::pack2(o[e], o[e + 1]), Elem<T>::pack2(o[e + 2], o[e + 3]), Elem<T>::pack2(o[e + 4], o[e + 5]),
-                   Elem<T>::pack2(o[e + 6], o[e + 7]));
-}
-__device__ __forceinline__ void store32(const float (&o)[32], float* out) {
-#pragma unroll
-  for (int e = 0; e < 32; e += 4) reinterpret_cast<float4*>(out)[e / 4] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+// 4 x 4 pieces of 16 bytes turned over four lanes: v[i] is piece i of this lane's
+// row and becomes piece (lane % 4) of row i of its four lanes.
+__device__ __forceinline__ void turn_pieces(uint4 (&v)[4]) {
+  const int lane = threadIdx.x & 31;
+  auto swap = [&](uint4& keep_low, uint4& keep_high, bool high, int o) {
+    // the lane with the bit set gives its low piece for the other's high one
+    uint4 x = high ? keep_low : keep_high;
+    x.x = __shfl_xor_sync(0xffffffffu, x.x, o);
+    x.y = __shfl_xor_sync(0xffffffffu, x.y, o);
+    x.z = __shfl_xor_sync(0xffffffffu, x.z, o);
+    x.w = __shfl_xor_sync(0xffffffffu, x.w, o);
+    if (high) keep_low = x; else keep_high = x;
+  };
+  swap(v[0], v[1], lane & 1, 1);
+  swap(v[2], v[3], lane & 1, 1);
+  swap(v[0], v[2], lane & 2, 2);
+  swap(v[1], v[3], lane & 2, 2);
 }
 
 // The end of a softmax warp's rows of a segment: O = w0 O_t (+ w1 O_1 where the
 // slots are joined), normalised, to the output or to the segment's partial
 // result.  flags: 1 the slot has an output of its own, 2 slot 1's is added.  A
 // function of its own: what it needs is read again from the segment, so the key
-// loop has its registers.
+// loop has its registers.  A thread holds a row; four lanes exchange 16-byte
+// pieces so that a store covers 64 bytes of each of 8 rows (each thread storing
+// its own row, 16 bytes of 32 rows at a time, took 6.8K cycles at D = 128).
 template <typename T, int D>
-__device__ __noinline__ void finish_rows(const ChunkParams& p, const Seg* sg, uint32_t tO, int t, float w0, float w1,
+__device__ __forceinline__ void finish_rows(const ChunkParams& p, const Seg* sg, uint32_t tO, int t, float w0, float w1,
                                          float row_lse, int flags) {
   const int r = threadIdx.x & (BM - 1), rtok = (int)fdiv((uint32_t)r, p.div_group);
   const bool single = sg->single;
   const int tok = (single ? 0 : t * p.TQ) + rtok, part = sg->part, head = sg->kvh * p.group + r - rtok * p.group;
   const bool valid = rtok < p.TQ && tok < sg->ntok;
   const int64_t grow = (int64_t)sg->q0 + tok;
-  T* orow = reinterpret_cast<T*>(p.out + grow * p.o_tok + (int64_t)head * p.o_head);
   const int64_t pidx = ((int64_t)(2 * blockIdx.x) + max(part, 0)) * p.part_rows + (single ? 0 : t * BM) + r;
+  char* mine = valid ? (part < 0 ? p.out + grow * p.o_tok + (int64_t)head * p.o_head
+                                 : reinterpret_cast<char*>(p.part_o + pidx * D))
+                     : nullptr;
+  char* row[4];  // the four lanes' rows, at this lane's piece
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    row[i] = reinterpret_cast<char*>(
+        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), (threadIdx.x & 28) + i));
+    if (row[i]) row[i] += (threadIdx.x & 3) * 16;
+  }
   const bool take0 = __any_sync(0xffffffffu, flags & 1), take1 = __any_sync(0xffffffffu, flags & 2);
 #pragma unroll 1
   for (int c = 0; c < D / 32; ++c) {
-    uint32_t a[32], b[32];
+    uint32_t a[32];
     float o[32];
-    if (take0) tmem_ld32(tO + t * D + c * 32, a);
-    if (take1) tmem_ld32(tO + D + c * 32, b);
-    tmem_wait_ld();
-#pragma unroll
-    for (int e = 0; e < 32; ++e) {
-      float y = flags & 1 ? __uint_as_float(a[e]) * w0 : 0.f;
-      if (flags & 2) y = fmaf(__uint_as_float(b[e]), w1, y);
-      o[e] = y;
+    if (take0) {
+      tmem_ld32(tO + t * D + c * 32, a);
+      tmem_wait_ld();
     }
-    if (valid) {
-      if (part < 0) store32(o, orow + c * 32);
-      else store32(o, p.part_o + pidx * D + c * 32);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) o[e] = flags & 1 ? __uint_as_float(a[e]) * w0 : 0.f;
+    if (take1) {
+      tmem_ld32(tO + D + c * 32, a);
+      tmem_wait_ld();
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] = flags & 2 ? fmaf(__uint_as_float(a[e]), w1, o[e]) : o[e];
+    }
+    uint4 v[4];
+    if (part < 0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        v[e] = make_uint4(Elem<T>::pack2(o[8 * e], o[8 * e + 1]), Elem<T>::pack2(o[8 * e + 2], o[8 * e + 3]),
+                          Elem<T>::pack2(o[8 * e + 4], o[8 * e + 5]), Elem<T>::pack2(o[8 * e + 6], o[8 * e + 7]));
+      turn_pieces(v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (row[i]) *reinterpret_cast<uint4*>(row[i] + c * 64) = v[i];
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] = make_uint4(__float_as_uint(o[16 * h + 4 * e]), __float_as_uint(o[16 * h + 4 * e + 1]),
+                            __float_as_uint(o[16 * h + 4 * e + 2]), __float_as_uint(o[16 * h + 4 * e + 3]));
+        turn_pieces(v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (row[i]) *reinterpret_cast<uint4*>(row[i] + c * 128 + h * 64) = v[i];
+      }
     }
   }
   if (valid) {
     if (part >= 0) p.part_lse[pidx] = row_lse;
     else if (p.lse) p.lse[grow * p.l_tok + (int64_t)head * p.l_head] = row_lse;
-    if (sg->noted) {
-      const int vis = sg->vis0 + tok;
-      if (part < 0) add_not_finite<T, D, T>(p, *sg, vis, orow);
-      else add_not_finite<T, D, float>(p, *sg, vis, p.part_o + pidx * D);
-    }
+  }
+  if (sg->noted) {
+    __syncwarp();  // the row was stored by four lanes
+    const int vis = sg->vis0 + tok;
+    if (valid && part < 0) add_not_finite<T, D, T>(p, *sg, vis, reinterpret_cast<T*>(mine));
+    if (valid && part >= 0) add_not_finite<T, D, float>(p, *sg, vis, reinterpret_cast<float*>(mine));
   }
 }
 
@@ -779,10 +831,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 unit_x += __shfl_sync(0xffffffffu, run, 31);
               }
             }
-            const int X = 2 * p.TQ, nt = unit_tiles(p, s, u), cost = kUnitCost + nt;
+            const int X = 2 * p.TQ, nt = unit_tiles(p, s, u), extra = unit_extra(p, s, u), cost = extra + nt;
             const int to = (int)min(x_end - unit_x, (int64_t)cost);
-            sg.t0 = max(0, (int)(x - unit_x) - kUnitCost);
-            sg.t1 = max(0, to - kUnitCost);
+            sg.t0 = max(0, (int)(x - unit_x) - extra);
+            sg.t1 = max(0, to - extra);
             // a range with none of the unit's tiles leaves it to the others (a unit without
             // any is the last one's, which writes zeros)
             const bool some = nt ? sg.t0 < sg.t1 : to == cost;
@@ -833,6 +885,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           sg.n1 = n;
         }
         more = sg.q0 >= 0;
+        if (!more) sg.n1 = -1;
         const int e = n_pub % kSegs;
         if (n_pub >= kSegs && !wait(&seg_empty[e], ((n_pub / kSegs) - 1) & 1)) {
           ok = false;
@@ -870,21 +923,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             unsigned char* v = smem + C::OFF_KV + st * C::KV_BYTES;
             const int rows = len - j * BN;  // the others are past the sequence
             const int r0 = min(max(p.causal ? vis0 - j * BN : rows, 0), BN);
-#pragma unroll 2
-            for (int c = lane; c < (BN - r0) * (D / 8); c += 32) {  // 16-byte pieces
-              const int r = r0 + c / (D / 8), ch = c % (D / 8);     // (the swizzle stays inside a row)
-              uint4* w = reinterpret_cast<uint4*>(v + (r >> 3) * C::GROUP + (ch >> 3) * C::HALF + (r & 7) * 128 + (ch & 7) * 16);
+            constexpr int PR = D / 8, RS = 32 / PR;  // 16-byte pieces of a row, rows a step
+            const int ch = lane % PR;
+            unsigned char* vc = v + (ch >> 3) * C::HALF + (ch & 7) * 16;  // (the swizzle stays inside a row)
+#pragma unroll 4
+            for (int r = r0 + lane / PR; r < BN; r += RS) {
+              uint4* w = reinterpret_cast<uint4*>(vc + (r >> 3) * C::GROUP + (r & 7) * 128);
+              const uint4 y = *w;
               if (r >= rows) {
                 *w = make_uint4(0, 0, 0, 0);
-              } else {
-                const uint4 y = *w;
-                const uint32_t m0 = not_finite2<T>(y.x), m1 = not_finite2<T>(y.y), m2 = not_finite2<T>(y.z),
-                               m3 = not_finite2<T>(y.w);
-                if (m0 | m1 | m2 | m3) {
-                  *w = make_uint4(y.x & ~m0, y.y & ~m1, y.z & ~m2, y.w & ~m3);
-                  atomicOr(&sg->bad[j - j_edge][r >> 5], 1u << (r & 31));
-                  sg->noted = 1;
-                }
+              } else if (not_finite2<T>(y.x) | not_finite2<T>(y.y) | not_finite2<T>(y.z) | not_finite2<T>(y.w)) {
+                *w = make_uint4(without_not_finite2<T>(y.x), without_not_finite2<T>(y.y), without_not_finite2<T>(y.z),
+                                without_not_finite2<T>(y.w));
+                atomicOr(&sg->bad[j - j_edge][r >> 5], 1u << (r & 31));
+                sg->noted = 1;
               }
             }
             fence_async_smem();
@@ -1096,10 +1148,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int k = 0; ok; ++k) {
         if (!wait_all(&seg_full[k % kSegs], (k / kSegs) & 1)) break;
         const Seg* sg = &segs[k % kSegs];
-        const int q0 = uni(sg->q0), single = uni(sg->single), tiles = uni(sg->t1 - sg->t0);
-        const int n0 = uni(sg->n0), n1 = uni(sg->n1);
+        const int w0 = uni(sg->n0 * 2 + sg->single), n1 = uni(sg->n1);
         if (lane == 0) mbar_arrive(&seg_empty[k % kSegs]);
-        if (q0 < 0) break;
+        if (n1 < 0) break;
+        const int single = w0 & 1, n0 = w0 >> 1, tiles = single ? n0 + n1 : n1;
         // both slots' first S, unless it went out at the end of the last segment
 #pragma unroll 1
         for (int t = 0; t < 2; ++t) {
@@ -1146,9 +1198,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           // share a K tile and slot 1's S releases it, so slot 1 never goes first.
           if (!uni(mbar_test(&seg_full[(k + 1) % kSegs], ((k + 1) / kSegs) & 1))) return true;
           const Seg* s2 = &segs[(k + 1) % kSegs];
-          const int single2 = uni(s2->single);
-          const bool turn = s2->q0 >= 0 && (single2 || t == 0 || (begun & 1u) || s2->n0 == 0);
-          const int nt2 = uni(turn ? (t ? s2->n1 : s2->n0) : 0);
+          const bool turn = s2->n1 >= 0 && (s2->single || t == 0 || (begun & 1u) || s2->n0 == 0);
+          const int w2 = uni(turn ? (t ? s2->n1 : s2->n0) * 2 + s2->single : 0), nt2 = w2 >> 1, single2 = w2 & 1;
           const uint32_t gs = base + 2 * tiles + ring_k(single2 ? t : 0);
           if (nt2 && uni(mbar_test(&q_full[t], par >> (2 + t) & 1u) &&
                          (gs < seen || mbar_test(&ready[gs % NS], (gs / NS) & 1)))) {
