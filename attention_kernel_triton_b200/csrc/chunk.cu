@@ -237,8 +237,11 @@ __device__ __forceinline__ void unit_at(const ChunkParams& p, const Tables& t, i
 }
 
 // Fills the tables (threads of one CTA, `nthreads` of them; cost and units in
-// shared or global memory) -- the caller syncs before and after.
-__device__ void build_tables(const ChunkParams& p, int64_t* cost, int* units, int nthreads) {
+// shared or global memory), and the costliest unit's cost, no less, into
+// *most_cost (shared memory).
+__device__ void build_tables(const ChunkParams& p, int64_t* cost, int* units, int* most_cost, int nthreads) {
+  if (threadIdx.x == 0) *most_cost = 1;
+  __syncthreads();
   // a team of threads per sequence sums its units' costs
   int team = 32;
   while (team > 1 && (nthreads / team) < p.B) team >>= 1;
@@ -256,6 +259,7 @@ __device__ void build_tables(const ChunkParams& p, int64_t* cost, int* units, in
     if (b < p.B && lane == 0) {
       cost[b + 1] = c * p.Hkv;
       units[b + 1] = U * p.Hkv;
+      if (U) atomicMax(most_cost, unit_tiles(p, load_seq(p, b, false), U - 1) + max(kUnitCost1, kUnitCost2));
     }
   }
   __syncthreads();
@@ -304,7 +308,7 @@ __device__ __forceinline__ int64_t div_small(int64_t a, int64_t b) {
 // Deals whole units and cuts the rest (at least p.grid threads of one CTA, all
 // call it).  share[c] .. share[c + 1] is CTA c's range of the cut part, in tiles
 // from plan.base.  scratch: an int64 per 32 CTAs.
-__device__ Plan make_plan(const ChunkParams& p, const Tables& t, int64_t* share, int* scratch) {
+__device__ Plan make_plan(const ChunkParams& p, const Tables& t, int most_cost, int64_t* share, int* scratch) {
   const int64_t W = t.cost[p.B];
   const int N = t.units[p.B], c = threadIdx.x;
   const int64_t per = div_small(W, p.grid), left = W - per * p.grid;
@@ -313,18 +317,29 @@ __device__ Plan make_plan(const ChunkParams& p, const Tables& t, int64_t* share,
   int64_t mine = 0;
   // Dealing pays by the CTAs of a round sharing K/V tiles in L2 and by fewer
   // parts; with one unit per (sequence, kv head) there is nothing to share.
+  // Rounds that cannot pass the target (all units as dear as the dearest) take no
+  // barrier; a thread's units run up the line, so it walks the sequences once.
   const int most = N > (int64_t)p.B * p.Hkv ? N / p.grid : 0;
-  for (int r = 0; r < most; ++r) {
-    int64_t cost = 0;
-    if (c < p.grid) {
-      int b, kvh, u;
-      Seq s;
-      unit_at(p, t, dealt_unit(p, r, c), b, s, kvh, u);
-      cost = unit_cost(p, s, u);
+  const int safe = (int)min((int64_t)most, div_small(target, most_cost));
+  int end = 0, start = 0, U = 1;
+  Seq s{};
+  auto cost_in_round = [&](int r) -> int {
+    const int i = dealt_unit(p, r, c);
+    if (i >= end) {
+      const int b = find_seq(t.units, p.B, i);
+      start = t.units[b];
+      end = t.units[b + 1];
+      s = load_seq(p, b, false);
+      U = num_units(p, s);
     }
+    return unit_cost(p, s, U - 1 - (i - start) % U);
+  };
+  if (c < p.grid)
+    for (int r = 0; r < safe; ++r) mine += cost_in_round(r);
+  for (pl.rounds = safe; pl.rounds < most; ++pl.rounds) {
+    const int cost = c < p.grid ? cost_in_round(pl.rounds) : 0;
     if (__syncthreads_or(mine + cost > target)) break;
     mine += cost;
-    ++pl.rounds;
   }
   if (!pl.rounds) {  // everything is cut: c W / grid, to the tile
     if (c <= p.grid) share[c] = c * per + (int64_t)((uint32_t)(c * left) / (uint32_t)p.grid);
@@ -667,8 +682,9 @@ __device__ __forceinline__ void finish_rows(const ChunkParams& p, const Seg* sg,
 // -------------------------------------------------------------------------
 __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
   __shared__ __align__(8) int scratch[64];
-  build_tables(p, p.plan_cost, p.plan_units, 1024);
-  const Plan pl = make_plan(p, Tables{p.plan_cost, p.plan_units}, p.plan_share, scratch);
+  __shared__ int most_cost;
+  build_tables(p, p.plan_cost, p.plan_units, &most_cost, 1024);
+  const Plan pl = make_plan(p, Tables{p.plan_cost, p.plan_units}, most_cost, p.plan_share, scratch);
   if (threadIdx.x == 0) *p.plan = pl;
 }
 
@@ -745,9 +761,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     int* units = reinterpret_cast<int*>(cost + p.B + 1);
     // the shares live where slot 0's Q tile goes later
     int64_t* share = reinterpret_cast<int64_t*>(smem + C::OFF_Q);
-    build_tables(p, cost, units, kThreads);
+    int* scratch = reinterpret_cast<int*>(share + p.grid + 1);
+    build_tables(p, cost, units, scratch + 63, kThreads);
     tab = Tables{cost, units};
-    plan = make_plan(p, tab, share, reinterpret_cast<int*>(share + p.grid + 1));
+    plan = make_plan(p, tab, scratch[63], share, scratch);
     begin = share[blockIdx.x];
     end = share[blockIdx.x + 1];
     // generic reads before the async-proxy writes of the Q tile
