@@ -209,10 +209,12 @@ __device__ __forceinline__ int unit_cost(const ChunkParams& p, const Seq& s, int
   return unit_extra(p, s, u) + unit_tiles(p, s, u);
 }
 
-// Tables: cost[b] and units[b] count the tiles and units before sequence b.
+// Tables: cost[b] and units[b] count the tiles and units before sequence b; seqs
+// (or null) holds the sequences while the plan is made.
 struct Tables {
   const int64_t* cost;
   const int* units;
+  const Seq* seqs;
 };
 
 // Largest b in [0, B) with t[b] <= x (the entry that holds x; empty ones are passed over).
@@ -239,7 +241,7 @@ __device__ __forceinline__ void unit_at(const ChunkParams& p, const Tables& t, i
 // Fills the tables (threads of one CTA, `nthreads` of them; cost and units in
 // shared or global memory), and the costliest unit's cost, no less, into
 // *most_cost (shared memory).
-__device__ void build_tables(const ChunkParams& p, int64_t* cost, int* units, int* most_cost, int nthreads) {
+__device__ void build_tables(const ChunkParams& p, int64_t* cost, int* units, Seq* seqs, int* most_cost, int nthreads) {
   if (threadIdx.x == 0) *most_cost = 1;
   __syncthreads();
   // a team of threads per sequence sums its units' costs
@@ -250,8 +252,9 @@ __device__ void build_tables(const ChunkParams& p, int64_t* cost, int* units, in
     const int b = b0 + threadIdx.x / team;
     int U = 0;
     int64_t c = 0;
+    Seq s{};
     if (b < p.B) {
-      const Seq s = load_seq(p, b, lane == 0);
+      s = load_seq(p, b, lane == 0);
       U = num_units(p, s);
       for (int u = lane; u < U; u += team) c += unit_cost(p, s, u);
     }
@@ -259,7 +262,8 @@ __device__ void build_tables(const ChunkParams& p, int64_t* cost, int* units, in
     if (b < p.B && lane == 0) {
       cost[b + 1] = c * p.Hkv;
       units[b + 1] = U * p.Hkv;
-      if (U) atomicMax(most_cost, unit_tiles(p, load_seq(p, b, false), U - 1) + max(kUnitCost1, kUnitCost2));
+      if (seqs) seqs[b] = s;
+      if (U) atomicMax(most_cost, unit_tiles(p, s, U - 1) + max(kUnitCost1, kUnitCost2));
     }
   }
   __syncthreads();
@@ -329,7 +333,7 @@ __device__ Plan make_plan(const ChunkParams& p, const Tables& t, int most_cost, 
       const int b = find_seq(t.units, p.B, i);
       start = t.units[b];
       end = t.units[b + 1];
-      s = load_seq(p, b, false);
+      s = t.seqs ? t.seqs[b] : load_seq(p, b, false);
       U = num_units(p, s);
     }
     return unit_cost(p, s, U - 1 - (i - start) % U);
@@ -683,8 +687,8 @@ __device__ __forceinline__ void finish_rows(const ChunkParams& p, const Seg* sg,
 __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
   __shared__ __align__(8) int scratch[64];
   __shared__ int most_cost;
-  build_tables(p, p.plan_cost, p.plan_units, &most_cost, 1024);
-  const Plan pl = make_plan(p, Tables{p.plan_cost, p.plan_units}, most_cost, p.plan_share, scratch);
+  build_tables(p, p.plan_cost, p.plan_units, nullptr, &most_cost, 1024);
+  const Plan pl = make_plan(p, Tables{p.plan_cost, p.plan_units, nullptr}, most_cost, p.plan_share, scratch);
   if (threadIdx.x == 0) *p.plan = pl;
 }
 
@@ -762,8 +766,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the shares live where slot 0's Q tile goes later
     int64_t* share = reinterpret_cast<int64_t*>(smem + C::OFF_Q);
     int* scratch = reinterpret_cast<int*>(share + p.grid + 1);
-    build_tables(p, cost, units, scratch + 63, kThreads);
-    tab = Tables{cost, units};
+    Seq* seqs = reinterpret_cast<Seq*>(smem + C::OFF_Q + 8192);
+    build_tables(p, cost, units, seqs, scratch + 63, kThreads);
+    tab = Tables{cost, units, seqs};
     plan = make_plan(p, tab, scratch[63], share, scratch);
     begin = share[blockIdx.x];
     end = share[blockIdx.x + 1];
@@ -771,7 +776,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_async_smem();
   } else {
     grid_dep_wait();
-    tab = Tables{p.plan_cost, p.plan_units};
+    tab = Tables{p.plan_cost, p.plan_units, nullptr};
     plan = *p.plan;
     begin = p.plan_share[blockIdx.x];
     end = p.plan_share[blockIdx.x + 1];
@@ -943,16 +948,27 @@ __global__ void __launch_bounds__(kThreads, 1)
             constexpr int PR = D / 8, RS = 32 / PR;  // 16-byte pieces of a row, rows a step
             const int ch = lane % PR;
             unsigned char* vc = v + (ch >> 3) * C::HALF + (ch & 7) * 16;  // (the swizzle stays inside a row)
-#pragma unroll 4
-            for (int r = r0 + lane / PR; r < BN; r += RS) {
-              uint4* w = reinterpret_cast<uint4*>(vc + (r >> 3) * C::GROUP + (r & 7) * 128);
-              const uint4 y = *w;
-              if (r >= rows) {
-                *w = make_uint4(0, 0, 0, 0);
-              } else if (not_finite2<T>(y.x) | not_finite2<T>(y.y) | not_finite2<T>(y.z) | not_finite2<T>(y.w)) {
-                *w = make_uint4(without_not_finite2<T>(y.x), without_not_finite2<T>(y.y), without_not_finite2<T>(y.z),
-                                without_not_finite2<T>(y.w));
-                atomicOr(&sg->bad[j - j_edge][r >> 5], 1u << (r & 31));
+            auto at = [&](int r) { return reinterpret_cast<uint4*>(vc + (r >> 3) * C::GROUP + (r & 7) * 128); };
+            const int top = min(rows, BN), mid = max(r0, top);
+            for (int r = mid + lane / PR; r < BN; r += RS) *at(r) = make_uint4(0, 0, 0, 0);
+            for (int r = r0 + lane / PR; r < top; r += 2 * RS) {  // two pieces at a time, one look
+              uint4 y[2];
+              uint32_t any = 0;
+#pragma unroll
+              for (int u = 0; u < 2; ++u) y[u] = r + u * RS < top ? *at(r + u * RS) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+              for (int u = 0; u < 2; ++u)
+                any |= not_finite2<T>(y[u].x) | not_finite2<T>(y[u].y) | not_finite2<T>(y[u].z) | not_finite2<T>(y[u].w);
+              if (!any) continue;
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const uint32_t x = not_finite2<T>(y[u].x) | not_finite2<T>(y[u].y) | not_finite2<T>(y[u].z) |
+                                   not_finite2<T>(y[u].w);
+                if (!x) continue;
+                const int q = r + u * RS;
+                *at(q) = make_uint4(without_not_finite2<T>(y[u].x), without_not_finite2<T>(y[u].y),
+                                    without_not_finite2<T>(y[u].z), without_not_finite2<T>(y[u].w));
+                atomicOr(&sg->bad[j - j_edge][q >> 5], 1u << (q & 31));
                 sg->noted = 1;
               }
             }
