@@ -9,6 +9,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import struct
 import threading
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint, c_void_p
 
@@ -314,6 +315,62 @@ def check(rc: int) -> None:
     raise AktError(rc, msg)
 
 
+def _layout(cls, base=0):
+    """(offset, size, format letter) of every plain field of a ctypes struct, nested ones flattened."""
+    letters = {c_void_p: "Q", c_int64: "q", c_int32: "i", c_float: "f"}
+    for name, kind in cls._fields_:
+        at = base + getattr(cls, name).offset
+        if issubclass(kind, Structure):
+            yield from _layout(kind, at)
+        else:
+            yield at, ctypes.sizeof(kind), letters[kind]
+
+
+class Entry:
+    """A C entry point whose argument struct is packed in one call: ``entry(values, ...)`` with the
+    struct's fields in order (filling a ctypes struct field by field costs 4 to 6 us of a small call)."""
+
+    def __init__(self, name, struct_cls, *rest, restype=c_int):
+        self._what = name, struct_cls, rest, restype
+        at, fmt = 0, "="
+        for offset, size, letter in _layout(struct_cls):
+            fmt += "x" * (offset - at) + letter
+            at = offset + size
+        fmt += "x" * (ctypes.sizeof(struct_cls) - at)
+        self._pack = struct.Struct(fmt).pack
+        self._fn = None
+
+    def __call__(self, values, *rest):
+        if self._fn is None:
+            name, _, kinds, restype = self._what
+            self._fn = ctypes.CFUNCTYPE(restype, c_char_p, *kinds)((name, lib()))
+        return self._fn(self._pack(*values), *rest)
+
+
+def device_index(*tensors: torch.Tensor) -> int:
+    """The CUDA device that holds every tensor; raises as ``require_cuda`` does."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != index or index < 0:
+            require_cuda(*tensors)
+    return index
+
+
+def on_index(index: int):
+    """``on_device`` by number, without building a device."""
+    return _SAME_DEVICE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def list_i32(t: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
+    """``t`` as a contiguous int32 tensor on the device of ``like`` (itself where it is one)."""
+    if t.dtype is torch.int32 and t.get_device() == like.get_device() and t.is_contiguous():
+        return t
+    return t.to(device=like.device, dtype=torch.int32).contiguous()
+
+
 def dtype_code(t: torch.Tensor) -> int:
     if t.dtype == torch.float16:
         return AKT_FLOAT16
@@ -331,6 +388,11 @@ def stream_ptr(device: torch.device) -> int:
     if _raw_stream is not None:
         return _raw_stream(device.index if device.index is not None else torch.cuda.current_device())
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def raw_stream(index: int) -> int:
+    """torch's current stream on device ``index`` as a ``cudaStream_t`` value."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 def on_device(device: torch.device):

@@ -15,7 +15,6 @@ torch's current stream.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
@@ -23,58 +22,51 @@ import torch
 from . import _lib
 
 
-def _i32(t, dev):
-    return _lib.as_int32(t, dev).contiguous()
+_chunk = _lib.Entry("akt_chunk_paged", _lib.ChunkPagedArgs, _lib.c_void_p, _lib.c_size_t, _lib.c_void_p)
+_workspace = _lib.Entry("akt_chunk_paged_workspace_size", _lib.ChunkPagedArgs, restype=_lib.c_size_t)
 
 
 def chunk_paged_into(out, q, q_indptr, paged_kv_cache, kv_page_indptr, kv_page_indices, kv_last_page_len, causal=True,
                      softmax_scale=None, lse=None):
     """Write the attention of ``q [T, Hq, D]`` into ``out [T, Hq, D]`` and, with ``lse`` (fp32
     ``[T, Hq]``), each row's natural-log sum-exp of the scaled scores (-inf where no key is seen)."""
-    dev = _lib.require_cuda(q, paged_kv_cache, out)
+    index = _lib.device_index(q, paged_kv_cache, out)
     if q.dtype != paged_kv_cache.dtype or out.dtype != q.dtype:
         raise TypeError("q, paged_kv_cache and the output must share one dtype")
-    if q.dim() != 3 or out.shape != q.shape:
+    shape, pool = q.shape, paged_kv_cache.shape
+    if len(shape) != 3 or out.shape != shape:
         raise ValueError("q and the output must be [T, Hq, D]")
-    T, Hq, D = q.shape
-    if paged_kv_cache.dim() != 5 or paged_kv_cache.shape[1] != 2 or paged_kv_cache.shape[4] != D:
+    T, Hq, D = shape
+    if len(pool) != 5 or pool[1] != 2 or pool[4] != D:
         raise ValueError("paged_kv_cache must be [num_pages, 2, Hkv, page_size, D]")
+    lp = (0, 0, 0)
     if lse is not None:
-        _lib.require_cuda(q, lse)
-        if lse.dtype != torch.float32 or lse.shape != (T, Hq):
+        _lib.device_index(q, lse)
+        if lse.dtype is not torch.float32 or lse.shape != shape[:2]:
             raise ValueError("lse must be fp32 [T, Hq]")
-    at, indptr = _i32(q_indptr, dev), _i32(kv_page_indptr, dev)
-    indices, last = _i32(kv_page_indices, dev), _i32(kv_last_page_len, dev)
+        lp = (lse.data_ptr(), *lse.stride())
+    at, indptr = _lib.list_i32(q_indptr, q), _lib.list_i32(kv_page_indptr, q)
+    indices, last = _lib.list_i32(kv_page_indices, q), _lib.list_i32(kv_last_page_len, q)
     B = indptr.numel() - 1
     if at.numel() != B + 1 or last.numel() != B:
         raise ValueError("q_indptr and kv_page_indptr must have B+1 entries and kv_last_page_len B entries")
+    scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
+    tail = (indptr.data_ptr(), indices.data_ptr(), last.data_ptr(), indices.numel(), out.data_ptr(), *out.stride(), *lp,
+            B, Hq, pool[2], pool[3], D, bool(causal), _lib.dtype_code(q), scale)
     t = {"q": q, "cache": paged_kv_cache}
-    a = _lib.ChunkPagedArgs()
-    a.q_indptr, a.num_tokens = at.data_ptr(), T
-    a.kv_page_indptr, a.kv_page_indices, a.kv_last_page_len = indptr.data_ptr(), indices.data_ptr(), last.data_ptr()
-    a.num_page_entries = indices.numel()
-    a.out, (a.out_stride_token, a.out_stride_head, a.out_stride_dim) = out.data_ptr(), out.stride()
-    if lse is not None:
-        a.lse, (a.lse_stride_token, a.lse_stride_head) = lse.data_ptr(), lse.stride()
-    a.batch, a.num_qo_heads, a.num_kv_heads = B, Hq, paged_kv_cache.shape[2]
-    a.page_size, a.head_dim, a.causal = paged_kv_cache.shape[3], D, int(bool(causal))
-    a.dtype = _lib.dtype_code(q)
-    a.softmax_scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
-    L = _lib.lib()
 
     def call():
         qq, cache = t["q"], t["cache"]
-        a.q, (a.q_stride_token, a.q_stride_head, a.q_stride_dim) = qq.data_ptr(), qq.stride()
-        a.kv_cache, a.num_pages = cache.data_ptr(), cache.shape[0]
-        (a.kv_stride_page, a.kv_stride_kv, a.kv_stride_head, a.kv_stride_token, a.kv_stride_dim) = cache.stride()
-        ws = _lib.workspace(L.akt_chunk_paged_workspace_size(ctypes.byref(a)), dev)
-        return L.akt_chunk_paged(ctypes.byref(a), ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev))
+        values = (qq.data_ptr(), *qq.stride(), at.data_ptr(), T, cache.data_ptr(), *cache.stride(), pool[0], *tail)
+        size = _workspace(values)
+        ws = qq.new_empty((size + 1) // 2)
+        return _chunk(values, ws.data_ptr(), size, _lib.raw_stream(index))
 
     def contiguous():
         for k in t:
             t[k] = t[k].contiguous()
 
-    with _lib.on_device(dev):
+    with _lib.on_index(index):
         _lib.run_with_layout_retry(call, contiguous)
     return out
 
@@ -88,7 +80,7 @@ def flash_attention_chunk_paged(q, q_indptr, paged_kv_cache, kv_page_indptr, kv_
         the page table with the new tokens in it
     returns O: [T, Hq, D] in q.dtype; scale 1/sqrt(D) unless given
     """
-    O = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    O = q.new_empty(q.shape)
     return chunk_paged_into(O, q, q_indptr, paged_kv_cache, kv_page_indptr, kv_page_indices, kv_last_page_len, causal,
                             softmax_scale)
 
@@ -98,8 +90,7 @@ def flash_attention_chunk_paged_with_lse(q, q_indptr, paged_kv_cache, kv_page_in
     """``flash_attention_chunk_paged`` returning ``(O, LSE)`` with fp32 ``LSE [T, Hq]``, the
     row's natural-log sum-exp of the scaled scores (-inf where no key is seen), which merges
     with other partial results (``akt_lse_merge``)."""
-    O = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    O, lse = q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
     chunk_paged_into(O, q, q_indptr, paged_kv_cache, kv_page_indptr, kv_page_indices, kv_last_page_len, causal,
                      softmax_scale, lse)
     return O, lse

@@ -13,51 +13,52 @@ Runs on torch's current stream (sm_100a, ``csrc/pages.cu``).
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
 
 
-def _pool(cache) -> _lib.PagePool:
-    if cache.dim() not in (5, 6) or cache.shape[-4] != 2:
+_TYPES = (torch.float16, torch.bfloat16)
+_copy = _lib.Entry("akt_copy_kv_pages", _lib.PagePool, _lib.c_void_p, _lib.c_void_p, _lib.c_int64, _lib.c_void_p)
+_fork_size = _lib.Entry("akt_fork_paged_workspace_size", _lib.ForkPagedArgs, restype=_lib.c_size_t)
+_fork = _lib.Entry("akt_fork_paged", _lib.ForkPagedArgs, _lib.c_void_p, _lib.c_size_t, _lib.c_void_p)
+_compact_size = _lib.Entry("akt_compact_paged_workspace_size", _lib.CompactPagedArgs, restype=_lib.c_size_t)
+_compact = _lib.Entry("akt_compact_paged", _lib.CompactPagedArgs, _lib.c_void_p, _lib.c_size_t, _lib.c_void_p)
+
+
+def _pool(cache):
+    """The fields of ``akt_page_pool``."""
+    shape, stride = cache.shape, cache.stride()
+    if len(shape) not in (5, 6) or shape[-4] != 2:
         raise ValueError("paged_kv_cache must be [num_pages, 2, Hkv, page_size, D], with layers before it or not")
-    if cache.dtype not in (torch.float16, torch.bfloat16):
+    if cache.dtype not in _TYPES:
         raise TypeError(f"unsupported dtype {cache.dtype}: float16 or bfloat16 expected")
-    q = _lib.PagePool()
-    q.kv_cache = cache.data_ptr()
-    stride = cache.stride()
-    q.num_layers = cache.shape[0] if cache.dim() == 6 else 1
-    q.stride_layer = stride[0] if cache.dim() == 6 else 0
-    q.stride_page, q.stride_kv, q.stride_head, q.stride_token, q.stride_dim = stride[-5:]
-    q.num_pages, q.num_kv_heads, q.page_size, q.head_dim = cache.shape[-5], *cache.shape[-3:]
-    return q
+    layers, step = (shape[0], stride[0]) if len(shape) == 6 else (1, 0)
+    return (cache.data_ptr(), step, *stride[-5:], shape[-5], layers, *shape[-3:])
 
 
-def _i32(t, dev):
-    return _lib.as_int32(t, dev).contiguous()
-
-
-def _reserved(mask, num_pages, dev):
+def _reserved(mask, num_pages, like):
     if mask is None:
         return None
-    if mask.dtype not in (torch.bool, torch.uint8) or mask.device != dev or mask.shape != (num_pages,):
+    if mask.dtype not in (torch.bool, torch.uint8) or mask.device != like.device or mask.shape != (num_pages,):
         raise ValueError("reserved must be a bool (or uint8) mask [num_pages] on the pool's device")
     return mask.contiguous()
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def copy_kv_pages(paged_kv_cache, src_pages, dst_pages):
     """Copy page ``src_pages[i]`` to page ``dst_pages[i]`` in every layer, in place.  No
     destination may be the source or destination of another copy."""
-    dev = _lib.require_cuda(paged_kv_cache)
+    index = _lib.device_index(paged_kv_cache)
     pool = _pool(paged_kv_cache)
-    src, dst = _i32(src_pages, dev), _i32(dst_pages, dev)
+    src, dst = _lib.list_i32(src_pages, paged_kv_cache), _lib.list_i32(dst_pages, paged_kv_cache)
     if src.dim() != 1 or src.shape != dst.shape:
         raise ValueError("src_pages and dst_pages must be lists of the same length")
-    with _lib.on_device(dev):
-        _lib.check(_lib.lib().akt_copy_kv_pages(ctypes.byref(pool), src.data_ptr(), dst.data_ptr(), src.numel(),
-                                                _lib.stream_ptr(dev)))
+    with _lib.on_index(index):
+        _lib.check(_copy(pool, src.data_ptr(), dst.data_ptr(), src.numel(), _lib.raw_stream(index)))
     return paged_kv_cache
 
 
@@ -77,32 +78,31 @@ def fork_paged_kv_cache(paged_kv_cache, kv_page_indptr, kv_page_indices, kv_last
     returns (kv_page_indptr [num_children + 1], kv_page_indices [max_entries],
         kv_last_page_len [num_children]), int32
     """
-    dev = _lib.require_cuda(paged_kv_cache)
-    a = _lib.ForkPagedArgs()
-    a.pool = _pool(paged_kv_cache)
-    indptr, indices, last = _i32(kv_page_indptr, dev), _i32(kv_page_indices, dev), _i32(kv_last_page_len, dev)
-    par = _i32(parents, dev)
+    index = _lib.device_index(paged_kv_cache)
+    pool = _pool(paged_kv_cache)
+    indptr, indices = _lib.list_i32(kv_page_indptr, paged_kv_cache), _lib.list_i32(kv_page_indices, paged_kv_cache)
+    last, par = _lib.list_i32(kv_last_page_len, paged_kv_cache), _lib.list_i32(parents, paged_kv_cache)
     B, F = indptr.numel() - 1, par.numel()
     if B < 0 or last.numel() != B or par.dim() != 1:
         raise ValueError("kv_page_indptr must have B+1 entries, kv_last_page_len B entries and parents be a list")
-    mask = _reserved(reserved, a.pool.num_pages, dev)
+    mask = _reserved(reserved, pool[7], paged_kv_cache)
     if max_entries is None:
         at = par.long().clamp(0, max(B - 1, 0))
         max_entries = int((indptr[at + 1] - indptr[at]).sum()) if B and F else 0
     if max_entries < 0:
         raise ValueError("max_entries must not be negative")
-    i32 = dict(dtype=torch.int32, device=dev)
-    out = (torch.empty(F + 1, **i32), torch.empty(max_entries, **i32), torch.empty(F, **i32))
-    a.kv_page_indptr, a.kv_page_indices, a.kv_last_page_len = indptr.data_ptr(), indices.data_ptr(), last.data_ptr()
-    a.num_page_entries = indices.numel()
-    a.parents, a.reserved = par.data_ptr(), mask.data_ptr() if mask is not None else None
-    a.out_indptr, a.out_indices, a.out_last_page_len = (t.data_ptr() for t in out)
-    a.max_entries, a.batch, a.num_children = max_entries, B, F
-    L = _lib.lib()
-    with _lib.on_device(dev):
-        ws = _lib.workspace(L.akt_fork_paged_workspace_size(ctypes.byref(a)), dev)
-        _lib.check(L.akt_fork_paged(ctypes.byref(a), ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev)))
-    return out
+    head = (*pool, indptr.data_ptr(), indices.data_ptr(), last.data_ptr(), indices.numel(), par.data_ptr(), _ptr(mask))
+    size = _fork_size((*head, 0, 0, 0, max_entries, B, F))
+    # one allocation: the workspace (a multiple of 16 bytes), then the new table
+    ws, out_indptr, out_indices, out_last = torch.empty(
+        size // 4 + 2 * F + 1 + max_entries, dtype=torch.int32, device=paged_kv_cache.device).split_with_sizes(
+            (size // 4, F + 1, max_entries, F))
+    with _lib.on_index(index):
+        rc = _fork((*head, out_indptr.data_ptr(), out_indices.data_ptr(), out_last.data_ptr(), max_entries, B, F),
+                   ws.data_ptr(), size, _lib.raw_stream(index))
+        if rc:
+            _lib.check(rc)
+    return out_indptr, out_indices, out_last
 
 
 def compact_paged_kv_cache(paged_kv_cache, kv_page_indices, reserved=None):
@@ -113,37 +113,36 @@ def compact_paged_kv_cache(paged_kv_cache, kv_page_indices, reserved=None):
     on the device) is one past the highest page then in use or reserved.  ``kv_page_indptr``
     and ``kv_last_page_len`` stay as they are.
     """
-    dev = _lib.require_cuda(paged_kv_cache)
-    a = _lib.CompactPagedArgs()
-    a.pool = _pool(paged_kv_cache)
-    indices = _i32(kv_page_indices, dev)
+    index = _lib.device_index(paged_kv_cache)
+    pool = _pool(paged_kv_cache)
+    indices = _lib.list_i32(kv_page_indices, paged_kv_cache)
     if indices.dim() != 1:
         raise ValueError("kv_page_indices must be a list")
-    mask = _reserved(reserved, a.pool.num_pages, dev)
-    out = torch.empty_like(indices)
-    used = torch.empty((), dtype=torch.int32, device=dev)
-    a.kv_page_indices, a.num_page_entries = indices.data_ptr(), indices.numel()
-    a.reserved = mask.data_ptr() if mask is not None else None
-    a.out_indices, a.pages_used = out.data_ptr(), used.data_ptr()
-    L = _lib.lib()
-    with _lib.on_device(dev):
-        ws = _lib.workspace(L.akt_compact_paged_workspace_size(ctypes.byref(a)), dev)
-        _lib.check(L.akt_compact_paged(ctypes.byref(a), ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev)))
-    return out, used
+    n = indices.shape[0]
+    mask = _reserved(reserved, pool[7], paged_kv_cache)
+    head = (*pool, indices.data_ptr(), n, _ptr(mask))
+    size = _compact_size((*head, 0, 0))
+    # one allocation: the workspace (a multiple of 16 bytes), the new index array and the count
+    ws, out, used = torch.empty(size // 4 + n + 1, dtype=torch.int32, device=indices.device).split_with_sizes(
+        (size // 4, n, 1))
+    with _lib.on_index(index):
+        rc = _compact((*head, out.data_ptr(), used.data_ptr()), ws.data_ptr(), size, _lib.raw_stream(index))
+        if rc:
+            _lib.check(rc)
+    return out, used.view(())
 
 
 def free_kv_pages(num_pages, kv_page_indices, reserved=None):
     """The pages that the table does not name, ascending: ``(pages [num_pages] int32, -1 past
     their count; count, int32 scalar on the device)``."""
-    dev = _lib.require_cuda(kv_page_indices)
-    indices = _i32(kv_page_indices, dev)
-    mask = _reserved(reserved, num_pages, dev)
-    out = torch.empty(num_pages, dtype=torch.int32, device=dev)
-    count = torch.empty((), dtype=torch.int32, device=dev)
+    index = _lib.device_index(kv_page_indices)
+    indices = _lib.list_i32(kv_page_indices, kv_page_indices)
+    mask = _reserved(reserved, num_pages, indices)
+    i32 = dict(dtype=torch.int32, device=indices.device)
+    out, count = torch.empty(num_pages, **i32), torch.empty((), **i32)
     L = _lib.lib()
-    with _lib.on_device(dev):
-        ws = _lib.workspace(L.akt_free_kv_pages_workspace_size(num_pages), dev)
-        _lib.check(L.akt_free_kv_pages(indices.data_ptr(), indices.numel(),
-                                       mask.data_ptr() if mask is not None else None, num_pages, out.data_ptr(),
-                                       count.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_ptr(dev)))
+    with _lib.on_index(index):
+        ws = _lib.workspace(L.akt_free_kv_pages_workspace_size(num_pages), indices.device)
+        _lib.check(L.akt_free_kv_pages(indices.data_ptr(), indices.numel(), _ptr(mask), num_pages, out.data_ptr(),
+                                       count.data_ptr(), ws.data_ptr(), ws.numel(), _lib.raw_stream(index)))
     return out, count

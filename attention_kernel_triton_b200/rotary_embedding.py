@@ -13,7 +13,6 @@ current stream.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
@@ -87,8 +86,12 @@ def rotary_cos_sin(max_positions, rotary_dim, base=10000.0, scaling=None, device
     return torch.cat((angle.cos() * factor, angle.sin() * factor), 1).float().to(device)
 
 
-def _check_table(cos_sin, D, dev):
-    if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32 or cos_sin.device != dev:
+_rotary = _lib.Entry("akt_rotary", _lib.RotaryArgs, _lib.c_void_p)
+_append_rotary = _lib.Entry("akt_append_rotary_paged_kv", _lib.AppendRotaryArgs, _lib.c_void_p)
+
+
+def _check_table(cos_sin, D):
+    if cos_sin.dim() != 2 or cos_sin.dtype is not torch.float32:
         raise ValueError("cos_sin must be fp32 [max_positions, rotary_dim] on the tensors' device")
     R = cos_sin.shape[1]
     if R % 2 or R > D:
@@ -103,42 +106,42 @@ def _unit(x):
 def rotary_into(q_out, k_out, q, k, cos_sin, positions, interleaved=False, inverse=False):
     """Rotate ``q [T, Hq, D]`` into ``q_out`` and, unless ``k`` is None, ``k [T, Hkv, D]``
     into ``k_out`` (either may be its input: in place)."""
-    ts = (q, q_out) if k is None else (q, q_out, k, k_out)
-    dev = _lib.require_cuda(*ts, cos_sin)
-    for t in ts:
-        if t.dim() != 3 or t.shape[0] != q.shape[0] or t.shape[2] != q.shape[2]:
-            raise ValueError("tensors must be [tokens, heads, head_dim] with the same tokens and head_dim")
-        if t.dtype != q.dtype:
+    shape = q.shape
+    if len(shape) != 3 or q_out.shape != shape:
+        raise ValueError("tensors must be [tokens, heads, head_dim], an output of its input's shape")
+    T, Hq, D = shape
+    if k is None:
+        index = _lib.device_index(q, q_out, cos_sin)
+        kp, Hkv = (0, 0, 0, 0, 0, 0, 0, 0), 0
+    else:
+        index = _lib.device_index(q, q_out, k, k_out, cos_sin)
+        ks = k.shape
+        if len(ks) != 3 or ks[0] != T or ks[2] != D or k_out.shape != ks:
+            raise ValueError("q and k must be [tokens, heads, head_dim] with the same tokens and head_dim")
+        if not (k.dtype == k_out.dtype == q.dtype):
             raise TypeError("q, k and the outputs must share one dtype")
-    if q_out.shape != q.shape or (k is not None and k_out.shape != k.shape):
-        raise ValueError("an output must have its input's shape")
-    T, Hq, D = q.shape
-    table = _check_table(cos_sin, D, dev)
-    pos = _lib.as_int32(positions, dev)
-    if pos.dim() != 1 or pos.numel() != T:
-        raise ValueError("positions must hold one position per token")
-    pos = pos.contiguous()
-    a = _lib.RotaryArgs()
-    q = _unit(q)
-    a.q, (a.q_stride_token, a.q_stride_head, a.q_stride_dim) = q.data_ptr(), q.stride()
-    a.q_out, (a.q_out_stride_token, a.q_out_stride_head, a.q_out_stride_dim) = q_out.data_ptr(), q_out.stride()
-    if k is not None:
         k = _unit(k)
-        a.k, (a.k_stride_token, a.k_stride_head, a.k_stride_dim) = k.data_ptr(), k.stride()
-        a.k_out, (a.k_out_stride_token, a.k_out_stride_head, a.k_out_stride_dim) = k_out.data_ptr(), k_out.stride()
-        a.num_kv_heads = k.shape[1]
-    a.cos_sin, a.cos_sin_stride, a.max_positions = table.data_ptr(), table.stride(0), table.shape[0]
-    a.positions, a.num_tokens = pos.data_ptr(), T
-    a.num_qo_heads, a.head_dim, a.rotary_dim = Hq, D, table.shape[1]
-    a.interleaved, a.inverse, a.dtype = int(bool(interleaved)), int(bool(inverse)), _lib.dtype_code(q)
-    with _lib.on_device(dev):
-        _lib.check(_lib.lib().akt_rotary(ctypes.byref(a), _lib.stream_ptr(dev)))
+        kp, Hkv = (k.data_ptr(), *k.stride(), k_out.data_ptr(), *k_out.stride()), ks[1]
+    if q_out.dtype != q.dtype:
+        raise TypeError("q, k and the outputs must share one dtype")
+    table = _check_table(cos_sin, D)
+    pos = _lib.list_i32(positions, q)
+    if pos.dim() != 1 or pos.shape[0] != T:
+        raise ValueError("positions must hold one position per token")
+    q = _unit(q)
+    top, R = table.shape
+    values = (q.data_ptr(), *q.stride(), *kp[:4], q_out.data_ptr(), *q_out.stride(), *kp[4:], table.data_ptr(),
+              table.stride(0), top, pos.data_ptr(), T, Hq, Hkv, D, R, bool(interleaved), bool(inverse),
+              _lib.dtype_code(q))
+    with _lib.on_index(index):
+        rc = _rotary(values, _lib.raw_stream(index))
+        if rc:
+            _lib.check(rc)
     return q_out, k_out
 
 
 def _forward(q, k, cos_sin, positions, interleaved, inverse):
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    q_out, k_out = q.new_empty(q.shape), None if k is None else k.new_empty(k.shape)
     return rotary_into(q_out, k_out, q, k, cos_sin, positions, interleaved, inverse)
 
 
@@ -202,49 +205,44 @@ def append_rotary_paged_kv_cache(paged_kv_cache, q, append_k, append_v, append_i
     describes the sequences after the append.  One pass: the rotated keys are never stored
     outside the pool.
     """
-    dev = _lib.require_cuda(paged_kv_cache, append_k, append_v, cos_sin)
-    if not (paged_kv_cache.dtype == append_k.dtype == append_v.dtype):
+    index = _lib.device_index(paged_kv_cache, append_k, append_v, cos_sin)
+    dtype = paged_kv_cache.dtype
+    if append_k.dtype != dtype or append_v.dtype != dtype:
         raise TypeError("the pool and the appended rows must share one dtype")
-    if paged_kv_cache.dim() != 5 or paged_kv_cache.shape[1] != 2:
+    pool = paged_kv_cache.shape
+    if len(pool) != 5 or pool[1] != 2:
         raise ValueError("paged_kv_cache must be [num_pages, 2, Hkv, page_size, D]")
-    _, _, Hkv, P, D = paged_kv_cache.shape
-    if append_k.dim() != 3 or append_k.shape[1:] != (Hkv, D) or append_v.shape != append_k.shape:
+    N, _, Hkv, P, D = pool
+    shape = append_k.shape
+    if len(shape) != 3 or shape[1] != Hkv or shape[2] != D or append_v.shape != shape:
         raise ValueError("append_k and append_v must be [num_append, Hkv, D]")
-    table = _check_table(cos_sin, D, dev)
-    indptr = _lib.as_int32(kv_page_indptr, dev).contiguous()
-    indices = _lib.as_int32(kv_page_indices, dev).contiguous()
-    last = _lib.as_int32(kv_last_page_len, dev).contiguous()
-    app = _lib.as_int32(append_indptr, dev).contiguous()
+    T = shape[0]
+    table = _check_table(cos_sin, D)
+    indptr = _lib.list_i32(kv_page_indptr, append_k)
+    indices = _lib.list_i32(kv_page_indices, append_k)
+    last = _lib.list_i32(kv_last_page_len, append_k)
+    app = _lib.list_i32(append_indptr, append_k)
     B = indptr.numel() - 1
     if app.numel() != B + 1 or last.numel() != B:
         raise ValueError("append_indptr and kv_page_indptr must have B+1 entries and kv_last_page_len B entries")
     k, v = _unit(append_k), _unit(append_v)
-    x = _lib.AppendRotaryArgs()
-    a = x.append
-    a.kv_cache = paged_kv_cache.data_ptr()
-    (a.kv_stride_page, a.kv_stride_kv, a.kv_stride_head, a.kv_stride_token, a.kv_stride_dim) = paged_kv_cache.stride()
-    a.num_pages = paged_kv_cache.shape[0]
-    a.kv_page_indptr, a.kv_page_indices, a.kv_last_page_len = indptr.data_ptr(), indices.data_ptr(), last.data_ptr()
-    a.num_page_entries = indices.numel()
-    a.append_k, (a.k_stride_token, a.k_stride_head, a.k_stride_dim) = k.data_ptr(), k.stride()
-    a.append_v, (a.v_stride_token, a.v_stride_head, a.v_stride_dim) = v.data_ptr(), v.stride()
-    a.append_indptr, a.num_append = app.data_ptr(), k.shape[0]
-    a.batch, a.num_kv_heads, a.page_size, a.head_dim = B, Hkv, P, D
-    a.dtype = _lib.dtype_code(k)
-    q_out = None
+    q_out, qp, Hq = None, (0, 0, 0, 0, 0, 0, 0, 0), 0
     if q is not None:
-        _lib.require_cuda(paged_kv_cache, q)
-        if q.dtype != append_k.dtype:
+        _lib.device_index(paged_kv_cache, q)
+        if q.dtype != dtype:
             raise TypeError("the pool and the appended rows must share one dtype")
-        if q.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != D:
+        if q.dim() != 3 or q.shape[0] != T or q.shape[2] != D:
             raise ValueError("q must be [num_append, Hq, D]")
         q = _unit(q)
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        x.q, (x.q_stride_token, x.q_stride_head, x.q_stride_dim) = q.data_ptr(), q.stride()
-        x.q_out, (x.q_out_stride_token, x.q_out_stride_head, x.q_out_stride_dim) = q_out.data_ptr(), q_out.stride()
-        x.num_qo_heads = q.shape[1]
-    x.cos_sin, x.cos_sin_stride, x.max_positions = table.data_ptr(), table.stride(0), table.shape[0]
-    x.rotary_dim, x.interleaved = table.shape[1], int(bool(interleaved))
-    with _lib.on_device(dev):
-        _lib.check(_lib.lib().akt_append_rotary_paged_kv(ctypes.byref(x), _lib.stream_ptr(dev)))
+        Hq = q.shape[1]
+        q_out = q.new_empty(q.shape)
+        qp = (q.data_ptr(), *q.stride(), q_out.data_ptr(), *q_out.stride())
+    top, R = table.shape
+    values = (paged_kv_cache.data_ptr(), *paged_kv_cache.stride(), N, indptr.data_ptr(), indices.data_ptr(),
+              last.data_ptr(), indices.numel(), k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(), app.data_ptr(), T,
+              B, Hkv, P, D, _lib.dtype_code(k), *qp, table.data_ptr(), table.stride(0), top, Hq, R, bool(interleaved))
+    with _lib.on_index(index):
+        rc = _append_rotary(values, _lib.raw_stream(index))
+        if rc:
+            _lib.check(rc)
     return q_out
