@@ -9,12 +9,13 @@
 // rotation is orthogonal, so its gradient is the turn by -s (inverse).
 //
 // Byte work: each value is read once and written once.  A head is cut into
-// pieces of W values (half layout: W values and their W partners), a thread
-// takes one piece, and the pieces of a token's q, k (and v) rows are numbered
-// one after the other so that neighbouring threads touch neighbouring bytes.
-// The table's values come through L1 (a token's heads share its row).  W is
-// the widest of 8 (16-byte accesses), 4, 2 and 1 that divides the pair count,
-// the copied part and every stride.
+// pieces of W values (half layout: W values and their W partners); a lane keeps
+// one piece number, so it loads that piece's cosines and sines once per token and
+// walks the heads by adding a stride.  (Numbering all pieces and dividing for each
+// took 150 instructions a piece and was bound by them: 75 us against 64 for an
+// append of 13K tokens, whose bytes need 49 at the measured copy rate.)  W is the
+// widest of 8 (16-byte accesses), 4, 2 and 1 that divides the pair count, the
+// copied part and every stride.
 #include "common.cuh"
 #include "profile.cuh"
 
@@ -48,12 +49,7 @@ struct RotaryParams {
   int64_t num_tokens;
   int Hq, Hkv, R, D;
   float sign;         // +1, or -1 for the inverse
-  FastDiv div_head;   // pieces of one rotated head
-  FastDiv div_vrow;   // pieces of one copied v row
-  int turned;         // rotating pieces per head; the head's remaining pieces are copied
-  int n_rot;          // pieces of the q and k heads of a token
-  int n_tok;          // pieces of a token in all (append: with v)
-  int tokens_per_cta;
+  int warps_per_token;
 };
 
 template <typename T, int W>
@@ -66,29 +62,6 @@ template <typename T>
 struct Vec<T, 2> { using type = uint32_t; };
 template <typename T>
 struct Vec<T, 1> { using type = uint16_t; };
-
-// W values at p (aligned to W values) as floats, and back
-template <typename T, int W>
-__device__ __forceinline__ void load_row(const char* p, float (&x)[W]) {
-  union {
-    typename Vec<T, W>::type v;
-    T e[W];
-  } u;
-  u.v = *reinterpret_cast<const typename Vec<T, W>::type*>(p);
-#pragma unroll
-  for (int i = 0; i < W; ++i) x[i] = Elem<T>::to_float(u.e[i]);
-}
-
-template <typename T, int W>
-__device__ __forceinline__ void store_row(char* p, const float (&x)[W]) {
-  union {
-    typename Vec<T, W>::type v;
-    T e[W];
-  } u;
-#pragma unroll
-  for (int i = 0; i < W; ++i) u.e[i] = Elem<T>::from_float(x[i]);
-  *reinterpret_cast<typename Vec<T, W>::type*>(p) = u.v;
-}
 
 // N consecutive floats of the table; 16-byte loads when N is a multiple of 4
 // (the host has checked the alignment)
@@ -106,60 +79,69 @@ __device__ __forceinline__ void load_angles(const float* p, float (&x)[N]) {
   }
 }
 
-// One rotating piece: pairs of `src` turned into `dst` (the same row offsets);
-// cs is the token's table row.  INTER with W == 1 takes one pair in two scalar
-// accesses, so a piece holds max(W / 2, 1) pairs there and W pairs otherwise.
-template <typename T, int W, bool INTER>
-__device__ __forceinline__ void turn_piece(const char* src, char* dst, int c, int R, const float* cs, float sign) {
-  if constexpr (INTER) {
-    constexpr int NP = W >= 2 ? W / 2 : 1;
-    constexpr int NV = 2 * NP;
-    float x[NV], y[NV], co[NP], si[NP];
-    const int64_t at = (int64_t)c * NV * 2;
-    if constexpr (W >= 2) {
-      load_row<T, NV>(src + at, x);
-    } else {
-      float t[1];
-      load_row<T, 1>(src + at, t); x[0] = t[0];
-      load_row<T, 1>(src + at + 2, t); x[1] = t[0];
-    }
-    load_angles<NP>(cs + c * NP, co);
-    load_angles<NP>(cs + R / 2 + c * NP, si);
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const float s = sign * si[i];
-      y[2 * i] = x[2 * i] * co[i] - x[2 * i + 1] * s;
-      y[2 * i + 1] = x[2 * i + 1] * co[i] + x[2 * i] * s;
-    }
-    if constexpr (W >= 2) {
-      store_row<T, NV>(dst + at, y);
-    } else {
-      const float y0[1] = {y[0]}, y1[1] = {y[1]};
-      store_row<T, 1>(dst + at, y0);
-      store_row<T, 1>(dst + at + 2, y1);
-    }
-  } else {
-    float a[W], b[W], ya[W], yb[W], co[W], si[W];
-    const int64_t at = (int64_t)c * W * 2, half = (int64_t)R;  // R/2 values of two bytes
-    load_row<T, W>(src + at, a);
-    load_row<T, W>(src + at + half, b);
-    load_angles<W>(cs + c * W, co);
-    load_angles<W>(cs + R / 2 + c * W, si);
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      const float s = sign * si[i];
-      ya[i] = a[i] * co[i] - b[i] * s;
-      yb[i] = b[i] * co[i] + a[i] * s;
-    }
-    store_row<T, W>(dst + at, ya);
-    store_row<T, W>(dst + at + half, yb);
-  }
-}
-
+// A piece as loaded: W values, and for a rotating piece of the half layout (or a
+// single interleaved pair) W more.
 template <typename T, int W>
-__device__ __forceinline__ void copy_piece(const char* src, char* dst) {
-  *reinterpret_cast<typename Vec<T, W>::type*>(dst) = *reinterpret_cast<const typename Vec<T, W>::type*>(src);
-}
+struct Raw {
+  typename Vec<T, W>::type a, b;
+};
+
+template <typename T, int W, bool INTER>
+struct PieceOp {
+  using V = typename Vec<T, W>::type;
+  static constexpr int NP = INTER ? (W >= 2 ? W / 2 : 1) : W;  // pairs
+  static constexpr bool TWO = !INTER || W == 1;                // a rotating piece takes two accesses
+  // byte offsets of the two accesses of rotating piece c
+  static __device__ __forceinline__ int64_t at_a(int c) { return (int64_t)c * (INTER ? 2 * NP : W) * 2; }
+  static __device__ __forceinline__ int64_t gap(int R) { return INTER ? 2 : (int64_t)R; }  // R / 2 values of two bytes
+
+  static __device__ __forceinline__ V load(const char* p) { return *reinterpret_cast<const V*>(p); }
+  static __device__ __forceinline__ void store(char* p, V v) { *reinterpret_cast<V*>(p) = v; }
+
+  static __device__ __forceinline__ void unpack(V v, float (&x)[W]) {
+    union {
+      V v;
+      T e[W];
+    } u;
+    u.v = v;
+#pragma unroll
+    for (int i = 0; i < W; ++i) x[i] = Elem<T>::to_float(u.e[i]);
+  }
+  static __device__ __forceinline__ V pack(const float (&x)[W]) {
+    union {
+      V v;
+      T e[W];
+    } u;
+#pragma unroll
+    for (int i = 0; i < W; ++i) u.e[i] = Elem<T>::from_float(x[i]);
+    return u.v;
+  }
+
+  // the piece's pairs turned by the angles' cosines and (signed) sines
+  static __device__ __forceinline__ void turn(Raw<T, W>& r, const float (&co)[NP], const float (&si)[NP]) {
+    float a[W], b[W];
+    unpack(r.a, a);
+    if constexpr (TWO) {
+      unpack(r.b, b);
+      float ya[W], yb[W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        ya[i] = a[i] * co[i] - b[i] * si[i];
+        yb[i] = b[i] * co[i] + a[i] * si[i];
+      }
+      r.a = pack(ya);
+      r.b = pack(yb);
+    } else {
+      float y[W];
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        y[2 * i] = a[2 * i] * co[i] - a[2 * i + 1] * si[i];
+        y[2 * i + 1] = a[2 * i + 1] * co[i] + a[2 * i] * si[i];
+      }
+      r.a = pack(y);
+    }
+  }
+};
 
 // Position and pool row (K half) of appended token `tok`, by one warp: a
 // search with 32 pivots a round for the sequence (two rounds up to 1024
@@ -187,115 +169,161 @@ __device__ __forceinline__ void place_token(const RotaryParams& p, int64_t tok, 
   const int last = __shfl_sync(0xffffffffu, v, 4);
   pos = -1;
   dst = nullptr;
-  if (lane) return;
+  unsigned bad = 0;
   if (a0 > tok || tok >= a1 || s < 0 || e <= s || e > p.num_page_entries) {
-    record_status(kStatusBadIndptr);
-    return;
+    bad = kStatusBadIndptr;
+  } else {
+    const int64_t len = (int64_t)(e - s - 1) * p.P + last;
+    const int64_t at = len - (a1 - a0) + (tok - a0);
+    if (last < 1 || last > p.P || at < 0 || at >= len || at >= p.max_positions) {
+      bad = kStatusBadToken;
+    } else {
+      const int entry = (int)(at / p.P), page = __ldg(p.indices + s + entry);
+      if (page < 0 || page >= p.num_pages) {
+        bad = kStatusBadPage;
+      } else {
+        pos = at;
+        dst = p.cache + (int64_t)page * p.s_page + (at - (int64_t)entry * p.P) * p.s_tok;
+      }
+    }
   }
-  const int64_t len = (int64_t)(e - s - 1) * p.P + last;
-  const int64_t at = len - (a1 - a0) + (tok - a0);
-  if (last < 1 || last > p.P || at < 0 || at >= len || at >= p.max_positions) {
-    record_status(kStatusBadToken);
-    return;
-  }
-  const int page = __ldg(p.indices + s + at / p.P);
-  if (page < 0 || page >= p.num_pages) {
-    record_status(kStatusBadPage);
-    return;
-  }
-  pos = at;
-  dst = p.cache + (int64_t)page * p.s_page + (at % p.P) * p.s_tok;
+  if (bad && lane == 0) record_status(bad);
 }
 
-constexpr int kThreads = 256;
-constexpr int kMaxTokens = 8;  // tokens of one CTA, one warp each while they are placed
+constexpr int kThreads = 128, kWarps = kThreads / 32;
 
+// How a warp's lanes share rows of n pieces: lane's piece and first row, and the
+// steps (n <= 32: several rows at a time; more: the pieces of one row in turns).
+struct Lanes {
+  int c, row, c_step, rows;
+  __device__ __forceinline__ Lanes(int n, int lane) {
+    if (n <= 32) {
+      rows = 32 / n;
+      row = lane / n;
+      c = row < rows ? lane - row * n : n;  // the last lanes may have none
+      c_step = n;
+    } else {
+      rows = 1;
+      row = 0;
+      c = lane;
+      c_step = 32;
+    }
+  }
+};
+
+// One or several warps per token, each with every warps_per_token-th group of
+// rows.  The first rows are asked for before the token is placed (a chain of four
+// dependent lookups) and its angles are read, since they need neither.
 template <typename T, int W, bool INTER, bool APPEND>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) {
-  __shared__ int64_t pos_s[kMaxTokens];
-  __shared__ char* dst_s[kMaxTokens];
-  const int64_t t0 = (int64_t)blockIdx.x * p.tokens_per_cta;
-  const int nt = (int)min((int64_t)p.tokens_per_cta, p.num_tokens - t0);
+  using Op = PieceOp<T, W, INTER>;
+  constexpr int U = 2;  // rows in flight per lane, and as many on their way (1: 74 us, 2: 64, 4: 74)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp < nt) {
-    int64_t pos;
-    char* dst = nullptr;
-    if constexpr (APPEND) {
-      place_token(p, t0 + warp, lane, pos, dst);
-    } else {
-      pos = __ldg(p.positions + t0 + warp);
-      if (pos < 0 || pos >= p.max_positions) {
-        if (lane == 0) record_status(kStatusBadToken);
-        pos = -1;
+  const int64_t tok = (int64_t)blockIdx.x * (kWarps / p.warps_per_token) + warp / p.warps_per_token;
+  if (tok >= p.num_tokens) return;
+  const int part = warp % p.warps_per_token, heads = p.Hq + p.Hkv, turned = p.R / 2 / Op::NP;
+  const char* q = p.q + tok * p.q_tok;
+  const char* k = p.k + tok * p.k_tok;
+  auto src_of = [&](int h) { return h < p.Hq ? q + h * p.q_head : k + (h - p.Hq) * p.k_head; };
+  Raw<T, W> raw[U];
+  const Lanes lt(max(turned, 1), lane);
+  const int h0 = part * lt.rows + lt.row, h_step = p.warps_per_token * lt.rows;
+  auto fetch = [&](int h, int c) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (h + u * h_step < heads) {
+        const char* src = src_of(h + u * h_step) + Op::at_a(c);
+        raw[u].a = Op::load(src);
+        if constexpr (Op::TWO) raw[u].b = Op::load(src + Op::gap(p.R));
       }
-    }
-    if (lane == 0) {
-      pos_s[warp] = pos;
-      dst_s[warp] = dst;
+  };
+  const bool some = lt.c < turned;
+  if (some) fetch(h0, lt.c);
+  int64_t pos;
+  char* row = nullptr;
+  if constexpr (APPEND) {
+    place_token(p, tok, lane, pos, row);
+  } else {
+    pos = __ldg(p.positions + tok);
+    if (pos < 0 || pos >= p.max_positions) {
+      if (lane == 0) record_status(kStatusBadToken);
+      pos = -1;
     }
   }
-  __syncthreads();
-  for (int i = 0; i < nt; ++i) {
-    const int64_t tok = t0 + i, pos = pos_s[i];
-    char* row = dst_s[i];
-    const float* cs = p.cos_sin + pos * p.cs_stride;
-    for (int w = threadIdx.x; w < p.n_tok; w += kThreads) {
-      if (APPEND && w >= p.n_rot) {  // v rows: copied
-        if (pos < 0) continue;
-        const int r = w - p.n_rot, h = (int)fdiv((uint32_t)r, p.div_vrow), c = r - h * (int)p.div_vrow.d;
-        copy_piece<T, W>(p.v + tok * p.v_tok + h * p.v_head + (int64_t)c * W * 2,
-                         row + p.s_kv + h * p.s_head + (int64_t)c * W * 2);
-        continue;
-      }
-      const int h = (int)fdiv((uint32_t)w, p.div_head);
-      int c = w - h * (int)p.div_head.d;
-      const bool is_q = h < p.Hq;
-      const int hk = h - p.Hq;
-      const char* src = is_q ? p.q + tok * p.q_tok + h * p.q_head : p.k + tok * p.k_tok + hk * p.k_head;
-      char* dst = is_q ? p.q_out + tok * p.qo_tok + h * p.qo_head
-                       : (APPEND ? row + hk * p.s_head : p.k_out + tok * p.ko_tok + hk * p.ko_head);
-      if (pos < 0) {
-        if (APPEND && !is_q) continue;
-        // no position: a row of zeros (every piece clears what it would write)
-        const float z[W] = {};
-        if (c >= p.turned) {
-          store_row<T, W>(dst + (int64_t)p.R * 2 + (int64_t)(c - p.turned) * W * 2, z);
-        } else if (INTER) {
-          constexpr int NV = W >= 2 ? W : 2;
+  const bool placed = pos >= 0;
+  char* qo = p.q_out + tok * p.qo_tok;
+  char* ko = APPEND ? row : p.k_out + tok * p.ko_tok;
+  const int64_t ko_head = APPEND ? p.s_head : p.ko_head;
+  // null: not written (a key of a token without a place)
+  auto dst_of = [&](int h) -> char* {
+    return h < p.Hq ? qo + h * p.qo_head : (APPEND && !placed ? nullptr : ko + (h - p.Hq) * ko_head);
+  };
+  const float* cs = p.cos_sin + pos * p.cs_stride;
+  for (int c = lt.c; c < turned; c += lt.c_step) {
+    float co[Op::NP] = {}, si[Op::NP] = {};
+    if (placed) {
+      load_angles<Op::NP>(cs + c * Op::NP, co);
+      load_angles<Op::NP>(cs + p.R / 2 + c * Op::NP, si);
 #pragma unroll
-          for (int o = 0; o < NV; o += W) store_row<T, W>(dst + (int64_t)c * NV * 2 + o * 2, z);
-        } else {
-          store_row<T, W>(dst + (int64_t)c * W * 2, z);
-          store_row<T, W>(dst + (int64_t)c * W * 2 + p.R, z);
-        }
-        continue;
-      }
-      if (c < p.turned) {
-        turn_piece<T, W, INTER>(src, dst, c, p.R, cs, p.sign);
-      } else {
-        const int64_t at = (int64_t)p.R * 2 + (int64_t)(c - p.turned) * W * 2;
-        copy_piece<T, W>(src + at, dst + at);
+      for (int i = 0; i < Op::NP; ++i) si[i] *= p.sign;
+    }
+    if (c != lt.c) fetch(h0, c);
+    for (int h = h0; h < heads; h += U * h_step) {
+      Raw<T, W> now[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) now[u] = raw[u];
+      fetch(h + U * h_step, c);  // the next rows while these are turned
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (h + u * h_step >= heads) continue;
+        char* dst = dst_of(h + u * h_step);
+        if (!dst) continue;
+        if (placed) Op::turn(now[u], co, si);
+        else now[u] = Raw<T, W>{};  // no position: a row of zeros
+        Op::store(dst + Op::at_a(c), now[u].a);
+        if constexpr (Op::TWO) Op::store(dst + Op::at_a(c) + Op::gap(p.R), now[u].b);
       }
     }
+  }
+  // the rest of the heads, and v: copied
+  auto copy_rows = [&](int n, int rows, int64_t first, auto from, auto to, bool zero) {
+    const Lanes lc(n, lane);
+    const int step = p.warps_per_token * lc.rows;
+    for (int c = lc.c; c < n; c += lc.c_step) {
+      constexpr int V = 4;
+      for (int h = part * lc.rows + lc.row; h < rows; h += V * step) {
+        typename Op::V v[V];
+#pragma unroll
+        for (int u = 0; u < V; ++u)
+          if (h + u * step < rows) v[u] = zero ? typename Op::V{} : Op::load(from(h + u * step) + first + (int64_t)c * W * 2);
+#pragma unroll
+        for (int u = 0; u < V; ++u)
+          if (h + u * step < rows) {
+            char* dst = to(h + u * step);
+            if (dst) Op::store(dst + first + (int64_t)c * W * 2, v[u]);
+          }
+      }
+    }
+  };
+  if (p.R < p.D) copy_rows((p.D - p.R) / W, heads, (int64_t)p.R * 2, src_of, dst_of, !placed);
+  if (APPEND && placed) {
+    const char* v = p.v + tok * p.v_tok;
+    copy_rows(p.D / W, p.Hkv, 0, [&](int h) { return v + h * p.v_head; },
+              [&](int h) { return row + p.s_kv + h * p.s_head; }, false);
   }
 }
 
-// Pieces per token for width W, and the launch.
+// Few tokens do not fill the GPU with a warp each: up to 512 a CTA's four warps
+// share one (64 tokens of 40 heads appended in 10.3 us against 12.3, 256 in 10.2
+// against 12.3); above, the lookups and angles that each warp repeats cost more
+// (2048 tokens in 16.4 us with one warp each, 22.6 with four).
+int warps_per_token(int64_t tokens) { return tokens <= 512 ? kWarps : 1; }
+
 template <typename T, int W, bool INTER, bool APPEND>
 int launch_rotary(RotaryParams p, cudaStream_t st) {
-  const int pairs = INTER ? (W >= 2 ? W / 2 : 1) : W;  // pairs of one piece
-  p.turned = p.R / 2 / pairs;
-  const int per_head = p.turned + (p.D - p.R) / W;
-  const int64_t n_rot = (int64_t)(p.Hq + p.Hkv) * per_head;
-  const int64_t n_tok = n_rot + (APPEND ? (int64_t)p.Hkv * (p.D / W) : 0);
-  if (n_tok > 0x3fffffff) return set_error(AKT_ERR_UNSUPPORTED, "rotary: token rows too large");
-  p.n_rot = (int)n_rot;
-  p.n_tok = (int)n_tok;
-  p.div_head = make_fastdiv((uint32_t)per_head);
-  p.div_vrow = make_fastdiv((uint32_t)(p.D / W));
-  p.tokens_per_cta = 1;
-  const int64_t ctas = (p.num_tokens + p.tokens_per_cta - 1) / p.tokens_per_cta;
-  if (ctas > 0x7fffffff) return set_error(AKT_ERR_INVALID, "rotary: too many tokens");
+  p.warps_per_token = warps_per_token(p.num_tokens);
+  const int per_cta = kWarps / p.warps_per_token;
+  const int64_t ctas = (p.num_tokens + per_cta - 1) / per_cta;
   {
     ProfileScope prof(st);
     rotary_kernel<T, W, INTER, APPEND><<<(unsigned)ctas, kThreads, 0, st>>>(p);
