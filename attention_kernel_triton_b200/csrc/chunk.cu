@@ -493,11 +493,11 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, i
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t src_bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// an arrival on bar when this thread's copies so far have landed
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // generic-proxy writes to shared memory before later async-proxy reads (the MMAs)
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -729,7 +729,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], TMA ? 1 : 32);  // cp.async: every lane of the loader
       mbar_init(&empty[s], 2);
       mbar_init(&ready[s], 1);
     }
@@ -937,6 +937,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = false;
             break;
           }
+          if (!TMA) {  // what the copies wrote, before the MMAs' reads
+            fence_async_smem();
+            __syncwarp();
+          }
           // V tiles are the even loads from the third on, and the last one
           const int j = t0 + (i + 1 == loads ? (i >> 1) : (i >> 1) - 1);
           const bool is_v = i + 1 == loads || (i >= 2 && !(i & 1));
@@ -996,15 +1000,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       const int boxes = TMA ? BN / p.box_rows : 0;  // of one tile, at most 16
       uint32_t loaded = 0;  // stages this warp has loaded (bits 0 ..) and the parity of the last load (16 ..)
-      int held = -1;  // cp.async: the stage whose copies are not known to have landed
-      auto hand_over = [&]() {
-        if (held < 0) return;
-        cp_async_wait<0>();
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&full[held]);
-        held = -1;
-      };
       for (int k = 0; ok; ++k) {
         if (!wait(&seg_full[k % kSegs], (k / kSegs) & 1)) break;
         const Seg* sg = &segs[k % kSegs];
@@ -1071,35 +1066,39 @@ __global__ void __launch_bounds__(kThreads, 1)
           // every half warp (D = 128) or quarter (D = 64) copies whole rows in 16-byte pieces
           constexpr int CH = D / 8, RW = 32 / CH;  // pieces of a row; rows a step
           const int ch = lane % CH, rl = lane / CH;
-          for (int j = t0; ok && j < t1; ++j) {
-            // the addresses of rows lane, lane + 32, ... of the tile's keys (null: zeros)
-            const char* src[BN / 32];
+          // the index entries of a tile's rows lane, lane + 32, ..., a tile ahead of their use
+          int id_next[BN / 32];
+          auto entries = [&](int j) {
 #pragma unroll
             for (int i = 0; i < BN / 32; ++i) {
               const int key = j * BN + i * 32 + lane;
-              src[i] = nullptr;
-              if (key < len) {
-                const int pg = (int)fdiv((uint32_t)key, p.div_page);
-                const int id = __ldg(p.indices + page0 + pg);
-                if (id >= 0 && id < p.num_pages)
-                  src[i] = p.kv + (op ? p.s_kv : 0) + (int64_t)id * p.s_page + (int64_t)kvh * p.s_head +
-                           (int64_t)(key - pg * p.P) * p.s_tok;
-                else record_status(kStatusBadPage);
-              }
+              id_next[i] = key < len ? __ldg(p.indices + page0 + (int)fdiv((uint32_t)key, p.div_page)) : -1;
             }
+          };
+          if (t0 < t1) entries(t0);
+          for (int j = t0; ok && j < t1; ++j) {
+            const char* src[BN / 32];  // the rows' addresses (null: zeros)
+#pragma unroll
+            for (int i = 0; i < BN / 32; ++i) {
+              const int key = j * BN + i * 32 + lane, id = id_next[i];
+              src[i] = nullptr;
+              if (id >= 0 && id < p.num_pages)
+                src[i] = p.kv + (op ? p.s_kv : 0) + (int64_t)id * p.s_page + (int64_t)kvh * p.s_head +
+                         (int64_t)(key - (int)fdiv((uint32_t)key, p.div_page) * p.P) * p.s_tok;
+              else if (key < len) record_status(kStatusBadPage);
+            }
+            if (j + 1 < t1) entries(j + 1);
             __syncwarp();
             const uint32_t g = base + (op ? ring_v(j - t0, t1 - t0) : ring_k(j - t0)), st = g % NS;
-            if (g >= NS && !__all_sync(0xffffffffu, mbar_try_wait(&empty[st], ((g / NS) - 1) & 1))) {
-              hand_over();  // nothing else to do: what was copied last need not wait for the next copy
-              if (!wait(&empty[st], ((g / NS) - 1) & 1)) {
-                ok = false;
-                break;
-              }
+            if (g >= NS && !wait(&empty[st], ((g / NS) - 1) & 1)) {
+              ok = false;
+              break;
             }
+            __syncwarp();
             const uint32_t tile = smem_u32(smem + C::OFF_KV + st * C::KV_BYTES);
 #pragma unroll
             for (int i = 0; i < BN / 32; ++i) {
-#pragma unroll 4
+#pragma unroll 8
               for (int r0 = 0; r0 < 32; r0 += RW) {
                 const int r = r0 + rl;
                 const char* row =
@@ -1109,16 +1108,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 cp_async16(dst, row ? row + ch * 16 : p.q, row ? 16u : 0u);
               }
             }
-            cp_async_commit();
-            if (held >= 0) {  // the stage before this one has landed
-              cp_async_wait<1>();
-              fence_async_smem();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&full[held]);
-            }
-            held = (int)st;
+            cp_async_arrive(&full[st]);  // each lane's arrival, once its copies have landed
           }
-          hand_over();  // the segment's last stage
         }
         base += 2 * (t1 - t0);
       }
@@ -1129,7 +1120,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (qn0) mbar_wait(&q_full[0], (qn0 - 1) & 1);
         if (qn1) mbar_wait(&q_full[1], (qn1 - 1) & 1);
       }
-      if (!TMA) cp_async_wait<0>();
+      if (!TMA) cp_async_wait_all();
     } else {
       // ============================ MMA issuer ============================
       // One warp issues both slots' MMAs, the slots in turn: P.V of slot t's tile,
