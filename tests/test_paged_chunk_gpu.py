@@ -297,3 +297,17 @@ def test_chunk_on_another_stream_and_in_a_graph():
     g.replay()
     torch.cuda.synchronize()
     c.close(out, flash_attention_chunk_paged_with_lse(*c.args())[1], True)
+
+
+def test_chunk_last_page_lengths_are_clamped():
+    c = Case([40, 32], [8, 4], Hkv=2, G=2, seed=16)
+    O = flash_attention_chunk_paged(*c.args())
+    last = c.last.clone()
+    last[1] = 999  # a full page of 16
+    assert torch.equal(flash_attention_chunk_paged(*c.args()[:5], last), O)
+    last[1] = 0  # a page that holds nothing yet: the sequence ends with the page before
+    O2 = flash_attention_chunk_paged(*c.args()[:5], last)
+    ref = flash_attention_chunk_paged(c.q, c.at, c.pool, torch.tensor([0, 3, 4], dtype=torch.int32, device=DEV),
+                                      c.indices[:4],
+                                      torch.tensor([8, 16], dtype=torch.int32, device=DEV))
+    assert torch.equal(O2, ref)
