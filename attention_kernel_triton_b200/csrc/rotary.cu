@@ -98,48 +98,38 @@ struct PieceOp {
   static __device__ __forceinline__ V load(const char* p) { return *reinterpret_cast<const V*>(p); }
   static __device__ __forceinline__ void store(char* p, V v) { *reinterpret_cast<V*>(p) = v; }
 
-  static __device__ __forceinline__ void unpack(V v, float (&x)[W]) {
-    union {
-      V v;
-      T e[W];
-    } u;
-    u.v = v;
-#pragma unroll
-    for (int i = 0; i < W; ++i) x[i] = Elem<T>::to_float(u.e[i]);
-  }
-  static __device__ __forceinline__ V pack(const float (&x)[W]) {
-    union {
-      V v;
-      T e[W];
-    } u;
-#pragma unroll
-    for (int i = 0; i < W; ++i) u.e[i] = Elem<T>::from_float(x[i]);
-    return u.v;
-  }
+  union Words {  // a vector as its 32-bit words (W >= 2) or its value
+    V v;
+    uint32_t w[W >= 2 ? W / 2 : 1];
+    T e[W];
+    __device__ __forceinline__ Words() {}
+  };
 
-  // the piece's pairs turned by the angles' cosines and (signed) sines
+  // The piece's pairs turned by the angles' cosines and (signed) sines, a word at
+  // a time and in place.
   static __device__ __forceinline__ void turn(Raw<T, W>& r, const float (&co)[NP], const float (&si)[NP]) {
-    float a[W], b[W];
-    unpack(r.a, a);
-    if constexpr (TWO) {
-      unpack(r.b, b);
-      float ya[W], yb[W];
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        ya[i] = a[i] * co[i] - b[i] * si[i];
-        yb[i] = b[i] * co[i] + a[i] * si[i];
-      }
-      r.a = pack(ya);
-      r.b = pack(yb);
+    Words a, b;
+    a.v = r.a;
+    if constexpr (TWO) b.v = r.b;
+    if constexpr (W == 1) {
+      const float x = Elem<T>::to_float(a.e[0]), y = Elem<T>::to_float(b.e[0]);
+      a.e[0] = Elem<T>::from_float(x * co[0] - y * si[0]);
+      b.e[0] = Elem<T>::from_float(y * co[0] + x * si[0]);
     } else {
-      float y[W];
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        y[2 * i] = a[2 * i] * co[i] - a[2 * i + 1] * si[i];
-        y[2 * i + 1] = a[2 * i + 1] * co[i] + a[2 * i] * si[i];
+      for (int i = 0; i < W / 2; ++i) {
+        const float2 x = Elem<T>::to_float2(a.w[i]);
+        if constexpr (TWO) {
+          const float2 y = Elem<T>::to_float2(b.w[i]);
+          a.w[i] = Elem<T>::pack2(x.x * co[2 * i] - y.x * si[2 * i], x.y * co[2 * i + 1] - y.y * si[2 * i + 1]);
+          b.w[i] = Elem<T>::pack2(y.x * co[2 * i] + x.x * si[2 * i], y.y * co[2 * i + 1] + x.y * si[2 * i + 1]);
+        } else {
+          a.w[i] = Elem<T>::pack2(x.x * co[i] - x.y * si[i], x.y * co[i] + x.x * si[i]);
+        }
       }
-      r.a = pack(y);
     }
+    r.a = a.v;
+    if constexpr (TWO) r.b = b.v;
   }
 };
 
@@ -211,11 +201,19 @@ struct Lanes {
   }
 };
 
+// CTAs per SM that the registers are cut for.  More warps cover more of the loads'
+// latency until the angles and rows in flight spill: interleaved pieces (half the
+// values) take 8 (append of 13K tokens 60 us against 64, plain rows of 8192 tokens
+// of 80 heads 134 against 146), half pieces 6 with the append's lookups (62 against
+// 68) and no cut on plain rows (132 us a training step's q and k and their
+// gradients; 226 at 6, 328 at 8).
+constexpr int min_ctas(bool inter, bool append) { return inter ? 8 : append ? 6 : 1; }
+
 // One or several warps per token, each with every warps_per_token-th group of
 // rows.  The first rows are asked for before the token is placed (a chain of four
 // dependent lookups) and its angles are read, since they need neither.
 template <typename T, int W, bool INTER, bool APPEND>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) {
+__global__ void __launch_bounds__(kThreads, min_ctas(INTER, APPEND)) rotary_kernel(const RotaryParams p) {
   using Op = PieceOp<T, W, INTER>;
   constexpr int U = 2;  // rows in flight per lane, and as many on their way (1: 74 us, 2: 64, 4: 74)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
