@@ -26,7 +26,8 @@
 //
 // Warps of a CTA (12):
 //   0-3 / 4-7  softmax of slot 0 / 1: thread i owns row i = TMEM lane i
-//   8 / 11     loaders of K / of V and Q into a ring of tiles: tensor-map boxes inside
+//   8 / 11     loaders of K / of V and Q (few rows: by plain loads, the rest of the tile
+//              cleared) into a ring of tiles: tensor-map boxes inside
 //              the pages, or 16-byte cp.async rows where no box fits a page (TMA template)
 //   9          issuer of both slots' MMAs (one thread)
 //   10         scheduler: the CTA's segments, a few ahead, through shared memory;
@@ -75,11 +76,20 @@ constexpr int kSegReaders = 12;    // 2 loaders, issuer, 8 softmax warps, schedu
 // 2 and 2 787, 6 and 1 682, 6 and 3 680, 8 and 3 686.  Eight prompts of 2048 tokens:
 // 451, then 400, 414, 398, 390.
 constexpr int kUnitCost1 = 6, kUnitCost2 = 3;
+// A unit with at most this many rows gets the rest of its Q tiles cleared; the
+// tensor map would fill it with the following sequences' rows, whose products nobody
+// reads but which draw power.  n tokens of 4 heads in each of 64 sequences of 512 to
+// 32768 keys, first calls / repeated for a second under the power cap: n = 1 644 / 695 us
+// (map: 652 / 736), 5 659 / 710 (667 / 780), 12 (48 rows) 673 / 758 (686 / 800); 16 rows
+// more take a warp's copy too long at a unit's start: 718 / 765 (685 / 810), n = 32
+// 920 / 969 (718 / 852).
+constexpr int kFewRows = 48;
 constexpr int kTableSeqs = 96;     // sequences whose table fits the CTA's shared memory
 constexpr int kMaxCtas = kThreads; // of the main kernel (one per SM)
 
 struct ChunkParams {
   const char* q;
+  int64_t q_tok, q_head;  // bytes
   const int32_t* q_indptr;
   int64_t num_tokens;
   const char* kv;
@@ -583,6 +593,34 @@ __device__ __forceinline__ void add_not_finite(const ChunkParams& p, const Seg& 
   }
 }
 
+// A warp's fill of the slots' Q tiles with a unit's rows and zeros up to row
+// `clear`, in the tiles' swizzled layout.
+template <int D>
+__device__ __forceinline__ void load_few_rows(const ChunkParams& p, unsigned char* tiles, int q0, int kvh, int rows,
+                                              int clear, bool slot0, bool slot1) {
+  constexpr int PIECES = D / 8, U = 4;
+  const char* q = p.q + (int64_t)q0 * p.q_tok + (int64_t)kvh * p.group * p.q_head;
+  for (int i0 = threadIdx.x & 31; i0 < clear * PIECES; i0 += 32 * U) {
+    uint4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + 32 * u, row = i / PIECES, tok = (int)fdiv((uint32_t)row, p.div_group);
+      v[u] = make_uint4(0, 0, 0, 0);
+      if (row < rows)
+        v[u] = __ldg(reinterpret_cast<const uint4*>(q + tok * p.q_tok + (row - tok * p.group) * p.q_head) + i % PIECES);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + 32 * u, row = i / PIECES, c = i % PIECES;
+      if (row >= clear) continue;
+      unsigned char* dst = tiles + (c >> 3) * (BM * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+      if (slot0) *reinterpret_cast<uint4*>(dst) = v[u];
+      if (slot1) *reinterpret_cast<uint4*>(dst + BM * D * 2) = v[u];
+    }
+  }
+  fence_async_smem();
+}
+
 // 4 x 4 pieces of 16 bytes turned over four lanes: v[i] is piece i of this lane's
 // row and becomes piece (lane % 4) of row i of its four lanes.
 __device__ __forceinline__ void turn_pieces(uint4 (&v)[4]) {
@@ -997,6 +1035,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // A warp each: one warp's boxes (72 cycles apiece) took as long as a tile's whole turn.
       const int op = warp == kLoadVWarp;
       uint32_t base = 0, qn0 = 0, qn1 = 0;  // ring loads before the segment; Q loads
+      int dirty = BM | BM << 8;             // rows of each slot's Q tile that are not zeros
       bool ok = true;
       const int boxes = TMA ? BN / p.box_rows : 0;  // of one tile, at most 16
       uint32_t loaded = 0;  // stages this warp has loaded (bits 0 ..) and the parity of the last load (16 ..)
@@ -1004,11 +1043,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!wait(&seg_full[k % kSegs], (k / kSegs) & 1)) break;
         const Seg* sg = &segs[k % kSegs];
         const int q0 = sg->q0, t0 = sg->t0, t1 = sg->t1, kvh = sg->kvh, page0 = sg->page0, len = sg->len;
-        const int single = sg->single, n0 = sg->n0, n1 = sg->n1;
+        const int single = sg->single, n0 = sg->n0, n1 = sg->n1, rows = sg->ntok * p.group;
         __syncwarp();
         if (lane == 0) mbar_arrive(&seg_empty[k % kSegs]);
         if (q0 < 0) break;
-        if (op) {  // Q of both slots: the buffer is free once the slot's last S before is done
+        if (op && single && rows <= kFewRows) {  // the same few rows for both slots
+          if ((n0 && qn0 && !wait(&q_empty[0], (qn0 - 1) & 1)) || (n1 && qn1 && !wait(&q_empty[1], (qn1 - 1) & 1))) break;
+          load_few_rows<D>(p, smem + C::OFF_Q, q0, kvh, rows, max(rows, max(n0 ? dirty & 255 : 0, n1 ? dirty >> 8 : 0)),
+                           n0, n1);
+          __syncwarp();
+          if (n0) {
+            ++qn0;
+            dirty = (dirty & ~255) | rows;
+            if (lane == 0) mbar_arrive(&q_full[0]);
+          }
+          if (n1) {
+            ++qn1;
+            dirty = (dirty & 255) | rows << 8;
+            if (lane == 0) mbar_arrive(&q_full[1]);
+          }
+        } else if (op) {  // Q of both slots: the buffer is free once the slot's last S before is done
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             uint32_t& qn = t ? qn1 : qn0;
@@ -1018,6 +1072,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               break;
             }
             ++qn;
+            dirty = t ? (dirty & 255) | BM << 8 : (dirty & ~255) | BM;
             if (lane == 0) {
               mbar_arrive_expect_tx(&q_full[t], (uint32_t)(p.TQ * p.group * 128 * C::DB));
 #pragma unroll
@@ -1678,6 +1733,8 @@ extern "C" int akt_chunk_paged(const akt_chunk_paged_args* a, void* workspace, s
     return set_error(AKT_ERR_WORKSPACE, "chunk_paged: workspace of " + std::to_string(y.bytes) + " bytes required");
   ChunkParams p{};
   p.q = static_cast<const char*>(a->q);
+  p.q_tok = a->q_stride_token * 2;
+  p.q_head = a->q_stride_head * 2;
   p.q_indptr = a->q_indptr;
   p.num_tokens = a->num_tokens;
   p.kv = static_cast<const char*>(a->kv_cache);
