@@ -993,23 +993,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             auto at = [&](int r) { return reinterpret_cast<uint4*>(vc + (r >> 3) * C::GROUP + (r & 7) * 128); };
             const int top = min(rows, BN), mid = max(r0, top);
             for (int r = mid + lane / PR; r < BN; r += RS) *at(r) = make_uint4(0, 0, 0, 0);
-            for (int r = r0 + lane / PR; r < top; r += 2 * RS) {  // two pieces at a time, one look
-              uint4 y[2];
+            constexpr int U = 8;  // pieces at a time, one look (8 prompts of 2048 tokens, D = 128: 2 310 us, 4 301, 8 299, 16 299)
+            for (int r = r0 + lane / PR; r < top; r += U * RS) {
               uint32_t any = 0;
 #pragma unroll
-              for (int u = 0; u < 2; ++u) y[u] = r + u * RS < top ? *at(r + u * RS) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-              for (int u = 0; u < 2; ++u)
-                any |= not_finite2<T>(y[u].x) | not_finite2<T>(y[u].y) | not_finite2<T>(y[u].z) | not_finite2<T>(y[u].w);
+              for (int u = 0; u < U; ++u) {  // (the last row again where there are no more)
+                const uint4 y = *at(min(r + u * RS, top - 1));
+                any |= not_finite2<T>(y.x) | not_finite2<T>(y.y) | not_finite2<T>(y.z) | not_finite2<T>(y.w);
+              }
               if (!any) continue;
-#pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                const uint32_t x = not_finite2<T>(y[u].x) | not_finite2<T>(y[u].y) | not_finite2<T>(y[u].z) |
-                                   not_finite2<T>(y[u].w);
-                if (!x) continue;
-                const int q = r + u * RS;
-                *at(q) = make_uint4(without_not_finite2<T>(y[u].x), without_not_finite2<T>(y[u].y),
-                                    without_not_finite2<T>(y[u].z), without_not_finite2<T>(y[u].w));
+#pragma unroll 1
+              for (int q = r; q < min(r + U * RS, top); q += RS) {
+                const uint4 y = *at(q);
+                if (!(not_finite2<T>(y.x) | not_finite2<T>(y.y) | not_finite2<T>(y.z) | not_finite2<T>(y.w))) continue;
+                *at(q) = make_uint4(without_not_finite2<T>(y.x), without_not_finite2<T>(y.y),
+                                    without_not_finite2<T>(y.z), without_not_finite2<T>(y.w));
                 atomicOr(&sg->bad[j - j_edge][q >> 5], 1u << (q & 31));
                 sg->noted = 1;
               }
