@@ -26,10 +26,10 @@
 //
 // Warps of a CTA (12):
 //   0-3 / 4-7  softmax of slot 0 / 1: thread i owns row i = TMEM lane i
-//   8 / 11     loaders of K / of V and Q (few rows: by plain loads, the rest of the tile
-//              cleared) into a ring of tiles: tensor-map boxes inside
-//              the pages, or 16-byte cp.async rows where no box fits a page (TMA template)
-//   9          issuer of both slots' MMAs (one thread)
+//   8 / 11     loaders of K / of V and Q into a ring of tiles: tensor-map boxes inside
+//              the pages, or 16-byte cp.async rows where no box fits a page (TMA template);
+//              a unit's few rows of Q come by plain loads, the rest of their tile cleared
+//   9          issuer of both slots' MMAs (one elected lane)
 //   10         scheduler: the CTA's segments, a few ahead, through shared memory;
 //              and the V tiles at the mask's edge (below)
 // TMEM (512 columns): S[2] (128 each), O[2] (D each).  P_t overwrites S_t: a
@@ -41,6 +41,12 @@
 // that a mask crosses the rows past the sequence are cleared, and values that are
 // not finite are cleared and their tokens noted; a row that does see such a token
 // gets the value added to its output at the end.
+//
+// Bounds and measured rates (fp16, 32 query heads on 8, pages of 16 keys, full clock).
+// Long prompts: the tensor pipe and the exponentials, 60 % busy each; 8192 tokens on top
+// of 24576, D = 128, 3.01 ms = 1280 TFLOP/s (D = 64: 2.53 ms).  Short prompts also their
+// units' ends and the causal edge: 8 of 2048 tokens, 295 us.  Few tokens: HBM; 5 in each
+// of 64 sequences of 512 to 32768 keys, 655 us = 6.66 TB/s.
 //
 // Built without -rdc (setmaxnreg needs whole-program device code).
 #define AKT_WHOLE_PROGRAM 1
@@ -74,7 +80,7 @@ constexpr int kSegReaders = 12;    // 2 loaders, issuer, 8 softmax warps, schedu
 // of one tile of rows, of two.  A verification of 5 tokens in 64 sequences of 512
 // to 32768: without it the CTAs with the short sequences were last, 1025 us; with
 // 2 and 2 787, 6 and 1 682, 6 and 3 680, 8 and 3 686.  Eight prompts of 2048 tokens:
-// 451, then 400, 414, 398, 390.
+// 451, then 400, 414, 398, 390.  (All before the later steps; see the rates above.)
 constexpr int kUnitCost1 = 6, kUnitCost2 = 3;
 // A unit with at most this many rows gets the rest of its Q tiles cleared; the
 // tensor map would fill it with the following sequences' rows, whose products nobody
