@@ -170,6 +170,27 @@ def test_chunk_many_segments_and_tiles_per_cta(new):
     assert _lib.device_status(0) == 0
 
 
+@pytest.mark.parametrize("dtype,D", [(FP16, 128), (BF16, 64)])
+def test_chunk_units_of_few_rows_among_others(dtype, D):
+    # units of less than a tile of rows have the rest of their query tile cleared: at the limit, around it, after and
+    # before whole tiles on the same CTA, queries apart in memory; other sequences' queries must not matter
+    news = [12, 13, 1, 40, 0, 3, 70, 11] * 8
+    c = Case([max(n, 200 + 53 * i) for i, n in enumerate(news)], news, Hkv=8, G=4, D=D, dtype=dtype, seed=12)
+    got, lse = c.check(True)
+    c.check(False)
+    wide = torch.full((c.q.shape[0], 2, 32, D), math.nan, dtype=dtype, device=DEV)
+    wide[:, 1] = c.q
+    strided = (wide[:, 1], *c.args()[1:])
+    assert torch.equal(flash_attention_chunk_paged(*strided), got)
+    at = c.at.tolist()
+    for b in range(0, 64, 2):  # the sequences of 13, 40, 3 and 11 tokens stay
+        c.q[at[b]:at[b + 1]] = math.nan
+    rest, lse2 = flash_attention_chunk_paged_with_lse(*c.args())
+    for b in range(1, 64, 2):
+        assert torch.equal(rest[at[b]:at[b + 1]], got[at[b]:at[b + 1]])
+        assert torch.equal(lse2[at[b]:at[b + 1]], lse[at[b]:at[b + 1]])
+
+
 def test_chunk_one_token_is_the_decode():
     lens = [1, 17, 500, 4000]
     c = Case(lens, [1] * 4, Hkv=2, G=4, seed=4)
