@@ -121,6 +121,7 @@ struct ChunkParams {
   float* part_o;       // [grid][2][part_rows][D]
   float* part_lse;     // [grid][2][part_rows] natural log, -inf: no key
   int part_rows;
+  int merge_rows;      // rows of a CTA of the merge
   // tables in the workspace, for more than kTableSeqs sequences
   int64_t* plan_cost;  // [B + 1]
   int* plan_units;     // [B + 1]
@@ -1477,8 +1478,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // -------------------------------------------------------------------------
 // O = sum_i e^{lse_i - M} O_i / sum_i e^{lse_i - M}.  The unit's parts are the one
 // with its first keys and then place 0 of the CTAs after it, up to the one with
-// its last keys.  CTA (x, y): place x, rows [32 y, 32 y + 32); a warp per row.
-constexpr int kMergeThreads = 256, kMergeRows = 32;
+// its last keys.  CTA (x, y): place x, rows [R y, R y + R), R = merge_rows; a warp per row.
+constexpr int kMergeThreads = 256;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const ChunkParams p) {
@@ -1505,7 +1506,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const ChunkP
   const Part me = p.parts[blockIdx.x];
   if (!me.used || !me.first) return;
   const int rows = me.single ? me.ntok * p.group : BM + (me.ntok - p.TQ) * p.group;
-  if ((int)blockIdx.y * kMergeRows >= rows) return;
+  if ((int)blockIdx.y * p.merge_rows >= rows) return;
   // how many CTAs follow with parts of this unit (those without one are passed over)
   int last = c0;
   for (int base = c0 + 1; base < p.grid; base += 32) {
@@ -1518,7 +1519,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const ChunkP
     }
   }
   const int count = last - c0 + 1;
-  for (int r = blockIdx.y * kMergeRows + warp; r < min(rows, (int)(blockIdx.y + 1) * kMergeRows); r += kMergeThreads / 32) {
+  for (int r = blockIdx.y * p.merge_rows + warp; r < min(rows, (int)(blockIdx.y + 1) * p.merge_rows); r += kMergeThreads / 32) {
     const int slot = me.single ? 0 : r >> 7, rr = r & (BM - 1);
     const int rtok = (int)fdiv((uint32_t)rr, p.div_group), tok = slot * p.TQ + rtok;
     if (rtok >= p.TQ || tok >= me.ntok) continue;
@@ -1538,19 +1539,24 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const ChunkP
     for (int i0 = 0; i0 < count; i0 += 32) {
       const float mine = fast_exp2((lse_of(i0 + lane) - Ms) * kLog2e);  // NaN stays NaN
       const int n = min(32, count - i0);
-#pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        const float w = __shfl_sync(0xffffffffu, mine, i);
-        if (w == 0.f) continue;
-        den += w;
-        const float* o = p.part_o + place(i0 + i) * D + lane * N;
-        if constexpr (N == 4) {
-          const float4 v = *reinterpret_cast<const float4*>(o);
-          acc[0] = fmaf(w, v.x, acc[0]); acc[1] = fmaf(w, v.y, acc[1]);
-          acc[2] = fmaf(w, v.z, acc[2]); acc[3] = fmaf(w, v.w, acc[3]);
-        } else {
-          const float2 v = *reinterpret_cast<const float2*>(o);
-          acc[0] = fmaf(w, v.x, acc[0]); acc[1] = fmaf(w, v.y, acc[1]);
+      for (int i1 = 0; i1 < n; i1 += 8) {  // eight parts' rows asked for at once
+        float w[8];
+        float v[8][N];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          w[u] = __shfl_sync(0xffffffffu, mine, i1 + u);  // (0 past the count)
+#pragma unroll
+          for (int e = 0; e < N; ++e) v[u][e] = 0.f;
+          if (w[u] == 0.f) continue;  // a part without keys for the row holds nothing
+          const float* o = p.part_o + place(i0 + i1 + u) * D + lane * N;
+          if constexpr (N == 4) *reinterpret_cast<float4*>(v[u]) = *reinterpret_cast<const float4*>(o);
+          else *reinterpret_cast<float2*>(v[u]) = *reinterpret_cast<const float2*>(o);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          den += w[u];
+#pragma unroll
+          for (int e = 0; e < N; ++e) acc[e] = fmaf(w[u], v[u][e], acc[e]);
         }
       }
     }
@@ -1695,7 +1701,7 @@ int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap
     else kern<<<p.grid, kThreads, smem, st>>>(mq, mk, mv, p);
   }
   if (e == cudaSuccess)
-    e = launch_dependent(chunk_merge_kernel<T, D>, dim3(2 * p.grid, (p.part_rows + kMergeRows - 1) / kMergeRows),
+    e = launch_dependent(chunk_merge_kernel<T, D>, dim3(2 * p.grid, (p.part_rows + p.merge_rows - 1) / p.merge_rows),
                          dim3(kMergeThreads), 0, st, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? AKT_OK : set_error(AKT_ERR_CUDA, std::string("chunk_paged: ") + cudaGetErrorString(e));
@@ -1774,6 +1780,11 @@ extern "C" int akt_chunk_paged(const akt_chunk_paged_args* a, void* workspace, s
   p.part_lse = reinterpret_cast<float*>(ws + y.lse);
   p.part_o = reinterpret_cast<float*>(ws + y.o);
   p.part_rows = y.part_rows;
+  // A row of a merge is a chain of lookups, so few rows get a warp each (4 tokens on 2048
+  // keys, whole call in a graph 20.3 us, 22.5 with four rows a warp; on 32768 keys 43.7, 47.8);
+  // many rows would be many CTAs that mostly find nothing to join (8 prompts of 2048
+  // tokens: 305 us, 316 with a row a warp).
+  p.merge_rows = y.part_rows <= 64 ? 8 : 32;
   if (p.B > kTableSeqs) {
     p.plan_cost = reinterpret_cast<int64_t*>(ws + y.cost);
     p.plan_units = reinterpret_cast<int*>(ws + y.units);
