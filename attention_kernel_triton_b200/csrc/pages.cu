@@ -84,29 +84,30 @@ __device__ __forceinline__ void copy_pieces(const PoolView& v, int layer, int64_
 // ---------------------------------------------------------------------------
 // block-wide helpers of the plans (kPlanThreads threads)
 // ---------------------------------------------------------------------------
-// Exclusive prefix sum of x over the block; total through `total`.  sums: 33 ints.
-__device__ __forceinline__ int block_scan(int x, int* sums, int& total) {
+// Exclusive prefix sum of x over the block; total through `total`.  sums: 33 of them.
+template <typename S>
+__device__ __forceinline__ S block_scan(S x, S* sums, S& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int v = x;
+  S v = x;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, v, o);
+    const S y = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += y;
   }
   if (lane == 31) sums[warp] = v;
   __syncthreads();
   if (warp == 0) {
-    int w = sums[lane];
+    S w = sums[lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, w, o);
+      const S y = __shfl_up_sync(0xffffffffu, w, o);
       if (lane >= o) w += y;
     }
     sums[lane] = w;
   }
   __syncthreads();
   total = sums[31];
-  const int before = warp ? sums[warp - 1] : 0;
+  const S before = warp ? sums[warp - 1] : 0;
   __syncthreads();
   return before + v - x;
 }
@@ -207,6 +208,7 @@ __device__ __forceinline__ bool fork_parent(const ForkParams& p, int c, int& b, 
 __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParams p) {
   extern __shared__ uint32_t bits_s[];
   __shared__ int sums[33];
+  __shared__ int64_t entry_sums[33];
   uint32_t* bits = p.bits_in_smem ? bits_s : p.bits;
   const int64_t words = (p.num_pages + 31) / 32;
   for (int64_t w = threadIdx.x; w < words; w += kPlanThreads) bits[w] = 0;
@@ -234,14 +236,15 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
     const int c = c0 + threadIdx.x;
     int b = 0, s = 0, n = 0, last = 0;
     if (c < p.F) fork_parent(p, c, b, s, n, last);
-    int total;
-    const int64_t begin = at + block_scan(n, sums, total);
+    // (64 bits: the children may name far more entries than max_entries holds)
+    int64_t total;
+    const int64_t begin = at + block_scan<int64_t>(n, entry_sums, total);
     const int64_t room = max((int64_t)0, p.max_entries - begin);
     const bool cut = n > room;
     const int kept = cut ? (int)room : n;
     const int own = c < p.F && n > 0 && !cut && last < p.P && p.first[b] != c;
     int n_own;
-    const int r = copies + block_scan(own, sums, n_own);
+    const int r = copies + block_scan<int>(own, sums, n_own);
     if (c < p.F) {
       if (cut) record_status(kStatusListOverflow);
       p.out_indptr[c] = (int)min(begin, p.max_entries);
