@@ -181,8 +181,9 @@ struct ForkParams {
   int64_t num_entries, max_entries, num_pages;
   int B, F, P;
   // workspace
-  uint32_t* bits;   // [words] when the bitmap is past shared memory
-  int32_t* first;   // [B] first child of each parent
+  uint32_t* bits;   // [2 * words] when the bitmaps are past shared memory
+  int32_t* first;   // [B] first child of each parent, then the child that keeps its partly filled last page
+  int32_t* owner;   // [num_pages] first child with the page as its partly filled last one (where parents share it)
   int32_t* start;   // [F] the parent's first entry
   int32_t* rank;    // [F] which copy, -1: none
   int32_t* dead;    // [F] dead pages for the copies, ascending; -1: none left
@@ -205,29 +206,70 @@ __device__ __forceinline__ bool fork_parent(const ForkParams& p, int c, int& b, 
   return true;
 }
 
+constexpr int kNoChild = 0x7fffffff;
+
+// The partly filled last page of a named parent (its bounds are good), or -1: it has none, or one outside the pool.
+__device__ __forceinline__ int partial_page(const ForkParams& p, int b) {
+  const int s = __ldg(p.indptr + b), e = __ldg(p.indptr + b + 1);
+  if (e <= s || __ldg(p.last + b) >= p.P) return -1;
+  const int id = __ldg(p.indices + e - 1);
+  return id >= 0 && id < p.num_pages ? id : -1;
+}
+
+// Two bits per page: `held`, a whole page of a named parent or reserved, which nobody may write; and `partial`, a
+// partly filled last page.  A partial page that is not held goes over to the first child that ends in it, whichever
+// parent's; all others get copies, since each child appends to its last page.  A page with neither bit is dead.
 __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParams p) {
   extern __shared__ uint32_t bits_s[];
   __shared__ int sums[33];
   __shared__ int64_t entry_sums[33];
-  uint32_t* bits = p.bits_in_smem ? bits_s : p.bits;
+  __shared__ int shared_s;  // whether two parents end in the same partial page
   const int64_t words = (p.num_pages + 31) / 32;
-  for (int64_t w = threadIdx.x; w < words; w += kPlanThreads) bits[w] = 0;
-  for (int b = threadIdx.x; b < p.B; b += kPlanThreads) p.first[b] = 0x7fffffff;
+  uint32_t* held = p.bits_in_smem ? bits_s : p.bits;
+  uint32_t* partial = held + words;
+  for (int64_t w = threadIdx.x; w < 2 * words; w += kPlanThreads) held[w] = 0;
+  for (int b = threadIdx.x; b < p.B; b += kPlanThreads) p.first[b] = kNoChild;
+  if (threadIdx.x == 0) shared_s = 0;
   __syncthreads();
   for (int c = threadIdx.x; c < p.F; c += kPlanThreads) {
     int b, s, n, last;
     if (fork_parent(p, c, b, s, n, last)) atomicMin(p.first + b, c);
     else record_status(kStatusBadIndptr);
   }
-  if (p.reserved) mark_reserved(bits, p.reserved, p.num_pages);
+  if (p.reserved) mark_reserved(held, p.reserved, p.num_pages);
   __syncthreads();
   // live pages: a team of threads per parent that has a child
   int team = kPlanThreads;
   while (team > 32 && (int64_t)(kPlanThreads / team) < p.B) team >>= 1;
   for (int b = threadIdx.x / team; b < p.B; b += kPlanThreads / team) {
-    if (p.first[b] == 0x7fffffff) continue;
+    if (p.first[b] == kNoChild) continue;
     const int s = __ldg(p.indptr + b), e = __ldg(p.indptr + b + 1);
-    mark_entries(bits, p.indices + s, e - s, p.num_pages, threadIdx.x % team, team, false);
+    const int whole = e - s - (e > s && __ldg(p.last + b) < p.P);
+    mark_entries(held, p.indices + s, whole, p.num_pages, threadIdx.x % team, team, false);
+    if (whole < e - s && threadIdx.x % team == 0) {
+      const int id = partial_page(p, b);
+      if (id < 0) record_status(kStatusBadPage);
+      else if (atomicOr(partial + (id >> 5), 1u << (id & 31)) >> (id & 31) & 1u) shared_s = 1;
+    }
+  }
+  __syncthreads();
+  // who keeps a partial page: first[b] stays where b's first child does, and becomes -1 where every child copies
+  const bool shared = shared_s;
+  if (shared) {
+    for (int b = threadIdx.x; b < p.B; b += kPlanThreads) {
+      const int id = p.first[b] == kNoChild ? -1 : partial_page(p, b);
+      if (id >= 0) p.owner[id] = kNoChild;
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < p.B; b += kPlanThreads) {
+      const int id = p.first[b] == kNoChild ? -1 : partial_page(p, b);
+      if (id >= 0) atomicMin(p.owner + id, p.first[b]);
+    }
+    __syncthreads();
+  }
+  for (int b = threadIdx.x; b < p.B; b += kPlanThreads) {
+    const int id = p.first[b] == kNoChild ? -1 : partial_page(p, b);
+    if (id >= 0 && ((held[id >> 5] >> (id & 31) & 1u) || (shared && p.owner[id] != p.first[b]))) p.first[b] = -1;
   }
   // the children's table bounds, and which of them need a page of their own
   int64_t at = 0;
@@ -261,7 +303,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
   int found = 0;
   for (int64_t w0 = 0; w0 < words && found < copies; w0 += kPlanThreads) {
     const int64_t w = w0 + threadIdx.x;
-    uint32_t d = w < words ? ~bits[w] & word_mask(p.num_pages, w) : 0u;
+    uint32_t d = w < words ? ~(held[w] | partial[w]) & word_mask(p.num_pages, w) : 0u;
     int total;
     int r = found + block_scan(__popc(d), sums, total);
     while (d && r < copies) {
@@ -540,8 +582,10 @@ extern "C" int akt_copy_kv_pages(const akt_page_pool* pool, const int32_t* src, 
 }
 
 static size_t fork_workspace(const akt_fork_paged_args* a) {
-  const size_t bits = a->pool.num_pages > kSmemPages ? bitmap_bytes(a->pool.num_pages) : 0;
-  return bits + round16((size_t)std::max(a->batch, 0) * 4) + 3 * round16((size_t)std::max(a->num_children, 0) * 4) + 16;
+  const int64_t pages = std::max<int64_t>(a->pool.num_pages, 0);
+  const size_t bits = pages > kSmemPages ? 2 * bitmap_bytes(pages) : 0;
+  return bits + round16((size_t)std::max(a->batch, 0) * 4) + 3 * round16((size_t)std::max(a->num_children, 0) * 4) +
+         round16((size_t)pages * 4) + 16;
 }
 
 extern "C" size_t akt_fork_paged_workspace_size(const akt_fork_paged_args* a) { return a ? fork_workspace(a) : 0; }
@@ -581,7 +625,7 @@ extern "C" int akt_fork_paged(const akt_fork_paged_args* a, void* workspace, siz
   char* ws = static_cast<char*>(workspace);
   if (!p.bits_in_smem) {
     p.bits = reinterpret_cast<uint32_t*>(ws);
-    ws += bitmap_bytes(p.num_pages);
+    ws += 2 * bitmap_bytes(p.num_pages);
   }
   p.first = reinterpret_cast<int32_t*>(ws);
   ws += round16((size_t)p.B * 4);
@@ -589,7 +633,8 @@ extern "C" int akt_fork_paged(const akt_fork_paged_args* a, void* workspace, siz
   p.start = reinterpret_cast<int32_t*>(ws);
   p.rank = reinterpret_cast<int32_t*>(ws + per_child);
   p.dead = reinterpret_cast<int32_t*>(ws + 2 * per_child);
-  const size_t smem = p.bits_in_smem ? bitmap_bytes(p.num_pages) : 0;
+  p.owner = reinterpret_cast<int32_t*>(ws + 3 * per_child);
+  const size_t smem = p.bits_in_smem ? 2 * bitmap_bytes(p.num_pages) : 0;
   cudaError_t e = ensure_smem_limit<fork_plan_kernel>(smem);
   if (e != cudaSuccess) return cuda_error("fork_paged", e);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

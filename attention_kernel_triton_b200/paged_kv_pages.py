@@ -66,11 +66,13 @@ def fork_paged_kv_cache(paged_kv_cache, kv_page_indptr, kv_page_indices, kv_last
                         max_entries=None):
     """A new batch of sequences: child ``c`` continues sequence ``parents[c]``.
 
-    The first child of a parent takes its pages over; each further child shares the full
-    pages and gets its own copy of a partly filled last page, in the lowest-numbered pages
-    that neither a named parent nor ``reserved`` holds.  Sequences that no child names are
-    dropped.  So beam search's reordering, several samples of one prompt and dropping
-    finished sequences (``parents`` = those that stay) are all this call.
+    Full pages are shared.  A partly filled last page, which the child will append to, goes
+    over to the first child that ends in it, unless ``reserved`` marks it (a prefix that a
+    store keeps) or a named parent has it as a full page (a sibling cut back into it); every
+    other child gets its own copy, in the lowest-numbered pages that neither a named parent
+    nor ``reserved`` holds.  Sequences that no child names are dropped.  So beam search's
+    reordering, several samples of one prompt and dropping finished sequences (``parents`` =
+    those that stay) are all this call.
 
     parents: [num_children] (int32)
     max_entries: length of the returned index array (``sum`` of the children's pages; a

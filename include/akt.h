@@ -529,9 +529,10 @@ int akt_copy_kv_pages(const akt_page_pool* pool, const int32_t* src_pages, const
                       int64_t num_copies, void* stream);
 
 /* A new batch of sequences from parents: child c continues sequence        */
-/* parents[c] of the table.  The first child of a parent takes its pages    */
-/* over; each further one shares the full pages and gets a copy of a partly */
-/* filled last page in the lowest-numbered dead page that no earlier child  */
+/* parents[c] of the table.  Full pages are shared.  A partly filled last   */
+/* page goes over to the first child that ends in it, unless `reserved`     */
+/* marks it or a named parent has it as a full page; every other child gets */
+/* a copy of it, in the lowest-numbered dead page that no earlier child     */
 /* took.  Dead is what neither a named parent's pages nor `reserved` holds, */
 /* so sequences that no child names are dropped.  Writes the children's     */
 /* table: out_indptr [num_children + 1], out_indices [max_entries] (-1 past */
