@@ -16,6 +16,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -146,18 +147,66 @@ def _forward(q, k, cos_sin, positions, interleaved, inverse):
 
 
 class _Rotary(torch.autograd.Function):
+    """The rotation is linear and orthogonal: its tangent is the same turn, its gradient the inverse
+    one.  Both rules apply the function itself, so that derivatives of every order have theirs."""
+
     @staticmethod
-    def forward(ctx, q, k, cos_sin, positions, interleaved, inverse):
-        ctx.save_for_backward(cos_sin, positions)
-        ctx.how = interleaved, inverse
+    def forward(q, k, cos_sin, positions, interleaved, inverse):
         return _forward(q, k, cos_sin, positions, interleaved, inverse)
 
     @staticmethod
+    def setup_context(ctx, inputs, output):
+        _, _, cos_sin, positions, interleaved, inverse = inputs
+        ctx.save_for_backward(cos_sin, positions)
+        ctx.save_for_forward(cos_sin, positions)
+        ctx.how = interleaved, inverse
+
+    @staticmethod
     def backward(ctx, dq, dk):
-        cos_sin, positions = ctx.saved_tensors
         interleaved, inverse = ctx.how
-        q_in, k_in = _forward(dq, dk, cos_sin, positions, interleaved, not inverse)
-        return q_in, k_in, None, None, None, None
+        return *_Rotary.apply(dq, dk, *ctx.saved_tensors, interleaved, not inverse), None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        return _Rotary.apply(tq, tk, *ctx.saved_tensors, *ctx.how)
+
+
+class _RotaryOne(torch.autograd.Function):
+    """``_Rotary`` for one tensor."""
+
+    @staticmethod
+    def forward(x, cos_sin, positions, interleaved, inverse):
+        return _forward(x, None, cos_sin, positions, interleaved, inverse)[0]
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        _, cos_sin, positions, interleaved, inverse = inputs
+        ctx.save_for_backward(cos_sin, positions)
+        ctx.save_for_forward(cos_sin, positions)
+        ctx.how = interleaved, inverse
+
+    @staticmethod
+    def backward(ctx, dx):
+        interleaved, inverse = ctx.how
+        return _RotaryOne.apply(dx, *ctx.saved_tensors, interleaved, not inverse), None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, tx, *_):
+        return _RotaryOne.apply(tx, *ctx.saved_tensors, *ctx.how)
+
+
+def _differentiated(cos_sin, q, k):
+    """Whether a derivative in q or k (or None) is asked for, backward or forward; the table has none."""
+    of_table = of_rows = False
+    if torch.is_grad_enabled():
+        of_table, of_rows = cos_sin.requires_grad, q.requires_grad or k is not None and k.requires_grad
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # (a tangent lives inside a dual level only)
+        def moves(t):
+            return t is not None and forward_ad.unpack_dual(t).tangent is not None
+        of_table, of_rows = of_table or moves(cos_sin), of_rows or moves(q) or moves(k)
+    if of_table:
+        raise ValueError("cos_sin is a constant of the rotation: it takes no gradient and no tangent")
+    return of_rows
 
 
 def apply_rotary_qk(q, k, cos_sin, positions, interleaved=False, inverse=False):
@@ -167,32 +216,19 @@ def apply_rotary_qk(q, k, cos_sin, positions, interleaved=False, inverse=False):
     returns (q', k') of the same shapes; a position outside the table gives zeros (status 3)
 
     ``inverse`` turns the other way, which is the gradient too: a training step either
-    calls it on the outputs' gradients or lets autograd do so.
+    calls it on the outputs' gradients or lets autograd do so (any order, and forward mode;
+    a table that requires a gradient is refused).
     """
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+    if _differentiated(cos_sin, q, k):
         return _Rotary.apply(q, k, cos_sin, positions, interleaved, inverse)
     return _forward(q, k, cos_sin, positions, interleaved, inverse)
 
 
 def apply_rotary(x, cos_sin, positions, interleaved=False, inverse=False):
     """``apply_rotary_qk`` for one tensor ``x [T, H, D]``."""
-    if torch.is_grad_enabled() and x.requires_grad:
+    if _differentiated(cos_sin, x, None):
         return _RotaryOne.apply(x, cos_sin, positions, interleaved, inverse)
     return _forward(x, None, cos_sin, positions, interleaved, inverse)[0]
-
-
-class _RotaryOne(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, cos_sin, positions, interleaved, inverse):
-        ctx.save_for_backward(cos_sin, positions)
-        ctx.how = interleaved, inverse
-        return _forward(x, None, cos_sin, positions, interleaved, inverse)[0]
-
-    @staticmethod
-    def backward(ctx, dx):
-        cos_sin, positions = ctx.saved_tensors
-        interleaved, inverse = ctx.how
-        return _forward(dx, None, cos_sin, positions, interleaved, not inverse)[0], None, None, None, None
 
 
 def append_rotary_paged_kv_cache(paged_kv_cache, q, append_k, append_v, append_indptr, kv_page_indptr,
