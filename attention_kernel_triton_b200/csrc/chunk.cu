@@ -1537,7 +1537,11 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const ChunkP
     const float Ms = M == -INFINITY ? 0.f : M;
     float acc[N] = {}, den = 0.f;
     for (int i0 = 0; i0 < count; i0 += 32) {
-      const float mine = fast_exp2((lse_of(i0 + lane) - Ms) * kLog2e);  // NaN stays NaN
+      const float part = lse_of(i0 + lane);
+      const float mine = fast_exp2((part - Ms) * kLog2e);  // NaN stays NaN
+      // A part without keys for the row is left out.  One whose weight is 0 is not: a value of it that is not
+      // finite is the row's, as it is where the unit is in one part.
+      const unsigned holds = __ballot_sync(0xffffffffu, part != -INFINITY);
       const int n = min(32, count - i0);
       for (int i1 = 0; i1 < n; i1 += 8) {  // eight parts' rows asked for at once
         float w[8];
@@ -1547,7 +1551,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const ChunkP
           w[u] = __shfl_sync(0xffffffffu, mine, i1 + u);  // (0 past the count)
 #pragma unroll
           for (int e = 0; e < N; ++e) v[u][e] = 0.f;
-          if (w[u] == 0.f) continue;  // a part without keys for the row holds nothing
+          if (!(holds >> (i1 + u) & 1u)) continue;
           const float* o = p.part_o + place(i0 + i1 + u) * D + lane * N;
           if constexpr (N == 4) *reinterpret_cast<float4*>(v[u]) = *reinterpret_cast<const float4*>(o);
           else *reinterpret_cast<float2*>(v[u]) = *reinterpret_cast<const float2*>(o);
