@@ -1486,20 +1486,31 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const ChunkP
   grid_dep_wait();
   constexpr int N = D / 32;  // columns per lane
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // padding rows of q (none in a batch that fills it)
+  // rows of no sequence: padding before and after all of them, and the rows of sequences with bad query bounds
   if (blockIdx.y == 0) {
     const int64_t lo = min(max((int64_t)__ldg(p.q_indptr), (int64_t)0), p.num_tokens);
     const int64_t hi = min(max((int64_t)__ldg(p.q_indptr + p.B), lo), p.num_tokens);
     const int64_t none = (lo + p.num_tokens - hi) * p.Hq;
-    for (int64_t i = (int64_t)blockIdx.x * (kMergeThreads / 32) + warp; i < none;
-         i += (int64_t)gridDim.x * (kMergeThreads / 32)) {
-      int64_t tok = i / p.Hq;
-      const int h = (int)(i - tok * p.Hq);
-      if (tok >= lo) tok += hi - lo;
+    const int64_t w0 = (int64_t)blockIdx.x * (kMergeThreads / 32) + warp, ws = (int64_t)gridDim.x * (kMergeThreads / 32);
+    auto clear = [&](int64_t tok, int h) {
       T* row = reinterpret_cast<T*>(p.out + tok * p.o_tok + (int64_t)h * p.o_head);
 #pragma unroll
       for (int e = 0; e < N; ++e) row[lane + 32 * e] = Elem<T>::from_float(0.f);
       if (p.lse && lane == 0) p.lse[tok * p.l_tok + (int64_t)h * p.l_head] = -INFINITY;
+    };
+    for (int64_t i = w0; i < none; i += ws) {
+      const int64_t tok = i / p.Hq;
+      clear(tok >= lo ? tok + hi - lo : tok, (int)(i - tok * p.Hq));
+    }
+    for (int64_t b0 = w0 * 32; b0 < p.B; b0 += ws * 32) {  // 32 sequences a look
+      const int64_t b = b0 + lane;
+      const int a0 = b < p.B ? __ldg(p.q_indptr + b) : 0, a1 = b < p.B ? __ldg(p.q_indptr + b + 1) : 0;
+      const int64_t r0 = max(a0, 0), r1 = min((int64_t)a1, p.num_tokens);
+      for (unsigned m = __ballot_sync(0xffffffffu, (a0 < 0 || a1 > p.num_tokens) && r0 < r1); m; m &= m - 1) {
+        const int64_t first = __shfl_sync(0xffffffffu, r0, __ffs(m) - 1);
+        const int64_t rows = (__shfl_sync(0xffffffffu, r1, __ffs(m) - 1) - first) * p.Hq;
+        for (int64_t i = 0; i < rows; ++i) clear(first + i / p.Hq, (int)(i % p.Hq));
+      }
     }
   }
   const int c0 = blockIdx.x >> 1;

@@ -424,10 +424,11 @@ int akt_sparse_index_to_mask(const akt_index_to_mask_args* args, void* stream);
 /* q_indptr[b] .. q_indptr[b+1] of q, the n_b newest: row i stands at       */
 /* position len_b - n_b + i and sees the keys up to it (causal) or all      */
 /* len_b keys.  A row that sees no key gives zeros and lse -inf, and so do  */
-/* rows before q_indptr[0] and from q_indptr[batch] on (padding).  Bad page */
-/* bounds make a sequence empty, bad query bounds leave its rows out (both  */
-/* status 4); K and V rows of pages outside the pool read as zeros (status  */
-/* 2).  A value row that is not finite reaches the rows that see it only.   */
+/* rows before q_indptr[0] and from q_indptr[batch] on (padding) and those  */
+/* between query bounds of which one is outside [0, num_tokens].  Bad page  */
+/* bounds make a sequence empty (both status 4); K and V rows of pages      */
+/* outside the pool read as zeros (status 2).  A value row that is not      */
+/* finite reaches the rows that see it only.                                */
 /* lse [num_tokens, num_qo_heads] (fp32, or NULL): natural-log sum-exp of   */
 /* the scaled scores.  head_dim 64 or 128.                                  */
 /* ------------------------------------------------------------------------ */
