@@ -53,22 +53,28 @@ def chunk_paged_into(out, q, q_indptr, paged_kv_cache, kv_page_indptr, kv_page_i
     scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
     tail = (indptr.data_ptr(), indices.data_ptr(), last.data_ptr(), indices.numel(), out.data_ptr(), *out.stride(), *lp,
             B, Hq, pool[2], pool[3], D, bool(causal), _lib.dtype_code(q), scale)
-    t = {"q": q, "cache": paged_kv_cache}
 
-    def call():
-        qq, cache = t["q"], t["cache"]
-        values = (qq.data_ptr(), *qq.stride(), at.data_ptr(), T, cache.data_ptr(), *cache.stride(), pool[0], *tail)
+    def call(q, cache):
+        values = (q.data_ptr(), *q.stride(), at.data_ptr(), T, cache.data_ptr(), *cache.stride(), pool[0], *tail)
         size = _workspace(values)
-        ws = qq.new_empty((size + 1) // 2)
+        ws = q.new_empty((size + 1) // 2)
         return _chunk(values, ws.data_ptr(), size, _lib.raw_stream(index))
 
-    def contiguous():
-        for k in t:
-            t[k] = t[k].contiguous()
-
     with _lib.on_index(index):
-        _lib.run_with_layout_retry(call, contiguous)
+        rc = call(q, paged_kv_cache)
+        if rc == _lib.AKT_ERR_UNSUPPORTED and D in (64, 128) and Hq <= 128 * pool[2] and _on_grid(out):
+            # a layout: what is off the 16-byte grid is copied, then both (strides that no tensor map takes)
+            q, cache = (t if _on_grid(t) else t.clone(memory_format=torch.contiguous_format) for t in (q, paged_kv_cache))
+            rc = call(q, cache)
+            if rc == _lib.AKT_ERR_UNSUPPORTED:
+                rc = call(q.contiguous(), cache.contiguous())
+        _lib.check(rc)
     return out
+
+
+def _on_grid(t):
+    *strides, unit = t.stride()
+    return unit == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in strides)
 
 
 def flash_attention_chunk_paged(q, q_indptr, paged_kv_cache, kv_page_indptr, kv_page_indices, kv_last_page_len,
