@@ -95,10 +95,9 @@ def fork_paged_kv_cache(paged_kv_cache, kv_page_indptr, kv_page_indices, kv_last
         raise ValueError("max_entries must not be negative")
     head = (*pool, indptr.data_ptr(), indices.data_ptr(), last.data_ptr(), indices.numel(), par.data_ptr(), _ptr(mask))
     size = _fork_size((*head, 0, 0, 0, max_entries, B, F))
-    # one allocation: the workspace (a multiple of 16 bytes), then the new table
-    ws, out_indptr, out_indices, out_last = torch.empty(
-        size // 4 + 2 * F + 1 + max_entries, dtype=torch.int32, device=paged_kv_cache.device).split_with_sizes(
-            (size // 4, F + 1, max_entries, F))
+    # the new table in one allocation; the workspace has its own, which goes when the call ends
+    ws = indptr.new_empty(size // 4)
+    out_indptr, out_indices, out_last = indptr.new_empty(2 * F + 1 + max_entries).split_with_sizes((F + 1, max_entries, F))
     with _lib.on_index(index):
         rc = _fork((*head, out_indptr.data_ptr(), out_indices.data_ptr(), out_last.data_ptr(), max_entries, B, F),
                    ws.data_ptr(), size, _lib.raw_stream(index))
@@ -124,9 +123,9 @@ def compact_paged_kv_cache(paged_kv_cache, kv_page_indices, reserved=None):
     mask = _reserved(reserved, pool[7], paged_kv_cache)
     head = (*pool, indices.data_ptr(), n, _ptr(mask))
     size = _compact_size((*head, 0, 0))
-    # one allocation: the workspace (a multiple of 16 bytes), the new index array and the count
-    ws, out, used = torch.empty(size // 4 + n + 1, dtype=torch.int32, device=indices.device).split_with_sizes(
-        (size // 4, n, 1))
+    # the new index array and the count in one allocation; the workspace has its own, which goes when the call ends
+    ws = indices.new_empty(size // 4)
+    out, used = indices.new_empty(n + 1).split_with_sizes((n, 1))
     with _lib.on_index(index):
         rc = _compact((*head, out.data_ptr(), used.data_ptr()), ws.data_ptr(), size, _lib.raw_stream(index))
         if rc:
