@@ -220,11 +220,13 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
   extern __shared__ uint32_t bits_s[];
   __shared__ int sums[33];
   __shared__ int64_t entry_sums[33];
+  __shared__ int again_s;
   const int64_t words = (p.num_pages + 31) / 32;
   uint32_t* held = p.bits_in_smem ? bits_s : p.bits;
   uint32_t* partial = held + words;
   for (int64_t w = threadIdx.x; w < 2 * words; w += kPlanThreads) held[w] = 0;
   for (int b = threadIdx.x; b < p.B; b += kPlanThreads) p.first[b] = kNoChild;
+  if (threadIdx.x == 0) again_s = 0;
   __syncthreads();
   for (int c = threadIdx.x; c < p.F; c += kPlanThreads) {
     int b, s, n, last;
@@ -236,11 +238,12 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
   // live pages: a team of threads per parent that has a child
   int team = kPlanThreads;
   while (team > 32 && (int64_t)(kPlanThreads / team) < p.B) team >>= 1;
-  bool shared = false;  // whether two parents end in the same partial page
+  int again = 0;  // partial pages marked, less those marked once
   constexpr int U = 4;
   for (int b = threadIdx.x / team; b < p.B; b += kPlanThreads / team) {
-    if (p.first[b] == kNoChild) continue;
-    const int s = __ldg(p.indptr + b), e = __ldg(p.indptr + b + 1), last = __ldg(p.last + b);
+    // (asked for together; the bounds of a parent without children may be anything)
+    const int child = p.first[b], s = __ldg(p.indptr + b), e = __ldg(p.indptr + b + 1), last = __ldg(p.last + b);
+    if (child == kNoChild) continue;
     const int n = e - s, whole = last < p.P ? n - 1 : n;  // the entries before it are whole pages
     for (int64_t i0 = threadIdx.x % team; i0 < n; i0 += (int64_t)U * team) {
       int id[U];
@@ -254,20 +257,25 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
           record_status(kStatusBadPage);
           continue;
         }
-        const uint32_t bit = 1u << (id[u] & 31);
-        if (i < whole) atomicOr(held + (id[u] >> 5), bit);
-        else shared |= (atomicOr(partial + (id[u] >> 5), bit) & bit) != 0;
+        atomicOr((i < whole ? held : partial) + (id[u] >> 5), 1u << (id[u] & 31));
+        again += i >= whole;
       }
     }
   }
   // Who keeps a partial page: first[b] stays where b's first child does, and becomes -1 where every child copies.
   // Only where two parents end in the same page, or one ends in a page that is held, does it change; the other
-  // batches pay for the look (fork of 16 beams 8.5 us in a graph against 7.6 without it, of 1024 children of 300
-  // parents 23.4 against 20.1).
-  shared = __syncthreads_or(shared);
+  // batches pay for the look (fork of 16 beams 8.6 us in a graph against 7.8 without it, of 1024 children of 300
+  // parents 25.3 against 22.1).
+  __syncthreads();
   bool both = false;
-  for (int64_t w = threadIdx.x; w < words; w += kPlanThreads) both |= (held[w] & partial[w]) != 0;
+  for (int64_t w = threadIdx.x; w < words; w += kPlanThreads) {
+    both |= (held[w] & partial[w]) != 0;
+    again -= __popc(partial[w]);
+  }
+  again = __reduce_add_sync(0xffffffffu, again);
+  if ((threadIdx.x & 31) == 0 && again) atomicAdd(&again_s, again);
   both = __syncthreads_or(both);
+  const bool shared = again_s != 0;
   if (shared) {
     for (int b = threadIdx.x; b < p.B; b += kPlanThreads) {
       const int id = p.first[b] == kNoChild ? -1 : partial_page(p, b);
