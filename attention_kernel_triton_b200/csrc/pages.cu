@@ -205,12 +205,12 @@ __device__ __forceinline__ bool fork_parent(const ForkParams& p, int c, int& b, 
 
 constexpr int kNoChild = 0x7fffffff;
 
-// The partly filled last page of a named parent (its bounds are good), or -1: it has none, or one outside the pool.
+// The partly filled last page of a named parent (its bounds are good); -1: it has none, -2: one outside the pool.
 __device__ __forceinline__ int partial_page(const ForkParams& p, int b) {
   const int s = __ldg(p.indptr + b), e = __ldg(p.indptr + b + 1);
   if (e <= s || __ldg(p.last + b) >= p.P) return -1;
   const int id = __ldg(p.indices + e - 1);
-  return id >= 0 && id < p.num_pages ? id : -1;
+  return id >= 0 && id < p.num_pages ? id : -2;
 }
 
 // Two bits per page: `held`, a whole page of a named parent or reserved, which nobody may write; and `partial`, a
@@ -238,7 +238,8 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
   // live pages: a team of threads per parent that has a child
   int team = kPlanThreads;
   while (team > 32 && (int64_t)(kPlanThreads / team) < p.B) team >>= 1;
-  int again = 0;  // partial pages marked, less those marked once
+  int again = 0;      // partial pages marked, less those marked once
+  bool look = false;  // whether the keepers have to be looked up
   constexpr int U = 4;
   for (int b = threadIdx.x / team; b < p.B; b += kPlanThreads / team) {
     // (asked for together; the bounds of a parent without children may be anything)
@@ -255,6 +256,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
         if (i >= n) continue;
         if (id[u] < 0 || id[u] >= p.num_pages) {
           record_status(kStatusBadPage);
+          look |= i >= whole;
           continue;
         }
         atomicOr((i < whole ? held : partial) + (id[u] >> 5), 1u << (id[u] & 31));
@@ -262,19 +264,18 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
       }
     }
   }
-  // Who keeps a partial page: first[b] stays where b's first child does, and becomes -1 where every child copies.
-  // Only where two parents end in the same page, or one ends in a page that is held, does it change; the other
-  // batches pay for the look (fork of 16 beams 8.6 us in a graph against 7.8 without it, of 1024 children of 300
-  // parents 25.3 against 22.1).
+  // Who keeps a partial page: first[b] stays where b's first child does, and becomes -1 where every child copies and
+  // kNoChild where there is nothing to copy.  Only where two parents end in the same page, or one ends in a page that
+  // is held or outside the pool, does it change; the other batches pay for the look (fork of 16 beams 8.5 us in a
+  // graph against 7.6 without it, of 1024 children of 300 parents 23.0 against 20.1).
   __syncthreads();
-  bool both = false;
   for (int64_t w = threadIdx.x; w < words; w += kPlanThreads) {
-    both |= (held[w] & partial[w]) != 0;
+    look |= (held[w] & partial[w]) != 0;
     again -= __popc(partial[w]);
   }
   again = __reduce_add_sync(0xffffffffu, again);
   if ((threadIdx.x & 31) == 0 && again) atomicAdd(&again_s, again);
-  both = __syncthreads_or(both);
+  look = __syncthreads_or(look);
   const bool shared = again_s != 0;
   if (shared) {
     for (int b = threadIdx.x; b < p.B; b += kPlanThreads) {
@@ -288,10 +289,11 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
     }
     __syncthreads();
   }
-  if (shared || both) {
+  if (shared || look) {
     for (int b = threadIdx.x; b < p.B; b += kPlanThreads) {
       const int id = p.first[b] == kNoChild ? -1 : partial_page(p, b);
-      if (id >= 0 && ((held[id >> 5] >> (id & 31) & 1u) || (shared && p.owner[id] != p.first[b]))) p.first[b] = -1;
+      if (id == -2) p.first[b] = kNoChild;
+      else if (id >= 0 && ((held[id >> 5] >> (id & 31) & 1u) || (shared && p.owner[id] != p.first[b]))) p.first[b] = -1;
     }
   }
   // the children's table bounds, and which of them need a page of their own
@@ -307,7 +309,8 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
     const int64_t room = max((int64_t)0, p.max_entries - begin);
     const bool cut = n > room;
     const int kept = cut ? (int)room : n;
-    const int own = c < p.F && n > 0 && !cut && last < p.P && p.first[b] != c;
+    const int keeper = c < p.F && n > 0 ? p.first[b] : kNoChild;
+    const int own = !cut && last < p.P && keeper != c && keeper != kNoChild;
     int n_own;
     const int r = copies + block_scan<int>(own, sums, n_own);
     if (c < p.F) {

@@ -1,4 +1,4 @@
-"""A fork whose children name more entries than its buffer, and than 32 bits, hold."""
+"""Forks at their limits: more entries than the buffer, and than 32 bits, hold; a last page outside the pool."""
 import pytest
 import torch
 
@@ -24,3 +24,14 @@ def test_sums_of_entries_past_32_bits():
     assert starts.tolist() == [0] + [most] * F
     assert torch.equal(out, indices[:most]) and last.tolist() == [1] + [0] * (F - 1)
     assert _lib.device_status(0, clear=True) == 5
+
+
+def test_last_pages_outside_the_pool_are_kept_by_every_child():
+    _lib.device_status(0, clear=True)
+    pool = torch.randn((8, 2, 1, 4, 16), device=DEV).half()
+    before = pool.clone()
+    for bad in (1 << 20, -7):
+        t = fork_paged_kv_cache(pool, i32([0, 2, 4]), i32([3, bad, 5, 6]), i32([2, 4]), i32([0, 0, 1, 0]))
+        assert t[1].tolist() == [3, bad, 3, bad, 5, 6, 3, bad] and t[2].tolist() == [2, 2, 4, 2]
+        assert torch.equal(pool, before)
+        assert _lib.device_status(0, clear=True) == 2
