@@ -1478,7 +1478,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // -------------------------------------------------------------------------
 // O = sum_i e^{lse_i - M} O_i / sum_i e^{lse_i - M}.  The unit's parts are the one
 // with its first keys and then place 0 of the CTAs after it, up to the one with
-// its last keys.  CTA (x, y): place x, rows [R y, R y + R), R = merge_rows; a warp per row.
+// its last keys; the ones without keys for the row (lse_i = -inf) are left out.  CTA (x, y): place x, rows [R y, R y + R), R = merge_rows; a warp per row.
 constexpr int kMergeThreads = 256;
 
 template <typename T, int D>
@@ -1796,7 +1796,7 @@ extern "C" int akt_chunk_paged(const akt_chunk_paged_args* a, void* workspace, s
   p.part_o = reinterpret_cast<float*>(ws + y.o);
   p.part_rows = y.part_rows;
   // A row of a merge is a chain of lookups, so few rows get a warp each (4 tokens on 2048
-  // keys, whole call in a graph 20.3 us, 22.5 with four rows a warp; on 32768 keys 43.7, 47.8);
+  // keys, whole call in a graph 20.6 us, 22.5 with four rows a warp; on 32768 keys 43.7, 47.8);
   // many rows would be many CTAs that mostly find nothing to join (8 prompts of 2048
   // tokens: 305 us, 316 with a row a warp).
   p.merge_rows = y.part_rows <= 64 ? 8 : 32;

@@ -7,7 +7,7 @@
 // every call gives the same result when it is repeated on the same table.
 //
 // Each call is a plan by one CTA and then, where pages are copied, a grid that
-// applies it.  The plan is integer work on one bit per page, held in shared
+// applies it.  The plan is integer work on a bit or two per page, held in shared
 // memory up to kSmemPages pages: mark the live pages, then walk the words with
 // block-wide prefix sums of their popcounts, which hands out dead pages in
 // ascending order.  Writes go to dead pages only and reads come from live

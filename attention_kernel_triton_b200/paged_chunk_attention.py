@@ -10,8 +10,10 @@ V are in the pool already (``append_paged_kv_cache`` or
 ``append_rotary_paged_kv_cache`` with the same ``indptr``): row ``i`` stands at
 position ``len_b - n_b + i``.  With ``causal`` it sees the keys up to its own
 position, else all ``len_b``.  A row that sees no key (an empty sequence, a chunk
-longer than its sequence) gives zeros.  Runs ``akt_chunk_paged`` (sm_100a) on
-torch's current stream.
+longer than its sequence) or that no sequence has gives zeros.  Scores, sums and
+partial results are in fp32; the softmax weights are rounded to the inputs' type
+for the product with V, as in the package's prefill and decode.  No gradient.
+Runs ``akt_chunk_paged`` (sm_100a) on torch's current stream.
 """
 from __future__ import annotations
 

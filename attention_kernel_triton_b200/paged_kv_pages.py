@@ -4,7 +4,7 @@ listed as free (the reference's drivers build one fixed page table).
 The page table ``(kv_page_indptr, kv_page_indices, kv_last_page_len)`` of the
 paged decodes is the only record: a page is live when the table names it, or
 when the optional ``reserved`` mask (``[num_pages]`` bool: pages that another
-holder keeps, a prefix store's say) marks it.  Every call below takes the table
+holder keeps, a prefix store's say, named by the table or not) marks it.  Every call below takes the table
 of the whole pool and returns a new one; the old table stays valid for what was
 launched before.  Dropping a sequence is leaving it out; there are no reference
 counts.  The pool is ``[num_pages, 2, Hkv, page_size, D]``, or

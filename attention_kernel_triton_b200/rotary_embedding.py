@@ -239,7 +239,7 @@ def append_rotary_paged_kv_cache(paged_kv_cache, q, append_k, append_v, append_i
     ``q`` (or None: nothing is returned), ``append_k`` and ``append_v`` are
     ``[num_append, heads, D]``, ragged by ``append_indptr [B + 1]``; the page table already
     describes the sequences after the append.  One pass: the rotated keys are never stored
-    outside the pool.
+    outside the pool.  For serving: no gradient.
     """
     index = _lib.device_index(paged_kv_cache, append_k, append_v, cos_sin)
     dtype = paged_kv_cache.dtype
