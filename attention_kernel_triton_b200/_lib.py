@@ -215,6 +215,47 @@ class CompactPagedArgs(Structure):
     ]
 
 
+class AttentionWeightsArgs(Structure):
+    _fields_ = [
+        ("q", c_void_p), ("q_stride_token", c_int64), ("q_stride_head", c_int64), ("q_stride_dim", c_int64),
+        ("q_indptr", c_void_p), ("num_tokens", c_int64),
+        ("kv_cache", c_void_p), ("kv_stride_page", c_int64), ("kv_stride_kv", c_int64), ("kv_stride_head", c_int64),
+        ("kv_stride_token", c_int64), ("kv_stride_dim", c_int64), ("num_pages", c_int64),
+        ("kv_page_indptr", c_void_p), ("kv_page_indices", c_void_p), ("kv_last_page_len", c_void_p),
+        ("num_page_entries", c_int64),
+        ("lse", c_void_p), ("lse_stride_token", c_int64), ("lse_stride_head", c_int64),
+        ("weights", c_void_p), ("weights_stride_batch", c_int64), ("weights_stride_head", c_int64),
+        ("out", c_void_p), ("out_stride_batch", c_int64), ("out_stride_head", c_int64), ("width", c_int64),
+        ("batch", c_int32), ("num_qo_heads", c_int32), ("num_kv_heads", c_int32), ("page_size", c_int32),
+        ("head_dim", c_int32), ("causal", c_int32), ("dtype", c_int32), ("softmax_scale", c_float),
+    ]
+
+
+class SelectTokensArgs(Structure):
+    _fields_ = [
+        ("weights", c_void_p), ("weights_stride_layer", c_int64), ("weights_stride_batch", c_int64),
+        ("weights_stride_head", c_int64), ("seq_lens", c_void_p),
+        ("keep_ind", c_void_p), ("keep_stride_layer", c_int64), ("keep_stride_batch", c_int64),
+        ("keep_stride_head", c_int64), ("keep_len", c_void_p), ("width", c_int64),
+        ("layers", c_int32), ("batch", c_int32), ("num_heads", c_int32), ("budget", c_int32), ("sinks", c_int32),
+        ("recent", c_int32),
+    ]
+
+
+class EvictPagedArgs(Structure):
+    _fields_ = [
+        ("pool", PagePool),
+        ("kv_page_indptr", c_void_p), ("kv_page_indices", c_void_p), ("kv_last_page_len", c_void_p),
+        ("num_page_entries", c_int64),
+        ("keep_ind", c_void_p), ("keep_stride_layer", c_int64), ("keep_stride_batch", c_int64),
+        ("keep_stride_head", c_int64), ("keep_len", c_void_p), ("max_kept", c_int64), ("reserved", c_void_p),
+        ("weights", c_void_p), ("weights_stride_layer", c_int64), ("weights_stride_batch", c_int64),
+        ("weights_stride_head", c_int64), ("width", c_int64),
+        ("out_indptr", c_void_p), ("out_indices", c_void_p), ("out_last_page_len", c_void_p),
+        ("max_entries", c_int64), ("batch", c_int32),
+    ]
+
+
 AKT_MAX_PEERS = 8
 
 
@@ -277,6 +318,11 @@ SIGNATURES = {
     "akt_fork_paged": (c_int, [POINTER(ForkPagedArgs), c_void_p, c_size_t, c_void_p]),
     "akt_compact_paged_workspace_size": (c_size_t, [POINTER(CompactPagedArgs)]),
     "akt_compact_paged": (c_int, [POINTER(CompactPagedArgs), c_void_p, c_size_t, c_void_p]),
+    "akt_attention_weights_workspace_size": (c_size_t, [POINTER(AttentionWeightsArgs)]),
+    "akt_attention_weights": (c_int, [POINTER(AttentionWeightsArgs), c_void_p, c_size_t, c_void_p]),
+    "akt_select_tokens": (c_int, [POINTER(SelectTokensArgs), c_void_p]),
+    "akt_evict_paged_workspace_size": (c_size_t, [POINTER(EvictPagedArgs)]),
+    "akt_evict_paged": (c_int, [POINTER(EvictPagedArgs), c_void_p, c_size_t, c_void_p]),
     "akt_free_kv_pages_workspace_size": (c_size_t, [c_int64]),
     "akt_free_kv_pages": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_size_t,
                                   c_void_p]),

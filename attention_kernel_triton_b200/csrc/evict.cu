@@ -1,0 +1,636 @@
+// Eviction from a paged KV cache: which tokens of each head stay, and the pool
+// with only those.  No reference counterpart (its sparse decodes take lists of
+// kept tokens, SD:7-66, that its drivers draw at random).
+//
+// Choice.  Of a head's n tokens the first `sinks`, the last `recent` and the k
+// heaviest of the others stay.  The k-th largest weight is found by a radix
+// select over an order-preserving map of fp32 to 32-bit keys (digits of 11, 11
+// and 10 bits from the top, a histogram each), then the list is written in
+// ascending order by ballots and prefix sums, the lowest of equal weights first.
+// A cluster of CTAs holds the head's keys in shared memory, so the weights are
+// read once; the histograms and counts are summed over distributed shared memory.
+//
+// Eviction.  Slot i of a head takes the row of token keep[i].  Lists ascend, so
+// keep[i] >= i: rows only move down and a sequence can stay in its own pages.  A
+// cluster walks a head's rows in order, a chunk in registers at a time: all of a
+// chunk is read before any of it is written (the cluster's barrier), and no later
+// chunk's source lies below a slot that is written by then.  So a chunk's reads
+// run ahead of the stores of the one before it.
+//
+// Pages that others have too (named twice by the table, or reserved) are never
+// written: one that keeps all its rows in place and is full stays shared, any
+// other is replaced by a dead page, in ascending order.  The plan is integer work
+// of one cluster on two bits per page.
+#include "cluster.cuh"
+#include "common.cuh"
+#include "profile.cuh"
+#include "scan.cuh"
+
+#include <algorithm>
+#include <string>
+
+namespace akt {
+int set_error(int code, const std::string& msg);
+
+namespace {
+
+int sm_count() {
+  int dev = 0, n = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n > 0 ? n : 148;
+}
+
+int cuda_error(const char* what, cudaError_t e) {
+  return set_error(AKT_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+}
+
+// ---------------------------------------------------------------------------
+// choice of the kept tokens
+// ---------------------------------------------------------------------------
+constexpr int kSelectThreads = 1024;
+constexpr int kBins = 2048;
+constexpr int kMaxKeys = 48 * 1024;  // of a CTA in shared memory
+
+struct SelectParams {
+  const float* w;
+  int64_t w_layer, w_batch, w_head;
+  const int32_t* lens;
+  int32_t* ind;
+  int64_t i_layer, i_batch, i_head;
+  int32_t* kept;
+  int B, H, width, budget, sinks, recent;
+  int cached;  // the CTA's share of a head fits its shared memory
+};
+
+// Larger floats have larger keys; -0 is 0, and NaN comes below everything.
+__device__ __forceinline__ uint32_t order_key(float f) {
+  if (f != f) return 0u;
+  const uint32_t u = __float_as_uint(f + 0.f);
+  return u >> 31 ? ~u : u | 0x80000000u;
+}
+
+__global__ void __launch_bounds__(kSelectThreads) select_kernel(const SelectParams p) {
+  extern __shared__ uint32_t keys_s[];
+  __shared__ int hist[3][kBins];
+  __shared__ int sums[33];
+  __shared__ int found[2];       // digit, how many are wanted of it
+  __shared__ int warp_count[2][32];
+  __shared__ int cta_count[2];   // tokens that stay for sure, tokens at the threshold
+  const int C = (int)cluster_size(), rank = (int)cluster_rank(), row = blockIdx.x / C;
+  const int h = row % p.H, b = row / p.H % p.B, l = row / p.H / p.B;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int asked = __ldg(p.lens + b), n = min(max(asked, 0), p.width);
+  if (asked != n && threadIdx.x == 0) record_status(kStatusBadToken);
+  int32_t* ind = p.ind + l * p.i_layer + b * p.i_batch + h * p.i_head;
+  if (l == 0 && h == 0 && rank == 0 && threadIdx.x == 0) p.kept[b] = min(n, p.budget);
+  if (n <= p.budget) {  // all stay
+    for (int i = rank * kSelectThreads + threadIdx.x; i < p.budget; i += C * kSelectThreads) ind[i] = i < n ? i : 0;
+    return;
+  }
+  const float* w = p.w + l * p.w_layer + b * p.w_batch + h * p.w_head;
+  const int slice = ((n + C - 1) / C + 31) / 32 * 32, lo = min(rank * slice, n), hi = min(lo + slice, n);
+  const int k = p.budget - p.sinks - p.recent, c0 = p.sinks, c1 = n - p.recent;  // candidates [c0, c1)
+  for (int i = threadIdx.x; i < 3 * kBins; i += kSelectThreads) (&hist[0][0])[i] = 0;
+  if (p.cached) {
+    constexpr int U = 8;
+    for (int j = lo + threadIdx.x; j < hi; j += U * kSelectThreads) {
+      float f[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) f[u] = j + u * kSelectThreads < hi ? __ldg(w + j + u * kSelectThreads) : 0.f;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (j + u * kSelectThreads < hi) keys_s[j + u * kSelectThreads - lo] = order_key(f[u]);
+    }
+  }
+  __syncthreads();
+  auto key = [&](int j) -> uint32_t { return p.cached ? keys_s[j - lo] : order_key(__ldg(w + j)); };
+  uint32_t top = 0, mask = 0;  // the threshold's digits so far
+  int want = k;
+  if (k > 0) {
+#pragma unroll 1
+    for (int d = 0; d < 3; ++d) {
+      const int shift = d == 0 ? 21 : (d == 1 ? 10 : 0);
+      const uint32_t digit_mask = d == 2 ? 0x3ffu : 0x7ffu;
+      for (int j = max(lo, c0) + threadIdx.x; j < min(hi, c1); j += kSelectThreads) {
+        const uint32_t x = key(j);
+        if ((x & mask) == top) atomicAdd(&hist[d][(x >> shift) & digit_mask], 1);
+      }
+      if (C > 1) cluster_sync(); else __syncthreads();
+      // the two bins of this thread, from the top
+      int own[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int bin = kBins - 1 - 2 * (int)threadIdx.x - e;
+        own[e] = 0;
+        for (int r = 0; r < C; ++r) own[e] += C > 1 ? cluster_read(&hist[d][bin], r) : hist[d][bin];
+      }
+      int all;
+      const int before = block_scan<int>(own[0] + own[1], sums, all);
+      if (before < want && want <= before + own[0] + own[1]) {
+        const int e = want > before + own[0];
+        found[0] = kBins - 1 - 2 * (int)threadIdx.x - e;
+        found[1] = want - before - (e ? own[0] : 0);
+      }
+      __syncthreads();
+      top |= (uint32_t)found[0] << shift;
+      mask |= digit_mask << shift;
+      want = found[1];
+    }
+  }
+  // which tokens stay: the ones always kept, the ones above the threshold, `want` of the ones at it
+  auto state = [&](int j) -> int {  // 2: stays, 1: at the threshold
+    if (j < c0 || j >= c1) return 2;
+    if (k == 0) return 0;
+    const uint32_t x = key(j);
+    return x > top ? 2 : (x == top ? 1 : 0);
+  };
+  const int seg = slice / 32 + 31 & ~31, s0 = min(lo + warp * seg, hi), s1 = min(s0 + seg, hi);
+  int n_sure = 0, n_equal = 0;
+  for (int j0 = s0; j0 < s1; j0 += 32) {
+    const int st = j0 + lane < s1 ? state(j0 + lane) : 0;
+    n_sure += __popc(__ballot_sync(0xffffffffu, st == 2));
+    n_equal += __popc(__ballot_sync(0xffffffffu, st == 1));
+  }
+  if (lane == 0) {
+    warp_count[0][warp] = n_sure;
+    warp_count[1][warp] = n_equal;
+  }
+  __syncthreads();
+  int sure = 0, equal = 0;  // before this warp's tokens
+  for (int i = 0; i < warp; ++i) {
+    sure += warp_count[0][i];
+    equal += warp_count[1][i];
+  }
+  if (threadIdx.x == kSelectThreads - 1) {
+    cta_count[0] = sure + n_sure;
+    cta_count[1] = equal + n_equal;
+  }
+  if (C > 1) {
+    cluster_sync();
+    for (int r = 0; r < rank; ++r) {
+      sure += cluster_read(&cta_count[0], r);
+      equal += cluster_read(&cta_count[1], r);
+    }
+  }
+  const unsigned below = (1u << lane) - 1u;
+  for (int j0 = s0; j0 < s1; j0 += 32) {
+    const int j = j0 + lane, st = j < s1 ? state(j) : 0;
+    const unsigned m2 = __ballot_sync(0xffffffffu, st == 2), m1 = __ballot_sync(0xffffffffu, st == 1);
+    const int eq = equal + __popc(m1 & below);
+    if (st == 2 || (st == 1 && eq < want)) ind[sure + __popc(m2 & below) + min(eq, want)] = j;
+    sure += __popc(m2);
+    equal += __popc(m1);
+  }
+  if (C > 1) cluster_sync();  // the others' reads of this CTA's counts
+}
+
+// ---------------------------------------------------------------------------
+// eviction: the plan
+// ---------------------------------------------------------------------------
+constexpr int kPlanThreads = 1024;
+
+struct EvictParams {
+  char* kv;
+  int64_t s_layer, s_page, s_kv, s_head, s_tok;  // bytes
+  int64_t num_pages, num_entries, max_entries;
+  const int32_t* indptr;
+  const int32_t* indices;
+  const int32_t* last;
+  const int32_t* keep;
+  int64_t k_layer, k_batch, k_head;
+  const int32_t* kept;
+  const uint8_t* reserved;
+  float* w;
+  int64_t w_layer, w_batch, w_head;
+  int32_t* out_indptr;
+  int32_t* out_indices;
+  int32_t* out_last;
+  int layers, B, H, P, M, width;
+  FastDiv div_page, div_piece;
+  int pieces;  // of a row
+  int rows;    // of a CTA's chunk
+  // workspace
+  uint32_t* seen;   // [words] live pages
+  uint32_t* again;  // [words] pages of more than one holder
+  int32_t* dead;    // [max_entries] the dead pages that are given out
+  int32_t* lens;    // [B] tokens before
+  int32_t* count;   // [B] tokens after
+  int32_t* moved;   // [B] first page that is replaced, or one past all
+};
+
+// What the lists say of the row of slot i: its token, or -1 where it is no good
+// (behind the sequence, below its slot, or not above the one before it).
+__device__ __forceinline__ int kept_token(const EvictParams& p, const int32_t* keep, int i, int len) {
+  const int j = __ldg(keep + i), before = i ? __ldg(keep + i - 1) : -1;
+  if (j >= i && j < len && j > before) return j;
+  record_status(kStatusBadToken);
+  return -1;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictParams p) {
+  __shared__ int64_t sums64[33];
+  __shared__ int sums[33];
+  __shared__ int n_fresh, n_dead;
+  const int C = (int)cluster_size(), rank = (int)cluster_rank(), tid = threadIdx.x;
+  const int64_t words = (p.num_pages + 31) / 32;
+  const int64_t w0 = words * rank / C, w1 = words * (rank + 1) / C;
+  for (int64_t w = w0 + tid; w < w1; w += kPlanThreads) p.seen[w] = p.again[w] = 0;
+  if (rank == 0) {  // the new table's bounds
+    int64_t at = 0;
+    for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
+      const int b = b0 + tid;
+      int len = 0, n = 0;
+      if (b < p.B) {
+        const int s = __ldg(p.indptr + b), e = __ldg(p.indptr + b + 1);
+        if (s < 0 || e < s || e > p.num_entries) record_status(kStatusBadIndptr);
+        else if (e > s) len = (e - s - 1) * p.P + min(max(__ldg(p.last + b), 0), p.P);
+        const int asked = __ldg(p.kept + b);
+        n = min(max(asked, 0), min(len, p.M));
+        if (n != asked) record_status(kStatusBadToken);
+      }
+      const int pages = (n + p.P - 1) / p.P;
+      int64_t total;
+      const int64_t begin = at + block_scan<int64_t>(pages, sums64, total);
+      const int64_t room = max((int64_t)0, p.max_entries - begin);
+      if (b < p.B) {
+        if (pages > room) {
+          record_status(kStatusListOverflow);
+          n = (int)room * p.P;
+        }
+        const int mine = (n + p.P - 1) / p.P;
+        p.out_indptr[b] = (int)min(begin, p.max_entries);
+        p.out_last[b] = mine ? n - (mine - 1) * p.P : 0;
+        p.lens[b] = len;
+        p.count[b] = n;
+        p.moved[b] = mine;
+      }
+      at += total;
+    }
+    if (tid == 0) p.out_indptr[p.B] = (int)min(at, p.max_entries);
+  }
+  cluster_sync();
+  // pages by how many hold them
+  constexpr int U = 4;
+  for (int64_t i = (int64_t)rank * kPlanThreads + tid; i < p.num_entries; i += (int64_t)U * C * kPlanThreads) {
+    int id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = i + (int64_t)u * C * kPlanThreads;
+      id[u] = at < p.num_entries ? __ldg(p.indices + at) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (id[u] < 0 || id[u] >= p.num_pages) {
+        if (id[u] >= 0) record_status(kStatusBadPage);
+        continue;
+      }
+      const uint32_t bit = 1u << (id[u] & 31);
+      if (atomicOr(p.seen + (id[u] >> 5), bit) & bit) atomicOr(p.again + (id[u] >> 5), bit);
+    }
+  }
+  if (p.reserved)
+    for (int64_t w = w0 + tid; w < w1; w += kPlanThreads) {
+      uint32_t m = 0;
+      for (int i = 0; i < 32 && w * 32 + i < p.num_pages; ++i) m |= (p.reserved[w * 32 + i] ? 1u : 0u) << i;
+      if (m) {
+        atomicOr(p.seen + w, m);
+        atomicOr(p.again + w, m);
+      }
+    }
+  cluster_sync();
+  // the new table's pages; one that has to be replaced is noted by its number among those
+  const int N = __ldcg(p.out_indptr + p.B);
+  const int g0 = (int)((int64_t)N * rank / C), g1 = (int)((int64_t)N * (rank + 1) / C);
+  int fresh = 0;
+  for (int t0 = g0; t0 < g1; t0 += kPlanThreads) {
+    const int g = t0 + tid;
+    int page = -1, replace = 0;
+    if (g < g1) {
+      int b = 0, hi = p.B - 1;
+      while (b < hi) {
+        const int mid = (b + hi + 1) >> 1;
+        if (__ldcg(p.out_indptr + mid) <= g) b = mid; else hi = mid - 1;
+      }
+      const int e = g - __ldcg(p.out_indptr + b), n = __ldcg(p.count + b);
+      page = __ldg(p.indices + __ldg(p.indptr + b) + e);
+      if (page >= 0 && page < p.num_pages && (__ldcg(p.again + (page >> 5)) >> (page & 31) & 1u)) {
+        const int end = min((e + 1) * p.P, n) - 1;  // the page's last row: in its place only if all are
+        replace = end + 1 < (e + 1) * p.P;
+        for (int i = 0; i < p.layers * p.H && !replace; ++i)
+          replace = __ldg(p.keep + i / p.H * p.k_layer + b * p.k_batch + i % p.H * p.k_head + end) != end;
+        if (replace) atomicMin(p.moved + b, e);
+      }
+    }
+    int here;
+    const int r = fresh + block_scan<int>(replace, sums, here);
+    if (g < g1) p.out_indices[g] = replace ? -2 - r : page;
+    fresh += here;
+  }
+  for (int64_t g = (int64_t)N + rank * kPlanThreads + tid; g < p.max_entries; g += (int64_t)C * kPlanThreads)
+    p.out_indices[g] = -1;
+  if (tid == 0) n_fresh = fresh;
+  cluster_sync();
+  int first = 0, all = 0;
+  for (int r = 0; r < C; ++r) {
+    const int x = cluster_read(&n_fresh, r);
+    if (r < rank) first += x;
+    all += x;
+  }
+  if (all) {  // the same in every CTA
+    // the lowest dead pages, in ascending order
+    int mine = 0, dead_here;
+    for (int64_t w = w0 + tid; w < w1; w += kPlanThreads) {
+      const int64_t left = p.num_pages - w * 32;
+      mine += __popc(~__ldcg(p.seen + w) & (left >= 32 ? 0xffffffffu : (1u << left) - 1u));
+    }
+    block_scan<int>(mine, sums, dead_here);
+    if (tid == 0) n_dead = dead_here;
+    cluster_sync();
+    int r0 = 0, found = 0;
+    for (int r = 0; r < C; ++r) {
+      const int x = cluster_read(&n_dead, r);
+      if (r < rank) r0 += x;
+      found += x;
+    }
+    for (int64_t v0 = w0; v0 < w1 && r0 < all; v0 += kPlanThreads) {
+      const int64_t w = v0 + tid, left = p.num_pages - w * 32;
+      uint32_t d = w < w1 ? ~__ldcg(p.seen + w) & (left >= 32 ? 0xffffffffu : (1u << left) - 1u) : 0u;
+      int total;
+      int r = r0 + block_scan<int>(__popc(d), sums, total);
+      for (; d && r < all; d &= d - 1) p.dead[r++] = (int)(w * 32) + __ffs(d) - 1;
+      r0 += total;
+    }
+    cluster_sync();
+    for (int g = g0 + tid; g < g1; g += kPlanThreads) {
+      const int v = p.out_indices[g];
+      if (v > -2) continue;
+      const int r = first + (-2 - v);
+      if (r >= found) record_status(kStatusNoDeadPage);
+      p.out_indices[g] = r < found ? __ldcg(p.dead + r) : -1;
+    }
+  }
+  cluster_sync();  // the others' reads of this CTA's counts
+}
+
+// ---------------------------------------------------------------------------
+// eviction: the rows
+// ---------------------------------------------------------------------------
+constexpr int kMoveThreads = 512;
+constexpr int kMovePieces = 8;    // of a thread in a chunk
+constexpr int kMaxRows = 512;     // of a CTA's chunk
+
+template <int W>
+struct Piece;
+template <>
+struct Piece<16> { using type = uint4; };
+template <>
+struct Piece<2> { using type = uint16_t; };
+
+// Cluster (layer, sequence, head, part): part 0 is K, 1 is V, 2 the weights.
+template <int W>
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictParams p) {
+  using V = typename Piece<W>::type;
+  constexpr int U = kMovePieces;
+  __shared__ int64_t from[2][kMaxRows], to[2][kMaxRows];  // bytes; from < 0: nothing moves
+  const int C = (int)cluster_size(), rank = (int)cluster_rank(), tid = threadIdx.x, parts = p.w ? 3 : 2;
+  int unit = blockIdx.x / C;
+  const int part = unit % parts;
+  unit /= parts;
+  const int h = unit % p.H, b = unit / p.H % p.B, l = unit / p.H / p.B;
+  grid_dep_wait();
+  const int n = p.count[b], len = p.lens[b];
+  const int s = __ldg(p.indptr + b), os = p.out_indptr[b];
+  const int32_t* keep = p.keep + l * p.k_layer + b * p.k_batch + h * p.k_head;
+  // the rows that stay in place are the first ones
+  const int step = (n + kMoveThreads - 1) / kMoveThreads;
+  int start = 0;
+  if (n) {
+    const int i = min((tid + 1) * step, n) - 1;
+    start = min(__syncthreads_count(__ldg(keep + i) == i) * step, n);
+  }
+  if (part == 2) {
+    float* w = p.w + l * p.w_layer + b * p.w_batch + h * p.w_head;
+    const int per = U * kMoveThreads, turns = (n - start + C * per - 1) / (C * per);
+    for (int it = 0; it < turns; ++it) {
+      const int i0 = start + (it * C + rank) * per + tid;
+      float v[U];
+      int ok = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * kMoveThreads, j = i < n ? kept_token(p, keep, i, len) : -1;
+        v[u] = 0.f;
+        if (j < 0 || j >= p.width) continue;
+        v[u] = w[j];
+        ok |= 1 << u;
+      }
+      cluster_sync();
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (ok >> u & 1) w[i0 + u * kMoveThreads] = v[u];
+    }
+    for (int i = n + rank * kMoveThreads + tid; i < min(len, p.width); i += C * kMoveThreads) w[i] = 0.f;
+    return;
+  }
+  // a page that is replaced takes its rows along even if they stay in their places
+  start = (int)min((int64_t)start, (int64_t)p.moved[b] * p.P);
+  const int R = p.rows, turns = (n - start + C * R - 1) / (C * R);
+  char* base = p.kv + l * p.s_layer + part * p.s_kv + h * p.s_head;
+  auto addresses = [&](int it) {  // of the rows of chunk `it`
+    for (int r = tid; r < R; r += kMoveThreads) {
+      const int i = start + (it * C + rank) * R + r;
+      int64_t f = -1, t = 0;
+      if (i < n) {
+        const int j = kept_token(p, keep, i, len);
+        if (j >= 0) {
+          const int pj = (int)fdiv((uint32_t)j, p.div_page), pi = (int)fdiv((uint32_t)i, p.div_page);
+          const int src = __ldg(p.indices + s + pj), dst = p.out_indices[os + pi];
+          if (src >= 0 && src < p.num_pages && dst >= 0 && dst < p.num_pages && (src != dst || i != j)) {
+            f = src * p.s_page + (j - pj * p.P) * p.s_tok;
+            t = dst * p.s_page + (i - pi * p.P) * p.s_tok;
+          }
+        }
+      }
+      from[it & 1][r] = f;
+      to[it & 1][r] = t;
+    }
+  };
+  V val[U];
+  auto load = [&](int it) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t x = u * kMoveThreads + tid, r = fdiv(x, p.div_piece);
+      if (r < R && from[it & 1][r] >= 0)
+        val[u] = *reinterpret_cast<const V*>(base + from[it & 1][r] + (x - r * p.pieces) * W);
+    }
+  };
+  for (int it = 0; it < turns; ++it) {
+    addresses(it);
+    __syncthreads();
+    load(it);
+    cluster_sync();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t x = u * kMoveThreads + tid, r = fdiv(x, p.div_piece);
+      if (r < R && from[it & 1][r] >= 0)
+        *reinterpret_cast<V*>(base + to[it & 1][r] + (x - r * p.pieces) * W) = val[u];
+    }
+  }
+}
+
+size_t round16(size_t n) { return (n + 15) & ~size_t(15); }
+
+struct EvictLayout {
+  size_t seen, again, dead, lens, count, moved, bytes;
+};
+
+EvictLayout evict_layout(const akt_evict_paged_args* a) {
+  EvictLayout y{};
+  const size_t words = ((size_t)std::max<int64_t>(a->pool.num_pages, 0) + 31) / 32;
+  const size_t batch = (size_t)std::max(a->batch, 0), most = (size_t)std::max<int64_t>(a->max_entries, 0);
+  y.again = round16(words * 4);
+  y.dead = 2 * y.again;
+  y.lens = y.dead + round16(most * 4);
+  y.count = y.lens + round16(batch * 4);
+  y.moved = y.count + round16(batch * 4);
+  y.bytes = y.moved + round16(batch * 4) + 16;
+  return y;
+}
+
+}  // namespace
+}  // namespace akt
+
+using namespace akt;
+
+extern "C" int akt_select_tokens(const akt_select_tokens_args* a, void* stream) {
+  if (!a) return set_error(AKT_ERR_INVALID, "null args");
+  if (a->layers < 0 || a->batch < 0 || a->num_heads < 0 || a->width < 0 || a->budget < 0 || a->sinks < 0 || a->recent < 0)
+    return set_error(AKT_ERR_INVALID, "select_tokens: bad sizes");
+  if ((int64_t)a->sinks + a->recent > a->budget)
+    return set_error(AKT_ERR_INVALID, "select_tokens: sinks and recent together must not exceed the budget");
+  const int64_t rows = (int64_t)a->layers * a->batch * a->num_heads;
+  if (a->width > 0x3fffffff || a->budget > 0x3fffffff || rows > 0x7ffffff)
+    return set_error(AKT_ERR_INVALID, "select_tokens: too many tokens");
+  if (a->batch > 0 && (!a->seq_lens || !a->keep_len)) return set_error(AKT_ERR_INVALID, "select_tokens: missing tensor");
+  if (rows == 0) return AKT_OK;
+  if ((a->width > 0 && !a->weights) || (a->budget > 0 && !a->keep_ind))
+    return set_error(AKT_ERR_INVALID, "select_tokens: missing tensor");
+  SelectParams p{};
+  p.w = a->weights;
+  p.w_layer = a->weights_stride_layer;
+  p.w_batch = a->weights_stride_batch;
+  p.w_head = a->weights_stride_head;
+  p.lens = a->seq_lens;
+  p.ind = a->keep_ind;
+  p.i_layer = a->keep_stride_layer;
+  p.i_batch = a->keep_stride_batch;
+  p.i_head = a->keep_stride_head;
+  p.kept = a->keep_len;
+  p.B = a->batch;
+  p.H = a->num_heads;
+  p.width = (int)a->width;
+  p.budget = a->budget;
+  p.sinks = a->sinks;
+  p.recent = a->recent;
+  int C = 8;
+  while (C > 1 && (rows * C > 8 * sm_count() || p.width / C < 2048)) C /= 2;
+  const int slice = ((p.width + C - 1) / C + 31) / 32 * 32;
+  p.cached = slice <= kMaxKeys;
+  const size_t smem = p.cached ? (size_t)slice * 4 : 0;
+  cudaError_t e = ensure_smem_limit<select_kernel>(smem);
+  if (e != cudaSuccess) return cuda_error("select_tokens", e);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  {
+    ProfileScope prof(st);
+    e = launch_cluster(select_kernel, dim3((unsigned)(rows * C)), dim3(kSelectThreads), C, false, smem, st, p);
+  }
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return e == cudaSuccess ? AKT_OK : cuda_error("select_tokens", e);
+}
+
+extern "C" size_t akt_evict_paged_workspace_size(const akt_evict_paged_args* a) { return a ? evict_layout(a).bytes : 0; }
+
+extern "C" int akt_evict_paged(const akt_evict_paged_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!a) return set_error(AKT_ERR_INVALID, "null args");
+  const akt_page_pool& q = a->pool;
+  if (q.num_layers <= 0 || q.num_kv_heads <= 0 || q.page_size <= 0 || q.head_dim <= 0 || q.num_pages < 0)
+    return set_error(AKT_ERR_INVALID, "evict_paged: bad pool sizes");
+  if (a->batch < 0 || a->num_page_entries < 0 || a->max_entries < 0 || a->max_kept < 0 || a->width < 0)
+    return set_error(AKT_ERR_INVALID, "evict_paged: bad sizes");
+  if (q.num_pages > 0x7fffff00 || a->num_page_entries > 0x3fffffff / q.page_size || a->max_entries > 0x3fffffff ||
+      a->max_kept > 0x3fffffff || a->width > 0x3fffffff)
+    return set_error(AKT_ERR_INVALID, "evict_paged: too many tokens");
+  if (!q.kv_cache && q.num_pages > 0) return set_error(AKT_ERR_INVALID, "evict_paged: missing pool");
+  if (!a->out_indptr || (a->max_entries > 0 && !a->out_indices) ||
+      (a->batch > 0 && (!a->kv_page_indptr || !a->kv_last_page_len || !a->out_last_page_len || !a->keep_len)) ||
+      (a->batch > 0 && a->max_kept > 0 && !a->keep_ind) || (a->num_page_entries > 0 && !a->kv_page_indices))
+    return set_error(AKT_ERR_INVALID, "evict_paged: missing table");
+  if (q.stride_dim != 1) return set_error(AKT_ERR_UNSUPPORTED, "evict_paged: unit dim stride required");
+  const int64_t row = (int64_t)q.head_dim * 2;
+  EvictParams p{};
+  p.kv = static_cast<char*>(q.kv_cache);
+  p.s_layer = q.num_layers > 1 ? q.stride_layer * 2 : 0;
+  p.s_page = q.stride_page * 2;
+  p.s_kv = q.stride_kv * 2;
+  p.s_head = q.stride_head * 2;
+  p.s_tok = q.stride_token * 2;
+  // 16-byte pieces where every row and stride allows them, else single values
+  const uint64_t bits = (uint64_t)(uintptr_t)q.kv_cache |
+                        (uint64_t)(p.s_layer | p.s_page | p.s_kv | (q.num_kv_heads > 1 ? p.s_head : 0) |
+                                   (q.page_size > 1 ? p.s_tok : 0) | row);
+  const int W = (bits & 15u) ? 2 : 16;
+  if (row / W > kMoveThreads * kMovePieces) return set_error(AKT_ERR_UNSUPPORTED, "evict_paged: head_dim too large");
+  const int64_t units = (int64_t)q.num_layers * a->batch * q.num_kv_heads;
+  if (units > 0x3ffffff) return set_error(AKT_ERR_INVALID, "evict_paged: too many heads");
+  const EvictLayout y = evict_layout(a);
+  if (!workspace || workspace_bytes < y.bytes)
+    return set_error(AKT_ERR_WORKSPACE, "evict_paged: workspace of " + std::to_string(y.bytes) + " bytes required");
+  p.num_pages = q.num_pages;
+  p.num_entries = a->num_page_entries;
+  p.max_entries = a->max_entries;
+  p.indptr = a->kv_page_indptr;
+  p.indices = a->kv_page_indices;
+  p.last = a->kv_last_page_len;
+  p.keep = a->keep_ind;
+  p.k_layer = a->keep_stride_layer;
+  p.k_batch = a->keep_stride_batch;
+  p.k_head = a->keep_stride_head;
+  p.kept = a->keep_len;
+  p.reserved = a->reserved;
+  p.w = a->weights;
+  p.w_layer = a->weights_stride_layer;
+  p.w_batch = a->weights_stride_batch;
+  p.w_head = a->weights_stride_head;
+  p.out_indptr = a->out_indptr;
+  p.out_indices = a->out_indices;
+  p.out_last = a->out_last_page_len;
+  p.layers = q.num_layers;
+  p.B = a->batch;
+  p.H = q.num_kv_heads;
+  p.P = q.page_size;
+  p.M = (int)a->max_kept;
+  p.width = (int)a->width;
+  p.div_page = make_fastdiv((uint32_t)p.P);
+  p.pieces = (int)(row / W);
+  p.div_piece = make_fastdiv((uint32_t)p.pieces);
+  p.rows = std::min(kMaxRows, kMoveThreads * kMovePieces / p.pieces);
+  char* ws = static_cast<char*>(workspace);
+  p.seen = reinterpret_cast<uint32_t*>(ws);
+  p.again = reinterpret_cast<uint32_t*>(ws + y.again);
+  p.dead = reinterpret_cast<int32_t*>(ws + y.dead);
+  p.lens = reinterpret_cast<int32_t*>(ws + y.lens);
+  p.count = reinterpret_cast<int32_t*>(ws + y.count);
+  p.moved = reinterpret_cast<int32_t*>(ws + y.moved);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const unsigned planners = p.num_entries > 4 * kPlanThreads ? 8 : 1;
+  cudaError_t e = launch_cluster(evict_plan_kernel, dim3(planners), dim3(kPlanThreads), planners, false, 0, st, p);
+  if (e == cudaSuccess && units > 0) {
+    ProfileScope prof(st);
+    const int64_t all = units * (p.w ? 3 : 2);
+    int C = 8;
+    while (C > 1 && (all * C > 2 * sm_count() || p.M / C < p.rows)) C /= 2;
+    const dim3 grid((unsigned)(all * C));
+    e = launch_cluster(W == 16 ? evict_move_kernel<16> : evict_move_kernel<2>, grid, dim3(kMoveThreads), C, true, 0, st, p);
+  }
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return e == cudaSuccess ? AKT_OK : cuda_error("evict_paged", e);
+}

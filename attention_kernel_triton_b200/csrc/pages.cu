@@ -14,6 +14,7 @@
 // ones, so the copies of one call never meet.
 #include "common.cuh"
 #include "profile.cuh"
+#include "scan.cuh"
 
 #include <algorithm>
 #include <string>
@@ -84,34 +85,6 @@ __device__ __forceinline__ void copy_pieces(const PoolView& v, int layer, int64_
 // ---------------------------------------------------------------------------
 // block-wide helpers of the plans (kPlanThreads threads)
 // ---------------------------------------------------------------------------
-// Exclusive prefix sum of x over the block; total through `total`.  sums: 33 of them.
-template <typename S>
-__device__ __forceinline__ S block_scan(S x, S* sums, S& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  S v = x;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const S y = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += y;
-  }
-  if (lane == 31) sums[warp] = v;
-  __syncthreads();
-  if (warp == 0) {
-    S w = sums[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const S y = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += y;
-    }
-    sums[lane] = w;
-  }
-  __syncthreads();
-  total = sums[31];
-  const S before = warp ? sums[warp - 1] : 0;
-  __syncthreads();
-  return before + v - x;
-}
-
 __device__ __forceinline__ uint32_t word_mask(int64_t num_pages, int64_t w) {  // the pages that word w stands for
   const int64_t left = num_pages - w * 32;
   return left >= 32 ? 0xffffffffu : (left <= 0 ? 0u : (1u << left) - 1u);

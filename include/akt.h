@@ -587,6 +587,106 @@ int akt_free_kv_pages(const int32_t* kv_page_indices, int64_t num_page_entries, 
                       int64_t num_pages, int32_t* free_pages, int32_t* num_free, void* workspace,
                       size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* eviction from a paged KV cache by accumulated attention weight (no       */
+/* reference counterpart: its sparse decodes take lists of kept tokens)     */
+/* ------------------------------------------------------------------------ */
+
+/* out[b, h, j] = weights[b, h, j] + the softmax weights that key j of       */
+/* sequence b gets from the new tokens' queries of the heads of kv head h:   */
+/* the sum of exp(scale q . k_j - lse) over the rows that see it.  Rows,     */
+/* table, causal and lse are those of akt_chunk_paged; a row whose lse is    */
+/* -inf adds nothing.  weights may be NULL (sums from zero) or out itself.   */
+/* Places past a sequence's length are not written; keys past `width` are    */
+/* left out and recorded (status 3).  Sums are in fp32, in an order that     */
+/* depends on the sizes alone.  head_dim 64 or 128.                          */
+typedef struct akt_attention_weights_args {
+  const void* q; /* [num_tokens, num_qo_heads, head_dim] */
+  int64_t q_stride_token, q_stride_head, q_stride_dim;
+  const int32_t* q_indptr; /* [batch + 1] */
+  int64_t num_tokens;
+  const void* kv_cache; /* [num_pages, 2, num_kv_heads, page_size, head_dim] */
+  int64_t kv_stride_page, kv_stride_kv, kv_stride_head, kv_stride_token, kv_stride_dim;
+  int64_t num_pages;
+  const int32_t* kv_page_indptr;   /* [batch + 1] */
+  const int32_t* kv_page_indices;  /* [num_page_entries] */
+  const int32_t* kv_last_page_len; /* [batch] */
+  int64_t num_page_entries;
+  const float* lse; /* [num_tokens, num_qo_heads] */
+  int64_t lse_stride_token, lse_stride_head;
+  const float* weights; /* [batch, num_kv_heads, width], unit stride in a row, or NULL */
+  int64_t weights_stride_batch, weights_stride_head;
+  float* out; /* [batch, num_kv_heads, width] */
+  int64_t out_stride_batch, out_stride_head;
+  int64_t width;
+  int32_t batch, num_qo_heads, num_kv_heads, page_size, head_dim;
+  int32_t causal;
+  int32_t dtype;
+  float softmax_scale;
+} akt_attention_weights_args;
+
+size_t akt_attention_weights_workspace_size(const akt_attention_weights_args* args);
+int akt_attention_weights(const akt_attention_weights_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Which min(seq_lens[b], budget) tokens of each head stay: the first        */
+/* `sinks`, the last `recent` and the heaviest of the others (the lowest     */
+/* index of equal weights; NaN counts as below everything).  keep_ind        */
+/* [layers, batch, num_heads, budget] ascends, 0 past the kept ones;         */
+/* keep_len [batch].  A length outside [0, width] is cut to it and recorded  */
+/* (status 3).  No workspace.                                                */
+typedef struct akt_select_tokens_args {
+  const float* weights; /* [layers, batch, num_heads, width], unit stride in a row */
+  int64_t weights_stride_layer, weights_stride_batch, weights_stride_head;
+  const int32_t* seq_lens; /* [batch] */
+  int32_t* keep_ind;       /* unit stride in a row */
+  int64_t keep_stride_layer, keep_stride_batch, keep_stride_head;
+  int32_t* keep_len; /* [batch] */
+  int64_t width;
+  int32_t layers, batch, num_heads, budget, sinks, recent;
+} akt_select_tokens_args;
+
+int akt_select_tokens(const akt_select_tokens_args* args, void* stream);
+
+/* The kept tokens of each head moved to the front of their sequence, in     */
+/* place: slot i of layer l, head h takes the row of token keep_ind[l, b, h, */
+/* i], for i < keep_len[b].  Lists ascend.  Writes the new table: out_indptr */
+/* [batch + 1], out_indices [max_entries] (-1 past its end),                 */
+/* out_last_page_len [batch].  A sequence stays in its first pages, but no   */
+/* page that another table entry names too or that `reserved` marks is       */
+/* written: one that is full of rows that stay in place is shared further,   */
+/* any other is replaced by the lowest-numbered dead page that none before   */
+/* it took (dead: named by no entry and not reserved); where none is left    */
+/* the entry is -1 and its rows are lost (status 6).  Slots behind the last  */
+/* kept row keep their contents.  weights [layers, batch, num_kv_heads,      */
+/* width] (fp32, or NULL) move along, zeros in the places they leave.  A     */
+/* list entry behind the sequence, below its slot or not above the one       */
+/* before it is skipped, keep_len past max_kept or the sequence is cut (both */
+/* status 3); a sequence with bad bounds is empty (status 4), pages past     */
+/* max_entries are cut (status 5), ids outside the pool stay as they are     */
+/* (status 2).  The new table must not overlap the old one.                  */
+typedef struct akt_evict_paged_args {
+  akt_page_pool pool;
+  const int32_t* kv_page_indptr;   /* [batch + 1] */
+  const int32_t* kv_page_indices;  /* [num_page_entries] */
+  const int32_t* kv_last_page_len; /* [batch] */
+  int64_t num_page_entries;
+  const int32_t* keep_ind; /* [num_layers, batch, num_kv_heads, max_kept], unit stride in a row */
+  int64_t keep_stride_layer, keep_stride_batch, keep_stride_head;
+  const int32_t* keep_len; /* [batch] */
+  int64_t max_kept;
+  const uint8_t* reserved; /* [num_pages] or NULL */
+  float* weights;          /* unit stride in a row, or NULL */
+  int64_t weights_stride_layer, weights_stride_batch, weights_stride_head, width;
+  int32_t* out_indptr;
+  int32_t* out_indices;
+  int32_t* out_last_page_len;
+  int64_t max_entries;
+  int32_t batch;
+} akt_evict_paged_args;
+
+size_t akt_evict_paged_workspace_size(const akt_evict_paged_args* args);
+int akt_evict_paged(const akt_evict_paged_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
