@@ -25,8 +25,8 @@ NVCC_FLAGS = ARCH + ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
                      "-I" + os.path.join(ROOT, "include"), "--expt-relaxed-constexpr"]
 # Files compiled as whole-program device code: ptxas ignores setmaxnreg in
 # relocatable device code, and the prefill kernel's warpgroup register split
-# (and the chunk kernel's) depends on it.  They reference no device symbol of another file.
-WHOLE_PROGRAM = {"prefill.cu", "chunk.cu"}
+# (and the chunk kernel's) depends on it.  These files reference no device symbol of another file.
+WHOLE_PROGRAM = {"prefill.cu", "chunk.cu", "weights.cu"}
 
 
 def flags_for(src: str):

@@ -49,6 +49,8 @@ cudaError_t prefill_status_read(unsigned int* v);
 cudaError_t prefill_status_clear();
 cudaError_t chunk_status_read(unsigned int* v);
 cudaError_t chunk_status_clear();
+cudaError_t weights_status_read(unsigned int* v);
+cudaError_t weights_status_clear();
 
 constexpr int kProducerWarps = 1;
 constexpr int kConsumerWarps = 4;
@@ -994,12 +996,14 @@ int akt_device_status(int device, unsigned int* status_out) {
   cudaGetDevice(&prev);
   cudaError_t e = cudaSetDevice(device);
   if (e == cudaSuccess) e = cudaDeviceSynchronize();
-  unsigned int v = 0, vp = 0, vc = 0;
+  unsigned int v = 0, vp = 0, vc = 0, vw = 0;
   if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, g_device_status, sizeof(v));
   if (e == cudaSuccess) e = prefill_status_read(&vp);
   if (e == cudaSuccess) e = chunk_status_read(&vc);
+  if (e == cudaSuccess) e = weights_status_read(&vw);
   if (v == 0) v = vp;
   if (v == 0) v = vc;
+  if (v == 0) v = vw;
   cudaSetDevice(prev);
   if (e != cudaSuccess) return set_error(AKT_ERR_CUDA, cudaGetErrorString(e));
   if (status_out) *status_out = v;
@@ -1014,6 +1018,7 @@ int akt_clear_device_status(int device) {
   if (e == cudaSuccess) e = cudaMemcpyToSymbol(g_device_status, &z, sizeof(z));
   if (e == cudaSuccess) e = prefill_status_clear();
   if (e == cudaSuccess) e = chunk_status_clear();
+  if (e == cudaSuccess) e = weights_status_clear();
   if (e == cudaSuccess) e = cudaDeviceSynchronize();
   cudaSetDevice(prev);
   if (e != cudaSuccess) return set_error(AKT_ERR_CUDA, cudaGetErrorString(e));
