@@ -20,13 +20,14 @@
 // sums in the workspace and weights_merge_kernel adds them, in the line's order, so
 // results depend on the sizes alone.
 //
-// Warps of a CTA (12):
-//   0-3 / 4-7  the exponentials of K tile 0 / 1 of the unit (S buffer 0 / 1)
-//   8 / 11     loaders of K / of Q and the log-sum-exps: tensor-map boxes inside the
-//              pages, or 16-byte cp.async rows where no box fits a page (TMA template)
-//   9          issuer of the MMAs (one elected lane)
-//   10         scheduler: the CTA's segments, a few ahead, through shared memory
-// TMEM (512 columns): two S buffers of 256.  A buffer is free once its last 64 columns
+// Warps of a CTA (20):
+//   0-15   the exponentials: four warps each for K tile 0 and 1 of the unit (S buffer 0
+//          and 1) and the left and right half of its columns
+//   16 / 19  loaders of K / of Q and the log-sum-exps: tensor-map boxes inside the
+//          pages, or 16-byte cp.async rows where no box fits a page (TMA template)
+//   17     issuer of the MMAs (one elected lane)
+//   18     scheduler: the CTA's segments, a few ahead, through shared memory
+// TMEM (512 columns): two S buffers of 256.  A buffer is free once its last columns
 // are in registers, so the tensor pipe works on while the exponentials run.
 //
 // Exponentials.  The special-function unit gives 16 a cycle and SM, half of what the
@@ -53,16 +54,15 @@ namespace {
 
 constexpr int BK = 128;            // keys of a tile
 constexpr int BR = 256;            // rows (tokens x heads) of a tile
-constexpr int kThreads = 384;
-constexpr int kLoadWarp = 8;       // K
-constexpr int kMmaWarp = 9;
-constexpr int kSchedWarp = 10;
-constexpr int kLoadQWarp = 11;
+constexpr int kExpWarps = 16;
+constexpr int kLoadWarp = kExpWarps;  // K
+constexpr int kMmaWarp = kExpWarps + 1;
+constexpr int kSchedWarp = kExpWarps + 2;
+constexpr int kLoadQWarp = kExpWarps + 3;
+constexpr int kThreads = 32 * (kExpWarps + 4);
 constexpr int kSegs = 4;           // segments in flight between the scheduler and the others
-constexpr int kSegReaders = 11;    // 2 loaders, issuer, 8 warps of exponentials
+constexpr int kSegReaders = kExpWarps + 3;  // and the 2 loaders and the issuer
 constexpr int QS = 2;              // Q tiles in shared memory
-constexpr int kMaxCtas = kThreads;
-constexpr int kPoly = 3;           // pairs of every 8 whose exponentials the FMA pipe computes
 
 struct WeightsParams {
   const char* q;
@@ -117,11 +117,13 @@ struct Cfg {
   static constexpr int KS = D == 64 ? 8 : 3;  // K tiles in shared memory
   static constexpr uint32_t OFF_Q = 0, OFF_K = QS * Q_BYTES, OFF_LSE = OFF_K + KS * K_BYTES;
   static constexpr uint32_t OFF_BAR = OFF_LSE + QS * BR * 4;
-  // k_full, k_empty [KS]; q_full, lse_full, q_empty [QS]; s_full, s_free [2]; seg_full, seg_empty [kSegs]; mma_idle
-  static constexpr int N_BARS = 2 * KS + 3 * QS + 4 + 2 * kSegs + 1;
+  // k_full, k_empty [KS]; q_full, lse_full, q_empty [QS]; s_full, s_free [2]; seg_full, seg_empty [kSegs]; red_full,
+  // red_empty [2]; mma_idle
+  static constexpr int N_BARS = 2 * KS + 3 * QS + 4 + 2 * kSegs + 5;
   static constexpr uint32_t OFF_MISC = OFF_BAR + (N_BARS * 8 + 15) / 16 * 16;  // TMEM address, abort flag
   static constexpr uint32_t OFF_SEG = OFF_MISC + 16;
-  static constexpr uint32_t SMEM = OFF_SEG + kSegs * sizeof(Seg);
+  static constexpr uint32_t OFF_RED = OFF_SEG + kSegs * sizeof(Seg);  // sums of a K tile's right half
+  static constexpr uint32_t SMEM = OFF_RED + BK * 4;
   static_assert(SMEM <= 227 * 1024, "shared memory budget");
 };
 
@@ -195,6 +197,10 @@ __device__ __forceinline__ int64_t cost_before(const WeightsParams& p, const Seq
 // -------------------------------------------------------------------------
 // exponentials
 // -------------------------------------------------------------------------
+// Whether the FMA pipe computes the exponentials of this pair of columns: one of four
+// (8192 tokens on top of 24576: 2.02 ms, none 2.08, three of eight 2.12, all 3.02).
+constexpr bool on_fma_pipe(int pair) { return pair % 4 == 0; }
+
 // 2^v of two values on the FMA pipe, as mantissas and scales.  The shift puts
 // n + 127 into the low bits of t; v below -127 gives a scale of 0, NaN stays NaN.
 __device__ __forceinline__ void poly_exp2(float2 v, float2& mant, float2& scale) {
@@ -210,7 +216,10 @@ __device__ __forceinline__ void poly_exp2(float2 v, float2& mant, float2& scale)
   r = ffma2(r, f, c(0.24022242f));
   r = ffma2(r, f, c(0.693147f));
   mant = ffma2(r, f, c(1.f));
-  scale = make_float2(__uint_as_float(__float_as_uint(t.x) << 23), __uint_as_float(__float_as_uint(t.y) << 23));
+  uint32_t sx, sy;  // (a shift on the ALU; a plain one may become a multiplication on the FMA pipe)
+  asm("shf.l.clamp.b32 %0, 0, %1, 23;" : "=r"(sx) : "r"(__float_as_uint(t.x)));
+  asm("shf.l.clamp.b32 %0, 0, %1, 23;" : "=r"(sy) : "r"(__float_as_uint(t.y)));
+  scale = make_float2(__uint_as_float(sx), __uint_as_float(sy));
 }
 
 // -------------------------------------------------------------------------
@@ -234,7 +243,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* s_free = s_full + 2;
   uint64_t* seg_full = s_free + 2;
   uint64_t* seg_empty = seg_full + kSegs;
-  uint64_t* mma_idle = seg_empty + kSegs;
+  uint64_t* red_full = seg_empty + kSegs;  // [K tile of the unit] the right half's sums are there
+  uint64_t* red_empty = red_full + 2;      // and read
+  uint64_t* mma_idle = red_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   Seg* segs = reinterpret_cast<Seg*>(smem + C::OFF_SEG);
@@ -250,15 +261,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < QS; ++s) {
       mbar_init(&q_full[s], 1);
       mbar_init(&lse_full[s], 1);
-      mbar_init(&q_empty[s], 1 + 8);
+      mbar_init(&q_empty[s], 1 + kExpWarps);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&s_free[t], 4);
+      mbar_init(&s_free[t], kExpWarps / 2);
     }
     for (int i = 0; i < kSegs; ++i) {
       mbar_init(&seg_full[i], 1);
       mbar_init(&seg_empty[i], kSegReaders);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&red_full[t], 4);
+      mbar_init(&red_empty[t], 4);
     }
     mbar_init(mma_idle, 1);
     *abort_flag = (smem_u32(smem) & 1023u) ? 1 : 0;  // swizzled tiles need a 1024-byte aligned base
@@ -271,8 +286,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   // ---- this CTA's range of the line, and the sequence that it starts in (scratch where Q goes later)
-  int64_t* sums = reinterpret_cast<int64_t*>(smem + C::OFF_Q);  // [12] of the warps
-  int64_t* found = sums + 16;                                   // [2] start of the sequence, its number
+  int64_t* sums = reinterpret_cast<int64_t*>(smem + C::OFF_Q);  // of the warps
+  int64_t* found = sums + kThreads / 32;                        // [2] start of the sequence, its number
   auto scan = [&](int64_t x, int64_t& total) -> int64_t {       // sum over the threads before this one
     int64_t v = x;
 #pragma unroll
@@ -333,9 +348,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
+  // the same answer in every lane, so a warp gives up as a whole
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-    if (mbar_try_wait(bar, parity)) return true;
-    return wait_or_abort_call(bar, parity, abort_flag);
+    return __all_sync(0xffffffffu, mbar_try_wait(bar, parity) || wait_or_abort_call(bar, parity, abort_flag));
   };
   if (warp == kSchedWarp) {
     // ============================ scheduler ============================
@@ -566,14 +581,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == kMmaWarp) {
     // ============================ MMA issuer ============================
     auto uni = [&](int v) { return (int)__reduce_or_sync(0xffffffffu, (unsigned)v); };
-    auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(bar, parity)); };
     const uint64_t dk = desc_sw128(smem_u32(smem + C::OFF_K), 16, C::GROUP);
     const uint64_t dq = desc_sw128(smem_u32(smem + C::OFF_Q), 16, 1024);
     const uint32_t tmem_u = uni(tmem);
     uint32_t gk = 0, gq = 0, gs = 0;  // K tiles, Q tiles, turns of the S buffers
     bool ok = true;
     for (int k = 0; ok; ++k) {
-      if (!wait_all(&seg_full[k % kSegs], (k / kSegs) & 1)) break;
+      if (!wait(&seg_full[k % kSegs], (k / kSegs) & 1)) break;
       const Seg* sp = &segs[k % kSegs];
       const int more = uni(sp->b >= 0), u0 = uni(sp->u0), u1 = uni(sp->u1), r0 = uni(sp->r0), r1 = uni(sp->r1), n = uni(sp->n);
       if (lane == 0) mbar_arrive(&seg_empty[k % kSegs]);
@@ -586,11 +600,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           // columns that the tile's rows fill, in steps of 16
           const int cols = toks > p.TQ ? BR : (toks * p.group + 15) / 16 * 16;
           const uint32_t idesc = idesc_f16(fmt, BK, 0, 0) | (uint32_t)(cols >> 3) << 17;
-          if (!wait_all(&q_full[slot], (gq / QS) & 1)) { ok = false; break; }
+          if (!wait(&q_full[slot], (gq / QS) & 1)) { ok = false; break; }
 #pragma unroll 1
           for (int t = 0; t < 2; ++t) {
             const uint32_t st = (gk + t) % KS;
-            if (!wait_all(&k_full[st], ((gk + t) / KS) & 1) || (gs && !wait_all(&s_free[t], (gs - 1) & 1))) {
+            if (!wait(&k_full[st], ((gk + t) / KS) & 1) || (gs && !wait(&s_free[t], (gs - 1) & 1))) {
               ok = false;
               break;
             }
@@ -623,10 +637,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_wait(mma_idle, 0);
   } else {
     // ============================ exponentials ============================
-    const int t = warp >> 2, row = threadIdx.x & (BK - 1);
-    const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * BR;
+    const int t = warp >> 2 & 1, half = warp >> 3, row = threadIdx.x & (BK - 1);
+    const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * BR + half * BK;
     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
-    uint32_t gq = 0, gs = 0;
+    float* red = reinterpret_cast<float*>(smem + C::OFF_RED);
+    uint32_t gq = 0, gs = 0, joins = 0;
     bool ok = true;
     for (int k = 0; ok; ++k) {
       if (!wait(&seg_full[k % kSegs], (k / kSegs) & 1)) break;
@@ -635,37 +650,42 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(&seg_empty[k % kSegs]);
       if (sg.b < 0) break;
       const bool stays = sg.u1 - sg.u0 > 1;
+      const bool wide = sg.n - sg.r0 * 2 * p.TQ > p.TQ;  // the right halves have columns
       for (int u = sg.u0; ok && u < sg.u1; ++u) {
         const int key0 = (2 * u + t) * BK, key = key0 + row;
         const bool mine = key < min(sg.len, p.width);
         float before = 0.f;
-        if (mine && sg.part < 0 && p.w) before = __ldg(p.w + sg.b * p.w_batch + sg.kvh * p.w_head + key);
+        if (mine && half == 0 && sg.part < 0 && p.w) before = __ldg(p.w + sg.b * p.w_batch + sg.kvh * p.w_head + key);
         float2 acc[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[e] = make_float2(0.f, 0.f);
         for (int r = sg.r0; r < sg.r1; ++r) {
-          const int slot = gq % QS, tok = r * 2 * p.TQ, toks = sg.n - tok;
+          // the half's first token, and its tokens
+          const int slot = gq % QS, tok = r * 2 * p.TQ + half * p.TQ, toks = min(sg.n - tok, p.TQ);
           if (!wait(&lse_full[slot], (gq / QS) & 1) || !wait(&s_full[t], gs & 1)) {
             ok = false;
             break;
           }
           ++gs;
           tc_fence_after();
-          // tokens of the tile that do not see this key yet, and whether any pair of the tile is hidden
+          // tokens of the half that do not see this key yet, and whether any pair of the half is hidden
           const int skip = p.causal ? key - (sg.len - sg.n) - tok : 0;
-          const bool masked = toks < 2 * p.TQ || (p.causal && key0 + BK - 1 - (sg.len - sg.n) - tok > 0);
-          const int chunks = toks > p.TQ ? BR / 64 : (toks * p.group + 63) / 64;
-          const float4* nl = reinterpret_cast<const float4*>(lse_s + slot * BR);
+          const bool masked = toks < p.TQ || (p.causal && key0 + BK - 1 - (sg.len - sg.n) - tok > 0);
+          const int chunks = (max(toks, 0) * p.group + 31) / 32;
+          const float4* nl = reinterpret_cast<const float4*>(lse_s + slot * BR + half * BK);
+          if (!chunks) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_free[t]);
+          }
 #pragma unroll 1
           for (int c = 0; c < chunks; ++c) {
-            float x[64];
+            float x[32];
             {
-              uint32_t rr[2][32];
-              tmem_ld32(tS + c * 64, rr[0]);
-              tmem_ld32(tS + c * 64 + 32, rr[1]);
+              uint32_t rr[32];
+              tmem_ld32(tS + c * 32, rr);
               tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 64; ++e) x[e] = __uint_as_float(rr[e >> 5][e & 31]);
+              for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(rr[e]);
             }
             if (c + 1 == chunks) {  // the buffer is free for the next MMAs
               tc_fence_before();
@@ -673,21 +693,19 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (lane == 0) mbar_arrive(&s_free[t]);
             }
             if (masked) {
-              const int first = (c >> 1) * p.TQ, at = (c & 1) * 64;  // the half's first token, the chunk's first column
-              const int lo = min(max(skip - first, 0), p.TQ) * p.group - at;
-              const int hi = min(max(toks - first, 0), p.TQ) * p.group - at;
+              const int lo = min(max(skip, 0), p.TQ) * p.group - c * 32, hi = toks * p.group - c * 32;
 #pragma unroll
-              for (int e = 0; e < 64; ++e) x[e] = e >= lo && e < hi ? x[e] : -INFINITY;
+              for (int e = 0; e < 32; ++e) x[e] = e >= lo && e < hi ? x[e] : -INFINITY;
             }
 #pragma unroll
-            for (int e = 0; e < 64; e += 4) {
-              const float4 l4 = nl[c * 16 + e / 4];
+            for (int e = 0; e < 32; e += 4) {
+              const float4 l4 = nl[c * 8 + e / 4];
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
                 const int pair = e / 2 + i;
                 const float2 v = ffma2(make_float2(x[e + 2 * i], x[e + 2 * i + 1]), sl2,
                                        i ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y));
-                if (pair % 8 < kPoly) {
+                if (on_fma_pipe(pair)) {
                   float2 mant, scale;
                   poly_exp2(v, mant, scale);
                   acc[pair & 3] = ffma2(mant, scale, acc[pair & 3]);
@@ -703,9 +721,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             ++gq;
           }
         }
-        if (!ok) break;
         const float2 a01 = __fadd2_rn(acc[0], acc[1]), a23 = __fadd2_rn(acc[2], acc[3]), a = __fadd2_rn(a01, a23);
-        const float sum = a.x + a.y;
+        float sum = a.x + a.y;
+        if (wide && ok) {  // left half + right half; one buffer, the unit's two K tiles in turn
+          if (half) {
+            ok = t ? wait(&red_empty[0], joins & 1) : !joins || wait(&red_empty[1], (joins - 1) & 1);
+            if (ok) red[row] = sum;
+          } else {
+            ok = wait(&red_full[t], joins & 1);
+            if (ok) sum += red[row];
+          }
+          __syncwarp();
+          if (ok && lane == 0) mbar_arrive(half ? &red_full[t] : &red_empty[t]);
+          ++joins;
+        }
+        if (!ok) break;
+        if (half) continue;
         if (sg.part >= 0) p.part_sum[((int64_t)(2 * blockIdx.x) + sg.part) * (2 * BK) + t * BK + row] = sum;
         else if (mine) p.out[sg.b * p.o_batch + sg.kvh * p.o_head + key] = before + sum;
       }
@@ -759,7 +790,7 @@ Layout make_layout(const akt_attention_weights_args* a) {
   Layout y{};
   const int64_t units = (a->num_page_entries * a->page_size / (2 * BK) + a->batch) * a->num_kv_heads;
   const int64_t tiles = a->num_tokens / (2 * (BK / (a->num_qo_heads / a->num_kv_heads))) + 1;
-  y.grid = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)sm_count(), (int64_t)kMaxCtas, units * tiles}));
+  y.grid = (int)std::max<int64_t>(1, std::min<int64_t>(sm_count(), units * tiles));
   y.sums = round256((size_t)y.grid * 2 * sizeof(Part));
   y.bytes = y.sums + (size_t)y.grid * 2 * 2 * BK * 4;
   return y;
