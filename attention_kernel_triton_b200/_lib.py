@@ -215,6 +215,13 @@ class CompactPagedArgs(Structure):
     ]
 
 
+class PrefixPagedArgs(Structure):
+    _fields_ = [
+        ("chunk", ChunkPagedArgs),
+        ("group_indptr", c_void_p), ("shared_pages", c_void_p), ("num_groups", c_int32),
+    ]
+
+
 class AttentionWeightsArgs(Structure):
     _fields_ = [
         ("q", c_void_p), ("q_stride_token", c_int64), ("q_stride_head", c_int64), ("q_stride_dim", c_int64),
@@ -318,6 +325,10 @@ SIGNATURES = {
     "akt_fork_paged": (c_int, [POINTER(ForkPagedArgs), c_void_p, c_size_t, c_void_p]),
     "akt_compact_paged_workspace_size": (c_size_t, [POINTER(CompactPagedArgs)]),
     "akt_compact_paged": (c_int, [POINTER(CompactPagedArgs), c_void_p, c_size_t, c_void_p]),
+    "akt_prefix_paged_workspace_size": (c_size_t, [POINTER(PrefixPagedArgs)]),
+    "akt_prefix_paged": (c_int, [POINTER(PrefixPagedArgs), c_void_p, c_size_t, c_void_p]),
+    "akt_shared_prefix_pages": (c_int, [c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int32,
+                                        c_void_p, c_void_p]),
     "akt_attention_weights_workspace_size": (c_size_t, [POINTER(AttentionWeightsArgs)]),
     "akt_attention_weights": (c_int, [POINTER(AttentionWeightsArgs), c_void_p, c_size_t, c_void_p]),
     "akt_select_tokens": (c_int, [POINTER(SelectTokensArgs), c_void_p]),

@@ -42,6 +42,14 @@
 // not finite are cleared and their tokens noted; a row that does see such a token
 // gets the value added to its output at the end.
 //
+// Shared prefixes (the SHARED template).  Groups of neighbouring sequences have their
+// first pages in common.  A planner turns the batch into virtual sequences: for each
+// group its sequences' rows on the shared keys, all visible, and for each sequence its
+// rows on its own keys behind them.  Both are cut into units as above, so the prefix's
+// K/V are read once for a group and the rows of all its sequences fill the tiles.  A
+// row of a sequence with a prefix leaves two partial results (or the parts of them),
+// which chunk_join_kernel joins; other rows go straight to the output.
+//
 // Bounds and measured rates (fp16, 32 query heads on 8, pages of 16 keys, full clock).
 // Long prompts: the tensor pipe and the exponentials, 60 % busy each; 8192 tokens on top
 // of 24576, D = 128, 3.01 ms = 1280 TFLOP/s (D = 64: 2.53 ms).  Short prompts also their
@@ -128,7 +136,19 @@ struct ChunkParams {
   int* plan_units;     // [B + 1]
   struct Plan* plan;
   int64_t* plan_share; // [grid + 1]
+  // shared prefixes: B counts the virtual sequences, `groups` prefixes and then the batch's
+  int groups, batch;
+  const int32_t* group_indptr;
+  const int32_t* shared_pages;
+  struct Seq* seqs;    // [B]
+  int* prefix_len;     // [batch] shared keys of each sequence
+  float* row_o;        // [2][rows][D] normalised outputs of a row on the prefix, on its own keys
+  float* row_lse;      // [2][rows]
+  int2* row_at;        // [2][rows] kWhole, kDone, or the place of the first part and the row there
 };
+
+constexpr int kWhole = -1;  // the row's result is in row_o
+constexpr int kDone = -2;   // the row is in the output
 
 // A unit's part that one CTA left in the workspace (written for both of a
 // CTA's places; keys == 0: none).
@@ -156,7 +176,9 @@ struct Seg {
   int single;  // one tile of rows: the slots take turns at the key tiles
   int part;    // -1: the whole unit; else the place of the partial result
   int noted;   // tokens in `bad`
-  int pad[3];
+  int causal;
+  int prefix;  // shared prefixes: 0 a sequence without one, 1 a prefix, 2 a sequence's own keys behind one
+  int pad;
   uint32_t bad[3][BN / 32];  // tokens from tile vis0 / BN on whose V row is not finite
 };
 
@@ -189,11 +211,16 @@ struct Cfg {
 // -------------------------------------------------------------------------
 struct Seq {
   int a0, n, page0, len;  // first row of q, queries, first index entry, keys
+  int causal, prefix;
 };
 
 // Sequence b's bounds; a malformed one is empty (recorded by the planner).
+template <bool SHARED = false>
 __device__ __forceinline__ Seq load_seq(const ChunkParams& p, int b, bool record) {
+  if constexpr (SHARED) return p.seqs[b];
   Seq s;
+  s.causal = p.causal;
+  s.prefix = 0;
   const int a1 = __ldg(p.q_indptr + b + 1), e = __ldg(p.indptr + b + 1), last = __ldg(p.last + b);
   s.a0 = __ldg(p.q_indptr + b);
   s.page0 = __ldg(p.indptr + b);
@@ -217,7 +244,7 @@ __device__ __forceinline__ int num_units(const ChunkParams& p, const Seq& s) {
 
 // Key tiles of unit u, and what it costs on the line
 __device__ __forceinline__ int unit_tiles(const ChunkParams& p, const Seq& s, int u) {
-  const int vis = p.causal ? s.len - s.n + min((u + 1) * 2 * p.TQ, s.n) : s.len;
+  const int vis = s.causal ? s.len - s.n + min((u + 1) * 2 * p.TQ, s.n) : s.len;
   return vis > 0 ? (vis - 1) / BN + 1 : 0;
 }
 __device__ __forceinline__ int unit_extra(const ChunkParams& p, const Seq& s, int u) {
@@ -248,9 +275,10 @@ __device__ __forceinline__ int find_seq(const V* t, int B, V x) {
 
 // Unit i of the line: its sequence, kv head and number (a sequence's units run
 // from the last, longest one down).
+template <bool SHARED>
 __device__ __forceinline__ void unit_at(const ChunkParams& p, const Tables& t, int i, int& b, Seq& s, int& kvh, int& u) {
   b = find_seq(t.units, p.B, i);
-  s = load_seq(p, b, false);
+  s = load_seq<SHARED>(p, b, false);
   const int U = num_units(p, s), r = i - t.units[b];
   kvh = r / U;
   u = U - 1 - (r - kvh * U);
@@ -259,6 +287,7 @@ __device__ __forceinline__ void unit_at(const ChunkParams& p, const Tables& t, i
 // Fills the tables (threads of one CTA, `nthreads` of them; cost and units in
 // shared or global memory), and the costliest unit's cost, no less, into
 // *most_cost (shared memory).
+template <bool SHARED>
 __device__ void build_tables(const ChunkParams& p, int64_t* cost, int* units, Seq* seqs, int* most_cost, int nthreads) {
   if (threadIdx.x == 0) *most_cost = 1;
   __syncthreads();
@@ -272,7 +301,7 @@ __device__ void build_tables(const ChunkParams& p, int64_t* cost, int* units, Se
     int64_t c = 0;
     Seq s{};
     if (b < p.B) {
-      s = load_seq(p, b, lane == 0);
+      s = load_seq<SHARED>(p, b, lane == 0);
       U = num_units(p, s);
       for (int u = lane; u < U; u += team) c += unit_cost(p, s, u);
     }
@@ -330,6 +359,7 @@ __device__ __forceinline__ int64_t div_small(int64_t a, int64_t b) {
 // Deals whole units and cuts the rest (at least p.grid threads of one CTA, all
 // call it).  share[c] .. share[c + 1] is CTA c's range of the cut part, in tiles
 // from plan.base.  scratch: an int64 per 32 CTAs.
+template <bool SHARED>
 __device__ Plan make_plan(const ChunkParams& p, const Tables& t, int most_cost, int64_t* share, int* scratch) {
   const int64_t W = t.cost[p.B];
   const int N = t.units[p.B], c = threadIdx.x;
@@ -351,7 +381,7 @@ __device__ Plan make_plan(const ChunkParams& p, const Tables& t, int most_cost, 
       const int b = find_seq(t.units, p.B, i);
       start = t.units[b];
       end = t.units[b + 1];
-      s = t.seqs ? t.seqs[b] : load_seq(p, b, false);
+      s = t.seqs ? t.seqs[b] : load_seq<SHARED>(p, b, false);
       U = num_units(p, s);
     }
     return unit_cost(p, s, U - 1 - (i - start) % U);
@@ -496,7 +526,7 @@ __device__ __forceinline__ void turn_pieces(uint4 (&v)[4]) {
 // loop has its registers.  A thread holds a row; four lanes exchange 16-byte
 // pieces so that a store covers 64 bytes of each of 8 rows (each thread storing
 // its own row, 16 bytes of 32 rows at a time, took 6.8K cycles at D = 128).
-template <typename T, int D>
+template <typename T, int D, bool SHARED>
 __device__ __forceinline__ void finish_rows(const ChunkParams& p, const Seg* sg, uint32_t tO, int t, float w0, float w1,
                                          float row_lse, int flags) {
   const int r = threadIdx.x & (BM - 1), rtok = (int)fdiv((uint32_t)r, p.div_group);
@@ -505,8 +535,10 @@ __device__ __forceinline__ void finish_rows(const ChunkParams& p, const Seg* sg,
   const bool valid = rtok < p.TQ && tok < sg->ntok;
   const int64_t grow = (int64_t)sg->q0 + tok;
   const int64_t pidx = ((int64_t)(2 * blockIdx.x) + max(part, 0)) * p.part_rows + (single ? 0 : t * BM) + r;
-  char* mine = valid ? (part < 0 ? p.out + grow * p.o_tok + (int64_t)head * p.o_head
-                                 : reinterpret_cast<char*>(p.part_o + pidx * D))
+  const bool done = part < 0 && (!SHARED || sg->prefix == 0);  // the row's final result
+  const int64_t ridx = SHARED ? (sg->prefix == 1 ? 0 : p.num_tokens * p.Hq) + grow * p.Hq + head : 0;
+  char* mine = valid ? (done ? p.out + grow * p.o_tok + (int64_t)head * p.o_head
+                             : reinterpret_cast<char*>(part < 0 ? p.row_o + ridx * D : p.part_o + pidx * D))
                      : nullptr;
   char* row[4];  // the four lanes' rows, at this lane's piece
 #pragma unroll
@@ -533,7 +565,7 @@ __device__ __forceinline__ void finish_rows(const ChunkParams& p, const Seg* sg,
       for (int e = 0; e < 32; ++e) o[e] = flags & 2 ? fmaf(__uint_as_float(a[e]), w1, o[e]) : o[e];
     }
     uint4 v[4];
-    if (part < 0) {
+    if (done) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         v[e] = make_uint4(Elem<T>::pack2(o[8 * e], o[8 * e + 1]), Elem<T>::pack2(o[8 * e + 2], o[8 * e + 3]),
@@ -556,33 +588,97 @@ __device__ __forceinline__ void finish_rows(const ChunkParams& p, const Seg* sg,
       }
     }
   }
+  if (SHARED && valid) {
+    if (part >= 0 && sg->t0 == 0) p.row_at[ridx] = make_int2(2 * blockIdx.x + part, (single ? 0 : t * BM) + r);
+    else if (part < 0) p.row_at[ridx] = make_int2(done ? kDone : kWhole, 0);
+    if (part < 0 && !done) p.row_lse[ridx] = row_lse;
+  }
   if (valid) {
     if (part >= 0) p.part_lse[pidx] = row_lse;
-    else if (p.lse) p.lse[grow * p.l_tok + (int64_t)head * p.l_head] = row_lse;
+    else if (done && p.lse) p.lse[grow * p.l_tok + (int64_t)head * p.l_head] = row_lse;
   }
   if (sg->noted) {
     __syncwarp();  // the row was stored by four lanes
     const int vis = sg->vis0 + tok;
-    if (valid && part < 0) add_not_finite<T, D, T>(p, *sg, vis, reinterpret_cast<T*>(mine));
-    if (valid && part >= 0) add_not_finite<T, D, float>(p, *sg, vis, reinterpret_cast<float*>(mine));
+    if (valid && done) add_not_finite<T, D, T>(p, *sg, vis, reinterpret_cast<T*>(mine));
+    if (valid && !done) add_not_finite<T, D, float>(p, *sg, vis, reinterpret_cast<float*>(mine));
   }
 }
 
 // -------------------------------------------------------------------------
 // the planner of batches past the CTA's own table
 // -------------------------------------------------------------------------
+// The virtual sequences of a batch with shared prefixes.  A group's prefix is as many
+// whole pages as it is said to share, as all its sequences with rows have and (causal)
+// as their first rows see; none where fewer than two have rows or one has bad bounds.
+__device__ void build_shared(const ChunkParams& p, int* bad) {
+  if (threadIdx.x == 0) *bad = 0;
+  __syncthreads();
+  for (int g = threadIdx.x; g <= p.groups; g += 1024) {
+    const int x = __ldg(p.group_indptr + g);
+    if (x < 0 || x > p.batch || (g && __ldg(p.group_indptr + g - 1) > x)) *bad = 1;
+  }
+  __syncthreads();
+  if (*bad && threadIdx.x == 0) record_status(kStatusBadIndptr);
+  const int lane = threadIdx.x & 31;
+  for (int g = threadIdx.x >> 5; g < p.groups; g += 32) {  // a warp per group
+    const int b0 = *bad ? 0 : __ldg(p.group_indptr + g), b1 = *bad ? 0 : __ldg(p.group_indptr + g + 1);
+    int keys = min(max(__ldg(p.shared_pages + g), 0), 0x3fffffff / p.P) * p.P, rows = 0, first = 0x7fffffff;
+    for (int b = b0 + lane; b < b1; b += 32) {
+      const Seq s = load_seq(p, b, false);
+      const int a0 = __ldg(p.q_indptr + b), a1 = __ldg(p.q_indptr + b + 1);
+      if (a0 < 0 || a1 < a0 || a1 > p.num_tokens) keys = 0;
+      if (s.n == 0) continue;
+      ++rows;
+      first = min(first, b);
+      keys = min(keys, max(p.causal ? s.len - s.n : s.len, 0));
+    }
+    keys = __reduce_min_sync(0xffffffffu, keys) / p.P * p.P;
+    rows = __reduce_add_sync(0xffffffffu, rows);
+    first = __reduce_min_sync(0xffffffffu, first);
+    Seq v{};
+    if (keys > 0 && rows > 1) {
+      v.a0 = __ldg(p.q_indptr + b0);
+      v.n = __ldg(p.q_indptr + b1) - v.a0;
+      v.page0 = __ldg(p.indptr + first);
+      v.len = keys;
+      v.prefix = 1;
+    }
+    if (lane == 0) p.seqs[g] = v;
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < p.batch; b += 1024) {
+    Seq s = load_seq(p, b, true);
+    int keys = 0;
+    if (p.groups && !*bad) {
+      const int g = find_seq(p.group_indptr, p.groups, b);
+      if (b >= __ldg(p.group_indptr + g) && b < __ldg(p.group_indptr + g + 1) && s.n) keys = p.seqs[g].len;
+    }
+    if (keys) {
+      s.page0 += keys / p.P;
+      s.len -= keys;
+      s.prefix = 2;
+    }
+    p.seqs[p.groups + b] = s;
+    p.prefix_len[b] = keys;
+  }
+  __syncthreads();
+}
+
+template <bool SHARED>
 __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
   __shared__ __align__(8) int scratch[64];
   __shared__ int most_cost;
-  build_tables(p, p.plan_cost, p.plan_units, nullptr, &most_cost, 1024);
-  const Plan pl = make_plan(p, Tables{p.plan_cost, p.plan_units, nullptr}, most_cost, p.plan_share, scratch);
+  if (SHARED) build_shared(p, &most_cost);
+  build_tables<SHARED>(p, p.plan_cost, p.plan_units, nullptr, &most_cost, 1024);
+  const Plan pl = make_plan<SHARED>(p, Tables{p.plan_cost, p.plan_units, nullptr}, most_cost, p.plan_share, scratch);
   if (threadIdx.x == 0) *p.plan = pl;
 }
 
 // -------------------------------------------------------------------------
 // main kernel
 // -------------------------------------------------------------------------
-template <typename T, int D, bool TMA>
+template <typename T, int D, bool TMA, bool SHARED>
 __global__ void __launch_bounds__(kThreads, 1)
     chunk_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ ChunkParams p) {
@@ -647,16 +743,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   int64_t begin, end;
   Plan plan;
   Tables tab;
-  if (p.B <= kTableSeqs) {
+  if (!SHARED && p.B <= kTableSeqs) {
     int64_t* cost = reinterpret_cast<int64_t*>(smem + C::OFF_TABLE);
     int* units = reinterpret_cast<int*>(cost + p.B + 1);
     // the shares live where slot 0's Q tile goes later
     int64_t* share = reinterpret_cast<int64_t*>(smem + C::OFF_Q);
     int* scratch = reinterpret_cast<int*>(share + p.grid + 1);
     Seq* seqs = reinterpret_cast<Seq*>(smem + C::OFF_Q + 8192);
-    build_tables(p, cost, units, seqs, scratch + 63, kThreads);
+    build_tables<SHARED>(p, cost, units, seqs, scratch + 63, kThreads);
     tab = Tables{cost, units, seqs};
-    plan = make_plan(p, tab, scratch[63], share, scratch);
+    plan = make_plan<SHARED>(p, tab, scratch[63], share, scratch);
     begin = share[blockIdx.x];
     end = share[blockIdx.x + 1];
     // generic reads before the async-proxy writes of the Q tile
@@ -700,12 +796,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (round < plan.rounds) {
           int bb, k, uu;
           Seq q;
-          unit_at(p, tab, dealt_unit(p, round, blockIdx.x), bb, q, k, uu);
+          unit_at<SHARED>(p, tab, dealt_unit(p, round, blockIdx.x), bb, q, k, uu);
           ++round;
           const int X = 2 * p.TQ;
           sg.q0 = q.a0 + uu * X;
           sg.ntok = min(X, q.n - uu * X);
-          sg.vis0 = p.causal ? q.len - q.n + uu * X + 1 : q.len;
+          sg.vis0 = q.causal ? q.len - q.n + uu * X + 1 : q.len;
+          sg.causal = q.causal;
+          sg.prefix = q.prefix;
           sg.kvh = k;
           sg.page0 = q.page0;
           sg.len = q.len;
@@ -716,7 +814,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           while (x < x_end) {
             if (b < 0) {  // the unit that holds x
               b = find_seq(tab.cost, p.B, x);
-              s = load_seq(p, b, false);
+              s = load_seq<SHARED>(p, b, false);
               U = num_units(p, s);
               const int64_t per_head = div_small(tab.cost[b + 1] - tab.cost[b], p.Hkv);
               const int64_t rel = x - tab.cost[b];
@@ -750,7 +848,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (some) {
               sg.q0 = s.a0 + u * X;
               sg.ntok = min(X, s.n - u * X);
-              sg.vis0 = p.causal ? s.len - s.n + u * X + 1 : s.len;
+              sg.vis0 = s.causal ? s.len - s.n + u * X + 1 : s.len;
+              sg.causal = s.causal;
+              sg.prefix = s.prefix;
               sg.kvh = kvh;
               sg.page0 = s.page0;
               sg.len = s.len;
@@ -789,7 +889,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           sg.n0 = (n + 1) >> 1;
           sg.n1 = n >> 1;
         } else {  // slot 1 holds the unit's last token, slot 0's may see fewer keys
-          const int vis = p.causal ? sg.vis0 + p.TQ - 1 : sg.len;
+          const int vis = sg.causal ? sg.vis0 + p.TQ - 1 : sg.len;
           sg.n0 = max(0, min(sg.t1, vis > 0 ? (vis - 1) / BN + 1 : 0) - sg.t0);
           sg.n1 = n;
         }
@@ -816,6 +916,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         Seg* sg = &segs[k % kSegs];
         const int t0 = sg->t0, t1 = sg->t1, vis0 = sg->vis0, len = sg->len, j_edge = max(vis0, 0) / BN;
+        const bool causal = SHARED ? sg->causal : p.causal;
         if (sg->q0 < 0) break;
         const int loads = 2 * (t1 - t0);
 #pragma unroll 1
@@ -831,11 +932,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           // V tiles are the even loads from the third on, and the last one
           const int j = t0 + (i + 1 == loads ? (i >> 1) : (i >> 1) - 1);
           const bool is_v = i + 1 == loads || (i >= 2 && !(i & 1));
-          if (is_v && ((p.causal && (j + 1) * BN > vis0) || (j + 1) * BN > len)) {
+          if (is_v && ((causal && (j + 1) * BN > vis0) || (j + 1) * BN > len)) {
             // rows that every row of the unit sees stay as they are
             unsigned char* v = smem + C::OFF_KV + st * C::KV_BYTES;
             const int rows = len - j * BN;  // the others are past the sequence
-            const int r0 = min(max(p.causal ? vis0 - j * BN : rows, 0), BN);
+            const int r0 = min(max(causal ? vis0 - j * BN : rows, 0), BN);
             constexpr int PR = D / 8, RS = 32 / PR;  // 16-byte pieces of a row, rows a step
             const int ch = lane % PR;
             unsigned char* vc = v + (ch >> 3) * C::HALF + (ch & 7) * 16;  // (the swizzle stays inside a row)
@@ -1171,8 +1272,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int tok0 = single ? 0 : t * p.TQ;                        // the slot's first token of the unit
       // keys past the slot's first tile that every row of the slot sees, and that this row sees more
       const int key0 = (sg->t0 + (single ? t : 0)) * BN, key_step = single ? 2 * BN : BN;
-      int vis_min = (p.causal ? sg->vis0 + tok0 : sg->len) - key0;
-      const int more = p.causal ? rtok : 0;
+      const bool causal = SHARED ? sg->causal : p.causal;
+      int vis_min = (causal ? sg->vis0 + tok0 : sg->len) - key0;
+      const int more = causal ? rtok : 0;
       const bool valid = rtok < p.TQ && tok0 + rtok < sg->ntok;
       const bool warp_valid = __any_sync(0xffffffffu, valid);
       float m_use = -INFINITY, l = 0.f;
@@ -1298,7 +1400,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       w0 *= inv;
       w1 *= inv;
       if (warp_valid)
-        finish_rows<T, D>(p, sg, tO, t, w0, w1, any ? (m_row + __log2f(total)) * kLn2 : -INFINITY,
+        finish_rows<T, D, SHARED>(p, sg, tO, t, w0, w1, any ? (m_row + __log2f(total)) * kLn2 : -INFINITY,
                           (mine && any ? 1 : 0) | (other ? 2 : 0));
       tc_fence_before();
       __syncwarp();
@@ -1431,21 +1533,124 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const ChunkP
 }
 
 // -------------------------------------------------------------------------
+// join of a row's results on a shared prefix and on its own keys
+// -------------------------------------------------------------------------
+// A warp per row (token, head).  The row's results are those of up to two units, whole
+// in row_o or in parts as chunk_merge_kernel finds them; rows of no sequence are zeros.
+template <typename T, int D>
+__global__ void __launch_bounds__(kMergeThreads) chunk_join_kernel(const ChunkParams p) {
+  constexpr int N = D / 32;  // columns per lane
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = p.num_tokens * p.Hq, row = (int64_t)blockIdx.x * (kMergeThreads / 32) + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int tok = (int)(row / p.Hq), head = (int)(row - (int64_t)tok * p.Hq);
+  const int b = find_seq(p.q_indptr, p.batch, tok);
+  const int a0 = __ldg(p.q_indptr + b), a1 = __ldg(p.q_indptr + b + 1);
+  const bool there = a0 >= 0 && tok >= a0 && tok < a1 && a1 <= p.num_tokens;
+  grid_dep_wait();
+  int count[2] = {0, 0}, at[2], rr[2];  // parts on the prefix and on the own keys, where they begin, the row there
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    at[k] = kWhole;
+    rr[k] = 0;
+    if (!there || (k == 0 && !p.prefix_len[b])) continue;
+    const int2 w = p.row_at[k * rows + row];
+    if (w.x == kDone) return;
+    at[k] = w.x;
+    rr[k] = w.y;
+    count[k] = 1;
+    if (w.x < 0 || p.parts[w.x].last) continue;
+    const int c0 = w.x >> 1;
+    for (int base = c0 + 1; base < p.grid; base += 32) {  // the CTA with the last part
+      const int c = base + lane;
+      const bool ends = c < p.grid && p.parts[2 * c].used && p.parts[2 * c].last;
+      const unsigned m = __ballot_sync(0xffffffffu, ends);
+      if (m) {
+        count[k] = base + __ffs(m) - c0;
+        break;
+      }
+    }
+  }
+  const int total = count[0] + count[1];
+  // result i: its log-sum-exp (-inf: nothing) and its row
+  auto find = [&](int i, const float*& o) -> float {
+    o = nullptr;
+    if (i >= total) return -INFINITY;
+    const int k = i >= count[0], e = i - (k ? count[0] : 0);
+    const int first = k ? at[1] : at[0], r = k ? rr[1] : rr[0];
+    if (first < 0) {
+      o = p.row_o + (k * rows + row) * D;
+      return p.row_lse[k * rows + row];
+    }
+    const int place = e ? 2 * ((first >> 1) + e) : first;
+    if (e && !p.parts[place].used) return -INFINITY;
+    const int64_t x = (int64_t)place * p.part_rows + r;
+    o = p.part_o + x * D;
+    return p.part_lse[x];
+  };
+  const float* o;
+  float M = -INFINITY;
+  for (int i = lane; i < total; i += 32) M = fmaxf(M, find(i, o));
+#pragma unroll
+  for (int s = 16; s; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
+  const float Ms = M == -INFINITY ? 0.f : M;
+  float acc[N] = {}, den = 0.f;
+  for (int i0 = 0; i0 < total; i0 += 32) {
+    const float part = find(i0 + lane, o);
+    const float mine = fast_exp2((part - Ms) * kLog2e);  // NaN stays NaN
+    const unsigned holds = __ballot_sync(0xffffffffu, part != -INFINITY);  // (a weight of 0 is not left out)
+    const int n = min(32, total - i0);
+    for (int i1 = 0; i1 < n; i1 += 8) {  // eight rows asked for at once
+      float w[8];
+      float v[8][N];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        w[u] = __shfl_sync(0xffffffffu, mine, i1 + u);
+        const float* src = reinterpret_cast<const float*>(
+            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(o), i1 + u));
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[u][e] = 0.f;
+        if (!(holds >> (i1 + u) & 1u)) continue;
+        if constexpr (N == 4) *reinterpret_cast<float4*>(v[u]) = *reinterpret_cast<const float4*>(src + lane * N);
+        else *reinterpret_cast<float2*>(v[u]) = *reinterpret_cast<const float2*>(src + lane * N);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        den += w[u];
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] = fmaf(w[u], v[u][e], acc[e]);
+      }
+    }
+  }
+  const bool any = den > 0.f || den != den;
+  const float inv = any ? 1.f / den : 0.f;
+  T* out = reinterpret_cast<T*>(p.out + (int64_t)tok * p.o_tok + (int64_t)head * p.o_head) + lane * N;
+  if constexpr (N == 4)
+    *reinterpret_cast<uint2*>(out) = make_uint2(Elem<T>::pack2(acc[0] * inv, acc[1] * inv), Elem<T>::pack2(acc[2] * inv, acc[3] * inv));
+  else
+    *reinterpret_cast<uint32_t*>(out) = Elem<T>::pack2(acc[0] * inv, acc[1] * inv);
+  if (p.lse && lane == 0)
+    p.lse[(int64_t)tok * p.l_tok + (int64_t)head * p.l_head] = any ? Ms + __log2f(den) * kLn2 : -INFINITY;
+}
+
+// -------------------------------------------------------------------------
 // host
 // -------------------------------------------------------------------------
 struct Layout {
   int grid, part_rows, TQ;
-  size_t parts, lse, o, cost, units, plan, share, bytes;
+  size_t parts, lse, o, cost, units, plan, share, seqs, prefix, row_o, row_lse, row_at, bytes;
 };
 
 // The grid is one CTA per SM, or less where the tables' bounds show that there
 // are fewer tiles: a sequence has at most one unit more per head than its rows
 // fill, and a unit at most as many tiles as all pages hold.
-Layout make_layout(const akt_chunk_paged_args* a) {
+Layout make_layout(const akt_chunk_paged_args* a, int groups, bool shared) {
   Layout y{};
   const int G = a->num_qo_heads / a->num_kv_heads;
   y.TQ = BM / G;
-  const int64_t units = ((int64_t)a->num_tokens / (2 * y.TQ) + std::min<int64_t>(a->batch, a->num_tokens)) * a->num_kv_heads;
+  int64_t units = (int64_t)a->num_tokens / (2 * y.TQ) + std::min<int64_t>(a->batch, a->num_tokens);
+  if (shared) units += (int64_t)a->num_tokens / (2 * y.TQ) + std::min<int64_t>(groups, a->num_tokens);
+  units *= a->num_kv_heads;
   const int64_t tiles = a->num_page_entries * a->page_size / BN + 1;
   y.grid = std::min(sm_count(), kMaxCtas - 1);  // (the planning threads are one more)
   if (units < y.grid && units * tiles < y.grid) y.grid = (int)std::max<int64_t>(1, units * tiles);
@@ -1459,11 +1664,20 @@ Layout make_layout(const akt_chunk_paged_args* a) {
   y.parts = take((size_t)y.grid * 2 * sizeof(Part));
   y.lse = take((size_t)y.grid * 2 * y.part_rows * 4);
   y.o = take((size_t)y.grid * 2 * y.part_rows * a->head_dim * 4);
-  if (a->batch > kTableSeqs) {
-    y.cost = take(((size_t)a->batch + 1) * 8);
-    y.units = take(((size_t)a->batch + 1) * 4);
+  const size_t seqs = (size_t)a->batch + (size_t)groups;
+  if (shared || a->batch > kTableSeqs) {
+    y.cost = take((seqs + 1) * 8);
+    y.units = take((seqs + 1) * 4);
     y.plan = take(sizeof(Plan));
     y.share = take(((size_t)y.grid + 1) * 8);
+  }
+  if (shared) {
+    const size_t rows = (size_t)a->num_tokens * a->num_qo_heads;
+    y.seqs = take(seqs * sizeof(Seq));
+    y.prefix = take((size_t)a->batch * 4);
+    y.row_o = take(2 * rows * a->head_dim * 4);
+    y.row_lse = take(2 * rows * 4);
+    y.row_at = take(2 * rows * sizeof(int2));
   }
   y.bytes = at;
   return y;
@@ -1502,10 +1716,10 @@ int check_args(const akt_chunk_paged_args* a) {
   return AKT_OK;
 }
 
-template <typename T, int D, bool TMA>
+template <typename T, int D, bool TMA, bool SHARED>
 int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const ChunkParams& p,
                  cudaStream_t st) {
-  auto kern = chunk_fwd_kernel<T, D, TMA>;
+  auto kern = chunk_fwd_kernel<T, D, TMA, SHARED>;
   constexpr int smem = (int)Cfg<D>::SMEM_ALL;
   // the register split in the kernel is only valid at the compiled count
   static const int regs = [&] {
@@ -1515,16 +1729,20 @@ int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap
   if (regs != kLaunchRegs)
     return set_error(AKT_ERR_CUDA, "chunk kernel compiled with " + std::to_string(regs) + " registers, expected " +
                                        std::to_string(kLaunchRegs));
-  cudaError_t e = ensure_smem_limit<chunk_fwd_kernel<T, D, TMA>>((size_t)smem);
+  cudaError_t e = ensure_smem_limit<chunk_fwd_kernel<T, D, TMA, SHARED>>((size_t)smem);
   if (e != cudaSuccess) return set_error(AKT_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
-  const bool planned = p.B > kTableSeqs;
-  if (planned) chunk_plan_kernel<<<1, 1024, 0, st>>>(p);
+  const bool planned = SHARED || p.B > kTableSeqs;
+  if (planned) chunk_plan_kernel<SHARED><<<1, 1024, 0, st>>>(p);
   {
     ProfileScope prof(st);
     if (planned) e = launch_dependent(kern, dim3(p.grid), dim3(kThreads), smem, st, mq, mk, mv, p);
     else kern<<<p.grid, kThreads, smem, st>>>(mq, mk, mv, p);
   }
-  if (e == cudaSuccess)
+  if (SHARED && e == cudaSuccess) {
+    constexpr int per = kMergeThreads / 32;
+    const int64_t rows = p.num_tokens * p.Hq;
+    e = launch_dependent(chunk_join_kernel<T, D>, dim3((unsigned)((rows + per - 1) / per)), dim3(kMergeThreads), 0, st, p);
+  } else if (e == cudaSuccess)
     e = launch_dependent(chunk_merge_kernel<T, D>, dim3(2 * p.grid, (p.part_rows + p.merge_rows - 1) / p.merge_rows),
                          dim3(kMergeThreads), 0, st, p);
   if (e == cudaSuccess) e = cudaGetLastError();
@@ -1534,7 +1752,9 @@ int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap
 template <typename T, int D>
 int dispatch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const ChunkParams& p,
                    cudaStream_t st) {
-  return p.box_rows ? launch_chunk<T, D, true>(mq, mk, mv, p, st) : launch_chunk<T, D, false>(mq, mk, mv, p, st);
+  if (p.row_o)
+    return p.box_rows ? launch_chunk<T, D, true, true>(mq, mk, mv, p, st) : launch_chunk<T, D, false, true>(mq, mk, mv, p, st);
+  return p.box_rows ? launch_chunk<T, D, true, false>(mq, mk, mv, p, st) : launch_chunk<T, D, false, false>(mq, mk, mv, p, st);
 }
 
 }  // namespace
@@ -1550,19 +1770,23 @@ cudaError_t chunk_status_clear() {
 
 using namespace akt;
 
-extern "C" size_t akt_chunk_paged_workspace_size(const akt_chunk_paged_args* a) {
-  if (!a || a->num_qo_heads <= 0 || a->num_kv_heads <= 0 || a->num_qo_heads % a->num_kv_heads || a->num_tokens <= 0 ||
+namespace {
+
+size_t workspace_size(const akt_chunk_paged_args* a, int groups, bool shared) {
+  if (a->num_qo_heads <= 0 || a->num_kv_heads <= 0 || a->num_qo_heads % a->num_kv_heads || a->num_tokens <= 0 ||
       a->batch <= 0 || a->num_qo_heads / a->num_kv_heads > BM || a->page_size <= 0 || a->head_dim <= 0 ||
       a->num_page_entries < 0)
     return 0;
-  return make_layout(a).bytes;
+  return make_layout(a, groups, shared).bytes;
 }
 
-extern "C" int akt_chunk_paged(const akt_chunk_paged_args* a, void* workspace, size_t workspace_bytes, void* stream) {
-  if (!a) return set_error(AKT_ERR_INVALID, "null args");
+// shared: the groups of a batch with shared prefixes, or null
+int run_chunk(const akt_chunk_paged_args* a, const akt_prefix_paged_args* shared, void* workspace, size_t workspace_bytes,
+              void* stream) {
   int rc = check_args(a);
   if (rc || a->num_tokens == 0) return rc;
-  const Layout y = make_layout(a);
+  const int groups = shared ? shared->num_groups : 0;
+  const Layout y = make_layout(a, groups, shared != nullptr);
   if (!workspace || workspace_bytes < y.bytes)
     return set_error(AKT_ERR_WORKSPACE, "chunk_paged: workspace of " + std::to_string(y.bytes) + " bytes required");
   ChunkParams p{};
@@ -1587,7 +1811,9 @@ extern "C" int akt_chunk_paged(const akt_chunk_paged_args* a, void* workspace, s
   p.lse = a->lse;
   p.l_tok = a->lse_stride_token;
   p.l_head = a->lse_stride_head;
-  p.B = a->batch;
+  p.batch = a->batch;
+  p.groups = groups;
+  p.B = a->batch + groups;
   p.Hq = a->num_qo_heads;
   p.Hkv = a->num_kv_heads;
   p.group = p.Hq / p.Hkv;
@@ -1609,7 +1835,16 @@ extern "C" int akt_chunk_paged(const akt_chunk_paged_args* a, void* workspace, s
   // many rows would be many CTAs that mostly find nothing to join (8 prompts of 2048
   // tokens: 305 us, 316 with a row a warp).
   p.merge_rows = y.part_rows <= 64 ? 8 : 32;
-  if (p.B > kTableSeqs) {
+  if (shared) {
+    p.group_indptr = shared->group_indptr;
+    p.shared_pages = shared->shared_pages;
+    p.seqs = reinterpret_cast<Seq*>(ws + y.seqs);
+    p.prefix_len = reinterpret_cast<int*>(ws + y.prefix);
+    p.row_o = reinterpret_cast<float*>(ws + y.row_o);
+    p.row_lse = reinterpret_cast<float*>(ws + y.row_lse);
+    p.row_at = reinterpret_cast<int2*>(ws + y.row_at);
+  }
+  if (shared || p.B > kTableSeqs) {
     p.plan_cost = reinterpret_cast<int64_t*>(ws + y.cost);
     p.plan_units = reinterpret_cast<int*>(ws + y.units);
     p.plan = reinterpret_cast<Plan*>(ws + y.plan);
@@ -1653,4 +1888,28 @@ extern "C" int akt_chunk_paged(const akt_chunk_paged_args* a, void* workspace, s
     return p.D == 64 ? dispatch_chunk<__half, 64>(mq, mk, mv, p, st) : dispatch_chunk<__half, 128>(mq, mk, mv, p, st);
   return p.D == 64 ? dispatch_chunk<__nv_bfloat16, 64>(mq, mk, mv, p, st)
                    : dispatch_chunk<__nv_bfloat16, 128>(mq, mk, mv, p, st);
+}
+
+}  // namespace
+
+extern "C" size_t akt_chunk_paged_workspace_size(const akt_chunk_paged_args* a) {
+  return a ? workspace_size(a, 0, false) : 0;
+}
+
+extern "C" int akt_chunk_paged(const akt_chunk_paged_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!a) return set_error(AKT_ERR_INVALID, "null args");
+  return run_chunk(a, nullptr, workspace, workspace_bytes, stream);
+}
+
+extern "C" size_t akt_prefix_paged_workspace_size(const akt_prefix_paged_args* a) {
+  return a && a->num_groups >= 0 ? workspace_size(&a->chunk, a->num_groups, true) : 0;
+}
+
+extern "C" int akt_prefix_paged(const akt_prefix_paged_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!a) return set_error(AKT_ERR_INVALID, "null args");
+  if (a->num_groups < 0 || (int64_t)a->num_groups + std::max(a->chunk.batch, 0) > 0x3fffffff)
+    return set_error(AKT_ERR_INVALID, "prefix_paged: bad number of groups");
+  if (a->num_groups > 0 && (!a->group_indptr || !a->shared_pages))
+    return set_error(AKT_ERR_INVALID, "prefix_paged: missing groups");
+  return run_chunk(&a->chunk, a, workspace, workspace_bytes, stream);
 }

@@ -489,6 +489,50 @@ __global__ void __launch_bounds__(kPlanThreads)
 }
 
 // ---------------------------------------------------------------------------
+// pages that the sequences of a group have in common
+// ---------------------------------------------------------------------------
+// A CTA per group: every sequence's entries against the first one's.
+__global__ void __launch_bounds__(kCopyThreads)
+    shared_pages_kernel(const int32_t* groups, const int32_t* indptr, const int32_t* indices, const int32_t* last,
+                        int batch, int64_t num_entries, int P, int32_t* out) {
+  __shared__ int common;
+  const int g = blockIdx.x, b0 = __ldg(groups + g), b1 = __ldg(groups + g + 1);
+  if (b0 < 0 || b1 < b0 || b1 > batch) {
+    if (threadIdx.x == 0) {
+      record_status(kStatusBadIndptr);
+      out[g] = 0;
+    }
+    return;
+  }
+  if (threadIdx.x == 0) common = b1 - b0 < 2 ? 0 : 0x7fffffff;
+  __syncthreads();
+  for (int b = b0 + threadIdx.x; b < b1; b += kCopyThreads) {  // full pages
+    const int s = __ldg(indptr + b), e = __ldg(indptr + b + 1);
+    if (s < 0 || e < s || e > num_entries) {
+      record_status(kStatusBadIndptr);
+      atomicMin(&common, 0);
+    } else {
+      atomicMin(&common, e > s && __ldg(last + b) < P ? e - s - 1 : e - s);
+    }
+  }
+  __syncthreads();
+  const int most = common, s0 = most > 0 ? __ldg(indptr + b0) : 0;
+  __syncthreads();
+  for (int b = b0 + 1; b < b1; ++b) {
+    const int n = min(most, common);  // (of any moment: it only falls)
+    if (n <= 0) break;
+    const int s = __ldg(indptr + b);
+    for (int i = threadIdx.x; i < n; i += kCopyThreads)
+      if (__ldg(indices + s + i) != __ldg(indices + s0 + i)) {
+        atomicMin(&common, i);
+        break;
+      }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) out[g] = common;
+}
+
+// ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
 size_t round16(size_t n) { return (n + 15) & ~size_t(15); }
@@ -733,4 +777,24 @@ extern "C" int akt_free_kv_pages(const int32_t* indices, int64_t num_entries, co
   }
   e = cudaGetLastError();
   return e == cudaSuccess ? AKT_OK : cuda_error("free_kv_pages", e);
+}
+
+extern "C" int akt_shared_prefix_pages(const int32_t* group_indptr, int32_t num_groups, const int32_t* kv_page_indptr,
+                                       const int32_t* kv_page_indices, const int32_t* kv_last_page_len, int32_t batch,
+                                       int64_t num_page_entries, int32_t page_size, int32_t* shared_pages, void* stream) {
+  if (num_groups < 0 || batch < 0 || num_page_entries < 0 || num_page_entries > 0x7fffffff || page_size <= 0)
+    return set_error(AKT_ERR_INVALID, "shared_prefix_pages: bad sizes");
+  if (num_groups == 0) return AKT_OK;
+  if (!group_indptr || !shared_pages || (batch > 0 && (!kv_page_indptr || !kv_last_page_len)) ||
+      (num_page_entries > 0 && !kv_page_indices))
+    return set_error(AKT_ERR_INVALID, "shared_prefix_pages: missing table");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  {
+    ProfileScope prof(st);
+    shared_pages_kernel<<<num_groups, kCopyThreads, 0, st>>>(group_indptr, kv_page_indptr, kv_page_indices,
+                                                             kv_last_page_len, batch, num_page_entries, page_size,
+                                                             shared_pages);
+  }
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? AKT_OK : cuda_error("shared_prefix_pages", e);
 }

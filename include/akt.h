@@ -588,6 +588,35 @@ int akt_free_kv_pages(const int32_t* kv_page_indices, int64_t num_page_entries, 
                       size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* attention behind shared prefixes (no reference counterpart)              */
+/* akt_chunk_paged for a batch in which the sequences group_indptr[g] ..    */
+/* group_indptr[g + 1] have their first shared_pages[g] pages in common (as */
+/* forked sequences do): the shared K and V are read once for the group.    */
+/* Results are those of akt_chunk_paged up to rounding.  The first sequence */
+/* of a group that has rows stands for the shared pages of all.  What of    */
+/* the shared pages a sequence does not have, or (causal) a row does not    */
+/* see, is not shared in its group.  group_indptr ascends within [0, batch];*/
+/* sequences outside it are groups of their own; bounds that do not ascend  */
+/* are recorded (status 4) and nothing is shared.                           */
+/* ------------------------------------------------------------------------ */
+typedef struct akt_prefix_paged_args {
+  akt_chunk_paged_args chunk;
+  const int32_t* group_indptr; /* [num_groups + 1] */
+  const int32_t* shared_pages; /* [num_groups] */
+  int32_t num_groups;
+} akt_prefix_paged_args;
+
+size_t akt_prefix_paged_workspace_size(const akt_prefix_paged_args* args);
+int akt_prefix_paged(const akt_prefix_paged_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* shared_pages[g] = how many full pages all sequences of the group have in  */
+/* common from the first on (0 for fewer than two sequences, and where the   */
+/* group's or a sequence's bounds are bad, recorded as status 4).            */
+int akt_shared_prefix_pages(const int32_t* group_indptr, int32_t num_groups, const int32_t* kv_page_indptr,
+                            const int32_t* kv_page_indices, const int32_t* kv_last_page_len, int32_t batch,
+                            int64_t num_page_entries, int32_t page_size, int32_t* shared_pages, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* eviction from a paged KV cache by accumulated attention weight (no       */
 /* reference counterpart: its sparse decodes take lists of kept tokens)     */
 /* ------------------------------------------------------------------------ */
