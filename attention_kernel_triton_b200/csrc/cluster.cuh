@@ -33,6 +33,23 @@ __device__ __forceinline__ int cluster_read(const int* local, uint32_t rank) {
   return v;
 }
 
+__device__ __forceinline__ int4 cluster_read4(const int* local, uint32_t rank) {
+  uint32_t a;
+  int4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(local)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+// Adds x to it.
+__device__ __forceinline__ void cluster_add(const int* local, uint32_t rank, int x) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(local)), "r"(rank));
+  asm volatile("red.relaxed.cluster.shared::cluster.add.s32 [%0], %1;" ::"r"(a), "r"(x) : "memory");
+}
+
 // `cluster` divides grid.x.  `dependent`: a programmatic dependent launch.
 template <typename... KArgs, typename... Args>
 cudaError_t launch_cluster(void (*kern)(KArgs...), dim3 grid, dim3 block, unsigned cluster, bool dependent, size_t smem,

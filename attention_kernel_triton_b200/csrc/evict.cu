@@ -7,8 +7,9 @@
 // select over an order-preserving map of fp32 to 32-bit keys (digits of 11, 11
 // and 10 bits from the top, a histogram each), then the list is written in
 // ascending order by ballots and prefix sums, the lowest of equal weights first.
-// A cluster of CTAs holds the head's keys in shared memory, so the weights are
-// read once; the histograms and counts are summed over distributed shared memory.
+// A first histogram, of the largest keys of groups of tokens, leaves few more than k
+// of them, which go into lists in shared memory.  A cluster of CTAs shares a head where
+// there are few; its histograms and counts are summed over distributed shared memory.
 //
 // Eviction.  Slot i of a head takes the row of token keep[i].  Lists ascend, so
 // keep[i] >= i: rows only move down and a sequence can stay in its own pages.  A
@@ -47,9 +48,10 @@ int cuda_error(const char* what, cudaError_t e) {
 // ---------------------------------------------------------------------------
 // choice of the kept tokens
 // ---------------------------------------------------------------------------
-constexpr int kSelectThreads = 1024;
+constexpr int kSelectThreads = 512;
+constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kBins = 2048;
-constexpr int kMaxKeys = 48 * 1024;  // of a CTA in shared memory
+constexpr int kList = 512;  // tokens of a warp's list
 
 struct SelectParams {
   const float* w;
@@ -59,128 +61,232 @@ struct SelectParams {
   int64_t i_layer, i_batch, i_head;
   int32_t* kept;
   int B, H, width, budget, sinks, recent;
-  int cached;  // the CTA's share of a head fits its shared memory
 };
 
-// Larger floats have larger keys; -0 is 0, and NaN comes below everything.
+// Larger floats have larger keys; -0 is 0, NaN comes below everything, and 0 is no float's key.
 __device__ __forceinline__ uint32_t order_key(float f) {
-  if (f != f) return 0u;
+  if (f != f) return 1u;
   const uint32_t u = __float_as_uint(f + 0.f);
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(kSelectThreads) select_kernel(const SelectParams p) {
-  extern __shared__ uint32_t keys_s[];
-  __shared__ int hist[3][kBins];
-  __shared__ int sums[33];
-  __shared__ int found[2];       // digit, how many are wanted of it
-  __shared__ int warp_count[2][32];
-  __shared__ int cta_count[2];   // tokens that stay for sure, tokens at the threshold
+// Sum of x over the threads before this one; `sums` holds a value per warp.
+__device__ __forceinline__ int select_scan(int x, int* sums, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int v = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  if (lane == 31) sums[warp] = v;
+  __syncthreads();
+  int y = lane < kSelectWarps ? sums[lane] : 0;
+  total = __reduce_add_sync(0xffffffffu, y);
+  const int before = __reduce_add_sync(0xffffffffu, lane < warp ? y : 0);
+  __syncthreads();
+  return before + v - x;
+}
+
+__global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectParams p) {
+  extern __shared__ uint32_t lists[];  // each warp's [kList] keys, then each warp's [kList] places in its segment
+  __shared__ __align__(16) int hist[4][kBins];
+  __shared__ int sums[kSelectWarps];
+  __shared__ int found[3];      // digit, how many are wanted of it, how many have it
+  __shared__ int cta_count[2];  // tokens that stay for sure, tokens at the threshold
   const int C = (int)cluster_size(), rank = (int)cluster_rank(), row = blockIdx.x / C;
   const int h = row % p.H, b = row / p.H % p.B, l = row / p.H / p.B;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int asked = __ldg(p.lens + b), n = min(max(asked, 0), p.width);
-  if (asked != n && threadIdx.x == 0) record_status(kStatusBadToken);
+  if (asked != n && tid == 0) record_status(kStatusBadToken);
   int32_t* ind = p.ind + l * p.i_layer + b * p.i_batch + h * p.i_head;
-  if (l == 0 && h == 0 && rank == 0 && threadIdx.x == 0) p.kept[b] = min(n, p.budget);
+  if (l == 0 && h == 0 && rank == 0 && tid == 0) p.kept[b] = min(n, p.budget);
   if (n <= p.budget) {  // all stay
-    for (int i = rank * kSelectThreads + threadIdx.x; i < p.budget; i += C * kSelectThreads) ind[i] = i < n ? i : 0;
+    for (int i = rank * kSelectThreads + tid; i < p.budget; i += C * kSelectThreads) ind[i] = i < n ? i : 0;
     return;
   }
   const float* w = p.w + l * p.w_layer + b * p.w_batch + h * p.w_head;
-  const int slice = ((n + C - 1) / C + 31) / 32 * 32, lo = min(rank * slice, n), hi = min(lo + slice, n);
+  // a CTA's slice of the tokens, a warp's segment of it (both multiples of 32)
+  const int seg = (((n + C - 1) / C + kSelectWarps - 1) / kSelectWarps + 31) / 32 * 32, slice = seg * kSelectWarps;
+  const int lo = min(rank * slice, n), hi = min(lo + slice, n);
+  const int s0 = min(lo + warp * seg, hi), s1 = min(s0 + seg, hi);
   const int k = p.budget - p.sinks - p.recent, c0 = p.sinks, c1 = n - p.recent;  // candidates [c0, c1)
-  for (int i = threadIdx.x; i < 3 * kBins; i += kSelectThreads) (&hist[0][0])[i] = 0;
-  if (p.cached) {
-    constexpr int U = 8;
-    for (int j = lo + threadIdx.x; j < hi; j += U * kSelectThreads) {
-      float f[U];
+  uint32_t* list_key = lists + warp * kList;
+  int32_t* list_at = reinterpret_cast<int32_t*>(lists + kSelectWarps * kList) + warp * kList;
+  for (int i = tid; i < 4 * kBins / 4; i += kSelectThreads) reinterpret_cast<int4*>(&hist[0][0])[i] = make_int4(0, 0, 0, 0);
+  if (C > 1) cluster_sync(); else __syncthreads();
+  // f(first token of a block of 32 U, the lanes' keys of it): 0 where there is no candidate
+  constexpr int U = 8;
+  auto blocks = [&](auto&& f) {
+    for (int j0 = s0; j0 < s1; j0 += 32 * U) {
+      uint32_t x[U];
+      if (j0 >= c0 && j0 + 32 * U <= min(s1, c1)) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) f[u] = j + u * kSelectThreads < hi ? __ldg(w + j + u * kSelectThreads) : 0.f;
+        for (int u = 0; u < U; ++u) x[u] = __float_as_uint(__ldg(w + j0 + 32 * u + lane));
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (j + u * kSelectThreads < hi) keys_s[j + u * kSelectThreads - lo] = order_key(f[u]);
+        for (int u = 0; u < U; ++u) x[u] = order_key(__uint_as_float(x[u]));
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int j = j0 + 32 * u + lane;
+          x[u] = j < s1 && j >= c0 && j < c1 ? order_key(__ldg(w + j)) : 0u;
+        }
+      }
+      f(j0, x);
     }
+  };
+  // The digit at which the sum of histogram d over the cluster, from the top, reaches
+  // `want`; how many are wanted of it and how many have it.  False: there are fewer.
+  // Rank 0 gets the others' counts.
+  auto find = [&](int d, int want) -> bool {
+    if (tid == 0) found[0] = -1;
+    __syncthreads();
+    constexpr int E = kBins / kSelectThreads;
+    static_assert(E == 4, "a thread's bins");
+    const int at = kBins - E * (tid + 1);  // this thread's bins, from the top down
+    int4 own = *reinterpret_cast<const int4*>(&hist[d][at]);
+    if (C > 1) {
+      if (rank) {
+        if (own.x) cluster_add(&hist[d][at], 0, own.x);
+        if (own.y) cluster_add(&hist[d][at + 1], 0, own.y);
+        if (own.z) cluster_add(&hist[d][at + 2], 0, own.z);
+        if (own.w) cluster_add(&hist[d][at + 3], 0, own.w);
+      }
+      cluster_sync();
+      own = cluster_read4(&hist[d][at], 0);
+    }
+    const int sum = own.x + own.y + own.z + own.w;
+    int all;
+    int before = select_scan(sum, sums, all);
+    if (before < want && want <= before + sum) {
+      const int c[E] = {own.w, own.z, own.y, own.x};
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (before < want && want <= before + c[e]) {
+          found[0] = at + E - 1 - e;
+          found[1] = want - before;
+          found[2] = c[e];
+        }
+        before += c[e];
+      }
+    }
+    __syncthreads();
+    return found[0] >= 0;
+  };
+  uint32_t least = 1;  // no key below it is one of the k largest
+  // The k-th largest of the largest keys of groups is no more than the k-th largest of all.
+  // So a histogram of those, of groups of 8 tokens or 2, leaves few more than k keys to
+  // look at (k of n: 3 % of 32768 leaves 3 %, 24 % of 131072 leaves 28 %).
+  const int group = (int64_t)16 * k <= n ? 8 : ((int64_t)3 * k <= n ? 2 : 0);
+  if (k > 0 && group) {
+    blocks([&](int, const uint32_t (&x)[U]) {
+      uint32_t m[U / 2];
+#pragma unroll
+      for (int u = 0; u < U / 2; ++u) m[u] = max(x[2 * u], x[2 * u + 1]);
+      if (group == 8) {
+        m[0] = max(max(m[0], m[1]), max(m[2], m[3]));
+        if (m[0]) atomicAdd(&hist[3][m[0] >> 21], 1);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U / 2; ++u)
+          if (m[u]) atomicAdd(&hist[3][m[u] >> 21], 1);
+      }
+    });
+    if (find(3, k)) least = max(1u, (uint32_t)found[0] << 21);
   }
-  __syncthreads();
-  auto key = [&](int j) -> uint32_t { return p.cached ? keys_s[j - lo] : order_key(__ldg(w + j)); };
+  // ---- each warp's tokens that are left, in order; where they are more than its list
+  // holds they are read again for every pass
+  int count = 0;
+  blocks([&](int j0, const uint32_t (&x)[U]) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + 32 * u + lane;
+      const bool left = j < s1 && (x[u] >= least || j < c0 || j >= c1);
+      const unsigned m = __ballot_sync(0xffffffffu, left);
+      if (!m) continue;
+      const int at = count + __popc(m & ((1u << lane) - 1u));
+      if (left && at < kList) {
+        list_key[at] = x[u];
+        list_at[at] = j;
+      }
+      count += __popc(m);
+    }
+  });
+  __syncwarp();
+  // f(whether there is one, token, its key) in order, 32 at a time
+  auto each = [&](auto&& f) {
+    if (count <= kList) {
+      for (int i0 = 0; i0 < count; i0 += 32) {
+        const bool there = i0 + lane < count;
+        f(there, there ? list_at[i0 + lane] : 0, there ? list_key[i0 + lane] : 0u);
+      }
+    } else {
+      blocks([&](int j0, const uint32_t (&x)[U]) {
+#pragma unroll 1
+        for (int u = 0; u < U; ++u) {
+          const int j = j0 + 32 * u + lane;
+          uint32_t key = 0;
+#pragma unroll
+          for (int e = 0; e < U; ++e) key = e == u ? x[e] : key;
+          f(j < s1, j, key);
+        }
+      });
+    }
+  };
   uint32_t top = 0, mask = 0;  // the threshold's digits so far
-  int want = k;
+  int want = k, have = 0;
   if (k > 0) {
 #pragma unroll 1
     for (int d = 0; d < 3; ++d) {
       const int shift = d == 0 ? 21 : (d == 1 ? 10 : 0);
       const uint32_t digit_mask = d == 2 ? 0x3ffu : 0x7ffu;
-      for (int j = max(lo, c0) + threadIdx.x; j < min(hi, c1); j += kSelectThreads) {
-        const uint32_t x = key(j);
-        if ((x & mask) == top) atomicAdd(&hist[d][(x >> shift) & digit_mask], 1);
-      }
-      if (C > 1) cluster_sync(); else __syncthreads();
-      // the two bins of this thread, from the top
-      int own[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int bin = kBins - 1 - 2 * (int)threadIdx.x - e;
-        own[e] = 0;
-        for (int r = 0; r < C; ++r) own[e] += C > 1 ? cluster_read(&hist[d][bin], r) : hist[d][bin];
-      }
-      int all;
-      const int before = block_scan<int>(own[0] + own[1], sums, all);
-      if (before < want && want <= before + own[0] + own[1]) {
-        const int e = want > before + own[0];
-        found[0] = kBins - 1 - 2 * (int)threadIdx.x - e;
-        found[1] = want - before - (e ? own[0] : 0);
-      }
-      __syncthreads();
+      each([&](bool, int, uint32_t x) {
+        if (x >= least && (x & mask) == top) atomicAdd(&hist[d][(x >> shift) & digit_mask], 1);
+      });
+      find(d, want);
       top |= (uint32_t)found[0] << shift;
       mask |= digit_mask << shift;
       want = found[1];
+      have = found[2];
     }
   }
-  // which tokens stay: the ones always kept, the ones above the threshold, `want` of the ones at it
-  auto state = [&](int j) -> int {  // 2: stays, 1: at the threshold
-    if (j < c0 || j >= c1) return 2;
-    if (k == 0) return 0;
-    const uint32_t x = key(j);
-    return x > top ? 2 : (x == top ? 1 : 0);
+  // ---- Which tokens stay: the ones always kept, the ones above the threshold and `want`
+  // of the `have` at it (the first ones; where they are all, their order does not matter).
+  const bool ties = want < have;
+  auto sure = [&](bool there, int j, uint32_t x) {
+    return there && (j < c0 || j >= c1 || (k > 0 && x && (ties ? x > top : x >= top)));
   };
-  const int seg = slice / 32 + 31 & ~31, s0 = min(lo + warp * seg, hi), s1 = min(s0 + seg, hi);
   int n_sure = 0, n_equal = 0;
-  for (int j0 = s0; j0 < s1; j0 += 32) {
-    const int st = j0 + lane < s1 ? state(j0 + lane) : 0;
-    n_sure += __popc(__ballot_sync(0xffffffffu, st == 2));
-    n_equal += __popc(__ballot_sync(0xffffffffu, st == 1));
+  each([&](bool there, int j, uint32_t x) {
+    n_sure += sure(there, j, x);
+    n_equal += ties && x == top;
+  });
+  int all;
+  int sure_before = select_scan(n_sure, sums, all);
+  if (tid == 0) cta_count[0] = all;
+  int equal_before = 0;
+  if (ties) {
+    equal_before = select_scan(n_equal, sums, all);
+    if (tid == 0) cta_count[1] = all;
   }
-  if (lane == 0) {
-    warp_count[0][warp] = n_sure;
-    warp_count[1][warp] = n_equal;
-  }
-  __syncthreads();
-  int sure = 0, equal = 0;  // before this warp's tokens
-  for (int i = 0; i < warp; ++i) {
-    sure += warp_count[0][i];
-    equal += warp_count[1][i];
-  }
-  if (threadIdx.x == kSelectThreads - 1) {
-    cta_count[0] = sure + n_sure;
-    cta_count[1] = equal + n_equal;
-  }
+  sure_before = __shfl_sync(0xffffffffu, sure_before, 0);  // before the warp
+  equal_before = __shfl_sync(0xffffffffu, equal_before, 0);
   if (C > 1) {
     cluster_sync();
     for (int r = 0; r < rank; ++r) {
-      sure += cluster_read(&cta_count[0], r);
-      equal += cluster_read(&cta_count[1], r);
+      sure_before += cluster_read(&cta_count[0], r);
+      if (ties) equal_before += cluster_read(&cta_count[1], r);
     }
   }
   const unsigned below = (1u << lane) - 1u;
-  for (int j0 = s0; j0 < s1; j0 += 32) {
-    const int j = j0 + lane, st = j < s1 ? state(j) : 0;
-    const unsigned m2 = __ballot_sync(0xffffffffu, st == 2), m1 = __ballot_sync(0xffffffffu, st == 1);
-    const int eq = equal + __popc(m1 & below);
-    if (st == 2 || (st == 1 && eq < want)) ind[sure + __popc(m2 & below) + min(eq, want)] = j;
-    sure += __popc(m2);
-    equal += __popc(m1);
-  }
+  each([&](bool there, int j, uint32_t x) {
+    const bool stays = sure(there, j, x), equal = ties && x == top;
+    const unsigned ms = __ballot_sync(0xffffffffu, stays), me = ties ? __ballot_sync(0xffffffffu, equal) : 0u;
+    const int eq = equal_before + __popc(me & below);
+    if (stays || (equal && eq < want)) ind[sure_before + __popc(ms & below) + min(eq, want)] = j;
+    sure_before += __popc(ms);
+    equal_before += __popc(me);
+  });
   if (C > 1) cluster_sync();  // the others' reads of this CTA's counts
 }
 
@@ -531,11 +637,10 @@ extern "C" int akt_select_tokens(const akt_select_tokens_args* a, void* stream) 
   p.budget = a->budget;
   p.sinks = a->sinks;
   p.recent = a->recent;
-  int C = 8;
-  while (C > 1 && (rows * C > 8 * sm_count() || p.width / C < 2048)) C /= 2;
-  const int slice = ((p.width + C - 1) / C + 31) / 32 * 32;
-  p.cached = slice <= kMaxKeys;
-  const size_t smem = p.cached ? (size_t)slice * 4 : 0;
+  // more CTAs to a head while there are SMs without one
+  int C = 1;
+  while (C < 8 && rows * C < sm_count() && p.width > C * 2048) C *= 2;
+  constexpr size_t smem = (size_t)kSelectWarps * kList * 8;
   cudaError_t e = ensure_smem_limit<select_kernel>(smem);
   if (e != cudaSuccess) return cuda_error("select_tokens", e);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
