@@ -70,7 +70,13 @@ __device__ __forceinline__ uint32_t order_key(float f) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// Sum of x over the threads before this one; `sums` holds a value per warp.
+// The least float with at least this key (no less than the one of -infinity).
+__device__ __forceinline__ float key_value(uint32_t key) {
+  return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key);
+}
+
+// Sum of x over the threads before this one; `sums` holds a value per warp (of one call
+// in two: a call's writes follow a barrier after the reads of the one before last).
 __device__ __forceinline__ int select_scan(int x, int* sums, int& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int v = x;
@@ -84,14 +90,13 @@ __device__ __forceinline__ int select_scan(int x, int* sums, int& total) {
   int y = lane < kSelectWarps ? sums[lane] : 0;
   total = __reduce_add_sync(0xffffffffu, y);
   const int before = __reduce_add_sync(0xffffffffu, lane < warp ? y : 0);
-  __syncthreads();
   return before + v - x;
 }
 
 __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectParams p) {
   extern __shared__ uint32_t lists[];  // each warp's [kList] keys, then each warp's [kList] places in its segment
   __shared__ __align__(16) int hist[4][kBins];
-  __shared__ int sums[kSelectWarps];
+  __shared__ int sums[2][kSelectWarps];
   __shared__ int found[3];      // digit, how many are wanted of it, how many have it
   __shared__ int cta_count[2];  // tokens that stay for sure, tokens at the threshold
   const int C = (int)cluster_size(), rank = (int)cluster_rank(), row = blockIdx.x / C;
@@ -114,32 +119,31 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectP
   uint32_t* list_key = lists + warp * kList;
   int32_t* list_at = reinterpret_cast<int32_t*>(lists + kSelectWarps * kList) + warp * kList;
   for (int i = tid; i < 4 * kBins / 4; i += kSelectThreads) reinterpret_cast<int4*>(&hist[0][0])[i] = make_int4(0, 0, 0, 0);
+  if (tid == 0) found[0] = -1;
   if (C > 1) cluster_sync(); else __syncthreads();
-  // f(first token of a block of 32 U, the lanes' keys of it): 0 where there is no candidate
+  // f(first token of a block of 32 U, whether all are candidates, the lanes' weights of it: NaN where there is none)
   constexpr int U = 8;
   auto blocks = [&](auto&& f) {
     for (int j0 = s0; j0 < s1; j0 += 32 * U) {
-      uint32_t x[U];
-      if (j0 >= c0 && j0 + 32 * U <= min(s1, c1)) {
+      float x[U];
+      const bool inside = j0 >= c0 && j0 + 32 * U <= min(s1, c1);
+      if (inside) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) x[u] = __float_as_uint(__ldg(w + j0 + 32 * u + lane));
-#pragma unroll
-        for (int u = 0; u < U; ++u) x[u] = order_key(__uint_as_float(x[u]));
+        for (int u = 0; u < U; ++u) x[u] = __ldg(w + j0 + 32 * u + lane);
       } else {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int j = j0 + 32 * u + lane;
-          x[u] = j < s1 && j >= c0 && j < c1 ? order_key(__ldg(w + j)) : 0u;
+          x[u] = j < s1 && j >= c0 && j < c1 ? __ldg(w + j) : __int_as_float(0x7fffffff);
         }
       }
-      f(j0, x);
+      f(j0, inside, x);
     }
   };
   // The digit at which the sum of histogram d over the cluster, from the top, reaches
   // `want`; how many are wanted of it and how many have it.  False: there are fewer.
   // Rank 0 gets the others' counts.
   auto find = [&](int d, int want) -> bool {
-    if (tid == 0) found[0] = -1;
     __syncthreads();
     constexpr int E = kBins / kSelectThreads;
     static_assert(E == 4, "a thread's bins");
@@ -157,7 +161,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectP
     }
     const int sum = own.x + own.y + own.z + own.w;
     int all;
-    int before = select_scan(sum, sums, all);
+    int before = select_scan(sum, sums[d & 1], all);
     if (before < want && want <= before + sum) {
       const int c[E] = {own.w, own.z, own.y, own.x};
 #pragma unroll
@@ -179,56 +183,69 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectP
   // look at (k of n: 3 % of 32768 leaves 3 %, 24 % of 131072 leaves 28 %).
   const int group = (int64_t)16 * k <= n ? 8 : ((int64_t)3 * k <= n ? 2 : 0);
   if (k > 0 && group) {
-    blocks([&](int, const uint32_t (&x)[U]) {
-      uint32_t m[U / 2];
+    blocks([&](int, bool, const float (&x)[U]) {
+      float m[U / 2];  // (NaN is passed over)
 #pragma unroll
-      for (int u = 0; u < U / 2; ++u) m[u] = max(x[2 * u], x[2 * u + 1]);
+      for (int u = 0; u < U / 2; ++u) m[u] = fmaxf(x[2 * u], x[2 * u + 1]);
       if (group == 8) {
-        m[0] = max(max(m[0], m[1]), max(m[2], m[3]));
-        if (m[0]) atomicAdd(&hist[3][m[0] >> 21], 1);
+        m[0] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+        if (m[0] == m[0]) atomicAdd(&hist[3][order_key(m[0]) >> 21], 1);
       } else {
 #pragma unroll
         for (int u = 0; u < U / 2; ++u)
-          if (m[u]) atomicAdd(&hist[3][m[u] >> 21], 1);
+          if (m[u] == m[u]) atomicAdd(&hist[3][order_key(m[u]) >> 21], 1);
       }
     });
-    if (find(3, k)) least = max(1u, (uint32_t)found[0] << 21);
+    if (find(3, k)) least = (uint32_t)found[0] << 21;
+    if (least <= order_key(-INFINITY)) least = 1;  // (NaN alone has a key below it)
   }
-  // ---- each warp's tokens that are left, in order; where they are more than its list
+  // ---- each warp's candidates that are left, in order; where they are more than its list
   // holds they are read again for every pass
   int count = 0;
-  blocks([&](int j0, const uint32_t (&x)[U]) {
+  const float bound = key_value(least);
+  const bool all_left = least == 1;
+  blocks([&](int j0, bool inside, const float (&x)[U]) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int j = j0 + 32 * u + lane;
-      const bool left = j < s1 && (x[u] >= least || j < c0 || j >= c1);
+      bool left = all_left || x[u] >= bound;
+      if (!inside) left = left && j < s1 && j >= c0 && j < c1;
       const unsigned m = __ballot_sync(0xffffffffu, left);
       if (!m) continue;
       const int at = count + __popc(m & ((1u << lane) - 1u));
       if (left && at < kList) {
-        list_key[at] = x[u];
+        list_key[at] = order_key(x[u]);
         list_at[at] = j;
       }
       count += __popc(m);
     }
   });
   __syncwarp();
-  // f(whether there is one, token, its key) in order, 32 at a time
+  // f(token, its key) in order, 32 at a time; key 0: none
   auto each = [&](auto&& f) {
     if (count <= kList) {
-      for (int i0 = 0; i0 < count; i0 += 32) {
-        const bool there = i0 + lane < count;
-        f(there, there ? list_at[i0 + lane] : 0, there ? list_key[i0 + lane] : 0u);
+      for (int i0 = 0; i0 < count; i0 += 128) {
+        int at[4];
+        uint32_t x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = i0 + 32 * e + lane;
+          at[e] = i < count ? list_at[i] : 0;
+          x[e] = i < count ? list_key[i] : 0u;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i0 + 32 * e < count) f(at[e], x[e]);
       }
     } else {
-      blocks([&](int j0, const uint32_t (&x)[U]) {
+      blocks([&](int j0, bool inside, const float (&x)[U]) {
 #pragma unroll 1
         for (int u = 0; u < U; ++u) {
           const int j = j0 + 32 * u + lane;
-          uint32_t key = 0;
+          float v = 0.f;
 #pragma unroll
-          for (int e = 0; e < U; ++e) key = e == u ? x[e] : key;
-          f(j < s1, j, key);
+          for (int e = 0; e < U; ++e) v = e == u ? x[e] : v;
+          f(j, inside || (j < s1 && j >= c0 && j < c1) ? order_key(v) : 0u);
         }
       });
     }
@@ -240,7 +257,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectP
     for (int d = 0; d < 3; ++d) {
       const int shift = d == 0 ? 21 : (d == 1 ? 10 : 0);
       const uint32_t digit_mask = d == 2 ? 0x3ffu : 0x7ffu;
-      each([&](bool, int, uint32_t x) {
+      each([&](int, uint32_t x) {
         if (x >= least && (x & mask) == top) atomicAdd(&hist[d][(x >> shift) & digit_mask], 1);
       });
       find(d, want);
@@ -250,37 +267,38 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectP
       have = found[2];
     }
   }
-  // ---- Which tokens stay: the ones always kept, the ones above the threshold and `want`
-  // of the `have` at it (the first ones; where they are all, their order does not matter).
+  // ---- Which candidates stay: the ones above the threshold and `want` of the `have` at it
+  // (the first ones; where they are all, their order does not matter).
   const bool ties = want < have;
-  auto sure = [&](bool there, int j, uint32_t x) {
-    return there && (j < c0 || j >= c1 || (k > 0 && x && (ties ? x > top : x >= top)));
-  };
+  auto sure = [&](uint32_t x) { return x && k > 0 && (ties ? x > top : x >= top); };
   int n_sure = 0, n_equal = 0;
-  each([&](bool there, int j, uint32_t x) {
-    n_sure += sure(there, j, x);
+  each([&](int, uint32_t x) {
+    n_sure += sure(x);
     n_equal += ties && x == top;
   });
   int all;
-  int sure_before = select_scan(n_sure, sums, all);
+  int sure_before = select_scan(n_sure, sums[1], all);
   if (tid == 0) cta_count[0] = all;
   int equal_before = 0;
   if (ties) {
-    equal_before = select_scan(n_equal, sums, all);
+    equal_before = select_scan(n_equal, sums[0], all);
     if (tid == 0) cta_count[1] = all;
   }
   sure_before = __shfl_sync(0xffffffffu, sure_before, 0);  // before the warp
   equal_before = __shfl_sync(0xffffffffu, equal_before, 0);
   if (C > 1) {
     cluster_sync();
-    for (int r = 0; r < rank; ++r) {
-      sure_before += cluster_read(&cta_count[0], r);
-      if (ties) equal_before += cluster_read(&cta_count[1], r);
-    }
+    // a lane per rank
+    sure_before += __reduce_add_sync(0xffffffffu, lane < rank ? cluster_read(&cta_count[0], lane) : 0);
+    if (ties) equal_before += __reduce_add_sync(0xffffffffu, lane < rank ? cluster_read(&cta_count[1], lane) : 0);
   }
+  // the tokens that always stay stand before and after them
+  for (int i = rank * kSelectThreads + tid; i < p.sinks + p.recent; i += C * kSelectThreads)
+    ind[i < p.sinks ? i : p.budget - p.recent + i - p.sinks] = i < p.sinks ? i : c1 + i - p.sinks;
   const unsigned below = (1u << lane) - 1u;
-  each([&](bool there, int j, uint32_t x) {
-    const bool stays = sure(there, j, x), equal = ties && x == top;
+  sure_before += p.sinks;
+  each([&](int j, uint32_t x) {
+    const bool stays = sure(x), equal = ties && x == top;
     const unsigned ms = __ballot_sync(0xffffffffu, stays), me = ties ? __ballot_sync(0xffffffffu, equal) : 0u;
     const int eq = equal_before + __popc(me & below);
     if (stays || (equal && eq < want)) ind[sure_before + __popc(ms & below) + min(eq, want)] = j;
