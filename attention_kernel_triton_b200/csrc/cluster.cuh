@@ -24,6 +24,10 @@ __device__ __forceinline__ void cluster_sync() {
           : "memory");
 }
 
+// Its two halves: arrivals order what came before them, waits what comes after.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // The int at the place of `local` in the shared memory of the cluster's CTA `rank`
 __device__ __forceinline__ int cluster_read(const int* local, uint32_t rank) {
   uint32_t a;

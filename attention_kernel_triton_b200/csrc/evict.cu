@@ -312,6 +312,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectP
 // eviction: the plan
 // ---------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024;
+constexpr int kPlanBounds = 4096;  // sequences whose bounds are looked up in shared memory
 
 struct EvictParams {
   char* kv;
@@ -342,10 +343,9 @@ struct EvictParams {
   int32_t* moved;   // [B] first page that is replaced, or one past all
 };
 
-// What the lists say of the row of slot i: its token, or -1 where it is no good
-// (behind the sequence, below its slot, or not above the one before it).
-__device__ __forceinline__ int kept_token(const EvictParams& p, const int32_t* keep, int i, int len) {
-  const int j = __ldg(keep + i), before = i ? __ldg(keep + i - 1) : -1;
+// The token that a list has for slot i, after `before`; -1 where it is no good (behind
+// the sequence, below its slot, or not above the one before it).
+__device__ __forceinline__ int checked_token(int i, int j, int before, int len) {
   if (j >= i && j < len && j > before) return j;
   record_status(kStatusBadToken);
   return -1;
@@ -355,11 +355,13 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
   __shared__ int64_t sums64[33];
   __shared__ int sums[33];
   __shared__ int n_fresh, n_dead;
+  __shared__ int bounds[kPlanBounds + 1];  // the new table's
   const int C = (int)cluster_size(), rank = (int)cluster_rank(), tid = threadIdx.x;
   const int64_t words = (p.num_pages + 31) / 32;
   const int64_t w0 = words * rank / C, w1 = words * (rank + 1) / C;
   for (int64_t w = w0 + tid; w < w1; w += kPlanThreads) p.seen[w] = p.again[w] = 0;
-  if (rank == 0) {  // the new table's bounds
+  cluster_sync();
+  if (rank == 0) {  // the new table's bounds (while the others begin to count)
     int64_t at = 0;
     for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
       const int b = b0 + tid;
@@ -392,14 +394,15 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
     }
     if (tid == 0) p.out_indptr[p.B] = (int)min(at, p.max_entries);
   }
-  cluster_sync();
   // pages by how many hold them
   constexpr int U = 4;
-  for (int64_t i = (int64_t)rank * kPlanThreads + tid; i < p.num_entries; i += (int64_t)U * C * kPlanThreads) {
+  const int counters = max(C - 1, 1), turn = C > 1 ? rank - 1 : 0;  // rank 0 only where it is alone
+  for (int64_t i = (int64_t)turn * kPlanThreads + tid; turn >= 0 && i < p.num_entries;
+       i += (int64_t)U * counters * kPlanThreads) {
     int id[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t at = i + (int64_t)u * C * kPlanThreads;
+      const int64_t at = i + (int64_t)u * counters * kPlanThreads;
       id[u] = at < p.num_entries ? __ldg(p.indices + at) : -1;
     }
 #pragma unroll
@@ -424,6 +427,11 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
   cluster_sync();
   // the new table's pages; one that has to be replaced is noted by its number among those
   const int N = __ldcg(p.out_indptr + p.B);
+  const bool bounds_here = p.B <= kPlanBounds;
+  if (bounds_here)
+    for (int i = tid; i <= p.B; i += kPlanThreads) bounds[i] = __ldcg(p.out_indptr + i);
+  __syncthreads();
+  auto bound = [&](int b) { return bounds_here ? bounds[b] : __ldcg(p.out_indptr + b); };
   const int g0 = (int)((int64_t)N * rank / C), g1 = (int)((int64_t)N * (rank + 1) / C);
   int fresh = 0;
   for (int t0 = g0; t0 < g1; t0 += kPlanThreads) {
@@ -433,15 +441,17 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
       int b = 0, hi = p.B - 1;
       while (b < hi) {
         const int mid = (b + hi + 1) >> 1;
-        if (__ldcg(p.out_indptr + mid) <= g) b = mid; else hi = mid - 1;
+        if (bound(mid) <= g) b = mid; else hi = mid - 1;
       }
-      const int e = g - __ldcg(p.out_indptr + b), n = __ldcg(p.count + b);
+      const int e = g - bound(b), n = __ldcg(p.count + b);
       page = __ldg(p.indices + __ldg(p.indptr + b) + e);
       if (page >= 0 && page < p.num_pages && (__ldcg(p.again + (page >> 5)) >> (page & 31) & 1u)) {
         const int end = min((e + 1) * p.P, n) - 1;  // the page's last row: in its place only if all are
         replace = end + 1 < (e + 1) * p.P;
-        for (int i = 0; i < p.layers * p.H && !replace; ++i)
-          replace = __ldg(p.keep + i / p.H * p.k_layer + b * p.k_batch + i % p.H * p.k_head + end) != end;
+        for (int l = 0; l < p.layers && !replace; ++l)
+#pragma unroll 8
+          for (int h = 0; h < p.H; ++h)
+            replace |= __ldg(p.keep + l * p.k_layer + b * p.k_batch + h * p.k_head + end) != end;
         if (replace) atomicMin(p.moved + b, e);
       }
     }
@@ -454,12 +464,15 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
     p.out_indices[g] = -1;
   if (tid == 0) n_fresh = fresh;
   cluster_sync();
-  int first = 0, all = 0;
-  for (int r = 0; r < C; ++r) {
-    const int x = cluster_read(&n_fresh, r);
-    if (r < rank) first += x;
-    all += x;
-  }
+  // over the ranks before this one, and over all: a lane per rank (at most 8)
+  const int lane = tid & 31;
+  auto over_ranks = [&](const int* count, int& total) -> int {
+    const int x = lane < C ? cluster_read(count, lane) : 0;
+    total = __reduce_add_sync(0xffffffffu, x);
+    return __reduce_add_sync(0xffffffffu, lane < rank ? x : 0);
+  };
+  int all;
+  const int first = over_ranks(&n_fresh, all);
   if (all) {  // the same in every CTA
     // the lowest dead pages, in ascending order
     int mine = 0, dead_here;
@@ -470,12 +483,8 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
     block_scan<int>(mine, sums, dead_here);
     if (tid == 0) n_dead = dead_here;
     cluster_sync();
-    int r0 = 0, found = 0;
-    for (int r = 0; r < C; ++r) {
-      const int x = cluster_read(&n_dead, r);
-      if (r < rank) r0 += x;
-      found += x;
-    }
+    int found;
+    int r0 = over_ranks(&n_dead, found);
     for (int64_t v0 = w0; v0 < w1 && r0 < all; v0 += kPlanThreads) {
       const int64_t w = v0 + tid, left = p.num_pages - w * 32;
       uint32_t d = w < w1 ? ~__ldcg(p.seen + w) & (left >= 32 ? 0xffffffffu : (1u << left) - 1u) : 0u;
@@ -500,8 +509,8 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
 // eviction: the rows
 // ---------------------------------------------------------------------------
 constexpr int kMoveThreads = 512;
-constexpr int kMovePieces = 8;    // of a thread in a chunk
-constexpr int kMaxRows = 512;     // of a CTA's chunk
+constexpr int kMovePieces = 4;    // of a thread in a chunk
+constexpr int kMaxRows = 256;     // of a CTA's chunk
 
 template <int W>
 struct Piece;
@@ -512,10 +521,13 @@ struct Piece<2> { using type = uint16_t; };
 
 // Cluster (layer, sequence, head, part): part 0 is K, 1 is V, 2 the weights.
 template <int W>
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(kMoveThreads, 2) evict_move_kernel(const EvictParams p) {
   using V = typename Piece<W>::type;
   constexpr int U = kMovePieces;
-  __shared__ int64_t from[2][kMaxRows], to[2][kMaxRows];  // bytes; from < 0: nothing moves
+  // Addresses of the rows of several chunks, a row a thread, in three turns: those that
+  // are moved, the next ones, and those before, which a warp may still store.  In bytes;
+  // from < 0: nothing moves.
+  __shared__ int64_t from[3][kMoveThreads], to[3][kMoveThreads];
   const int C = (int)cluster_size(), rank = (int)cluster_rank(), tid = threadIdx.x, parts = p.w ? 3 : 2;
   int unit = blockIdx.x / C;
   const int part = unit % parts;
@@ -534,6 +546,7 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictPar
   }
   if (part == 2) {
     float* w = p.w + l * p.w_layer + b * p.w_batch + h * p.w_head;
+    constexpr int U = 8;
     const int per = U * kMoveThreads, turns = (n - start + C * per - 1) / (C * per);
     for (int it = 0; it < turns; ++it) {
       const int i0 = start + (it * C + rank) * per + tid;
@@ -541,7 +554,8 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictPar
       int ok = 0;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * kMoveThreads, j = i < n ? kept_token(p, keep, i, len) : -1;
+        const int i = i0 + u * kMoveThreads;
+        const int j = i < n ? checked_token(i, __ldg(keep + i), i ? __ldg(keep + i - 1) : -1, len) : -1;
         v[u] = 0.f;
         if (j < 0 || j >= p.width) continue;
         v[u] = w[j];
@@ -559,45 +573,79 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictPar
   start = (int)min((int64_t)start, (int64_t)p.moved[b] * p.P);
   const int R = p.rows, turns = (n - start + C * R - 1) / (C * R);
   char* base = p.kv + l * p.s_layer + part * p.s_kv + h * p.s_head;
-  auto addresses = [&](int it) {  // of the rows of chunk `it`
-    for (int r = tid; r < R; r += kMoveThreads) {
-      const int i = start + (it * C + rank) * R + r;
-      int64_t f = -1, t = 0;
-      if (i < n) {
-        const int j = kept_token(p, keep, i, len);
-        if (j >= 0) {
-          const int pj = (int)fdiv((uint32_t)j, p.div_page), pi = (int)fdiv((uint32_t)i, p.div_page);
-          const int src = __ldg(p.indices + s + pj), dst = p.out_indices[os + pi];
-          if (src >= 0 && src < p.num_pages && dst >= 0 && dst < p.num_pages && (src != dst || i != j)) {
-            f = src * p.s_page + (j - pj * p.P) * p.s_tok;
-            t = dst * p.s_page + (i - pi * p.P) * p.s_tok;
-          }
+  const int span = kMoveThreads / R;  // chunks whose addresses are made at once (at least 2)
+  const int mine = tid / R, r_mine = tid - mine * R;
+  auto slot = [&](int q) { return start + ((q * span + mine) * C + rank) * R + r_mine; };
+  int2 next;  // the list's entry for this thread's row of the next span, and the one before it
+  auto ask = [&](int q) {
+    const int i = slot(q);
+    next = mine < span && i < n ? make_int2(__ldg(keep + i), i ? __ldg(keep + i - 1) : -1) : make_int2(-1, -1);
+  };
+  auto address = [&](int q) {
+    const int i = slot(q);
+    int64_t f = -1, t = 0;
+    if (mine < span && i < n) {
+      const int j = checked_token(i, next.x, next.y, len);
+      if (j >= 0) {
+        const int pj = (int)fdiv((uint32_t)j, p.div_page), pi = (int)fdiv((uint32_t)i, p.div_page);
+        const int src = __ldg(p.indices + s + pj), dst = p.out_indices[os + pi];
+        if (src >= 0 && src < p.num_pages && dst >= 0 && dst < p.num_pages && (src != dst || i != j)) {
+          f = src * p.s_page + (j - pj * p.P) * p.s_tok;
+          t = dst * p.s_page + (i - pi * p.P) * p.s_tok;
         }
       }
-      from[it & 1][r] = f;
-      to[it & 1][r] = t;
     }
+    from[q % 3][tid] = f;
+    to[q % 3][tid] = t;
   };
-  V val[U];
-  auto load = [&](int it) {
+  V val[2][U];
+  auto load = [&](int at, V (&v)[U]) {
+    const int64_t* f = &from[0][0] + at;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint32_t x = u * kMoveThreads + tid, r = fdiv(x, p.div_piece);
-      if (r < R && from[it & 1][r] >= 0)
-        val[u] = *reinterpret_cast<const V*>(base + from[it & 1][r] + (x - r * p.pieces) * W);
+      if (r < R && f[r] >= 0) v[u] = *reinterpret_cast<const V*>(base + f[r] + (x - r * p.pieces) * W);
     }
   };
-  for (int it = 0; it < turns; ++it) {
-    addresses(it);
+  if (!turns) return;
+  ask(0);
+  address(0);
+  ask(1);
+  __syncthreads();
+  load(0, val[0]);
+  if (C > 1) cluster_arrive();
+  int here = 0, ahead_at = R, in_span = 0, q = 0;  // this chunk's and the next one's place in the addresses
+  // Chunk `it` is stored once all of it has been loaded, and the one after it is on its
+  // way by then.  Inside a CTA a barrier orders the accesses; in a cluster the arrival
+  // for a chunk waits for its loads and for stores of a turn ago.
+  auto turn = [&](int it, V (&cur)[U], V (&ahead)[U]) {
+    if (it + 1 < turns) load(ahead_at, ahead);
+    if (in_span == 0 && it + span < turns) {
+      address(q + 1);
+      ask(q + 2);
+    }
+    if (C > 1) {
+      cluster_wait();
+      if (it + 1 < turns) cluster_arrive();
+    }
     __syncthreads();
-    load(it);
-    cluster_sync();
+    const int64_t *f = &from[0][0] + here, *t = &to[0][0] + here;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint32_t x = u * kMoveThreads + tid, r = fdiv(x, p.div_piece);
-      if (r < R && from[it & 1][r] >= 0)
-        *reinterpret_cast<V*>(base + to[it & 1][r] + (x - r * p.pieces) * W) = val[u];
+      if (r < R && f[r] >= 0) *reinterpret_cast<V*>(base + t[r] + (x - r * p.pieces) * W) = cur[u];
     }
+    here = ahead_at;
+    if (++in_span == span) {
+      in_span = 0;
+      ++q;
+    }
+    ahead_at = in_span + 1 < span ? here + R : (q + 1) % 3 * kMoveThreads;
+  };
+#pragma unroll 1
+  for (int it = 0; it < turns; it += 2) {
+    turn(it, val[0], val[1]);
+    if (it + 1 < turns) turn(it + 1, val[1], val[0]);
   }
 }
 
