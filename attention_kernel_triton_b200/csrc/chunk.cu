@@ -58,6 +58,7 @@
 //
 // Built without -rdc (setmaxnreg needs whole-program device code).
 #define AKT_WHOLE_PROGRAM 1
+#include "attn_mma.cuh"
 #include "common.cuh"
 #include "profile.cuh"
 #include "tcgen05.cuh"
@@ -99,6 +100,11 @@ constexpr int kUnitCost1 = 6, kUnitCost2 = 3;
 // more take a warp's copy too long at a unit's start: 718 / 765 (685 / 810), n = 32
 // 920 / 969 (718 / 852).
 constexpr int kFewRows = 48;
+// Units of a sequence's own keys behind a prefix that take the warp-level kernel: a
+// unit's chain of steps here (Q, S, the exponentials, P.V, the output) takes 4 us however
+// few its rows and tiles are.  One token in each of 64 sequences of 64 to 1024 own keys
+// behind 8192: KSMALL_MEASURED.
+constexpr int kSmallRows = 32, kSmallKeys = 2048;
 constexpr int kTableSeqs = 96;     // sequences whose table fits the CTA's shared memory
 constexpr int kMaxCtas = kThreads; // of the main kernel (one per SM)
 
@@ -141,6 +147,7 @@ struct ChunkParams {
   const int32_t* group_indptr;
   const int32_t* shared_pages;
   struct Seq* seqs;    // [B]
+  struct Seq* own;     // [batch] the sequences on their own keys; those with few have no rows in `seqs`
   int* prefix_len;     // [batch] shared keys of each sequence
   float* row_o;        // [2][rows][D] normalised outputs of a row on the prefix, on its own keys
   float* row_lse;      // [2][rows]
@@ -608,6 +615,11 @@ __device__ __forceinline__ void finish_rows(const ChunkParams& p, const Seg* sg,
 // -------------------------------------------------------------------------
 // the planner of batches past the CTA's own table
 // -------------------------------------------------------------------------
+// Sequences with so few rows and own keys are left to chunk_small_kernel.
+__device__ __forceinline__ bool is_small(const ChunkParams& p, const Seq& s) {
+  return s.n > 0 && s.n <= kSmallRows / p.group && s.len <= kSmallKeys;
+}
+
 // The virtual sequences of a batch with shared prefixes.  A group's prefix is as many
 // whole pages as it is said to share, as all its sequences with rows have and (causal)
 // as their first rows see; none where fewer than two have rows or one has bad bounds.
@@ -659,6 +671,8 @@ __device__ void build_shared(const ChunkParams& p, int* bad) {
       s.len -= keys;
       s.prefix = 2;
     }
+    p.own[b] = s;
+    if (is_small(p, s)) s.n = 0;
     p.seqs[p.groups + b] = s;
     p.prefix_len[b] = keys;
   }
@@ -710,6 +724,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  if (threadIdx.x == 32) {
+    prefetch_tensor_map(&tmQ);
+    prefetch_tensor_map(&tmK);
+    prefetch_tensor_map(&tmV);
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&full[s], TMA ? 1 : 32);  // cp.async: every lane of the loader
@@ -759,6 +778,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_async_smem();
   } else {
     grid_dep_wait();
+    if (SHARED) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the planner is done)
     tab = Tables{p.plan_cost, p.plan_units, nullptr};
     plan = *p.plan;
     begin = p.plan_share[blockIdx.x];
@@ -1535,76 +1555,66 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const ChunkP
 // -------------------------------------------------------------------------
 // join of a row's results on a shared prefix and on its own keys
 // -------------------------------------------------------------------------
-// A warp per row (token, head).  The row's results are those of up to two units, whole
-// in row_o or in parts as chunk_merge_kernel finds them; rows of no sequence are zeros.
-template <typename T, int D>
-__global__ void __launch_bounds__(kMergeThreads) chunk_join_kernel(const ChunkParams p) {
-  constexpr int N = D / 32;  // columns per lane
-  const int lane = threadIdx.x & 31;
-  const int64_t rows = p.num_tokens * p.Hq, row = (int64_t)blockIdx.x * (kMergeThreads / 32) + (threadIdx.x >> 5);
-  if (row >= rows) return;
-  const int tok = (int)(row / p.Hq), head = (int)(row - (int64_t)tok * p.Hq);
-  const int b = find_seq(p.q_indptr, p.batch, tok);
-  const int a0 = __ldg(p.q_indptr + b), a1 = __ldg(p.q_indptr + b + 1);
-  const bool there = a0 >= 0 && tok >= a0 && tok < a1 && a1 <= p.num_tokens;
-  grid_dep_wait();
-  int count[2] = {0, 0}, at[2], rr[2];  // parts on the prefix and on the own keys, where they begin, the row there
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    at[k] = kWhole;
-    rr[k] = 0;
-    if (!there || (k == 0 && !p.prefix_len[b])) continue;
-    const int2 w = p.row_at[k * rows + row];
-    if (w.x == kDone) return;
-    at[k] = w.x;
-    rr[k] = w.y;
-    count[k] = 1;
-    if (w.x < 0 || p.parts[w.x].last) continue;
-    const int c0 = w.x >> 1;
-    for (int base = c0 + 1; base < p.grid; base += 32) {  // the CTA with the last part
-      const int c = base + lane;
-      const bool ends = c < p.grid && p.parts[2 * c].used && p.parts[2 * c].last;
-      const unsigned m = __ballot_sync(0xffffffffu, ends);
-      if (m) {
-        count[k] = base + __ffs(m) - c0;
-        break;
-      }
+// Results of row `row` in unit kind k (0 the prefix, 1 its own keys): whole, or parts as
+// chunk_merge_kernel finds them.  The whole warp calls it.
+struct RowParts {
+  int count;  // 0: none
+  int first;  // place of the first part, kWhole, or kDone
+  int r;      // the row there
+};
+
+__device__ __forceinline__ RowParts row_parts(const ChunkParams& p, int k, int64_t row) {
+  const int2 w = p.row_at[k * p.num_tokens * p.Hq + row];
+  RowParts x{1, w.x, w.y};
+  if (w.x < 0 || p.parts[w.x].last) return x;
+  const int lane = threadIdx.x & 31, c0 = w.x >> 1;
+  for (int base = c0 + 1; base < p.grid; base += 32) {  // the CTA with the last part
+    const int c = base + lane;
+    const bool ends = c < p.grid && p.parts[2 * c].used && p.parts[2 * c].last;
+    const unsigned m = __ballot_sync(0xffffffffu, ends);
+    if (m) {
+      x.count = base + __ffs(m) - c0;
+      break;
     }
   }
-  const int total = count[0] + count[1];
-  // result i: its log-sum-exp (-inf: nothing) and its row
-  auto find = [&](int i, const float*& o) -> float {
-    o = nullptr;
-    if (i >= total) return -INFINITY;
-    const int k = i >= count[0], e = i - (k ? count[0] : 0);
-    const int first = k ? at[1] : at[0], r = k ? rr[1] : rr[0];
-    if (first < 0) {
-      o = p.row_o + (k * rows + row) * D;
-      return p.row_lse[k * rows + row];
-    }
-    const int place = e ? 2 * ((first >> 1) + e) : first;
-    if (e && !p.parts[place].used) return -INFINITY;
-    const int64_t x = (int64_t)place * p.part_rows + r;
-    o = p.part_o + x * D;
-    return p.part_lse[x];
-  };
-  const float* o;
-  float M = -INFINITY;
-  for (int i = lane; i < total; i += 32) M = fmaxf(M, find(i, o));
-#pragma unroll
-  for (int s = 16; s; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
-  const float Ms = M == -INFINITY ? 0.f : M;
-  float acc[N] = {}, den = 0.f;
-  for (int i0 = 0; i0 < total; i0 += 32) {
-    const float part = find(i0 + lane, o);
+  return x;
+}
+
+// Result i of these: its log-sum-exp (-inf: nothing) and its row.
+template <int D>
+__device__ __forceinline__ float row_result(const ChunkParams& p, int k, int64_t row, const RowParts& x, int i,
+                                            const float*& o) {
+  const int64_t rows = p.num_tokens * p.Hq;
+  o = nullptr;
+  if (i >= x.count) return -INFINITY;
+  if (x.first < 0) {
+    o = p.row_o + (k * rows + row) * D;
+    return p.row_lse[k * rows + row];
+  }
+  const int place = i ? 2 * ((x.first >> 1) + i) : x.first;
+  if (i && !p.parts[place].used) return -INFINITY;
+  const int64_t at = (int64_t)place * p.part_rows + x.r;
+  o = p.part_o + at * D;
+  return p.part_lse[at];
+}
+
+// A row's results, a weight each; lane columns [N lane, N lane + N).  `M` is the largest
+// log-sum-exp so far (all lanes), den and acc the sums in its scale.
+template <int D, int N>
+__device__ __forceinline__ void add_results(const ChunkParams& p, int k, int64_t row, const RowParts& x, float Ms,
+                                            float& den, float (&acc)[N]) {
+  const int lane = threadIdx.x & 31;
+  for (int i0 = 0; i0 < x.count; i0 += 32) {
+    const float* o;
+    const float part = row_result<D>(p, k, row, x, i0 + lane, o);
     const float mine = fast_exp2((part - Ms) * kLog2e);  // NaN stays NaN
     const unsigned holds = __ballot_sync(0xffffffffu, part != -INFINITY);  // (a weight of 0 is not left out)
-    const int n = min(32, total - i0);
-    for (int i1 = 0; i1 < n; i1 += 8) {  // eight rows asked for at once
-      float w[8];
-      float v[8][N];
+    const int n = min(32, x.count - i0);
+    for (int i1 = 0; i1 < n; i1 += 4) {  // four rows asked for at once
+      float w[4];
+      float v[4][N];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
+      for (int u = 0; u < 4; ++u) {
         w[u] = __shfl_sync(0xffffffffu, mine, i1 + u);
         const float* src = reinterpret_cast<const float*>(
             __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(o), i1 + u));
@@ -1615,22 +1625,388 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_join_kernel(const ChunkPa
         else *reinterpret_cast<float2*>(v[u]) = *reinterpret_cast<const float2*>(src + lane * N);
       }
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
+      for (int u = 0; u < 4; ++u) {
         den += w[u];
 #pragma unroll
         for (int e = 0; e < N; ++e) acc[e] = fmaf(w[u], v[u][e], acc[e]);
       }
     }
   }
+}
+
+template <int D>
+__device__ __forceinline__ float largest_result(const ChunkParams& p, int k, int64_t row, const RowParts& x) {
+  const float* o;
+  float M = -INFINITY;
+  for (int i = threadIdx.x & 31; i < x.count; i += 32) M = fmaxf(M, row_result<D>(p, k, row, x, i, o));
+#pragma unroll
+  for (int s = 16; s; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
+  return M;
+}
+
+// The joined row: sum of the weighted results over the sum of the weights.
+template <typename T, int N>
+__device__ __forceinline__ void store_row(const ChunkParams& p, int64_t tok, int head, float Ms, float den,
+                                          const float (&acc)[N]) {
+  const int lane = threadIdx.x & 31;
   const bool any = den > 0.f || den != den;
   const float inv = any ? 1.f / den : 0.f;
-  T* out = reinterpret_cast<T*>(p.out + (int64_t)tok * p.o_tok + (int64_t)head * p.o_head) + lane * N;
+  T* out = reinterpret_cast<T*>(p.out + tok * p.o_tok + (int64_t)head * p.o_head) + lane * N;
   if constexpr (N == 4)
     *reinterpret_cast<uint2*>(out) = make_uint2(Elem<T>::pack2(acc[0] * inv, acc[1] * inv), Elem<T>::pack2(acc[2] * inv, acc[3] * inv));
   else
     *reinterpret_cast<uint32_t*>(out) = Elem<T>::pack2(acc[0] * inv, acc[1] * inv);
-  if (p.lse && lane == 0)
-    p.lse[(int64_t)tok * p.l_tok + (int64_t)head * p.l_head] = any ? Ms + __log2f(den) * kLn2 : -INFINITY;
+  if (p.lse && lane == 0) p.lse[tok * p.l_tok + (int64_t)head * p.l_head] = any ? Ms + __log2f(den) * kLn2 : -INFINITY;
+}
+
+constexpr int kJoinRows = 8;  // of a warp
+constexpr int64_t kFoldRows = 32768;  // up to so many rows CTAs of the kernel of small units join them
+
+// Warps of kJoinRows rows (token, head) each.  Rows of no sequence are zeros.
+template <typename T, int D>
+__device__ void join_rows(const ChunkParams& p, int64_t warp) {
+  constexpr int N = D / 32;  // columns per lane
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = p.num_tokens * p.Hq, row0 = warp * kJoinRows;
+  // a lane looks a row up
+  int2 w0 = make_int2(kDone, 0), w1 = make_int2(kDone, 0);
+  float lse0 = -INFINITY, lse1 = -INFINITY;
+  int none = 0;
+  if (lane < kJoinRows && row0 + lane < rows) {
+    const int64_t row = row0 + lane;
+    const int tok = (int)(row / p.Hq), b = find_seq(p.q_indptr, p.batch, tok);
+    const int a0 = __ldg(p.q_indptr + b), a1 = __ldg(p.q_indptr + b + 1);
+    none = !(a0 >= 0 && tok >= a0 && tok < a1 && a1 <= p.num_tokens);
+    if (!none && !is_small(p, p.own[b])) {
+      w1 = p.row_at[rows + row];
+      if (w1.x == kWhole) lse1 = p.row_lse[rows + row];
+      if (p.prefix_len[b]) {
+        w0 = p.row_at[row];
+        if (w0.x == kWhole) lse0 = p.row_lse[row];
+      }
+    }
+  }
+#pragma unroll
+  for (int i0 = 0; i0 < kJoinRows; i0 += 4) {
+    // rows that are whole in both places, four at a time
+    float v[4][2][N];
+    unsigned simple = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int at0 = __shfl_sync(0xffffffffu, w0.x, i0 + u), at1 = __shfl_sync(0xffffffffu, w1.x, i0 + u);
+      if (at0 != kWhole || at1 != kWhole) continue;
+      simple |= 1u << u;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float* o = p.row_o + (k * rows + row0 + i0 + u) * D + lane * N;
+        if constexpr (N == 4) *reinterpret_cast<float4*>(v[u][k]) = *reinterpret_cast<const float4*>(o);
+        else *reinterpret_cast<float2*>(v[u][k]) = *reinterpret_cast<const float2*>(o);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t row = row0 + i0 + u;
+      const int64_t tok = row / p.Hq;
+      const int head = (int)(row - tok * p.Hq);
+      const float x0 = __shfl_sync(0xffffffffu, lse0, i0 + u), x1 = __shfl_sync(0xffffffffu, lse1, i0 + u);
+      const int at1 = __shfl_sync(0xffffffffu, w1.x, i0 + u), nobody = __shfl_sync(0xffffffffu, none, i0 + u);
+      const bool prefixed = __shfl_sync(0xffffffffu, w0.x, i0 + u) != kDone;
+      float acc[N] = {}, den = 0.f, M;
+      if (simple >> u & 1u) {
+        M = fmaxf(x0, x1);
+        const float Ms = M == -INFINITY ? 0.f : M;
+        const float e[2] = {fast_exp2((x0 - Ms) * kLog2e), fast_exp2((x1 - Ms) * kLog2e)};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if ((k ? x1 : x0) == -INFINITY) continue;
+          den += e[k];
+#pragma unroll
+          for (int c = 0; c < N; ++c) acc[c] = fmaf(e[k], v[u][k][c], acc[c]);
+        }
+      } else if (nobody) {
+        M = -INFINITY;
+      } else {
+        if (at1 == kDone) continue;
+        const RowParts own = row_parts(p, 1, row), front = prefixed ? row_parts(p, 0, row) : RowParts{0, kWhole, 0};
+        M = fmaxf(largest_result<D>(p, 1, row, own), largest_result<D>(p, 0, row, front));
+        const float Ms = M == -INFINITY ? 0.f : M;
+        add_results<D, N>(p, 0, row, front, Ms, den, acc);
+        add_results<D, N>(p, 1, row, own, Ms, den, acc);
+      }
+      store_row<T, N>(p, tok, head, M == -INFINITY ? 0.f : M, den, acc);
+    }
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kMergeThreads) chunk_join_kernel(const ChunkParams p) {
+  grid_dep_wait();
+  join_rows<T, D>(p, (int64_t)blockIdx.x * (kMergeThreads / 32) + (threadIdx.x >> 5));
+}
+
+// -------------------------------------------------------------------------
+// few rows on few own keys, at warp level
+// -------------------------------------------------------------------------
+// A CTA per (sequence, kv head).  Its four warps take 16 keys at a time in turn, each
+// with a ring of its own that cp.async fills (no barrier in the loop):
+//   S^T[16 keys x 8 NT rows] = K . q^T,   O^T[D x 8 NT rows] += V^T . P^T
+// in warp-level products, the softmax's running maximum and sum in fp32 per row.  The
+// warps' results and the ones on the prefix are joined at the end, so the row is written
+// once and the loop runs beside the end of the kernel that works on the prefixes.
+constexpr int kSmallThreads = 128;
+constexpr int kSmallStages = 3;
+
+template <int D>
+struct SmallCfg {
+  static constexpr int TILE = 16 * D * 2;               // bytes of K (or V) of a step
+  static constexpr int WARP = kSmallStages * 2 * TILE;  // a warp's ring
+  static constexpr int RING = kSmallThreads / 32 * WARP;
+  // after the loop: each warp's [rows][D] sums
+  static constexpr int SUMS = kSmallThreads / 32 * kSmallRows * D * 4;
+  static constexpr int SMEM = RING > SUMS ? RING : SUMS;
+};
+
+// byte offset of 16-byte piece c of row r of a tile: rows of D values, pieces exchanged within 128 bytes
+template <int D>
+__device__ __forceinline__ uint32_t small_at(int r, int c) {
+  return (uint32_t)(r * D * 2 + ((c & ~7) | ((c & 7) ^ (r & 7))) * 16);
+}
+
+template <typename T, int D, int NT>
+__device__ void small_unit(const ChunkParams& p, const Seq& s, int b, int kvh, unsigned char* smem, float* stat,
+                           uint32_t* bad) {
+  constexpr int KS = D / 16, PIECES = D / 8;
+  using C = SmallCfg<D>;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = kSmallThreads / 32;
+  const int rows = s.n * p.group;
+  // this lane's rows of each 8: columns 2 (lane % 4) and the next of the products
+  int vis[NT][2];
+  uint32_t qb[NT][KS][2];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = t * 8 + 2 * (lane & 3) + i;
+      vis[t][i] = r >= rows ? 0 : (s.causal ? s.len - s.n + (int)fdiv((uint32_t)r, p.div_group) + 1 : s.len);
+    }
+    const int r = t * 8 + (lane >> 2), tok = (int)fdiv((uint32_t)r, p.div_group);
+    const T* q = reinterpret_cast<const T*>(p.q + (int64_t)(s.a0 + tok) * p.q_tok +
+                                            (int64_t)(kvh * p.group + r - tok * p.group) * p.q_head) + 2 * (lane & 3);
+#pragma unroll
+    for (int e = 0; e < KS; ++e) {
+      qb[t][e][0] = r < rows ? __ldg(reinterpret_cast<const uint32_t*>(q + 16 * e)) : 0u;
+      qb[t][e][1] = r < rows ? __ldg(reinterpret_cast<const uint32_t*>(q + 16 * e + 8)) : 0u;
+    }
+  }
+  const int all_see = s.causal ? max(s.len - s.n + 1, 0) : s.len;  // keys that every row sees
+  const int steps = (s.len + 15) / 16;
+  const uint32_t ring = smem_u32(smem) + warp * C::WARP;
+  const char* kv = p.kv + (int64_t)kvh * p.s_head;
+  // lane r < 16: key r of a step; its index entry is asked for a step ahead
+  auto entry = [&](int j) -> int {
+    const int key = j * 16 + (lane & 15);
+    return j < steps && key < s.len ? __ldg(p.indices + s.page0 + (int)fdiv((uint32_t)key, p.div_page)) : -1;
+  };
+  int id_next = entry(warp);
+  auto load = [&](int j, int st) {  // step j's K and V into stage st (an empty group past the end)
+    if (j < steps) {
+      const int key = j * 16 + (lane & 15), id = id_next;
+      const char* src = nullptr;
+      if (id >= 0 && id < p.num_pages)
+        src = kv + (int64_t)id * p.s_page + (int64_t)(key - (int)fdiv((uint32_t)key, p.div_page) * p.P) * p.s_tok;
+      else if (key < s.len && lane < 16) record_status(kStatusBadPage);
+      id_next = entry(j + warps);
+      const uint32_t dst = ring + st * 2 * C::TILE;
+#pragma unroll
+      for (int i = 0; i < PIECES / 2; ++i) {
+        const int x = i * 32 + lane, r = x / PIECES, c = x % PIECES;
+        const char* row =
+            reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), r));
+        cp_async16(dst + small_at<D>(r, c), row ? row + c * 16 : p.q, row ? 16u : 0u);
+        cp_async16(dst + C::TILE + small_at<D>(r, c), row ? row + p.s_kv + c * 16 : p.q, row ? 16u : 0u);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int st = 0; st < kSmallStages - 1; ++st) load(warp + st * warps, st);
+  float o[NT][KS][4], m[NT][2], l[NT][2];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    m[t][0] = m[t][1] = -INFINITY;
+    l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+    for (int e = 0; e < KS; ++e) o[t][e][0] = o[t][e][1] = o[t][e][2] = o[t][e][3] = 0.f;
+  }
+  int st = 0, to = kSmallStages - 1;
+#pragma unroll 1
+  for (int j = warp; j < steps; j += warps) {
+    load(j + (kSmallStages - 1) * warps, to);  // (the stage of the step before, which the warp is done with)
+    asm volatile("cp.async.wait_group %0;" ::"n"(kSmallStages - 1) : "memory");
+    __syncwarp();
+    const uint32_t kt = ring + st * 2 * C::TILE, vt = kt + C::TILE;
+    const int base = j * 16;
+    if (base + 16 > all_see) {
+      // values that some rows do not see must be finite (0 x NaN is NaN): others are cleared and noted
+      unsigned char* v = smem + (vt - smem_u32(smem));
+      for (int x = lane; x < 16 * PIECES; x += 32) {
+        const int r = x / PIECES, key = base + r;
+        if (key < all_see || key >= s.len) continue;
+        uint4* piece = reinterpret_cast<uint4*>(v + small_at<D>(r, x % PIECES));
+        const uint4 y = *piece;
+        if (!(not_finite2<T>(y.x) | not_finite2<T>(y.y) | not_finite2<T>(y.z) | not_finite2<T>(y.w))) continue;
+        *piece = make_uint4(without_not_finite2<T>(y.x), without_not_finite2<T>(y.y), without_not_finite2<T>(y.z),
+                            without_not_finite2<T>(y.w));
+        atomicOr(bad, 1u << (key - all_see));  // (fewer than kSmallRows keys)
+      }
+      __syncwarp();
+    }
+    // ---- S^T = K q^T
+    float x[NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) x[t][0] = x[t][1] = x[t][2] = x[t][3] = 0.f;
+#pragma unroll
+    for (int e = 0; e < KS; ++e) {
+      uint32_t a[4];  // keys 0-7 | 8-15 of dims 0-7, then of dims 8-15
+      ldsm_x4(a, kt + small_at<D>(lane & 15, 2 * e + (lane >> 4)));
+#pragma unroll
+      for (int t = 0; t < NT; ++t) MmaOp<T>::run(x[t], a, qb[t][e][0], qb[t][e][1]);
+    }
+    const bool edge = base + 16 > all_see;  // (columns past the rows are nobody's)
+    const int k0 = base + (lane >> 2);
+    uint32_t pb[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if (edge) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[t][e] = k0 + (e >> 1) * 8 < vis[t][e & 1] ? x[t][e] : -INFINITY;
+      }
+      float alpha[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float mx = fmaxf(x[t][i], x[t][2 + i]);
+#pragma unroll
+        for (int w = 4; w <= 16; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+        const float m_new = fmaxf(m[t][i], mx * p.scale_log2), m_sub = m_new == -INFINITY ? 0.f : m_new;
+        alpha[i] = fast_exp2(m[t][i] - m_sub);
+        m[t][i] = m_new;
+        x[t][i] = fast_exp2(fmaf(x[t][i], p.scale_log2, -m_sub));
+        x[t][2 + i] = fast_exp2(fmaf(x[t][2 + i], p.scale_log2, -m_sub));
+        l[t][i] = fmaf(l[t][i], alpha[i], x[t][i] + x[t][2 + i]);
+      }
+      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+        for (int e = 0; e < KS; ++e) {
+          o[t][e][0] *= alpha[0];
+          o[t][e][1] *= alpha[1];
+          o[t][e][2] *= alpha[0];
+          o[t][e][3] *= alpha[1];
+        }
+      }
+      pb[t][0] = movmatrix_trans(Elem<T>::pack2(x[t][0], x[t][1]));
+      pb[t][1] = movmatrix_trans(Elem<T>::pack2(x[t][2], x[t][3]));
+    }
+    // ---- O^T += V^T P^T
+#pragma unroll
+    for (int e = 0; e < KS; ++e) {
+      uint32_t a[4];  // dims 0-7 | 8-15 of keys 0-7, then of keys 8-15
+      ldsm_x4_trans(a, vt + small_at<D>((lane & 7) + (lane >> 4) * 8, 2 * e + (lane >> 3 & 1)));
+#pragma unroll
+      for (int t = 0; t < NT; ++t) MmaOp<T>::run(o[t][e], a, pb[t][0], pb[t][1]);
+    }
+    __syncwarp();  // the stage may be filled again
+    st = st + 1 == kSmallStages ? 0 : st + 1;
+    to = to + 1 == kSmallStages ? 0 : to + 1;
+  }
+  cp_async_wait_all();
+  __syncthreads();
+  // ---- the warps' results, a row at a time
+  float* sums = reinterpret_cast<float*>(smem) + warp * (kSmallRows * D);  // [row][D]
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = t * 8 + 2 * (lane & 3) + i;
+#pragma unroll
+      for (int w = 4; w <= 16; w <<= 1) l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], w);
+      if (lane < 4) {
+        stat[(warp * kSmallRows + r) * 2] = m[t][i];
+        stat[(warp * kSmallRows + r) * 2 + 1] = l[t][i];
+      }
+#pragma unroll
+      for (int e = 0; e < KS; ++e) {
+        sums[r * D + 16 * e + (lane >> 2)] = o[t][e][i];
+        sums[r * D + 16 * e + 8 + (lane >> 2)] = o[t][e][2 + i];
+      }
+    }
+  }
+  __syncthreads();
+  grid_dep_wait();
+  constexpr int N = D / 32;
+  for (int r = warp; r < rows; r += warps) {
+    const int tok = (int)fdiv((uint32_t)r, p.div_group), head = kvh * p.group + r - tok * p.group;
+    const int64_t row = (int64_t)(s.a0 + tok) * p.Hq + head;
+    float ml = -INFINITY;  // log2 units
+#pragma unroll
+    for (int w = 0; w < warps; ++w) ml = fmaxf(ml, stat[(w * kSmallRows + r) * 2]);
+    const RowParts front = s.prefix ? row_parts(p, 0, row) : RowParts{0, kWhole, 0};
+    const float M = fmaxf(ml * kLn2, largest_result<D>(p, 0, row, front)), Ms = M == -INFINITY ? 0.f : M;
+    float acc[N] = {}, den = 0.f;
+    add_results<D, N>(p, 0, row, front, Ms, den, acc);
+#pragma unroll
+    for (int w = 0; w < warps; ++w) {
+      const float mw = stat[(w * kSmallRows + r) * 2], lw = stat[(w * kSmallRows + r) * 2 + 1];
+      if (!(lw > 0.f || lw != lw)) continue;  // no key of the warp's is seen
+      const float e = fast_exp2(mw - Ms * kLog2e);
+      den = fmaf(e, lw, den);
+      const float* src = reinterpret_cast<const float*>(smem) + (w * kSmallRows + r) * D + lane * N;
+#pragma unroll
+      for (int c = 0; c < N; ++c) acc[c] = fmaf(e, src[c], acc[c]);
+    }
+    if (*bad) {  // the values that were cleared, where the row sees them
+      const int sees = s.causal ? s.len - s.n + tok + 1 : s.len;
+      for (uint32_t left = *bad; left; left &= left - 1) {
+        const int key = all_see + __ffs(left) - 1;
+        if (key >= sees) break;
+        const int pg = (int)fdiv((uint32_t)key, p.div_page), page = __ldg(p.indices + s.page0 + pg);
+        if (page < 0 || page >= p.num_pages) continue;
+        const T* v = reinterpret_cast<const T*>(kv + p.s_kv + (int64_t)page * p.s_page + (int64_t)(key - pg * p.P) * p.s_tok);
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+          const float y = Elem<T>::to_float(v[lane * N + c]);
+          if (!isfinite(y)) acc[c] += y;
+        }
+      }
+    }
+    store_row<T, N>(p, s.a0 + tok, head, Ms, den, acc);
+  }
+}
+
+// CTAs past the units join the other rows (launched that way where they are few).
+template <typename T, int D>
+__global__ void __launch_bounds__(kSmallThreads) chunk_small_kernel(const ChunkParams p) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  __shared__ float stat[kSmallThreads / 32 * kSmallRows * 2];
+  __shared__ uint32_t bad;
+  const int unit = blockIdx.x;
+  if (unit >= p.batch * p.Hkv) {
+    grid_dep_wait();
+    join_rows<T, D>(p, (int64_t)(unit - p.batch * p.Hkv) * (kSmallThreads / 32) + (threadIdx.x >> 5));
+    return;
+  }
+  const int b = unit / p.Hkv, kvh = unit - b * p.Hkv;
+  const Seq s = p.own[b];
+  if (threadIdx.x == 0) bad = 0;
+  __syncthreads();
+  if (!is_small(p, s)) {
+    grid_dep_wait();  // (a kernel after this one relies on the one before it)
+    return;
+  }
+  const int rows = s.n * p.group;
+  if (rows <= 8) small_unit<T, D, 1>(p, s, b, kvh, smem, stat, &bad);
+  else if (rows <= 16) small_unit<T, D, 2>(p, s, b, kvh, smem, stat, &bad);
+  else if (rows <= 24) small_unit<T, D, 3>(p, s, b, kvh, smem, stat, &bad);
+  else small_unit<T, D, 4>(p, s, b, kvh, smem, stat, &bad);
 }
 
 // -------------------------------------------------------------------------
@@ -1638,7 +2014,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_join_kernel(const ChunkPa
 // -------------------------------------------------------------------------
 struct Layout {
   int grid, part_rows, TQ;
-  size_t parts, lse, o, cost, units, plan, share, seqs, prefix, row_o, row_lse, row_at, bytes;
+  size_t parts, lse, o, cost, units, plan, share, seqs, own, prefix, row_o, row_lse, row_at, bytes;
 };
 
 // The grid is one CTA per SM, or less where the tables' bounds show that there
@@ -1674,6 +2050,7 @@ Layout make_layout(const akt_chunk_paged_args* a, int groups, bool shared) {
   if (shared) {
     const size_t rows = (size_t)a->num_tokens * a->num_qo_heads;
     y.seqs = take(seqs * sizeof(Seq));
+    y.own = take((size_t)a->batch * sizeof(Seq));
     y.prefix = take((size_t)a->batch * 4);
     y.row_o = take(2 * rows * a->head_dim * 4);
     y.row_lse = take(2 * rows * 4);
@@ -1739,9 +2116,17 @@ int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap
     else kern<<<p.grid, kThreads, smem, st>>>(mq, mk, mv, p);
   }
   if (SHARED && e == cudaSuccess) {
-    constexpr int per = kMergeThreads / 32;
+    constexpr int per = kMergeThreads / 32 * kJoinRows, per_small = kSmallThreads / 32 * kJoinRows;
     const int64_t rows = p.num_tokens * p.Hq;
-    e = launch_dependent(chunk_join_kernel<T, D>, dim3((unsigned)((rows + per - 1) / per)), dim3(kMergeThreads), 0, st, p);
+    const bool fold = rows <= kFoldRows;
+    const int64_t units = (int64_t)p.batch * p.Hkv;
+    constexpr size_t smem_small = SmallCfg<D>::SMEM;
+    e = ensure_smem_limit<chunk_small_kernel<T, D>>(smem_small);
+    if (e == cudaSuccess)
+      e = launch_dependent(chunk_small_kernel<T, D>, dim3((unsigned)(units + (fold ? (rows + per_small - 1) / per_small : 0))),
+                           dim3(kSmallThreads), smem_small, st, p);
+    if (e == cudaSuccess && !fold)
+      e = launch_dependent(chunk_join_kernel<T, D>, dim3((unsigned)((rows + per - 1) / per)), dim3(kMergeThreads), 0, st, p);
   } else if (e == cudaSuccess)
     e = launch_dependent(chunk_merge_kernel<T, D>, dim3(2 * p.grid, (p.part_rows + p.merge_rows - 1) / p.merge_rows),
                          dim3(kMergeThreads), 0, st, p);
@@ -1839,6 +2224,7 @@ int run_chunk(const akt_chunk_paged_args* a, const akt_prefix_paged_args* shared
     p.group_indptr = shared->group_indptr;
     p.shared_pages = shared->shared_pages;
     p.seqs = reinterpret_cast<Seq*>(ws + y.seqs);
+    p.own = reinterpret_cast<Seq*>(ws + y.own);
     p.prefix_len = reinterpret_cast<int*>(ws + y.prefix);
     p.row_o = reinterpret_cast<float*>(ws + y.row_o);
     p.row_lse = reinterpret_cast<float*>(ws + y.row_lse);
@@ -1909,6 +2295,8 @@ extern "C" int akt_prefix_paged(const akt_prefix_paged_args* a, void* workspace,
   if (!a) return set_error(AKT_ERR_INVALID, "null args");
   if (a->num_groups < 0 || (int64_t)a->num_groups + std::max(a->chunk.batch, 0) > 0x3fffffff)
     return set_error(AKT_ERR_INVALID, "prefix_paged: bad number of groups");
+  if ((int64_t)std::max(a->chunk.batch, 0) * std::max(a->chunk.num_kv_heads, 0) > 0x3fffffff)
+    return set_error(AKT_ERR_INVALID, "prefix_paged: too many sequences");
   if (a->num_groups > 0 && (!a->group_indptr || !a->shared_pages))
     return set_error(AKT_ERR_INVALID, "prefix_paged: missing groups");
   return run_chunk(&a->chunk, a, workspace, workspace_bytes, stream);
