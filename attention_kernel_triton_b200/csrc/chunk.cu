@@ -105,6 +105,7 @@ constexpr int kFewRows = 48;
 // few its rows and tiles are.  One token in each of 64 sequences of 64 to 1024 own keys
 // behind 8192: KSMALL_MEASURED.
 constexpr int kSmallRows = 32, kSmallKeys = 2048;
+constexpr int kOrderSeqs = 1024;   // sequences that the planner orders by length for it
 constexpr int kTableSeqs = 96;     // sequences whose table fits the CTA's shared memory
 constexpr int kMaxCtas = kThreads; // of the main kernel (one per SM)
 
@@ -149,6 +150,7 @@ struct ChunkParams {
   struct Seq* seqs;    // [B]
   struct Seq* own;     // [batch] the sequences on their own keys; those with few have no rows in `seqs`
   int* prefix_len;     // [batch] shared keys of each sequence
+  int* order;          // [batch] the sequences, those with the most own keys first
   float* row_o;        // [2][rows][D] normalised outputs of a row on the prefix, on its own keys
   float* row_lse;      // [2][rows]
   int2* row_at;        // [2][rows] kWhole, kDone, or the place of the first part and the row there
@@ -675,7 +677,20 @@ __device__ void build_shared(const ChunkParams& p, int* bad) {
     if (is_small(p, s)) s.n = 0;
     p.seqs[p.groups + b] = s;
     p.prefix_len[b] = keys;
+    p.order[b] = b;
   }
+  __syncthreads();
+  // long ones first, so that none of them begins last (past kOrderSeqs the sorting would take longer than it saves)
+  if (p.batch <= kOrderSeqs)
+    for (int b = threadIdx.x; b < p.batch; b += 1024) {
+      const int len = p.own[b].len;
+      int before = 0;
+      for (int e = 0; e < p.batch; ++e) {
+        const int other = p.own[e].len;
+        before += other > len || (other == len && e < b);
+      }
+      p.order[before] = b;
+    }
   __syncthreads();
 }
 
@@ -1555,16 +1570,15 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const ChunkP
 // -------------------------------------------------------------------------
 // join of a row's results on a shared prefix and on its own keys
 // -------------------------------------------------------------------------
-// Results of row `row` in unit kind k (0 the prefix, 1 its own keys): whole, or parts as
-// chunk_merge_kernel finds them.  The whole warp calls it.
+// Results of a row in unit kind k (0 the prefix, 1 its own keys), whose entry of row_at is
+// w: whole, or parts as chunk_merge_kernel finds them.  The whole warp calls it.
 struct RowParts {
   int count;  // 0: none
   int first;  // place of the first part, kWhole, or kDone
   int r;      // the row there
 };
 
-__device__ __forceinline__ RowParts row_parts(const ChunkParams& p, int k, int64_t row) {
-  const int2 w = p.row_at[k * p.num_tokens * p.Hq + row];
+__device__ __forceinline__ RowParts row_parts(const ChunkParams& p, int2 w) {
   RowParts x{1, w.x, w.y};
   if (w.x < 0 || p.parts[w.x].last) return x;
   const int lane = threadIdx.x & 31, c0 = w.x >> 1;
@@ -1600,7 +1614,7 @@ __device__ __forceinline__ float row_result(const ChunkParams& p, int k, int64_t
 
 // A row's results, a weight each; lane columns [N lane, N lane + N).  `M` is the largest
 // log-sum-exp so far (all lanes), den and acc the sums in its scale.
-template <int D, int N>
+template <int D, int N, int U = 4>
 __device__ __forceinline__ void add_results(const ChunkParams& p, int k, int64_t row, const RowParts& x, float Ms,
                                             float& den, float (&acc)[N]) {
   const int lane = threadIdx.x & 31;
@@ -1610,22 +1624,23 @@ __device__ __forceinline__ void add_results(const ChunkParams& p, int k, int64_t
     const float mine = fast_exp2((part - Ms) * kLog2e);  // NaN stays NaN
     const unsigned holds = __ballot_sync(0xffffffffu, part != -INFINITY);  // (a weight of 0 is not left out)
     const int n = min(32, x.count - i0);
-    for (int i1 = 0; i1 < n; i1 += 4) {  // four rows asked for at once
-      float w[4];
-      float v[4][N];
+    for (int i1 = 0; i1 < n; i1 += U) {  // U rows asked for at once
+      float w[U];
+      float v[U][N];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < U; ++u) {
         w[u] = __shfl_sync(0xffffffffu, mine, i1 + u);
         const float* src = reinterpret_cast<const float*>(
             __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(o), i1 + u));
 #pragma unroll
         for (int e = 0; e < N; ++e) v[u][e] = 0.f;
-        if (!(holds >> (i1 + u) & 1u)) continue;
+        if (i1 + u >= n || !(holds >> (i1 + u) & 1u)) continue;
         if constexpr (N == 4) *reinterpret_cast<float4*>(v[u]) = *reinterpret_cast<const float4*>(src + lane * N);
         else *reinterpret_cast<float2*>(v[u]) = *reinterpret_cast<const float2*>(src + lane * N);
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < U; ++u) {
+        if (i1 + u >= n) continue;
         den += w[u];
 #pragma unroll
         for (int e = 0; e < N; ++e) acc[e] = fmaf(w[u], v[u][e], acc[e]);
@@ -1727,7 +1742,8 @@ __device__ void join_rows(const ChunkParams& p, int64_t warp) {
         M = -INFINITY;
       } else {
         if (at1 == kDone) continue;
-        const RowParts own = row_parts(p, 1, row), front = prefixed ? row_parts(p, 0, row) : RowParts{0, kWhole, 0};
+        const RowParts own = row_parts(p, p.row_at[rows + row]);
+        const RowParts front = prefixed ? row_parts(p, p.row_at[row]) : RowParts{0, kWhole, 0};
         M = fmaxf(largest_result<D>(p, 1, row, own), largest_result<D>(p, 0, row, front));
         const float Ms = M == -INFINITY ? 0.f : M;
         add_results<D, N>(p, 0, row, front, Ms, den, acc);
@@ -1777,7 +1793,8 @@ __device__ void small_unit(const ChunkParams& p, const Seq& s, int b, int kvh, u
                            uint32_t* bad) {
   constexpr int KS = D / 16, PIECES = D / 8;
   using C = SmallCfg<D>;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = kSmallThreads / 32;
+  constexpr int warps = kSmallThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rows = s.n * p.group;
   // this lane's rows of each 8: columns 2 (lane % 4) and the next of the products
   int vis[NT][2];
@@ -1942,17 +1959,51 @@ __device__ void small_unit(const ChunkParams& p, const Seq& s, int b, int kvh, u
   }
   __syncthreads();
   grid_dep_wait();
-  constexpr int N = D / 32;
-  for (int r = warp; r < rows; r += warps) {
+  constexpr int N = D / 32, RW = NT * 8 / warps;  // rows of a warp
+  // where the prefix's results of the warp's rows are: a lane per row, and the parts' log-sum-exps of all rows at once
+  auto row_of = [&](int r) -> int64_t {
+    const int tok = (int)fdiv((uint32_t)r, p.div_group);
+    return (int64_t)(s.a0 + tok) * p.Hq + kvh * p.group + r - tok * p.group;
+  };
+  int2 at = make_int2(kDone, 0);
+  if (s.prefix && lane < RW && warp + lane * warps < rows) at = p.row_at[row_of(warp + lane * warps)];
+  RowParts parts[RW];
+  float largest[RW];
+#pragma unroll
+  for (int i = 0; i < RW; ++i) {
+    const int2 w = make_int2(__shfl_sync(0xffffffffu, at.x, i), __shfl_sync(0xffffffffu, at.y, i));
+    if (w.x == kDone) parts[i] = RowParts{0, kWhole, 0};
+    else if (i && w.x == parts[i - 1].first && parts[i - 1].count) parts[i] = RowParts{parts[i - 1].count, w.x, w.y};
+    else parts[i] = row_parts(p, w);
+    const float* o;  // (the first 32 of them)
+    largest[i] = row_result<D>(p, 0, row_of(warp + i * warps), parts[i], lane, o);
+  }
+#pragma unroll 1
+  for (int i = 0; i < RW; ++i) {
+    const int r = warp + i * warps;
+    if (r >= rows) break;
+    RowParts front = parts[0];
+    float big = largest[0];
+#pragma unroll
+    for (int e = 1; e < RW; ++e)
+      if (e == i) {
+        front = parts[e];
+        big = largest[e];
+      }
     const int tok = (int)fdiv((uint32_t)r, p.div_group), head = kvh * p.group + r - tok * p.group;
-    const int64_t row = (int64_t)(s.a0 + tok) * p.Hq + head;
+    const int64_t row = row_of(r);
     float ml = -INFINITY;  // log2 units
 #pragma unroll
     for (int w = 0; w < warps; ++w) ml = fmaxf(ml, stat[(w * kSmallRows + r) * 2]);
-    const RowParts front = s.prefix ? row_parts(p, 0, row) : RowParts{0, kWhole, 0};
-    const float M = fmaxf(ml * kLn2, largest_result<D>(p, 0, row, front)), Ms = M == -INFINITY ? 0.f : M;
+    if (front.count > 32) {
+      big = largest_result<D>(p, 0, row, front);
+    } else {
+#pragma unroll
+      for (int w = 16; w; w >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, w));
+    }
+    const float M = fmaxf(ml * kLn2, big), Ms = M == -INFINITY ? 0.f : M;
     float acc[N] = {}, den = 0.f;
-    add_results<D, N>(p, 0, row, front, Ms, den, acc);
+    add_results<D, N, 16>(p, 0, row, front, Ms, den, acc);
 #pragma unroll
     for (int w = 0; w < warps; ++w) {
       const float mw = stat[(w * kSmallRows + r) * 2], lw = stat[(w * kSmallRows + r) * 2 + 1];
@@ -1994,7 +2045,7 @@ __global__ void __launch_bounds__(kSmallThreads) chunk_small_kernel(const ChunkP
     join_rows<T, D>(p, (int64_t)(unit - p.batch * p.Hkv) * (kSmallThreads / 32) + (threadIdx.x >> 5));
     return;
   }
-  const int b = unit / p.Hkv, kvh = unit - b * p.Hkv;
+  const int b = p.order[unit / p.Hkv], kvh = unit % p.Hkv;
   const Seq s = p.own[b];
   if (threadIdx.x == 0) bad = 0;
   __syncthreads();
@@ -2014,7 +2065,7 @@ __global__ void __launch_bounds__(kSmallThreads) chunk_small_kernel(const ChunkP
 // -------------------------------------------------------------------------
 struct Layout {
   int grid, part_rows, TQ;
-  size_t parts, lse, o, cost, units, plan, share, seqs, own, prefix, row_o, row_lse, row_at, bytes;
+  size_t parts, lse, o, cost, units, plan, share, seqs, own, prefix, order, row_o, row_lse, row_at, bytes;
 };
 
 // The grid is one CTA per SM, or less where the tables' bounds show that there
@@ -2052,6 +2103,7 @@ Layout make_layout(const akt_chunk_paged_args* a, int groups, bool shared) {
     y.seqs = take(seqs * sizeof(Seq));
     y.own = take((size_t)a->batch * sizeof(Seq));
     y.prefix = take((size_t)a->batch * 4);
+    y.order = take((size_t)a->batch * 4);
     y.row_o = take(2 * rows * a->head_dim * 4);
     y.row_lse = take(2 * rows * 4);
     y.row_at = take(2 * rows * sizeof(int2));
@@ -2226,6 +2278,7 @@ int run_chunk(const akt_chunk_paged_args* a, const akt_prefix_paged_args* shared
     p.seqs = reinterpret_cast<Seq*>(ws + y.seqs);
     p.own = reinterpret_cast<Seq*>(ws + y.own);
     p.prefix_len = reinterpret_cast<int*>(ws + y.prefix);
+    p.order = reinterpret_cast<int*>(ws + y.order);
     p.row_o = reinterpret_cast<float*>(ws + y.row_o);
     p.row_lse = reinterpret_cast<float*>(ws + y.row_lse);
     p.row_at = reinterpret_cast<int2*>(ws + y.row_at);
