@@ -397,11 +397,18 @@ class Entry:
         self._pack = struct.Struct(fmt).pack
         self._fn = None
 
-    def __call__(self, values, *rest):
+    def pack(self, values):
+        """The argument struct, for ``packed``: one struct for two entry points that take it."""
+        return self._pack(*values)
+
+    def packed(self, args, *rest):
         if self._fn is None:
             name, _, kinds, restype = self._what
             self._fn = ctypes.CFUNCTYPE(restype, c_char_p, *kinds)((name, lib()))
-        return self._fn(self._pack(*values), *rest)
+        return self._fn(args, *rest)
+
+    def __call__(self, values, *rest):
+        return self.packed(self._pack(*values), *rest)
 
 
 def device_index(*tensors: torch.Tensor) -> int:

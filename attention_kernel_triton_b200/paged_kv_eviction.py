@@ -77,7 +77,7 @@ def accumulate_attention_weights_paged(weights, q, q_indptr, paged_kv_cache, kv_
     B = indptr.numel() - 1
     if at.numel() != B + 1 or last.numel() != B:
         raise ValueError("q_indptr and kv_page_indptr must have B+1 entries and kv_last_page_len B entries")
-    for t in (out,) if weights is None else (out, weights):
+    for t in (out,) if weights is None or weights is out else (out, weights):
         if t.dtype is not torch.float32 or len(t.shape) != 3 or t.shape[:2] != (B, pool[2]) or t.shape != out.shape:
             raise ValueError("weights and out must be fp32 [B, Hkv, L]")
         if not _unit(t):
@@ -94,9 +94,10 @@ def accumulate_attention_weights_paged(weights, q, q_indptr, paged_kv_cache, kv_
 
     def call(q, cache):
         values = (q.data_ptr(), *q.stride(), at.data_ptr(), T, cache.data_ptr(), *cache.stride(), pool[0], *tail)
-        size = _weights_size(values)
+        args = _weights.pack(values)
+        size = _weights_size.packed(args)
         ws = q.new_empty((size + 1) // 2)
-        return _weights(values, ws.data_ptr(), size, _lib.raw_stream(index))
+        return _weights.packed(args, ws.data_ptr(), size, _lib.raw_stream(index))
 
     with _lib.on_index(index):
         rc = call(q, paged_kv_cache)
@@ -189,10 +190,11 @@ def evict_paged_kv_cache(paged_kv_cache, kv_page_indptr, kv_page_indices, kv_las
     values = (*pool, indptr.data_ptr(), indices.data_ptr(), last.data_ptr(), indices.numel(), keep.data_ptr(),
               ks[0] if layered else 0, *ks[-3:-1], kept.data_ptr(), M, _ptr(mask), *wp, out_indptr.data_ptr(),
               out_indices.data_ptr(), out_last.data_ptr(), most, B)
-    size = _evict_size(values)
+    args = _evict.pack(values)
+    size = _evict_size.packed(args)
     ws = indptr.new_empty(size // 4 + 1)
     with _lib.on_index(index):
-        rc = _evict(values, ws.data_ptr(), size, _lib.raw_stream(index))
+        rc = _evict.packed(args, ws.data_ptr(), size, _lib.raw_stream(index))
         if rc:
             _lib.check(rc)
     return out_indptr, out_indices, out_last

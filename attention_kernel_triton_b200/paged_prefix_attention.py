@@ -81,9 +81,10 @@ def shared_prefix_paged_into(out, q, q_indptr, paged_kv_cache, kv_page_indptr, k
 
     def call(q, cache):
         values = (q.data_ptr(), *q.stride(), at.data_ptr(), T, cache.data_ptr(), *cache.stride(), pool[0], *tail)
-        size = _workspace(values)
+        args = _prefix.pack(values)
+        size = _workspace.packed(args)
         ws = q.new_empty((size + 1) // 2)
-        return _prefix(values, ws.data_ptr(), size, _lib.raw_stream(index))
+        return _prefix.packed(args, ws.data_ptr(), size, _lib.raw_stream(index))
 
     with _lib.on_index(index):
         rc = call(q, paged_kv_cache)

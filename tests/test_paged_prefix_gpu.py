@@ -122,6 +122,25 @@ def test_prompts_behind_documents():
     Family([(60, [1100, 513], [1100, 400])], Hkv=1, G=2, D=128, P=16, seed=5).check(True)
 
 
+def test_borders_of_the_warp_level_units():
+    Family([(4, [2047, 2048, 2049, 2050], [1, 8, 8, 9])], Hkv=2, G=4, seed=20).check(True)
+    Family([(4, [31, 32, 33, 2047], [31, 32, 33, 2])], Hkv=1, G=1, D=64, dtype=BF16, seed=21).check(True)
+    Family([(2, [5, 16, 40, 7], [1, 2, 4, 3])], Hkv=2, G=8, D=64, seed=22).check(True)
+    Family([(2, [5, 16, 40, 7], [1, 2, 4, 3])], Hkv=1, G=7, seed=23).check(False)
+
+
+def test_more_sequences_than_are_ordered():
+    Family([(3, [1 + i % 5 for i in range(1100)], [1] * 1100)], Hkv=1, G=2, D=64, seed=24).check(True)
+
+
+def test_rows_that_a_kernel_of_their_own_joins():
+    Family([(20, [700, 600], [700, 600]), (3, [33], [33])], Hkv=4, G=8, D=64, seed=25).check(True)
+
+
+def test_a_long_sequence_without_a_prefix_beside_a_group():
+    Family([(0, [9000], [1]), (40, [3, 5], [1, 1]), (0, [5000], [3])], Hkv=2, G=4, seed=26).check(True)
+
+
 def test_scale_and_large_scores():
     Family([(9, [30, 31], [3, 4])], D=64, seed=6, std=2.0).check(True, scale=0.3)
 
