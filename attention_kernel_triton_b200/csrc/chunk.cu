@@ -103,7 +103,9 @@ constexpr int kFewRows = 48;
 // Units of a sequence's own keys behind a prefix that take the warp-level kernel: a
 // unit's chain of steps here (Q, S, the exponentials, P.V, the output) takes 4 us however
 // few its rows and tiles are.  One token in each of 64 sequences of 64 to 1024 own keys
-// behind 8192: KSMALL_MEASURED.
+// behind 8192, 4 rows a unit: 72 us, all units here 101; five tokens in each of 64 behind
+// eight prefixes, 20 rows: 167, here 181.  (More rows take a multiple of the warp-level
+// products; longer keys are better cut over several SMs.)
 constexpr int kSmallRows = 32, kSmallKeys = 2048;
 constexpr int kOrderSeqs = 1024;   // sequences that the planner orders by length for it
 constexpr int kTableSeqs = 96;     // sequences whose table fits the CTA's shared memory
