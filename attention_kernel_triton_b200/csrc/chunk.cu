@@ -104,7 +104,7 @@ constexpr int kFewRows = 48;
 // unit's chain of steps here (Q, S, the exponentials, P.V, the output) takes 4 us however
 // few its rows and tiles are.  One token in each of 64 sequences of 64 to 1024 own keys
 // behind 8192, 4 rows a unit: 72 us, all units here 101; five tokens in each of 64 behind
-// eight prefixes, 20 rows: 167, here 181.  (More rows take a multiple of the warp-level
+// eight prefixes, 20 rows: 159, here 181.  (More rows take a multiple of the warp-level
 // products; longer keys are better cut over several SMs.)
 constexpr int kSmallRows = 32, kSmallKeys = 2048;
 constexpr int kOrderSeqs = 1024;   // sequences that the planner orders by length for it
@@ -1614,40 +1614,45 @@ __device__ __forceinline__ float row_result(const ChunkParams& p, int k, int64_t
   return p.part_lse[at];
 }
 
-// A row's results, a weight each; lane columns [N lane, N lane + N).  `M` is the largest
-// log-sum-exp so far (all lanes), den and acc the sums in its scale.
-template <int D, int N, int U = 4>
+// n results of a row, result i's log-sum-exp `part` and row `o` with lane i; lane columns
+// [N lane, N lane + N).  Ms is the largest log-sum-exp, den and acc the sums in its scale.
+template <int N, int U>
+__device__ __forceinline__ void add_weighted(int n, float part, const float* o, float Ms, float& den, float (&acc)[N]) {
+  const int lane = threadIdx.x & 31;
+  const float mine = fast_exp2((part - Ms) * kLog2e);  // NaN stays NaN
+  const unsigned holds = __ballot_sync(0xffffffffu, part != -INFINITY);  // (a weight of 0 is not left out)
+  for (int i1 = 0; i1 < n; i1 += U) {  // U rows asked for at once
+    float w[U];
+    float v[U][N];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      w[u] = __shfl_sync(0xffffffffu, mine, i1 + u);
+      const float* src = reinterpret_cast<const float*>(
+          __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(o), i1 + u));
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[u][e] = 0.f;
+      if (i1 + u >= n || !(holds >> (i1 + u) & 1u)) continue;
+      if constexpr (N == 4) *reinterpret_cast<float4*>(v[u]) = *reinterpret_cast<const float4*>(src + lane * N);
+      else *reinterpret_cast<float2*>(v[u]) = *reinterpret_cast<const float2*>(src + lane * N);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i1 + u >= n) continue;
+      den += w[u];
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] = fmaf(w[u], v[u][e], acc[e]);
+    }
+  }
+}
+
+// All results of a row.
+template <int D, int N>
 __device__ __forceinline__ void add_results(const ChunkParams& p, int k, int64_t row, const RowParts& x, float Ms,
                                             float& den, float (&acc)[N]) {
-  const int lane = threadIdx.x & 31;
   for (int i0 = 0; i0 < x.count; i0 += 32) {
     const float* o;
-    const float part = row_result<D>(p, k, row, x, i0 + lane, o);
-    const float mine = fast_exp2((part - Ms) * kLog2e);  // NaN stays NaN
-    const unsigned holds = __ballot_sync(0xffffffffu, part != -INFINITY);  // (a weight of 0 is not left out)
-    const int n = min(32, x.count - i0);
-    for (int i1 = 0; i1 < n; i1 += U) {  // U rows asked for at once
-      float w[U];
-      float v[U][N];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        w[u] = __shfl_sync(0xffffffffu, mine, i1 + u);
-        const float* src = reinterpret_cast<const float*>(
-            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(o), i1 + u));
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[u][e] = 0.f;
-        if (i1 + u >= n || !(holds >> (i1 + u) & 1u)) continue;
-        if constexpr (N == 4) *reinterpret_cast<float4*>(v[u]) = *reinterpret_cast<const float4*>(src + lane * N);
-        else *reinterpret_cast<float2*>(v[u]) = *reinterpret_cast<const float2*>(src + lane * N);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (i1 + u >= n) continue;
-        den += w[u];
-#pragma unroll
-        for (int e = 0; e < N; ++e) acc[e] = fmaf(w[u], v[u][e], acc[e]);
-      }
-    }
+    const float part = row_result<D>(p, k, row, x, i0 + (int)(threadIdx.x & 31), o);
+    add_weighted<N, 4>(min(32, x.count - i0), part, o, Ms, den, acc);
   }
 }
 
@@ -1997,6 +2002,7 @@ __device__ void small_unit(const ChunkParams& p, const Seq& s, int b, int kvh, u
     float ml = -INFINITY;  // log2 units
 #pragma unroll
     for (int w = 0; w < warps; ++w) ml = fmaxf(ml, stat[(w * kSmallRows + r) * 2]);
+    const float part = big;
     if (front.count > 32) {
       big = largest_result<D>(p, 0, row, front);
     } else {
@@ -2005,7 +2011,14 @@ __device__ void small_unit(const ChunkParams& p, const Seq& s, int b, int kvh, u
     }
     const float M = fmaxf(ml * kLn2, big), Ms = M == -INFINITY ? 0.f : M;
     float acc[N] = {}, den = 0.f;
-    add_results<D, N, 16>(p, 0, row, front, Ms, den, acc);
+    if (front.count > 32) {
+      add_results<D, N>(p, 0, row, front, Ms, den, acc);
+    } else if (front.count) {
+      const int place = lane ? 2 * ((front.first >> 1) + lane) : front.first;
+      const float* o = front.first < 0 ? p.row_o + row * D : p.part_o + ((int64_t)place * p.part_rows + front.r) * D;
+      if (front.count <= 4) add_weighted<N, 4>(front.count, part, o, Ms, den, acc);
+      else add_weighted<N, 16>(front.count, part, o, Ms, den, acc);
+    }
 #pragma unroll
     for (int w = 0; w < warps; ++w) {
       const float mw = stat[(w * kSmallRows + r) * 2], lw = stat[(w * kSmallRows + r) * 2 + 1];
