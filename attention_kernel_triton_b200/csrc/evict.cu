@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictPar
     }
     int here;
     const int r = fresh + block_scan<int>(replace, sums, here);
-    if (g < g1) p.out_indices[g] = replace ? -2 - r : page;
+    if (g < g1) p.out_indices[g] = replace ? -2 - r : max(page, -1);
     fresh += here;
   }
   for (int64_t g = (int64_t)N + rank * kPlanThreads + tid; g < p.max_entries; g += (int64_t)C * kPlanThreads)
@@ -553,10 +553,8 @@ __global__ void __launch_bounds__(kMoveThreads, 2) evict_move_kernel(const Evict
       for (int u = 0; u < U; ++u) {
         const int i = i0 + u * kMoveThreads;
         const int j = i < n ? checked_token(i, __ldg(keep + i), i ? __ldg(keep + i - 1) : -1, len) : -1;
-        v[u] = 0.f;
-        if (j < 0 || j >= p.width) continue;
-        v[u] = w[j];
-        ok |= 1 << u;
+        v[u] = j >= 0 && j < p.width ? w[j] : 0.f;
+        ok |= (j >= 0 && i < p.width) << u;
       }
       cluster_sync();
 #pragma unroll

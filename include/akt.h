@@ -692,7 +692,8 @@ int akt_select_tokens(const akt_select_tokens_args* args, void* stream);
 /* before it is skipped, keep_len past max_kept or the sequence is cut (both */
 /* status 3); a sequence with bad bounds is empty (status 4), pages past     */
 /* max_entries are cut (status 5), ids outside the pool stay as they are     */
-/* (status 2).  The new table must not overlap the old one.                  */
+/* (status 2; negative ones become -1).  Tokens past `width` have weight 0.  */
+/* The new table must not overlap the old one.                               */
 typedef struct akt_evict_paged_args {
   akt_page_pool pool;
   const int32_t* kv_page_indptr;   /* [batch + 1] */

@@ -286,6 +286,41 @@ def test_bad_lists_and_tables_are_skipped_and_recorded():
             assert same(dev[page].cpu(), want[0, page]), what
 
 
+def test_negative_page_ids_take_no_dead_page():
+    # an id below -1 in a sequence beside pages that have to be replaced
+    pool, starts, indices, last, keep, kept, w = case([40, 40, 40], 20, 8, share=2, spare=6)
+    bad = list(indices)
+    bad[starts[2]] = -2
+    bad[starts[2] + 1] = -3
+    want = pool.clone()
+    a, b, c = plain_evict(want, starts[:3], indices[:starts[2]], last[:2], keep[:, :2], kept[:2], 8,
+                          reserved=set(bad[starts[2] + 2:]))
+    dev = pool[0].to(DEV)
+    got = evict_paged_kv_cache(dev, i32(starts), i32(bad), i32(last), keep[0].to(DEV), i32(kept))
+    # (the two pages that the bad ids hide are dead: the lowest dead ones are found again)
+    dead = sorted(set(range(pool.shape[1])) - {x for x in bad if x >= 0})
+    fresh = [x for x in got[1].tolist()[:a[-1]] if x not in indices[:starts[2]]]
+    assert fresh == dead[:len(fresh)] and len(fresh) == len(set(fresh)) > 0
+    assert got[1].tolist()[a[2]:a[2] + 2] == [-1, -1]
+    for b in range(2):  # every row of the good sequences
+        pages = got[1].tolist()[a[b]:a[b + 1]]
+        mine = indices[starts[b]:starts[b + 1]]
+        for h in range(2):
+            for i in range(20):
+                j = int(keep[0, b, h, i])
+                assert same(dev[pages[i // 8], :, h, i % 8].cpu(), pool[0, mine[j // 8], :, h, j % 8])
+
+
+def test_weights_narrower_than_the_sequences():
+    pool, starts, indices, last, keep, kept, w = case([60], 30, 8)
+    narrow = w[0, :, :, :40].contiguous()
+    dw = narrow.to(DEV)
+    evict_paged_kv_cache(pool[0].to(DEV), i32(starts), i32(indices), i32(last), keep[0].to(DEV), i32(kept), weights=dw)
+    for h in range(2):
+        want = [narrow[0, h, j].item() if j < 40 else 0.0 for j in keep[0, 0, h].tolist()] + [0.0] * 10
+        assert dw[0, h].tolist() == want
+
+
 def test_empty_calls():
     pool = torch.zeros(3, 2, 1, 4, 64, dtype=torch.float16, device=DEV)
     got = evict_paged_kv_cache(pool, i32([0]), i32([]), i32([]), i32([]).view(0, 1, 0), i32([]))
