@@ -597,8 +597,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int u = u0; ok && u < u1; ++u) {
         for (int r = r0; r < r1; ++r) {
           const int slot = gq % QS, toks = n - r * 2 * p.TQ;
-          // columns that the tile's rows fill, in steps of 16
-          const int cols = toks > p.TQ ? BR : (toks * p.group + 15) / 16 * 16;
+          // columns that the tile's rows fill, in steps of 16; a half that is full of tokens is read
+          // whole and without a mask, so all of its columns are written (by rows of zeros, if it must be)
+          const int cols = toks > p.TQ ? BR : (toks == p.TQ ? BK : (toks * p.group + 15) / 16 * 16);
           const uint32_t idesc = idesc_f16(fmt, BK, 0, 0) | (uint32_t)(cols >> 3) << 17;
           if (!wait(&q_full[slot], (gq / QS) & 1)) { ok = false; break; }
 #pragma unroll 1
