@@ -630,7 +630,7 @@ __device__ __forceinline__ bool is_small(const ChunkParams& p, const Seq& s) {
 __device__ void build_shared(const ChunkParams& p, int* bad) {
   if (threadIdx.x == 0) *bad = 0;
   __syncthreads();
-  for (int g = threadIdx.x; g <= p.groups; g += 1024) {
+  for (int g = threadIdx.x; p.groups && g <= p.groups; g += 1024) {  // (no groups need no bounds)
     const int x = __ldg(p.group_indptr + g);
     if (x < 0 || x > p.batch || (g && __ldg(p.group_indptr + g - 1) > x)) *bad = 1;
   }

@@ -305,6 +305,27 @@ def test_graph_and_another_stream():
     assert same(got, want) and same(lse, ref) and same(found, want)
 
 
+def test_no_groups_need_no_pointers():
+    c = Family([(4, [20, 40], [2, 3])], seed=27)
+    out, lse = torch.empty_like(c.q), torch.empty(c.q.shape[:2], device=DEV)
+    q, at, pool, indptr, indices, last = c.args()
+    a = _lib.PrefixPagedArgs()
+    k = a.chunk
+    k.q, (k.q_stride_token, k.q_stride_head, k.q_stride_dim) = q.data_ptr(), q.stride()
+    k.q_indptr, k.num_tokens, k.kv_cache, k.num_pages = at.data_ptr(), q.shape[0], pool.data_ptr(), pool.shape[0]
+    (k.kv_stride_page, k.kv_stride_kv, k.kv_stride_head, k.kv_stride_token, k.kv_stride_dim) = pool.stride()
+    k.kv_page_indptr, k.kv_page_indices, k.kv_last_page_len = indptr.data_ptr(), indices.data_ptr(), last.data_ptr()
+    k.num_page_entries, k.out, k.lse = indices.numel(), out.data_ptr(), lse.data_ptr()
+    (k.out_stride_token, k.out_stride_head, k.out_stride_dim) = out.stride()
+    (k.lse_stride_token, k.lse_stride_head) = lse.stride()
+    k.batch, k.num_qo_heads, k.num_kv_heads, k.page_size, k.head_dim, k.causal = 2, 8, 2, 16, 128, 1
+    k.dtype, k.softmax_scale = _lib.AKT_FLOAT16, 128 ** -0.5
+    L = _lib.lib()
+    ws = torch.empty(L.akt_prefix_paged_workspace_size(a), dtype=torch.uint8, device=DEV)
+    assert L.akt_prefix_paged(a, ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream) == _lib.AKT_OK
+    c.close(out, lse, True)
+
+
 def test_nothing_to_do():
     c = Family([(2, [3, 4], [0, 0])], seed=19)
     assert c.run(True)[0].shape == (0, 8, 128)
