@@ -678,7 +678,8 @@ extern "C" int akt_select_tokens(const akt_select_tokens_args* a, void* stream) 
   if (a->width > 0x3fffffff || a->budget > 0x3fffffff || rows > 0x7ffffff)
     return set_error(AKT_ERR_INVALID, "select_tokens: too many tokens");
   if (a->batch > 0 && (!a->seq_lens || !a->keep_len)) return set_error(AKT_ERR_INVALID, "select_tokens: missing tensor");
-  if (rows == 0) return AKT_OK;
+  if (a->batch == 0) return AKT_OK;
+  if (rows == 0) return set_error(AKT_ERR_INVALID, "select_tokens: sequences without heads");
   if ((a->width > 0 && !a->weights) || (a->budget > 0 && !a->keep_ind))
     return set_error(AKT_ERR_INVALID, "select_tokens: missing tensor");
   SelectParams p{};

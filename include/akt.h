@@ -624,8 +624,9 @@ int akt_shared_prefix_pages(const int32_t* group_indptr, int32_t num_groups, con
 /* out[b, h, j] = weights[b, h, j] + the softmax weights that key j of       */
 /* sequence b gets from the new tokens' queries of the heads of kv head h:   */
 /* the sum of exp(scale q . k_j - lse) over the rows that see it.  Rows,     */
-/* table, causal and lse are those of akt_chunk_paged; a row whose lse is    */
-/* -inf adds nothing.  weights may be NULL (sums from zero) or out itself.   */
+/* table, causal and lse are those of akt_chunk_paged (lse over all of the   */
+/* row's keys, so that no weight is above 1); a row whose lse is -inf adds   */
+/* nothing.  weights may be NULL (sums from zero) or out itself.            */
 /* Places past a sequence's length are not written; keys past `width` are    */
 /* left out and recorded (status 3).  Sums are in fp32, in an order that     */
 /* depends on the sizes alone.  head_dim 64 or 128.                          */

@@ -90,7 +90,8 @@ def test_select_entry_refuses_bad_arguments():
 
     for kw in (dict(batch=-1), dict(layers=-1), dict(num_heads=-1), dict(width=-1), dict(budget=-1), dict(sinks=9),
                dict(recent=10), dict(sinks=-1), dict(weights=None), dict(seq_lens=None), dict(keep_ind=None),
-               dict(keep_len=None), dict(width=1 << 40), dict(sinks=1 << 30, recent=1 << 30, budget=100)):
+               dict(keep_len=None), dict(num_heads=0), dict(layers=0), dict(width=1 << 40),
+               dict(sinks=1 << 30, recent=1 << 30, budget=100)):
         assert rc(**kw) == _lib.AKT_ERR_INVALID, kw
     assert rc(batch=0) == _lib.AKT_OK
     assert L.akt_select_tokens(None, None) == _lib.AKT_ERR_INVALID
