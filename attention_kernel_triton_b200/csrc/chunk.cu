@@ -1580,6 +1580,12 @@ struct RowParts {
   int r;      // the row there
 };
 
+// Entry i of row_at.  Where a wait ran out (recorded) it may never have been written: no place outside the workspace.
+__device__ __forceinline__ int2 row_place(const ChunkParams& p, int64_t i) {
+  const int2 w = p.row_at[i];
+  return w.x >= 2 * p.grid || (w.x >= 0 && (unsigned)w.y >= (unsigned)p.part_rows) ? make_int2(kDone, 0) : w;
+}
+
 __device__ __forceinline__ RowParts row_parts(const ChunkParams& p, int2 w) {
   RowParts x{1, w.x, w.y};
   if (w.x < 0 || p.parts[w.x].last) return x;
@@ -1700,10 +1706,10 @@ __device__ void join_rows(const ChunkParams& p, int64_t warp) {
     const int a0 = __ldg(p.q_indptr + b), a1 = __ldg(p.q_indptr + b + 1);
     none = !(a0 >= 0 && tok >= a0 && tok < a1 && a1 <= p.num_tokens);
     if (!none && !is_small(p, p.own[b])) {
-      w1 = p.row_at[rows + row];
+      w1 = row_place(p, rows + row);
       if (w1.x == kWhole) lse1 = p.row_lse[rows + row];
       if (p.prefix_len[b]) {
-        w0 = p.row_at[row];
+        w0 = row_place(p, row);
         if (w0.x == kWhole) lse0 = p.row_lse[row];
       }
     }
@@ -1749,8 +1755,8 @@ __device__ void join_rows(const ChunkParams& p, int64_t warp) {
         M = -INFINITY;
       } else {
         if (at1 == kDone) continue;
-        const RowParts own = row_parts(p, p.row_at[rows + row]);
-        const RowParts front = prefixed ? row_parts(p, p.row_at[row]) : RowParts{0, kWhole, 0};
+        const RowParts own = row_parts(p, row_place(p, rows + row));
+        const RowParts front = prefixed ? row_parts(p, row_place(p, row)) : RowParts{0, kWhole, 0};
         M = fmaxf(largest_result<D>(p, 1, row, own), largest_result<D>(p, 0, row, front));
         const float Ms = M == -INFINITY ? 0.f : M;
         add_results<D, N>(p, 0, row, front, Ms, den, acc);
@@ -1973,7 +1979,7 @@ __device__ void small_unit(const ChunkParams& p, const Seq& s, int b, int kvh, u
     return (int64_t)(s.a0 + tok) * p.Hq + kvh * p.group + r - tok * p.group;
   };
   int2 at = make_int2(kDone, 0);
-  if (s.prefix && lane < RW && warp + lane * warps < rows) at = p.row_at[row_of(warp + lane * warps)];
+  if (s.prefix && lane < RW && warp + lane * warps < rows) at = row_place(p, row_of(warp + lane * warps));
   RowParts parts[RW];
   float largest[RW];
 #pragma unroll
