@@ -639,6 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ============================ exponentials ============================
     const int t = warp >> 2 & 1, half = warp >> 3, row = threadIdx.x & (BK - 1);
+    const bool ragged = used % 32;  // a full half reads columns of cleared rows of Q
     const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * BR + half * BK;
     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
     float* red = reinterpret_cast<float*>(smem + C::OFF_RED);
@@ -673,6 +674,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int skip = p.causal ? key - (sg.len - sg.n) - tok : 0;
           const bool masked = toks < p.TQ || (p.causal && key0 + BK - 1 - (sg.len - sg.n) - tok > 0);
           const int chunks = (max(toks, 0) * p.group + 31) / 32;
+          // In a full half the last chunk ends in columns of cleared rows, which an infinite key makes NaN.  They are
+          // looked at first (2048 tokens on top of 6144 of four sequences, 28 heads on 4, D = 64: 444 us; hidden
+          // without a look 480, not at all 436).
+          const int cleared_in = ragged ? chunks - 1 : -1;
           const float4* nl = reinterpret_cast<const float4*>(lse_s + slot * BR + half * BK);
           if (!chunks) {
             __syncwarp();
@@ -693,7 +698,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               __syncwarp();
               if (lane == 0) mbar_arrive(&s_free[t]);
             }
-            if (masked) {
+            if (masked || (c == cleared_in && __any_sync(0xffffffffu, x[31] != x[31]))) {
               const int lo = min(max(skip, 0), p.TQ) * p.group - c * 32, hi = toks * p.group - c * 32;
 #pragma unroll
               for (int e = 0; e < 32; ++e) x[e] = e >= lo && e < hi ? x[e] : -INFINITY;

@@ -1,0 +1,35 @@
+"""Accumulated attention weights where keys, queries or log-sum-exps are at their limits, and what a call copies."""
+import math
+
+import pytest
+import torch
+
+from test_attention_weights_gpu import DEV, check, make, reference_lse, same
+
+from attention_kernel_triton_b200.paged_kv_eviction import accumulate_attention_weights_paged
+
+pytestmark = pytest.mark.gpu
+
+
+def key_place(c, b, j):
+    """Page and row of key j of sequence b."""
+    P = c["cache"].shape[3]
+    return int(c["indices"][int(c["starts"][b]) + j // P]), j % P
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.float16, 64), (torch.bfloat16, 128)])
+@pytest.mark.parametrize("G", [1, 3, 5, 6, 7, 12, 28, 33, 64, 65, 96, 100])
+def test_a_key_that_every_row_scores_minus_infinity_gets_nothing(G, dtype, D):
+    # half tiles full of tokens, whose last columns no row fills where 128 is no multiple of the group
+    for n in (128 // G, 2 * (128 // G), 5 * (128 // G)):
+        c = make([n + 300], [n], G, 1, D, 16, dtype, seed=G)
+        c["q"][..., 3] = c["q"][..., 3].abs() + 0.125
+        for j in (0, 7, 200, n + 40):
+            page, row = key_place(c, 0, j)
+            c["cache"][page, 0, :, row, 3] = -math.inf
+        for causal in (True, False):
+            start = torch.rand(1, 1, n + 300, device=DEV)
+            got = check(c, causal, start=start)
+            assert torch.isfinite(got).all()
+            for j in (0, 7, 200, n + 40):
+                assert got[0, 0, j] == start[0, 0, j]
