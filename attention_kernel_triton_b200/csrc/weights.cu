@@ -123,7 +123,8 @@ struct Cfg {
   static constexpr uint32_t OFF_MISC = OFF_BAR + (N_BARS * 8 + 15) / 16 * 16;  // TMEM address, abort flag
   static constexpr uint32_t OFF_SEG = OFF_MISC + 16;
   static constexpr uint32_t OFF_RED = OFF_SEG + kSegs * sizeof(Seg);  // sums of a K tile's right half
-  static constexpr uint32_t SMEM = OFF_RED + BK * 4;
+  static constexpr uint32_t OFF_NONE = (OFF_RED + BK * 4 + 15) / 16 * 16;  // rows of Q that add nothing
+  static constexpr uint32_t SMEM = OFF_NONE + QS * (BR / 32) * 4;
   static_assert(SMEM <= 227 * 1024, "shared memory budget");
 };
 
@@ -201,6 +202,9 @@ __device__ __forceinline__ int64_t cost_before(const WeightsParams& p, const Seq
 // (8192 tokens on top of 24576: 2.02 ms, none 2.08, three of eight 2.12, all 3.02).
 constexpr bool on_fma_pipe(int pair) { return pair % 4 == 0; }
 
+// bits below n
+__device__ __forceinline__ unsigned below(int n) { return n >= 32 ? 0xffffffffu : (1u << max(n, 0)) - 1u; }
+
 // 2^v of two values on the FMA pipe, as mantissas and scales.  The shift puts
 // n + 127 into the low bits of t; v below -127 gives a scale of 0, NaN stays NaN.
 __device__ __forceinline__ void poly_exp2(float2 v, float2& mant, float2& scale) {
@@ -250,6 +254,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   Seg* segs = reinterpret_cast<Seg*>(smem + C::OFF_SEG);
   float* lse_s = reinterpret_cast<float*>(smem + C::OFF_LSE);  // [QS][BR]: -lse log2 e, -inf: no such row
+
+  unsigned* none_s = reinterpret_cast<unsigned*>(smem + C::OFF_NONE);  // [QS][BR / 32] bits: rows whose lse is -inf
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -570,8 +576,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                           (int64_t)(sg.kvh * p.group + rr - rt * p.group) * p.l_head) * kLog2e;
         }
 #pragma unroll
-        for (int i = 0; i < BR / 32; ++i)  // lse = -inf: the row adds nothing
+        for (int i = 0; i < BR / 32; ++i) {  // lse = -inf: the row adds nothing
+          const unsigned nothing = __ballot_sync(0xffffffffu, v[i] == INFINITY);
+          if (lane == 0) none_s[slot * (BR / 32) + i] = nothing;
           lse_s[slot * BR + i * 32 + lane] = v[i] == INFINITY ? -INFINITY : v[i];
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(&lse_full[slot]);
       }
@@ -675,10 +684,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           const bool masked = toks < p.TQ || (p.causal && key0 + BK - 1 - (sg.len - sg.n) - tok > 0);
           const int chunks = (max(toks, 0) * p.group + 31) / 32;
           // In a full half the last chunk ends in columns of cleared rows, which an infinite key makes NaN.  They are
-          // looked at first (2048 tokens on top of 6144 of four sequences, 28 heads on 4, D = 64: 444 us; hidden
-          // without a look 480, not at all 436).
+          // looked at first (2048 tokens on top of 6144 of four sequences, 28 heads on 4, D = 64: 421 us; hidden
+          // without a look 437).
           const int cleared_in = ragged ? chunks - 1 : -1;
           const float4* nl = reinterpret_cast<const float4*>(lse_s + slot * BR + half * BK);
+          const unsigned* none = none_s + slot * (BR / 32) + half * (BK / 32);
+          const uint4 n4 = *reinterpret_cast<const uint4*>(none);
+          const bool hides = masked || (n4.x | n4.y | n4.z | n4.w);
           if (!chunks) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_free[t]);
@@ -698,10 +710,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               __syncwarp();
               if (lane == 0) mbar_arrive(&s_free[t]);
             }
-            if (masked || (c == cleared_in && __any_sync(0xffffffffu, x[31] != x[31]))) {
+            if (hides || (c == cleared_in && __any_sync(0xffffffffu, x[31] != x[31]))) {
               const int lo = min(max(skip, 0), p.TQ) * p.group - c * 32, hi = toks * p.group - c * 32;
+              const unsigned hidden = none[c] | below(lo) | ~below(hi);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) x[e] = e >= lo && e < hi ? x[e] : -INFINITY;
+              for (int e = 0; e < 32; ++e) x[e] = hidden >> e & 1u ? -INFINITY : x[e];
             }
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {

@@ -33,3 +33,22 @@ def test_a_key_that_every_row_scores_minus_infinity_gets_nothing(G, dtype, D):
             assert torch.isfinite(got).all()
             for j in (0, 7, 200, n + 40):
                 assert got[0, 0, j] == start[0, 0, j]
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(4, 1), (6, 2), (1, 1)])
+def test_a_row_whose_lse_is_minus_infinity_adds_nothing_whatever_it_holds(Hq, Hkv):
+    c = make([300, 200], [70, 200], Hq, Hkv, 64, 16, seed=20)
+    lse = reference_lse(c, True, 0.125)
+    off = torch.zeros(270, dtype=torch.bool, device=DEV)
+    off[[0, 1, 33, 69, 70, 71, 140, 269]] = True
+    lse[off] = -math.inf
+    c["q"][off] = math.nan
+    c["q"][1] = math.inf
+    got = check(c, lse=lse)
+    assert torch.isfinite(got).all()
+    # a head of a row alone
+    c = make([90], [40], 4, 1, 128, 8, seed=21)
+    lse = reference_lse(c, False, 128 ** -0.5)
+    lse[5, 2] = -math.inf
+    c["q"][5, 2] = math.nan
+    assert torch.isfinite(check(c, False, lse=lse)).all()
