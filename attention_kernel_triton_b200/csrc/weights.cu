@@ -206,11 +206,14 @@ constexpr bool on_fma_pipe(int pair) { return pair % 4 == 0; }
 __device__ __forceinline__ unsigned below(int n) { return n >= 32 ? 0xffffffffu : (1u << max(n, 0)) - 1u; }
 
 // 2^v of two values on the FMA pipe, as mantissas and scales.  The shift puts
-// n + 127 into the low bits of t; v below -127 gives a scale of 0, NaN stays NaN.
+// n + 127 into the low bits of t; v below -127 gives a scale of 0, from 127.5 on one of
+// infinity (only with a log-sum-exp that is not the row's own), NaN stays NaN.
 __device__ __forceinline__ void poly_exp2(float2 v, float2& mant, float2& scale) {
   constexpr float kShift = 12582912.f + 127.f;  // 1.5 * 2^23 + 127
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(v.x) : "f"(v.x), "f"(-127.f));
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(v.y) : "f"(v.y), "f"(-127.f));
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(v.x) : "f"(v.x), "f"(128.f));
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(v.y) : "f"(v.y), "f"(128.f));
   const float2 t = __fadd2_rn(v, make_float2(kShift, kShift));
   const float2 n = __fadd2_rn(t, make_float2(-kShift, -kShift));
   const float2 f = __fadd2_rn(v, make_float2(-n.x, -n.y));

@@ -52,3 +52,21 @@ def test_a_row_whose_lse_is_minus_infinity_adds_nothing_whatever_it_holds(Hq, Hk
     lse[5, 2] = -math.inf
     c["q"][5, 2] = math.nan
     assert torch.isfinite(check(c, False, lse=lse)).all()
+
+
+@pytest.mark.parametrize("n,G", [(1, 1), (1, 4), (5, 1), (40, 2), (130, 1)])
+def test_weights_past_the_range_of_fp32_are_infinite(n, G):
+    # log-sum-exps that are not the rows' own: 60 below them (weights up to e^60), then 100 (past fp32)
+    c = make([300], [n], G, 1, 64, 16, seed=22, scale=0.125)
+    lse = reference_lse(c, False, 0.125)
+    check(c, False, lse=lse - 60)
+    args = c["q"], c["at"], c["cache"], c["starts"], c["indices"], c["last"]
+    for far in (100, 1000):
+        got = accumulate_attention_weights_paged(None, *args, lse - far, causal=False, out=torch.zeros(1, 1, 300, device=DEV))
+        assert (got == math.inf).all()  # exp(-|q k| - log 300 + 100) > e^89
+    # a key that every row scores +infinity, beside finite ones
+    c["q"][..., 0] = 1
+    page, row = key_place(c, 0, 17)
+    c["cache"][page, 0, 0, row, 0] = math.inf
+    got = accumulate_attention_weights_paged(None, *args, lse, causal=False, out=torch.zeros(1, 1, 300, device=DEV))
+    assert got[0, 0, 17] == math.inf and torch.isfinite(got[0, 0, :17]).all() and torch.isfinite(got[0, 0, 18:]).all()
