@@ -32,6 +32,7 @@ import math
 import torch
 
 from . import _lib
+from .paged_chunk_attention import _on_grid
 from .paged_kv_pages import _pool, _ptr, _reserved
 
 _weights = _lib.Entry("akt_attention_weights", _lib.AttentionWeightsArgs, _lib.c_void_p, _lib.c_size_t, _lib.c_void_p)
@@ -101,11 +102,12 @@ def accumulate_attention_weights_paged(weights, q, q_indptr, paged_kv_cache, kv_
 
     with _lib.on_index(index):
         rc = call(q, paged_kv_cache)
-        if rc == _lib.AKT_ERR_UNSUPPORTED and D in (64, 128) and Hq <= 128 * pool[2]:  # strides that no tensor map takes
-            rc = call(q.contiguous(), paged_kv_cache)
+        if rc == _lib.AKT_ERR_UNSUPPORTED and D in (64, 128) and Hq <= 128 * pool[2]:
+            # a layout: what is off the 16-byte grid is copied, then both (strides that no tensor map takes)
+            q, cache = (t if _on_grid(t) else t.clone(memory_format=torch.contiguous_format) for t in (q, paged_kv_cache))
+            rc = call(q, cache)
             if rc == _lib.AKT_ERR_UNSUPPORTED:
-                rc = call(q.clone(memory_format=torch.contiguous_format),
-                          paged_kv_cache.clone(memory_format=torch.contiguous_format))
+                rc = call(q.contiguous(), cache.contiguous())
         _lib.check(rc)
     return out
 

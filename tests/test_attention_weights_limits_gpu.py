@@ -70,3 +70,30 @@ def test_weights_past_the_range_of_fp32_are_infinite(n, G):
     c["cache"][page, 0, 0, row, 0] = math.inf
     got = accumulate_attention_weights_paged(None, *args, lse, causal=False, out=torch.zeros(1, 1, 300, device=DEV))
     assert got[0, 0, 17] == math.inf and torch.isfinite(got[0, 0, :17]).all() and torch.isfinite(got[0, 0, 18:]).all()
+
+
+def test_queries_off_the_grid_are_copied_and_the_pool_is_not():
+    c = make([300, 90], [40, 1], 8, 8, 128, 16, seed=23)
+    args = c["at"], c["starts"], c["indices"], c["last"], reference_lse(c, True, 128 ** -0.5)
+
+    def run(q, pool):
+        return accumulate_attention_weights_paged(None, q, args[0], pool, *args[1:], out=torch.zeros(2, 8, 300, device=DEV))
+
+    want = run(c["q"], c["cache"])
+    pool = torch.zeros(600, *c["cache"].shape[1:], dtype=c["cache"].dtype, device=DEV)  # 39 MB
+    pool[:c["cache"].shape[0]] = c["cache"]
+    flat = torch.zeros(c["q"].numel() + 1, dtype=c["q"].dtype, device=DEV)
+    shifted = flat[1:].view(c["q"].shape)  # contiguous, and off the grid
+    odd = torch.zeros(*c["q"].shape[:2], 129, dtype=c["q"].dtype, device=DEV)[..., 1:]
+    for q in (shifted, odd):
+        q.copy_(c["q"])
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        got = run(q, pool)
+        assert same(got, want)
+        assert torch.cuda.max_memory_allocated() - before < 8 << 20
+    flat = torch.zeros(c["cache"].numel() + 1, dtype=c["cache"].dtype, device=DEV)
+    moved = flat[1:].view(c["cache"].shape)
+    moved.copy_(c["cache"])
+    assert same(run(shifted, moved), want) and same(run(c["q"], moved), want)
