@@ -525,6 +525,7 @@ __global__ void __launch_bounds__(kMoveThreads, 2) evict_move_kernel(const Evict
   // are moved, the next ones, and those before, which a warp may still store.  In bytes;
   // from < 0: nothing moves.
   __shared__ int64_t from[3][kMoveThreads], to[3][kMoveThreads];
+  __shared__ int in_place[kMoveThreads / 32];
   const int C = (int)cluster_size(), rank = (int)cluster_rank(), tid = threadIdx.x, parts = p.w ? 3 : 2;
   int unit = blockIdx.x / C;
   const int part = unit % parts;
@@ -534,12 +535,15 @@ __global__ void __launch_bounds__(kMoveThreads, 2) evict_move_kernel(const Evict
   const int n = p.count[b], len = p.lens[b];
   const int s = __ldg(p.indptr + b), os = p.out_indptr[b];
   const int32_t* keep = p.keep + l * p.k_layer + b * p.k_batch + h * p.k_head;
-  // the rows that stay in place are the first ones
+  // the rows that stay in place are the first ones: as many as stand before the first entry looked at that is not its slot
   const int step = (n + kMoveThreads - 1) / kMoveThreads;
   int start = 0;
   if (n) {
     const int i = min((tid + 1) * step, n) - 1;
-    start = min(__syncthreads_count(__ldg(keep + i) == i) * step, n);
+    const unsigned moves = __ballot_sync(0xffffffffu, __ldg(keep + i) != i);
+    if ((tid & 31) == 0) in_place[tid >> 5] = moves ? (tid + __ffs(moves) - 1) * step : n;
+    __syncthreads();
+    start = __reduce_min_sync(0xffffffffu, min(in_place[tid & (kMoveThreads / 32 - 1)], n));
   }
   if (part == 2) {
     float* w = p.w + l * p.w_layer + b * p.w_batch + h * p.w_head;
