@@ -589,8 +589,13 @@ __global__ void __launch_bounds__(kMoveThreads, 2) evict_move_kernel(const Evict
         const int pj = (int)fdiv((uint32_t)j, p.div_page), pi = (int)fdiv((uint32_t)i, p.div_page);
         const int src = __ldg(p.indices + s + pj), dst = p.out_indices[os + pi];
         if (src >= 0 && src < p.num_pages && dst >= 0 && dst < p.num_pages && (src != dst || i != j)) {
-          f = src * p.s_page + (j - pj * p.P) * p.s_tok;
-          t = dst * p.s_page + (i - pi * p.P) * p.s_tok;
+          // a page of several holders that was not replaced: the list does not ascend
+          if (p.again[dst >> 5] >> (dst & 31) & 1u) {
+            record_status(kStatusBadToken);
+          } else {
+            f = src * p.s_page + (j - pj * p.P) * p.s_tok;
+            t = dst * p.s_page + (i - pi * p.P) * p.s_tok;
+          }
         }
       }
     }

@@ -690,10 +690,12 @@ int akt_select_tokens(const akt_select_tokens_args* args, void* stream);
 /* kept row keep their contents.  weights [layers, batch, num_kv_heads,      */
 /* width] (fp32, or NULL) move along, zeros in the places they leave.  A     */
 /* list entry behind the sequence, below its slot or not above the one       */
-/* before it is skipped, keep_len past max_kept or the sequence is cut (both */
-/* status 3); a sequence with bad bounds is empty (status 4), pages past     */
-/* max_entries are cut (status 5), ids outside the pool stay as they are     */
-/* (status 2; negative ones become -1).  Tokens past `width` have weight 0.  */
+/* before it is skipped, and so is a row that, in a list that does not       */
+/* ascend, would go to a page of several holders; keep_len past max_kept or  */
+/* the sequence is cut (all status 3); a sequence with bad bounds is empty   */
+/* (status 4), pages past max_entries are cut (status 5), ids outside the    */
+/* pool stay as they are (status 2; negative ones become -1).  Tokens past   */
+/* `width` have weight 0.                                                    */
 /* The new table must not overlap the old one.                               */
 typedef struct akt_evict_paged_args {
   akt_page_pool pool;
