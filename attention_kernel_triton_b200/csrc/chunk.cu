@@ -741,7 +741,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 32) {
+  if (SHARED && threadIdx.x == 32) {  // (in the form without shared prefixes it spills at D = 64)
     prefetch_tensor_map(&tmQ);
     prefetch_tensor_map(&tmK);
     prefetch_tensor_map(&tmV);
