@@ -153,8 +153,8 @@ struct ChunkParams {
   struct Seq* own;     // [batch] the sequences on their own keys; those with few have no rows in `seqs`
   int* prefix_len;     // [batch] shared keys of each sequence
   int* order;          // [batch] the sequences, those with the most own keys first
-  float* row_o;        // [2][rows][D] normalised outputs of a row on the prefix, on its own keys
-  float* row_lse;      // [2][rows]
+  float* row_o;        // [2][rows][D] (none without groups) normalised outputs of a row on the prefix, on its own keys
+  float* row_lse;      // [2][rows] (none without groups)
   int2* row_at;        // [2][rows] kWhole, kDone, or the place of the first part and the row there
 };
 
@@ -1583,7 +1583,8 @@ struct RowParts {
 // Entry i of row_at.  Where a wait ran out (recorded) it may never have been written: no place outside the workspace.
 __device__ __forceinline__ int2 row_place(const ChunkParams& p, int64_t i) {
   const int2 w = p.row_at[i];
-  return w.x >= 2 * p.grid || (w.x >= 0 && (unsigned)w.y >= (unsigned)p.part_rows) ? make_int2(kDone, 0) : w;
+  const bool nowhere = w.x < 0 ? !p.groups : w.x >= 2 * p.grid || (unsigned)w.y >= (unsigned)p.part_rows;
+  return nowhere ? make_int2(kDone, 0) : w;
 }
 
 __device__ __forceinline__ RowParts row_parts(const ChunkParams& p, int2 w) {
@@ -2125,8 +2126,9 @@ Layout make_layout(const akt_chunk_paged_args* a, int groups, bool shared) {
     y.own = take((size_t)a->batch * sizeof(Seq));
     y.prefix = take((size_t)a->batch * 4);
     y.order = take((size_t)a->batch * 4);
-    y.row_o = take(2 * rows * a->head_dim * 4);
-    y.row_lse = take(2 * rows * 4);
+    const size_t results = groups ? 2 * rows : 0;  // (rows without a prefix have theirs in the output or in parts)
+    y.row_o = take(results * a->head_dim * 4);
+    y.row_lse = take(results * 4);
     y.row_at = take(2 * rows * sizeof(int2));
   }
   y.bytes = at;
@@ -2210,7 +2212,7 @@ int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap
 template <typename T, int D>
 int dispatch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const ChunkParams& p,
                    cudaStream_t st) {
-  if (p.row_o)
+  if (p.row_at)
     return p.box_rows ? launch_chunk<T, D, true, true>(mq, mk, mv, p, st) : launch_chunk<T, D, false, true>(mq, mk, mv, p, st);
   return p.box_rows ? launch_chunk<T, D, true, false>(mq, mk, mv, p, st) : launch_chunk<T, D, false, false>(mq, mk, mv, p, st);
 }

@@ -11,6 +11,9 @@ pool, table, masks and results are those of
 drafted tokens and prompt chunks alike.  The two results are kept in fp32 until they
 are joined.  No gradient.  Runs ``akt_prefix_paged`` (sm_100a) on torch's current stream.
 
+The workspace of a call with groups holds both fp32 results of every row, ``8 T Hq D``
+bytes: chunks of long prompts are better small.
+
 The sequences of a group stand side by side in the batch: group ``g`` is
 ``group_indptr[g]:group_indptr[g + 1]`` (a fork's ``parents`` in that order give it).
 """
