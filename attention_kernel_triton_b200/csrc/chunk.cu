@@ -107,7 +107,10 @@ constexpr int kFewRows = 48;
 // eight prefixes, 20 rows: 159, here 181.  (More rows take a multiple of the warp-level
 // products; longer keys are better cut over several SMs.)
 constexpr int kSmallRows = 32, kSmallKeys = 2048;
-constexpr int kOrderSeqs = 1024;   // sequences that the planner orders by length for it
+// The planner gives that kernel the longest first up to so many sequences (a quadratic count).  One token in each of n
+// sequences of up to 1024 own keys behind 2048, eight kv heads, in order / as they come: n = 16 32.8 / 35.6 us, 64
+// 66.0 / 67.0, 128 98 / 90, 256 168 / 143, 1024 536 / 459; one kv head, 1024 160 / 120.
+constexpr int kOrderSeqs = 64;
 constexpr int kTableSeqs = 96;     // sequences whose table fits the CTA's shared memory
 constexpr int kMaxCtas = kThreads; // of the main kernel (one per SM)
 
@@ -682,7 +685,7 @@ __device__ void build_shared(const ChunkParams& p, int* bad) {
     p.order[b] = b;
   }
   __syncthreads();
-  // long ones first, so that none of them begins last (past kOrderSeqs the sorting would take longer than it saves)
+  // long ones first, so that none of them begins last
   if (p.batch <= kOrderSeqs)
     for (int b = threadIdx.x; b < p.batch; b += 1024) {
       const int len = p.own[b].len;
