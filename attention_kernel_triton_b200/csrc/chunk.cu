@@ -103,9 +103,12 @@ constexpr int kFewRows = 48;
 // Units of a sequence's own keys behind a prefix that take the warp-level kernel: a
 // unit's chain of steps here (Q, S, the exponentials, P.V, the output) takes 4 us however
 // few its rows and tiles are.  One token in each of 64 sequences of 64 to 1024 own keys
-// behind 8192, 4 rows a unit: 72 us, all units here 101; five tokens in each of 64 behind
-// eight prefixes, 20 rows: 159, here 181.  (More rows take a multiple of the warp-level
-// products; longer keys are better cut over several SMs.)
+// behind 8192, 4 rows a unit: 74 us, all units here 151; five tokens in each of 64 behind
+// eight prefixes, 20 rows: 160, here 216.  So too where few units leave SMs without one,
+// n sequences of 2048 own keys behind 2048 on eight kv heads, n = 2 45 / 67, 8 48 / 66, 16
+// 60 / 93, 64 122 / 190.  Past 2048 it depends on n: 4096 own keys, n = 2 70 / 66, 16
+// 87 / 106, 64 198 / 314; 8192, n = 2 128 / 72, 16 140 / 149, 64 351 / 449.  (More rows take
+// a multiple of the warp-level products.)
 constexpr int kSmallRows = 32, kSmallKeys = 2048;
 // The planner gives that kernel the longest first up to so many sequences (a quadratic count).  One token in each of n
 // sequences of up to 1024 own keys behind 2048, eight kv heads, in order / as they come: n = 16 32.8 / 35.6 us, 64

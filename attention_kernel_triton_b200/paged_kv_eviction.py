@@ -55,7 +55,8 @@ def accumulate_attention_weights_paged(weights, q, q_indptr, paged_kv_cache, kv_
 
     weights: [B, Hkv, L] fp32, L no less than the longest sequence; None: from zero, into ``out``
     q .. softmax_scale: those of ``flash_attention_chunk_paged_with_lse``, whose second result is
-    lse: [T, Hq] fp32; a row of -inf adds nothing
+    lse: [T, Hq] fp32, over all keys that the row sees (with another one the sums are not of
+        softmax weights, and may pass fp32's range); a row of -inf adds nothing
     out: [B, Hkv, L] fp32 for the sums; None: ``weights`` itself
     returns out; its places past a sequence's length stay as they were
     """
